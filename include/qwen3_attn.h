@@ -347,6 +347,50 @@ int qwen3_padded_prefill_bf16(const void* q, const int64_t q_strides[3], const v
                               size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Attention of a chunk of new tokens over the paged cache (no counterpart in the
+ * reference engine, which prefills a prompt whole and then decodes): a prompt
+ * prefilled in pieces, new turns behind a cached prefix, draft tokens to verify,
+ * and all of these with decoding sequences in one batch.
+ *
+ * Sequence b has the tokens cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of q and
+ * seq_lens[row] tokens before them (row = row_ids[b]; NULL: b); their keys and
+ * values are in the pool already, at positions seq_lens[row] + i.  Token i attends
+ * positions 0 .. seq_lens[row] + i.
+ *   q           (total_tokens, num_heads, head_dim), packed
+ *   k_cache, v_cache, block_table, seq_lens, row_ids: as qwen3_paged_decode_bf16
+ *   cu_seqlens  device int32 (B + 1), non-decreasing; a range outside
+ *               [0, total_tokens] counts as empty
+ *   max_chunk   host bound of the chunks' lengths: tokens of a longer chunk
+ *               behind it may be left unwritten
+ *   out         (total_tokens, num_heads, head_dim); rows that belong to no
+ *               sequence are left as they are, rows that may attend nothing (no
+ *               row of the table, negative length) are zero
+ *   scale       positive and finite
+ *   workspace   qwen3_paged_chunk_workspace_bytes(...) bytes, needs no
+ *               initialisation; calls that share one must not overlap
+ * Positions behind what a table row addresses, and pages whose id is no block of
+ * the pool, are not attended.  Slots behind a sequence's last token are not read.
+ * The new tokens' values must be finite: a value that is not reaches the chunk's
+ * earlier tokens too.
+ * Supported: head_dim 128; block_size a multiple of 16; num_heads / num_kv_heads up
+ * to 16; slot strides from head_dim to 2^24 elements; 16-byte aligned rows.
+ * ---------------------------------------------------------------------- */
+size_t qwen3_paged_chunk_workspace_bytes(int B, int max_chunk, int64_t total_tokens,
+                                         int num_heads, int num_kv_heads, int head_dim);
+
+int qwen3_paged_chunk_bf16(const void* q, const int64_t q_strides[2],
+                           const void* k_cache, const int64_t k_strides[3],
+                           const void* v_cache, const int64_t v_strides[3],
+                           int64_t num_blocks, const int32_t* block_table,
+                           int64_t bt_row_stride, int64_t max_rows, int64_t max_pages,
+                           const int32_t* seq_lens, const int32_t* row_ids,
+                           const int32_t* cu_seqlens, void* out,
+                           const int64_t out_strides[2], int B, int max_chunk,
+                           int64_t total_tokens, int num_heads, int num_kv_heads,
+                           int head_dim, int block_size, float scale, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Fused pre-attention step: QK-RMSNorm + RoPE + K/V pool write.
  *
  * Replaces, in one launch, q_norm / k_norm (qwen3/attention.py:91-92 with

@@ -117,6 +117,14 @@ _SIGNATURES = {
          ctypes.POINTER(ctypes.c_int32), _i, _i,
          _i, _i, _i, ctypes.c_float, _i, _vp, ctypes.c_size_t, _vp],
     ),
+    "qwen3_paged_chunk_workspace_bytes": (ctypes.c_size_t, [_i, _i, _i64, _i, _i, _i]),
+    "qwen3_paged_chunk_bf16": (
+        _i,
+        [_vp, _c_i64p, _vp, _c_i64p, _vp, _c_i64p, _i64,
+         _vp, _i64, _i64, _i64, _vp, _vp, _vp,
+         _vp, _c_i64p,
+         _i, _i, _i64, _i, _i, _i, _i, ctypes.c_float, _vp, ctypes.c_size_t, _vp],
+    ),
     "qwen3_qk_norm_rope_decode_bf16": (
         _i,
         [_vp, _c_i64p, _vp, _c_i64p, _vp, _c_i64p, _vp, _vp, ctypes.c_float,
@@ -169,7 +177,7 @@ _SIGNATURES = {
     ),
 }
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 _lib = None
 

@@ -1,0 +1,521 @@
+// Attention of a chunk of new tokens over the paged cache, for gfx950 (GQA).
+//
+// Sequence s of the batch has n_s new tokens, packed in q from row cu[s], and
+// c_s = seq_lens[row_s] tokens before them; the new tokens' keys and values are
+// in its pages already.  Token i attends the keys j <= c_s + i of its row of the
+// block table:
+//   o_i = sum_j exp(scale q_i k_j) v_j / sum_j exp(scale q_i k_j),
+// in one pass with a running maximum and sum in fp32; P is rounded to bf16 for
+// the PV product (a relative error of at most 2^-8 per term of a weighted mean),
+// the output once to bf16.  A row without keys is zero.
+//
+//  * Query rows of one KV head are packed: row r is token r / G, head r % G of
+//    the group, so one staged K/V tile serves every head of the group whatever
+//    G is.  A work item is (sequence, KV head, 128 packed rows); each of the
+//    four waves of a workgroup owns 32 of them.
+//  * K/V tiles of 64 keys go from HBM into LDS by buffer loads that write LDS,
+//    16 keys a wave, so a wave reads one page per tile: its base is a scalar and
+//    the lanes' offsets never change.  The descriptor ends at the sequence's
+//    last key (or holds nothing where the table names no page of the pool), so
+//    slots behind it are never read.  Page ids come 64 at a time into a
+//    register (16 tiles' worth), the next 64 before they are needed.
+#include "prefill_tile.hpp"
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kRows = 32 * kWaves;   // packed query rows of an item
+constexpr int kMaxG = 16;
+constexpr float kRescaleSlack = 8.f;  // log2 headroom before the running maximum is raised
+constexpr int kGroup = 16;           // keys a wave loads of a tile: inside one page
+
+struct ChunkArgs {
+  const uint16_t* q;
+  int64_t q_st, q_sh;
+  const uint16_t* k;
+  int64_t k_blk, k_sh, k_slot;
+  const uint16_t* v;
+  int64_t v_blk, v_sh, v_slot;
+  int64_t num_blocks;
+  const int32_t* bt;
+  int64_t bt_stride, max_rows, max_pages;
+  const int32_t* seq_lens;
+  const int32_t* row_ids;  // nullable: identity
+  const int32_t* cu;
+  uint16_t* o;
+  int64_t o_st, o_sh;
+  int64_t total;   // rows of q
+  int B, Hkv, G, bs;
+  int n_mtiles;    // items of the longest chunk of one KV head
+  float scale_log2;
+};
+
+// One sequence of the batch.
+struct Seq {
+  int64_t q0;   // its first row of q
+  int n;        // its new tokens (0: nothing is computed)
+  int64_t row;  // its row of the block table, -1: none
+  int ctx;      // tokens before the new ones
+  int cap;      // keys that may be attended: at most what its tokens reach and a row holds
+};
+
+__device__ __forceinline__ Seq seq_at(const ChunkArgs& a, int b) {
+  Seq s;
+  const int64_t s0 = a.cu[b], s1 = a.cu[b + 1];
+  const bool ok = s0 >= 0 && s1 > s0 && s1 <= a.total;
+  s.q0 = ok ? s0 : 0;
+  s.n = ok ? static_cast<int>(s1 - s0) : 0;
+  const int64_t row = a.row_ids ? a.row_ids[b] : b;
+  s.row = row >= 0 && row < a.max_rows ? row : -1;
+  s.ctx = s.row >= 0 ? a.seq_lens[s.row] : 0;
+  const int64_t len = static_cast<int64_t>(s.ctx) + s.n, most = a.max_pages * a.bs;
+  const int64_t cap = len < most ? len : most;
+  s.cap = s.row >= 0 && cap > 0 ? static_cast<int>(cap) : 0;
+  return s;
+}
+
+// Keys that packed rows r0 .. r1 - 1 of a sequence reach.
+__device__ __forceinline__ int keys_of(const ChunkArgs& a, const Seq& s, int r1) {
+  const int tokens = min(s.n, (r1 + a.G - 1) / a.G);
+  const int64_t reach = static_cast<int64_t>(s.ctx) + tokens;
+  return static_cast<int>(reach < 0 ? 0 : reach < s.cap ? reach : s.cap);
+}
+
+struct TileBufs {
+  uint16_t* k0;
+  uint16_t* v0;
+  uint16_t* k1;
+  uint16_t* v1;
+};
+
+constexpr int kDma = kGroup * kRowBytes / (64 * 16);  // 16-byte loads a lane of a K or V tile
+
+struct LaneOffsets {
+  uint32_t kdma[kDma], vdma[kDma];  // source offsets within the wave's 16 keys
+  uint32_t kread, vread;
+};
+
+__device__ __forceinline__ LaneOffsets lane_offsets(const ChunkArgs& a, int lane) {
+  LaneOffsets o;
+  // Load j of a wave fills rows 4 j .. 4 j + 3 of its 16; lane i writes slot
+  // i % 16 of row 4 j + i / 16, i.e. source chunk slot ^ swz(row).
+#pragma unroll
+  for (int j = 0; j < kDma; ++j) {
+    const int row = 4 * j + (lane >> 4);
+    const int slot = lane & 15;
+    o.kdma[j] = static_cast<uint32_t>(row * a.k_slot * 2) + ((slot ^ (row & 15)) << 4);
+    o.vdma[j] = static_cast<uint32_t>(row * a.v_slot * 2) + ((slot ^ (4 * (row & 3))) << 4);
+  }
+  read_offsets(o, lane);
+  return o;
+}
+
+// The pages of the item's next 64 groups of 16 keys (16 tiles), a lane each,
+// and of the 64 after them.
+struct PageWindow {
+  int base;           // group of lane 0
+  int32_t cur, next;
+  uint64_t ok;        // groups of the window whose page is a block of the pool
+};
+
+__device__ __forceinline__ int32_t page_of_group(const ChunkArgs& a, int64_t row, int group) {
+  const int64_t page = static_cast<int64_t>(group) * kGroup / a.bs;
+  return row >= 0 && page < a.max_pages ? a.bt[row * a.bt_stride + page] : -1;
+}
+__device__ __forceinline__ void window_check(PageWindow& w, const ChunkArgs& a) {
+  w.ok = __ballot(w.cur >= 0 && w.cur < a.num_blocks);
+}
+__device__ __forceinline__ void window_start(PageWindow& w, const ChunkArgs& a, int64_t row,
+                                             int tile, int lane) {
+  w.base = tile * (kBN / kGroup);
+  w.cur = page_of_group(a, row, w.base + lane);
+  w.next = page_of_group(a, row, w.base + 64 + lane);
+  window_check(w, a);
+}
+// Moves on once `tile` lies behind the window (tiles come in order).
+__device__ __forceinline__ void window_to(PageWindow& w, const ChunkArgs& a, int64_t row, int tile,
+                                          int lane) {
+  if (tile * (kBN / kGroup) < w.base + 64) return;
+  w.base += 64;
+  w.cur = w.next;
+  w.next = page_of_group(a, row, w.base + 64 + lane);
+  window_check(w, a);
+}
+
+// Issues this wave's share (16 keys) of the loads of key tile `tile` into (sk, sv).
+// Returns which of the tile's four groups lie in the pool's blocks.
+__device__ __forceinline__ uint32_t tile_dma(const ChunkArgs& a, const LaneOffsets& off,
+                                             PageWindow& w, const Seq& s, int kvh, int tile,
+                                             uint16_t* sk, uint16_t* sv, int wave, int lane) {
+  window_to(w, a, s.row, tile, lane);
+  const int g0 = tile * (kBN / kGroup) - w.base;
+  const int64_t phys = __builtin_amdgcn_readlane(w.cur, g0 + wave);
+  const uint32_t ok = static_cast<uint32_t>(w.ok >> g0) & 15u;
+  const int key = tile * kBN + wave * kGroup;
+  const int rows = (ok >> wave) & 1u ? min(kGroup, s.cap - key) : 0;
+  const int64_t sub = key % a.bs;
+  const uint16_t* kb = a.k + kvh * a.k_sh;
+  const uint16_t* vb = a.v + kvh * a.v_sh;
+  if (rows > 0) {
+    kb += phys * a.k_blk + sub * a.k_slot;
+    vb += phys * a.v_blk + sub * a.v_slot;
+  }
+  const int k_bytes = rows > 0 ? static_cast<int>((rows - 1) * a.k_slot * 2) + kRowBytes : 0;
+  const int v_bytes = rows > 0 ? static_cast<int>((rows - 1) * a.v_slot * 2) + kRowBytes : 0;
+  const __amdgpu_buffer_rsrc_t kr =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(kb), 0, k_bytes, 0x00020000);
+  const __amdgpu_buffer_rsrc_t vr =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(vb), 0, v_bytes, 0x00020000);
+#pragma unroll
+  for (int j = 0; j < kDma; ++j) {
+    const int blk = (kDma * wave + j) * 512;  // elements: 1 KiB per load
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void_t*)(sk + blk), 16, off.kdma[j], 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void_t*)(sv + blk), 16, off.vdma[j], 0, 0, 0);
+  }
+  return ok;
+}
+
+// A wave's 32 packed rows: lane l holds row r0 + l % 32.
+struct WaveRows {
+  int r0;         // first packed row
+  int tok, head;  // this lane's token and head of the group
+  int last;       // last key of this lane's token (-1: none)
+  int lo, hi;     // least and greatest such key of the wave's rows (uniform)
+  bool active;    // the wave has rows of the sequence
+};
+
+__device__ __forceinline__ WaveRows wave_rows(const ChunkArgs& a, const Seq& s, int mt, int wave,
+                                              int lane) {
+  WaveRows w;
+  w.r0 = mt * kRows + wave * 32;
+  const int r = w.r0 + (lane & 31);
+  w.tok = r / a.G;
+  w.head = r - w.tok * a.G;
+  auto last = [&](int tok) {
+    const int64_t p = static_cast<int64_t>(s.ctx) + min(tok, s.n - 1);
+    return static_cast<int>(p < s.cap - 1 ? (p < -1 ? -1 : p) : s.cap - 1);
+  };
+  w.last = last(w.tok);
+  w.lo = last(w.r0 / a.G);
+  w.hi = last((w.r0 + 31) / a.G);
+  w.active = w.r0 < s.n * a.G;
+  return w;
+}
+
+__device__ __forceinline__ void load_q(const ChunkArgs& a, const Seq& s, const WaveRows& w,
+                                       int kvh, int lane, q3::bf16x8 (&qv)[8]) {
+  const bool ok = w.tok < s.n;
+  const uint16_t* p = a.q + (s.q0 + (ok ? w.tok : 0)) * a.q_st +
+                      (static_cast<int64_t>(kvh) * a.G + (ok ? w.head : 0)) * a.q_sh +
+                      8 * (lane >> 5);
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    qv[c] = q3::as_bf16x8(ok ? q3::ld16(p + 16 * c) : q3::u32x4{0u, 0u, 0u, 0u});
+}
+
+// One 64-key tile (staged in kt / vt) folded into this wave's online softmax
+// state; c: the softmax scale times log2(e).  mask(s) sets the scores of masked
+// keys to -inf: s[kb][r] of a lane is key 32 kb + 8 (r / 4) + r % 4 + 4 (lane / 32)
+// of the tile.
+template <typename Off, typename Mask>
+__device__ __forceinline__ void tile_fold(const Off& off, float c, const Mask& mask,
+                                          const uint16_t* kt, const uint16_t* vt, const q3::bf16x8 (&qv)[8],
+                                          float& m_run, float& l_run, q3::f32x16 (&acc)[4]) {
+  // ---- S^T = K Q^T for two 32-key blocks ----
+  // Step u covers key block u % 2, dims 16 (u / 2) .. +15; the two blocks'
+  // chains alternate and K operands are read 4 steps ahead (the scheduling
+  // fences keep that distance).
+  q3::f32x16 s[2];
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
+  {
+    q3::bf16x8 kf[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) kf[u] = lds_ld16(kt, qk_operand(off, u));
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      s[u & 1] = q3::mfma32x32x16(kf[u % kAhead], qv[u >> 1], s[u & 1]);
+      if (u + kAhead < 16) kf[u % kAhead] = lds_ld16(kt, qk_operand(off, u + kAhead));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  mask(s);
+  // Row max as a v_max3 chain over the lane's 32 scores.  The scores were
+  // written by the QK MFMAs just above: 24 wait states cover the
+  // MFMA-to-VALU dependency.
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7");
+  float bm = max3_scores(s);
+  bm = cross_half_max(bm);
+  const float m_cand = bm * c;
+  const bool raise = m_cand > m_run + kRescaleSlack;
+  if (__any(raise)) {
+    const float m_new = raise ? m_cand : m_run;
+    const float alpha = raise ? q3::fast_exp2(m_run - m_new) : 1.f;
+    m_run = m_new;
+    l_run *= alpha;
+#pragma unroll
+    for (int db = 0; db < 4; ++db) acc[db] *= alpha;
+  }
+  // V^T operands of the first PV steps are read before the exponentials,
+  // which hide their latency.
+  q3::bf16x8 vf[kAhead];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) vf[u] = lds_vt(vt, pv_operand(off, u));
+  __builtin_amdgcn_sched_barrier(0);
+  const float m_use = m_run == q3::kNegInf ? 0.f : m_run;
+  // ---- P = exp2(s * c - m) as P^T B operands (chunk g = 2 kb + kc:
+  // scores s[kb][8 kc .. 8 kc + 7]) and O^T += V^T P^T, step u covering
+  // key chunk u / 4, dims 32 (u % 4) .. +31.  Chunk 0 is computed first;
+  // the exponentials of chunk g + 1 are issued between the four MFMAs of
+  // chunk g, two per step, so the VALU works while the matrix core runs.
+  q3::u32x4 pk[4];
+  float psum[4];  // four independent sum chains, started by chunk 0
+  auto exp_pair = [&](int g, int h) {  // scores 2h, 2h + 1 of chunk g
+    const int kb = g >> 1, kc = g & 1;
+    const float e0 = q3::fast_exp2(__builtin_fmaf(s[kb][8 * kc + 2 * h], c, -m_use));
+    const float e1 = q3::fast_exp2(__builtin_fmaf(s[kb][8 * kc + 2 * h + 1], c, -m_use));
+    if (g == 0 && h < 2) {
+      psum[2 * h] = e0;
+      psum[2 * h + 1] = e1;
+    } else {
+      psum[(2 * h) & 3] += e0;
+      psum[(2 * h + 1) & 3] += e1;
+    }
+    pk[g][h] = q3::pack_bf16x2(e0, e1);
+  };
+#pragma unroll
+  for (int h = 0; h < 4; ++h) exp_pair(0, h);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int u = 0; u < 16; ++u) {
+    acc[u & 3] = q3::mfma32x32x16(vf[u % kAhead], q3::as_bf16x8(pk[u >> 2]), acc[u & 3]);
+    if (u + kAhead < 16) vf[u % kAhead] = lds_vt(vt, pv_operand(off, u + kAhead));
+    if (u < 12) exp_pair((u >> 2) + 1, u & 3);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  l_run += (psum[0] + psum[1]) + (psum[2] + psum[3]);
+}
+
+// Key tiles [t0, t1) of an item folded into a fresh state.  Every thread of the
+// workgroup calls it; the tile buffers are free when it returns.
+__device__ __forceinline__ void run_tiles(const ChunkArgs& a, const LaneOffsets& off, const Seq& s,
+                                          const WaveRows& w, int kvh, int t0, int t1,
+                                          const TileBufs& tb, int lane, int wave, float& m_run,
+                                          float& l_run, q3::f32x16 (&acc)[4]) {
+  m_run = q3::kNegInf;
+  l_run = 0.f;
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[db][r] = 0.f;
+  if (t0 >= t1) return;
+  PageWindow pw;
+  window_start(pw, a, s.row, t0, lane);
+  uint32_t ok = tile_dma(a, off, pw, s, kvh, t0, tb.k0, tb.v0, wave, lane);
+  q3::bf16x8 qv[8];
+  load_q(a, s, w, kvh, lane, qv);
+  wait_loads();
+  __syncthreads();
+  auto tile = [&](int it, const uint16_t* kt, const uint16_t* vt, uint16_t* nk, uint16_t* nv) {
+    const uint32_t here = ok;
+    if (it + 1 < t1) ok = tile_dma(a, off, pw, s, kvh, it + 1, nk, nv, wave, lane);
+    const int n0 = it * kBN;
+    if (w.active && n0 <= w.hi) {
+      auto mask = [&](q3::f32x16 (&x)[2]) {
+        if (n0 + kBN - 1 > w.lo || here != 15u) {
+          // score (kb, r): key n0 + 4 (lane / 32) + kr of group 2 kb + r / 8
+          const int lim = w.last - n0 - 4 * (lane >> 5);
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int kr = kb * 32 + 8 * (r / 4) + (r % 4);
+              const int l = (here >> (2 * kb + r / 8)) & 1u ? lim : -1;
+              x[kb][r] = kr <= l ? x[kb][r] : q3::kNegInf;
+            }
+        }
+      };
+      tile_fold(off, a.scale_log2, mask, kt, vt, qv, m_run, l_run, acc);
+    }
+    wait_loads();
+    __syncthreads();
+  };
+  for (int it = t0; it < t1; it += 2) {
+    tile(it, tb.k0, tb.v0, tb.k1, tb.v1);
+    if (it + 1 < t1) tile(it + 1, tb.k1, tb.v1, tb.k0, tb.v0);
+  }
+}
+
+// Normalises this wave's rows (l: a row's full sum) and writes those of the
+// sequence, through 8 KiB of LDS at `stage` so that 16 lanes write a head row.
+__device__ __forceinline__ void store_output(const ChunkArgs& a, const Seq& s, const WaveRows& w,
+                                             int kvh, int lane, float l,
+                                             const q3::f32x16 (&acc)[4], char* stage) {
+  const int l32 = lane & 31, hl = lane >> 5;
+  const float inv = l > 0.f ? 1.f / l : 0.f;  // 0: no key
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4) {
+      const int ch = 4 * db + g4;
+      q3::u32x2 x = {q3::pack_bf16x2(acc[db][4 * g4] * inv, acc[db][4 * g4 + 1] * inv),
+                     q3::pack_bf16x2(acc[db][4 * g4 + 2] * inv, acc[db][4 * g4 + 3] * inv)};
+      *reinterpret_cast<q3::u32x2*>(stage + l32 * 256 + ((ch ^ (l32 & 15)) << 4) + hl * 8) = x;
+    }
+  const int oc = lane & 15;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int rr = 4 * j + (lane >> 4);
+    const q3::u32x4 x =
+        *reinterpret_cast<const q3::u32x4*>(stage + rr * 256 + ((oc ^ (rr & 15)) << 4));
+    const int r = w.r0 + rr, tok = r / a.G;
+    if (tok < s.n)
+      q3::st16(a.o + (s.q0 + tok) * a.o_st +
+                   (static_cast<int64_t>(kvh) * a.G + (r - tok * a.G)) * a.o_sh + 8 * oc,
+               x);
+  }
+}
+
+__device__ __forceinline__ char* stage_of(const TileBufs& tb, int wave) {
+  const int sb = wave >> 1;
+  return reinterpret_cast<char*>(sb == 0 ? tb.k0 : tb.v0) + (wave & 1) * 8192;
+}
+
+// One workgroup per item, KV head fastest (neighbouring workgroups go to
+// different XCDs, and an XCD's L2 holds few heads), longest reach first.
+__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void paged_chunk_flat_kernel(ChunkArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint16_t s_k0[kTileElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t s_v0[kTileElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t s_k1[kTileElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t s_v1[kTileElems];
+  const TileBufs tb{s_k0, s_v0, s_k1, s_v1};
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int id = blockIdx.x;
+  const int kvh = id % a.Hkv;
+  const int b = id / a.Hkv % a.B;
+  const int mt = a.n_mtiles - 1 - id / a.Hkv / a.B;
+  const Seq s = seq_at(a, b);
+  if (mt * kRows >= static_cast<int64_t>(s.n) * a.G) return;
+  const LaneOffsets off = lane_offsets(a, lane);
+  const WaveRows w = wave_rows(a, s, mt, wave, lane);
+  const int tiles = (keys_of(a, s, (mt + 1) * kRows) + kBN - 1) / kBN;
+  float m_run, l_run;
+  q3::f32x16 acc[4];
+  run_tiles(a, off, s, w, kvh, 0, tiles, tb, lane, wave, m_run, l_run, acc);
+  l_run = cross_half_sum(l_run);
+  if (w.active) store_output(a, s, w, kvh, lane, l_run, acc, stage_of(tb, wave));
+}
+
+}  // namespace
+
+extern "C" size_t qwen3_paged_chunk_workspace_bytes(int B, int max_chunk, int64_t total_tokens,
+                                                    int num_heads, int num_kv_heads,
+                                                    int head_dim) {
+  if (B <= 0 || total_tokens <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
+      num_heads / num_kv_heads > kMaxG || head_dim != kD || max_chunk <= 0)
+    return 0;
+  return 256;
+}
+
+extern "C" int qwen3_paged_chunk_bf16(
+    const void* q, const int64_t q_strides[2], const void* k_cache, const int64_t k_strides[3],
+    const void* v_cache, const int64_t v_strides[3], int64_t num_blocks,
+    const int32_t* block_table, int64_t bt_row_stride, int64_t max_rows, int64_t max_pages,
+    const int32_t* seq_lens, const int32_t* row_ids, const int32_t* cu_seqlens, void* out,
+    const int64_t out_strides[2], int B, int max_chunk, int64_t total_tokens, int num_heads,
+    int num_kv_heads, int head_dim, int block_size, float scale, void* workspace,
+    size_t workspace_bytes, void* stream) {
+  const char* who = "qwen3_paged_chunk_bf16";
+  if (!q || !k_cache || !v_cache || !block_table || !seq_lens || !cu_seqlens || !out ||
+      !q_strides || !k_strides || !v_strides || !out_strides)
+    return q3::fail(QWEN3_EINVAL, "%s: null pointer argument", who);
+  if (head_dim != kD)
+    return q3::fail(QWEN3_EUNSUPPORTED, "%s: head_dim %d not supported (built for %d)", who,
+                    head_dim, kD);
+  if (block_size <= 0 || block_size % kGroup != 0)
+    return q3::fail(QWEN3_EUNSUPPORTED, "%s: block_size %d must be a multiple of %d", who,
+                    block_size, kGroup);
+  if (num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads != 0 ||
+      num_heads / num_kv_heads > kMaxG)
+    return q3::fail(QWEN3_EUNSUPPORTED, "%s: num_heads %d / num_kv_heads %d unsupported", who,
+                    num_heads, num_kv_heads);
+  if (B < 0 || max_chunk < 0 || total_tokens < 0 || total_tokens > 0x7fffffff ||
+      num_blocks <= 0 || max_rows <= 0 || max_pages <= 0 || bt_row_stride < max_pages)
+    return q3::fail(QWEN3_EINVAL, "%s: bad sizes (B=%d max_chunk=%d total_tokens=%lld "
+                    "num_blocks=%lld max_rows=%lld max_pages=%lld bt_row_stride=%lld)", who, B,
+                    max_chunk, (long long)total_tokens, (long long)num_blocks,
+                    (long long)max_rows, (long long)max_pages, (long long)bt_row_stride);
+  if (!(scale > 0.f) || !(scale < __builtin_inff()))
+    return q3::fail(QWEN3_EINVAL, "%s: scale must be positive and finite", who);
+  if (max_pages * block_size > (int64_t(1) << 30))
+    return q3::fail(QWEN3_EINVAL, "%s: max_pages * block_size too large", who);
+  const int64_t vec_strides[] = {q_strides[0], q_strides[1], k_strides[0], k_strides[1],
+                                 k_strides[2], v_strides[0], v_strides[1], v_strides[2],
+                                 out_strides[0], out_strides[1]};
+  bool ok = q3::aligned16(q) && q3::aligned16(k_cache) && q3::aligned16(v_cache) &&
+            q3::aligned16(out);
+  for (int64_t st : vec_strides) ok = ok && st % 8 == 0;
+  if (!ok)
+    return q3::fail(QWEN3_EALIGN, "%s: q/K/V/out need 16-byte aligned rows (strides multiple "
+                    "of 8 elements)", who);
+  // Rows behind a descriptor's end must lie outside it, and 16 of them inside 32-bit offsets.
+  for (int64_t st : {k_strides[2], v_strides[2]})
+    if (st < kD || st > (int64_t(1) << 24))
+      return q3::fail(QWEN3_EUNSUPPORTED, "%s: slot stride %lld outside %d..2^24", who,
+                      (long long)st, kD);
+  const int64_t total_rows = total_tokens * (num_heads / num_kv_heads);
+  if (total_rows > 0x7fffffff - kRows)
+    return q3::fail(QWEN3_EINVAL, "%s: too many tokens", who);
+  if (B == 0 || max_chunk == 0 || total_tokens == 0) return QWEN3_OK;
+  const size_t need = qwen3_paged_chunk_workspace_bytes(B, max_chunk, total_tokens, num_heads,
+                                                        num_kv_heads, head_dim);
+  if (!workspace || workspace_bytes < need)
+    return q3::fail(QWEN3_EWORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need,
+                    workspace ? workspace_bytes : (size_t)0);
+  if (!q3::aligned16(workspace))
+    return q3::fail(QWEN3_EALIGN, "%s: workspace must be 16-byte aligned", who);
+  ChunkArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_st = q_strides[0];
+  a.q_sh = q_strides[1];
+  a.k = static_cast<const uint16_t*>(k_cache);
+  a.k_blk = k_strides[0];
+  a.k_sh = k_strides[1];
+  a.k_slot = k_strides[2];
+  a.v = static_cast<const uint16_t*>(v_cache);
+  a.v_blk = v_strides[0];
+  a.v_sh = v_strides[1];
+  a.v_slot = v_strides[2];
+  a.num_blocks = num_blocks;
+  a.bt = block_table;
+  a.bt_stride = bt_row_stride;
+  a.max_rows = max_rows;
+  a.max_pages = max_pages;
+  a.seq_lens = seq_lens;
+  a.row_ids = row_ids;
+  a.cu = cu_seqlens;
+  a.o = static_cast<uint16_t*>(out);
+  a.o_st = out_strides[0];
+  a.o_sh = out_strides[1];
+  a.total = total_tokens;
+  a.B = B;
+  a.Hkv = num_kv_heads;
+  a.G = num_heads / num_kv_heads;
+  a.bs = block_size;
+  a.scale_log2 = scale * q3::kLog2e;
+  const int64_t longest = max_chunk < total_tokens ? max_chunk : total_tokens;
+  a.n_mtiles = static_cast<int>(q3::cdiv(longest * a.G, kRows));
+  const int64_t items = static_cast<int64_t>(a.Hkv) * B * a.n_mtiles;
+  if (items > 0x7fffffff)
+    return q3::fail(QWEN3_EINVAL, "%s: grid too large (KV heads %d, batch %d, max_chunk %d)", who,
+                    num_kv_heads, B, max_chunk);
+  q3::clear_error();
+  hipLaunchKernelGGL(paged_chunk_flat_kernel, dim3(static_cast<unsigned>(items)),
+                     dim3(kWaves * 64), 0, static_cast<hipStream_t>(stream), a);
+  return q3::launch_status(who);
+}

@@ -17,10 +17,12 @@ from .. import _lib
 
 __all__ = [
     "paged_attention_decode_hip",
+    "paged_attention_chunk_hip",
     "hip_paged_attention_decode",
     "hip_paged_attention_decode_batch",
     "update_kv_batch_hip",
     "paged_decode_workspace_bytes",
+    "paged_chunk_workspace_bytes",
     # reference names
     "paged_attention_decode_triton",
     "triton_paged_attention_decode",
@@ -175,6 +177,91 @@ def paged_attention_decode_partials_hip(q, k_buffer, v_buffer, block_table_2d, s
         B, num_heads, num_kv_heads, head_dim, block_size, 1.0 / math.sqrt(head_dim),
         workspace.data_ptr(), workspace.numel(), _lib.stream_of(dev))
     _lib.check(rc, "qwen3_paged_decode_partials_bf16")
+    return out
+
+
+def paged_chunk_workspace_bytes(batch: int, max_chunk: int, total_tokens: int, num_heads: int,
+                                num_kv_heads: int, head_dim: int) -> int:
+    """Workspace size of paged_attention_chunk_hip on the current device; depends
+    only on the launch shape, so a captured call stays valid for any lengths."""
+    return int(_lib.load().qwen3_paged_chunk_workspace_bytes(
+        batch, max_chunk, total_tokens, num_heads, num_kv_heads, head_dim))
+
+
+def paged_attention_chunk_hip(q, k_buffer, v_buffer, block_table_2d, seq_lens_full, row_ids,
+                              cu_seqlens, block_size, *, max_chunk: int | None = None,
+                              scale: float | None = None, out: torch.Tensor | None = None,
+                              workspace: torch.Tensor | None = None):
+    """Attention of each sequence's new tokens over its pages, causal inside the
+    chunk: a prompt prefilled in pieces, a new turn behind a cached prefix, draft
+    tokens to verify, or these beside decoding sequences (one token each) in one
+    batch.  The tokens' keys and values must be in the pool already.
+
+    q:              (total_tokens, num_heads, head_dim) bf16, the sequences' new
+                    tokens packed
+    k_buffer/v_buffer, block_table_2d, row_ids: as paged_attention_decode_hip
+    seq_lens_full:  (max_requests,) int32, lengths BEFORE this step: token i of a
+                    sequence is at position seq_lens_full[row] + i and attends all
+                    positions up to its own
+    cu_seqlens:     int32 (num_seqs + 1,) cumulative chunk lengths
+    max_chunk:      host bound of the chunk lengths (None: read from cu_seqlens,
+                    which synchronises and cannot be captured)
+    Returns out (total_tokens, num_heads, head_dim) bf16.  Rows behind
+    cu_seqlens[-1] are left as they are; a token without keys is zero.  scale:
+    1/sqrt(head_dim) unless given.  workspace: paged_chunk_workspace_bytes(...)
+    bytes, a fresh one per call by default.
+    """
+    assert q.dim() == 3
+    T, num_heads, head_dim = q.shape
+    num_blocks, num_kv_heads, block_size_check, head_dim_check = k_buffer.shape
+    assert block_size_check == block_size and head_dim_check == head_dim
+    assert v_buffer.shape == k_buffer.shape
+    assert q.dtype == torch.bfloat16 and k_buffer.dtype == torch.bfloat16 \
+        and v_buffer.dtype == torch.bfloat16, "HIP chunk kernel is bf16 only"
+    assert block_table_2d.dtype == torch.int32 and seq_lens_full.dtype == torch.int32
+    assert block_table_2d.dim() == 2 and block_table_2d.stride(1) == 1, \
+        "block_table_2d rows must be contiguous"
+    assert seq_lens_full.dim() == 1 and seq_lens_full.shape[0] >= block_table_2d.shape[0]
+    assert cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1
+    assert k_buffer.stride(3) == 1 and v_buffer.stride(3) == 1
+    B = cu_seqlens.numel() - 1
+    if row_ids is not None:
+        assert row_ids.dtype == torch.int32 and row_ids.numel() == B
+        row_ids = row_ids.contiguous()
+    else:
+        assert B <= block_table_2d.shape[0], "more sequences than rows of the block table"
+    dev = _lib.require_hip(q, k_buffer, v_buffer, block_table_2d, seq_lens_full, row_ids,
+                           cu_seqlens, out, workspace)
+    cu_seqlens = cu_seqlens.contiguous()
+    seq_lens_full = seq_lens_full.contiguous()
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    if max_chunk is None:
+        lens = cu_seqlens.cpu().diff()
+        max_chunk = int(lens.max()) if B else 0
+    if scale is None:
+        scale = 1.0 / math.sqrt(head_dim)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        assert out.shape == q.shape and out.dtype == torch.bfloat16 and out.stride(2) == 1, \
+            "out must be a bf16 (total_tokens, num_heads, head_dim) tensor with unit last stride"
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        need = paged_chunk_workspace_bytes(B, max_chunk, T, num_heads, num_kv_heads, head_dim)
+        if workspace is None or workspace.numel() * workspace.element_size() < need:
+            workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        rc = lib.qwen3_paged_chunk_bf16(
+            q.data_ptr(), _lib.strides(q, (0, 1)),
+            k_buffer.data_ptr(), _lib.strides(k_buffer, (0, 1, 2)),
+            v_buffer.data_ptr(), _lib.strides(v_buffer, (0, 1, 2)), num_blocks,
+            block_table_2d.data_ptr(), block_table_2d.stride(0), *block_table_2d.shape,
+            seq_lens_full.data_ptr(), _lib.ptr(row_ids), cu_seqlens.data_ptr(),
+            out.data_ptr(), _lib.strides(out, (0, 1)),
+            B, int(max_chunk), T, num_heads, num_kv_heads, head_dim, block_size, float(scale),
+            workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+            _lib.stream_of(dev))
+    _lib.check(rc, "qwen3_paged_chunk_bf16")
     return out
 
 
