@@ -458,6 +458,65 @@ int qwen3_qk_norm_rope_slots_bf16(const void* q, const int64_t q_strides[2],
                                   int block_size, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Rotary positions (the reference's RotaryEmbedding and apply_rotary_pos_emb,
+ * qwen3/rope.py:42-110, without their tables: any position, any frequencies, half
+ * or interleaved pairs, a whole head or the first rotary_dim elements of it).  For
+ * pair i of element a and b, angle t = positions[token] * inv_freq[i]:
+ *   out_a = factor (x_a cos t - x_b sin t), out_b = factor (x_b cos t + x_a sin t)
+ * layout 0: (a, b) = (i, i + rotary_dim / 2); 1: (2 i, 2 i + 1).  Elements from
+ * rotary_dim on are copied.  inverse: the angle's sign is turned (the transpose of
+ * the map: its gradient).  Angles in 64 bits, products in fp32, one rounding.
+ *   q (tokens, num_heads, head_dim), k (tokens, num_kv_heads, head_dim) through
+ *               strides [token, head]; k and k_out may be NULL together.  q_out and
+ *               k_out may be q and k themselves; they must not overlap otherwise.
+ *   inv_freq    device, rotary_dim / 2 doubles;  positions: int64 of magnitude
+ *               below 2^31
+ *   dtype       0: bf16, 1: fp16, 2: fp32
+ * Supported: head_dim a multiple of 8, rotary_dim of 16, up to 512; 16-byte aligned
+ * rows.
+ * ---------------------------------------------------------------------- */
+int qwen3_rotary(const void* q, const int64_t q_strides[2], const void* k,
+                 const int64_t k_strides[2], void* q_out, const int64_t q_out_strides[2],
+                 void* k_out, const int64_t k_out_strides[2], int dtype,
+                 const double* inv_freq, float factor, int layout, int inverse,
+                 const int64_t* positions, int64_t num_tokens, int num_heads,
+                 int num_kv_heads, int head_dim, int rotary_dim, void* stream);
+
+/* The same (bf16) with the pool write of qwen3_qk_norm_rope_slots_bf16: rotated k and v
+ * unchanged go to slot_mapping[token] (negative or outside the pool: not written).
+ * k_out may be NULL. */
+int qwen3_rotary_slots_bf16(const void* q, const int64_t q_strides[2], const void* k,
+                            const int64_t k_strides[2], const void* v,
+                            const int64_t v_strides[2], void* q_out,
+                            const int64_t q_out_strides[2], void* k_out,
+                            const int64_t k_out_strides[2], const double* inv_freq,
+                            float factor, int layout, const int64_t* positions,
+                            const int64_t* slot_mapping, void* k_cache,
+                            const int64_t k_cache_strides[4], void* v_cache,
+                            const int64_t v_cache_strides[4], int64_t num_blocks,
+                            int layer_idx, int num_layers, int64_t num_tokens,
+                            int num_heads, int num_kv_heads, int head_dim, int rotary_dim,
+                            int block_size, void* stream);
+
+/* The decode form: one token a sequence, written at seq_lens[row] through the block
+ * table as in qwen3_kv_write_decode_bf16 and rotated at positions[b] (NULL: at
+ * seq_lens[row]; a row outside the table at 0).  Nothing is written where the table
+ * names no block of the pool. */
+int qwen3_rotary_decode_bf16(const void* q, const int64_t q_strides[2], const void* k,
+                             const int64_t k_strides[2], const void* v,
+                             const int64_t v_strides[2], void* q_out,
+                             const int64_t q_out_strides[2], const double* inv_freq,
+                             float factor, int layout, void* k_cache,
+                             const int64_t k_cache_strides[4], void* v_cache,
+                             const int64_t v_cache_strides[4], int64_t num_blocks,
+                             int layer_idx, int num_layers, const int32_t* seq_lens,
+                             const int32_t* block_table, int64_t bt_row_stride,
+                             int64_t max_rows, int64_t max_pages, const int32_t* row_ids,
+                             const int64_t* positions, int B, int num_heads,
+                             int num_kv_heads, int head_dim, int rotary_dim,
+                             int block_size, void* stream);
+
+/* ------------------------------------------------------------------------
  * Streaming read reference (no counterpart in the reference engine; for the
  * measurement of the HBM-bound entry points above): reads `bytes` bytes
  * (a multiple of 16) at `src` with 16-byte loads, non-temporal when

@@ -234,6 +234,40 @@ int qwen3_page_in_bf16(int32_t* block_table, int64_t bt_row_stride, int64_t max_
                        void* k_cache, void* v_cache, int64_t block_elems,
                        int64_t num_blocks, void* stream);
 
+/* Pages of the pool copied, forked and moved (no counterpart in the reference
+ * engine, whose requests never share a page).  k_cache, v_cache: the pool's
+ * contiguous blocks of block_elems bf16 values, slots of slot_elems (head_dim)
+ * inside [.., block_size, slot_elems] arrays.  The lists are HOST arrays of n
+ * entries, read before the call returns; the plan travels in the launch (several
+ * launches above 240 entries).  Refused before anything is launched: an id outside
+ * the pool or the table, a destination named twice, one that is also a source (the
+ * copies of a call run at the same time). */
+
+/* Block dst[i] becomes a copy of block src[i], K and V, all layers: of its first
+ * tokens[i] slots, the others zero (NULL: of all slots). */
+int qwen3_page_copy_bf16(void* k_cache, void* v_cache, int64_t block_elems, int slot_elems,
+                         int block_size, int64_t num_blocks, const int32_t* src,
+                         const int32_t* dst, const int32_t* tokens, int n, void* stream);
+
+/* Row dst_rows[i] of the block table takes over the pages of the first tokens[i]
+ * tokens of row src_rows[i]; where they end inside a page, block new_blocks[i]
+ * becomes a copy of its first slots (the others zero) and takes its place.  The
+ * row's other entries become -1, seq_lens[dst_rows[i]] = tokens[i].  new_blocks[i]
+ * is not read where the tokens fill whole pages.  A last page whose entry is no
+ * block of the pool is not copied. */
+int qwen3_page_fork_bf16(void* k_cache, void* v_cache, int64_t block_elems, int slot_elems,
+                         int block_size, int64_t num_blocks, int32_t* block_table,
+                         int64_t bt_row_stride, int64_t max_rows, int64_t max_pages,
+                         int32_t* seq_lens, const int32_t* src_rows, const int32_t* dst_rows,
+                         const int32_t* tokens, const int32_t* new_blocks, int n, void* stream);
+
+/* Block src[i] moves to dst[i]: its K and V are copied and every entry of the table
+ * that names it names dst[i] afterwards.  No source may be named twice. */
+int qwen3_page_move_bf16(void* k_cache, void* v_cache, int64_t block_elems, int slot_elems,
+                         int block_size, int64_t num_blocks, int32_t* block_table,
+                         int64_t bt_row_stride, int64_t max_rows, int64_t max_pages,
+                         const int32_t* src, const int32_t* dst, int n, void* stream);
+
 /* Samples one token per row of bf16 logits (out[r], int64), per-row
  * parameters as device arrays (NULL: temperature 0, top_k 0, top_p 1):
  *   temperature[r] <= 0  the first index of the largest logit (NaN highest);

@@ -10,6 +10,13 @@ and the batched prefill write, which the reference runs as a per-request
 loop of PagedKVCache.update (qwen3/attention.py:160-161), is one
 slot-mapped launch (write_prefill_batch / qwen3_kv_write_slots_bf16).
 
+Beyond the reference, requests can share pages (fork, fork_caches), give tokens back
+(truncate) and have the pool's live pages moved together (KVCachePool.compact), on
+the kernels of kernels/paged_cache.py.  One rule keeps every write path as it is:
+the page that a request's next token falls into is never shared -- fork copies a
+partly filled last page, truncate copies one that it leaves partly filled -- so only
+whole, finished pages have several holders.  The pool counts them on the host.
+
 Pool layout (num_blocks, num_layers, num_kv_heads, block_size, head_dim):
 one (block, layer, head) chunk is block_size * head_dim contiguous bf16
 (4 KiB at 16 x 128), the unit the decode kernel streams.
@@ -21,8 +28,9 @@ import torch
 
 from . import _lib
 from .kernels.paged_attention import update_kv_batch_hip
+from .kernels.paged_cache import copy_pages_hip, fork_pages_hip, move_pages_hip
 
-__all__ = ["KVCachePool", "PagedKVCache", "prefill_slot_mapping", "write_prefill_batch",
+__all__ = ["KVCachePool", "PagedKVCache", "fork_caches", "prefill_slot_mapping", "write_prefill_batch",
            "reserve_pages_bulk", "set_seq_lens_bulk", "PageIn"]
 
 
@@ -54,6 +62,7 @@ class KVCachePool:
 
         self.free_block_ids = list(range(num_blocks))
         self.total_blocks = num_blocks
+        self._extra_holders = {}  # shared block -> its holders beyond the first
 
     def alloc(self, n: int):
         """Pops n block ids (LIFO from the tail) and zeroes their K/V, so a
@@ -80,7 +89,55 @@ class KVCachePool:
         return allocated
 
     def free(self, block_ids: list):
-        self.free_block_ids.extend(block_ids)
+        """Returns blocks; one that other requests still hold stays theirs."""
+        if not self._extra_holders:
+            self.free_block_ids.extend(block_ids)
+            return
+        for b in block_ids:
+            left = self._extra_holders.get(b, 0)
+            if left == 0:
+                self.free_block_ids.append(b)
+            elif left == 1:
+                del self._extra_holders[b]
+            else:
+                self._extra_holders[b] = left - 1
+
+    def share(self, block_ids: list):
+        """One more holder for each of the blocks."""
+        for b in block_ids:
+            self._extra_holders[b] = self._extra_holders.get(b, 0) + 1
+
+    def is_shared(self, block_id: int) -> bool:
+        return block_id in self._extra_holders
+
+    def compact(self, caches) -> int:
+        """Moves the pages of the given handles into the lowest blocks (one launch per
+        240 moves, the block table with them), so that what is free lies together at
+        the pool's end; returns how many moved.  Blocks in use that these handles do
+        not account for -- another handle's, a captured graph's own page -- stay where
+        they are.  Tables change in place, so captured graphs stay valid; nothing may
+        write into the pool on another stream meanwhile.  Blocks taken next come from
+        the low end."""
+        handles = list({id(c): c for c in caches}.values())
+        holders: dict = {}
+        for c in handles:
+            if c._pool is not self:
+                raise ValueError("a handle of another pool")
+            for b in c.block_table:
+                holders[b] = holders.get(b, 0) + 1
+        used = self.total_blocks - len(self.free_block_ids)
+        src = sorted(b for b, n in holders.items()
+                     if b >= used and n == 1 + self._extra_holders.get(b, 0))
+        dst = sorted(b for b in self.free_block_ids if b < used)[:len(src)]
+        if src:
+            move_pages_hip(self.k_buffer, self.v_buffer, self.block_table_2d, src, dst)
+            to = dict(zip(src, dst))
+            for c in handles:
+                c.block_table = [to.get(b, b) for b in c.block_table]
+            self._extra_holders = {to.get(b, b): n for b, n in self._extra_holders.items()}
+            self.free_block_ids = list(set(self.free_block_ids).difference(dst).union(src))
+        self.free_block_ids.sort(reverse=True)
+        return len(src)
 
     @property
     def free_count(self):
@@ -199,6 +256,40 @@ class PagedKVCache:
         self.seq_len += n
         self._pool.seq_lens[self.row_id] = self.seq_len
 
+    def fork(self, tokens: int | None = None) -> "PagedKVCache":
+        """A new handle that starts with this one's first `tokens` tokens (None: all):
+        parallel samples of one prompt, requests behind a common prefix.  Whole pages
+        are shared, a partly filled last one is copied; one launch."""
+        return fork_caches([self], None if tokens is None else [tokens])[0]
+
+    def truncate(self, tokens: int):
+        """Gives back everything behind the first `tokens` tokens (draft tokens that
+        were not accepted): pages that hold nothing of the rest are freed, and one
+        that is left partly filled and has other holders is replaced by a copy."""
+        if not 0 <= tokens <= self.seq_len:
+            raise ValueError(f"cannot keep {tokens} of {self.seq_len} tokens")
+        pool = self._pool
+        bs = pool.block_size
+        keep, rest = -(-tokens // bs), tokens % bs
+        if rest and pool.is_shared(self.block_table[keep - 1]):
+            old = self.block_table[keep - 1]
+            new = pool.take_blocks(1)[0]
+            try:
+                copy_pages_hip(pool.k_buffer, pool.v_buffer, [old], [new], [rest])
+            except Exception:
+                pool.free([new])
+                raise
+            self.block_table[keep - 1] = new
+            self.block_table_tensor[keep - 1] = new
+            pool.free([old])
+        if keep < self.num_pages:
+            pool.free(self.block_table[keep:])
+            del self.block_table[keep:]
+            self.block_table_tensor[keep:self.num_pages] = -1
+            self.num_pages = keep
+        self.seq_len = tokens
+        pool.seq_lens[self.row_id] = tokens
+
     def free(self):
         if self.block_table:
             self._pool.free(self.block_table)
@@ -206,6 +297,55 @@ class PagedKVCache:
             self.num_pages = 0
         self.seq_len = 0
         self._pool.free_row(self.row_id)
+
+
+def fork_caches(parents: list, tokens: list | None = None) -> list:
+    """A new handle for every entry of `parents` (the same one may come several
+    times), starting with its first tokens[i] tokens (None: all of them), in one
+    launch: the block-table rows, the copies of the partly filled last pages and the
+    lengths.  Takes a row a fork, and a block where the tokens end inside a page; a
+    pool that has too few raises before anything changes."""
+    if not parents:
+        return []
+    pool = parents[0]._pool
+    bs = pool.block_size
+    if tokens is None:
+        tokens = [p.seq_len for p in parents]
+    if len(tokens) != len(parents):
+        raise ValueError(f"{len(tokens)} lengths for {len(parents)} forks")
+    for p, n in zip(parents, tokens):
+        if p._pool is not pool:
+            raise ValueError("forks of several pools in one call")
+        if not 0 <= n <= p.seq_len:
+            raise ValueError(f"cannot fork {n} of {p.seq_len} tokens")
+    if len(pool._free_rows) < len(parents):
+        raise RuntimeError(f"OOM: {len(parents)} request rows needed, {len(pool._free_rows)} free")
+    ends_inside = [n % bs != 0 for n in tokens]
+    need = sum(ends_inside)
+    if pool.free_count < need:
+        raise RuntimeError(
+            f"OOM: requested {need} blocks, {pool.free_count} / {pool.total_blocks} free")
+    rows = pool._free_rows[-len(parents):][::-1]
+    fresh = iter(pool.free_block_ids[len(pool.free_block_ids) - need:])
+    blocks = [next(fresh) if e else -1 for e in ends_inside]
+    fork_pages_hip(pool.k_buffer, pool.v_buffer, pool.block_table_2d, pool.seq_lens,
+                   [p.row_id for p in parents], rows, tokens, blocks)
+    if need:
+        pool.take_blocks(need)
+    children = []
+    for p, n, row, block in zip(parents, tokens, rows, blocks):
+        c = PagedKVCache.__new__(PagedKVCache)
+        c._pool = pool
+        c.seq_len = n
+        c.row_id = row  # its length is written by the launch
+        pool._free_rows.pop()
+        c.block_table_tensor = pool.block_table_2d[row]
+        shared = p.block_table[:n // bs]
+        pool.share(shared)
+        c.block_table = shared if block < 0 else shared + [block]
+        c.num_pages = len(c.block_table)
+        children.append(c)
+    return children
 
 
 class PageIn:

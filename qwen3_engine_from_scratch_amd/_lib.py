@@ -18,6 +18,8 @@ _c_i32p = ctypes.c_void_p  # device pointers travel as void*
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
+_i32p = ctypes.POINTER(ctypes.c_int32)  # host arrays
+
 
 class DecodeChainArgs(ctypes.Structure):
     """qwen3_decode_chain_args of include/qwen3_model_ops.h."""
@@ -140,6 +142,23 @@ _SIGNATURES = {
          _vp, _c_i64p, _vp, _c_i64p, _vp, _c_i64p, _vp, _c_i64p, _i64, _i, _i,
          _i64, _i, _i, _i, _i, _vp],
     ),
+    "qwen3_rotary": (
+        _i,
+        [_vp, _c_i64p, _vp, _c_i64p, _vp, _c_i64p, _vp, _c_i64p, _i, _vp, ctypes.c_float, _i, _i,
+         _vp, _i64, _i, _i, _i, _i, _vp],
+    ),
+    "qwen3_rotary_slots_bf16": (
+        _i,
+        [_vp, _c_i64p, _vp, _c_i64p, _vp, _c_i64p, _vp, _c_i64p, _vp, _c_i64p,
+         _vp, ctypes.c_float, _i, _vp, _vp, _vp, _c_i64p, _vp, _c_i64p, _i64, _i, _i,
+         _i64, _i, _i, _i, _i, _i, _vp],
+    ),
+    "qwen3_rotary_decode_bf16": (
+        _i,
+        [_vp, _c_i64p, _vp, _c_i64p, _vp, _c_i64p, _vp, _c_i64p,
+         _vp, ctypes.c_float, _i, _vp, _c_i64p, _vp, _c_i64p, _i64, _i, _i,
+         _vp, _vp, _i64, _i64, _i64, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
+    ),
     # include/qwen3_model_ops.h
     "qwen3_add_rms_norm_bf16": (
         _i,
@@ -150,6 +169,11 @@ _SIGNATURES = {
     "qwen3_argmax_bf16": (_i, [_vp, _i64, _i64, _i64, _vp, _vp]),
     "qwen3_advance_seq_lens": (_i, [_vp, _i64, _vp, _i, _i, _i, _vp]),
     "qwen3_page_in_bf16": (_i, [_vp, _i64, _i64, _i64, _vp, _i, _vp, _vp, _i64, _i64, _vp]),
+    "qwen3_page_copy_bf16": (_i, [_vp, _vp, _i64, _i, _i, _i64, _i32p, _i32p, _i32p, _i, _vp]),
+    "qwen3_page_fork_bf16": (_i, [_vp, _vp, _i64, _i, _i, _i64, _vp, _i64, _i64, _i64, _vp,
+                                  _i32p, _i32p, _i32p, _i32p, _i, _vp]),
+    "qwen3_page_move_bf16": (_i, [_vp, _vp, _i64, _i, _i, _i64, _vp, _i64, _i64, _i64,
+                                  _i32p, _i32p, _i, _vp]),
     "qwen3_sample_bf16": (_i, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, ctypes.c_uint64, _vp, _vp]),
     "qwen3_sample_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
     "qwen3_sample_ws_bf16": (_i, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, ctypes.c_uint64, _vp, _vp,

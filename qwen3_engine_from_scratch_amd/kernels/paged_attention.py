@@ -246,6 +246,8 @@ def paged_attention_chunk_hip(q, k_buffer, v_buffer, block_table_2d, seq_lens_fu
     else:
         assert out.shape == q.shape and out.dtype == torch.bfloat16 and out.stride(2) == 1, \
             "out must be a bf16 (total_tokens, num_heads, head_dim) tensor with unit last stride"
+    if T == 0 or B == 0:
+        return out
     lib = _lib.load()
     with torch.cuda.device(dev):
         need = paged_chunk_workspace_bytes(B, max_chunk, T, num_heads, num_kv_heads, head_dim)

@@ -283,3 +283,14 @@ def test_calls_on_two_streams(gpu):
         check(outs[i][0], t, f"stream {i}")
         for o in outs[i][1:]:
             assert torch.equal(o, outs[i][0]), "the same call gave other bits"
+
+
+def test_nothing_to_do(gpu):
+    announce("chunk: no tokens, no sequences")
+    t = make_case([0, 0], [5, 0], 16, 8, 16, gpu)
+    assert run(t, gpu).shape == (0, 16, 128)
+    t = make_case([3], [5], 16, 8, 16, gpu)
+    t.update(cu=torch.zeros(1, dtype=torch.int32), row_ids=t["row_ids"][:0])
+    out = torch.full_like(t["q"], 2.0)
+    assert (run(t, gpu, out=out) == 2.0).all()
+    assert (run(t, gpu, out=out, max_chunk=None) == 2.0).all()
