@@ -29,6 +29,13 @@ constexpr int kMaxG = 16;
 constexpr float kRescaleSlack = 8.f;  // log2 headroom before the running maximum is raised
 constexpr int kGroup = 16;           // keys a wave loads of a tile: inside one page
 
+// A cut item, noted by the range that holds its first tile: its parts lie in slot
+// 2 v + 1 of that range v and in slots 2 (v + 1), 2 (v + 2), ... of the next ones.
+struct CutItem {
+  int32_t parts;  // 0: this range holds no cut item's first tile
+  int32_t b, kvh, mt;
+};
+
 struct ChunkArgs {
   const uint16_t* q;
   int64_t q_st, q_sh;
@@ -48,6 +55,10 @@ struct ChunkArgs {
   int B, Hkv, G, bs;
   int n_mtiles;    // items of the longest chunk of one KV head
   float scale_log2;
+  // range schedule
+  float* po;       // [2 ranges][kRows][kD] partial outputs, not normalised
+  float2* pml;     // [2 ranges][kRows] their running maximum (log2 domain) and sum
+  CutItem* cuts;   // [ranges]
 };
 
 // One sequence of the batch.
@@ -384,15 +395,18 @@ __device__ __forceinline__ char* stage_of(const TileBufs& tb, int wave) {
   return reinterpret_cast<char*>(sb == 0 ? tb.k0 : tb.v0) + (wave & 1) * 8192;
 }
 
+#define Q3_CHUNK_TILE_BUFFERS                                          \
+  __shared__ __attribute__((aligned(1024))) uint16_t s_k0[kTileElems]; \
+  __shared__ __attribute__((aligned(1024))) uint16_t s_v0[kTileElems]; \
+  __shared__ __attribute__((aligned(1024))) uint16_t s_k1[kTileElems]; \
+  __shared__ __attribute__((aligned(1024))) uint16_t s_v1[kTileElems]; \
+  const TileBufs tb{s_k0, s_v0, s_k1, s_v1}
+
 // One workgroup per item, KV head fastest (neighbouring workgroups go to
 // different XCDs, and an XCD's L2 holds few heads), longest reach first.
 __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_chunk_flat_kernel(ChunkArgs a) {
-  __shared__ __attribute__((aligned(1024))) uint16_t s_k0[kTileElems];
-  __shared__ __attribute__((aligned(1024))) uint16_t s_v0[kTileElems];
-  __shared__ __attribute__((aligned(1024))) uint16_t s_k1[kTileElems];
-  __shared__ __attribute__((aligned(1024))) uint16_t s_v1[kTileElems];
-  const TileBufs tb{s_k0, s_v0, s_k1, s_v1};
+  Q3_CHUNK_TILE_BUFFERS;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int id = blockIdx.x;
@@ -411,6 +425,259 @@ void paged_chunk_flat_kernel(ChunkArgs a) {
   if (w.active) store_output(a, s, w, kvh, lane, l_run, acc, stage_of(tb, wave));
 }
 
+// ---------------------------------------------------------------------------
+// Range schedule: too few items for the device (a few long contexts).  The items'
+// key tiles, each of weight kUnits, with kItemUnits for an item's start and end, lie
+// end to end, KV head by KV head; they are cut into equal ranges, one per resident
+// workgroup.  Neighbouring ranges run on one XCD, so its L2 serves one KV head.  A
+// tile belongs to the range that holds its midpoint.  An item cut by a border leaves
+// a partial state per part, which a second launch joins, a wave per row: with up to
+// 64 parts to a row, joining inside one workgroup would take as long as the tiles.
+constexpr int kUnits = 16;
+constexpr int kItemUnits = 40;
+constexpr int kMinRangeTiles = 4;
+constexpr int kMaxEntries = 1024;   // (sequence, row tile) pairs tabulated in LDS
+
+// Exclusive prefix sum of v[0 .. n) in LDS, in place, n <= kMaxEntries; returns the
+// total.  Every thread of the workgroup calls it.
+template <typename T>
+__device__ __forceinline__ T block_scan(T* v, int n, T* s_wsum) {
+  constexpr int kPer = kMaxEntries / (kWaves * 64);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  T x[kPer], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    x[i] = tid * kPer + i < n ? v[tid * kPer + i] : 0;
+    sum += x[i];
+  }
+  T incl = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const T y = __shfl_up(incl, o, 64);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 63) s_wsum[wave] = incl;
+  __syncthreads();
+  T run = incl - sum, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    run += w < wave ? s_wsum[w] : 0;
+    total += s_wsum[w];
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (tid * kPer + i < n) v[tid * kPer + i] = run;
+    run += x[i];
+  }
+  __syncthreads();
+  return total;
+}
+
+// Largest index i < n with v[i] <= p (v ascending, v[0] <= p).
+template <typename T>
+__device__ __forceinline__ int last_at_most(const T* v, int n, T p) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (v[mid] <= p) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x >> 32));
+  return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+}
+
+__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void paged_chunk_range_kernel(ChunkArgs a) {
+  Q3_CHUNK_TILE_BUFFERS;
+  __shared__ int64_t s_pos[kMaxEntries];  // weight before each (sequence, row tile)
+  __shared__ int s_first[kMaxEntries];    // row tiles before each sequence
+  __shared__ int64_t s_wsum[kWaves];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  for (int b = tid; b < a.B; b += kWaves * 64) {
+    const int64_t s0 = a.cu[b], s1 = a.cu[b + 1];
+    const bool ok = s0 >= 0 && s1 > s0 && s1 <= a.total;
+    s_first[b] = ok ? static_cast<int>(((s1 - s0) * a.G + kRows - 1) / kRows) : 0;
+  }
+  __syncthreads();
+  // (the bound matters only where cu_seqlens is not ascending)
+  const int E = min(kMaxEntries, block_scan<int>(s_first, a.B, reinterpret_cast<int*>(s_wsum)));
+  for (int e = tid; e < E; e += kWaves * 64) {
+    const int b = last_at_most(s_first, a.B, e);
+    const Seq s = seq_at(a, b);
+    const int tiles = (keys_of(a, s, (e - s_first[b] + 1) * kRows) + kBN - 1) / kBN;
+    s_pos[e] = static_cast<int64_t>(kUnits) * tiles + kItemUnits;
+  }
+  __syncthreads();
+  const int64_t H = block_scan<int64_t>(s_pos, E, s_wsum);
+  const int nwg = gridDim.x;
+  const int64_t U = H * a.Hkv;
+  int64_t N = U / (kMinRangeTiles * kUnits);
+  N = N < 1 ? 1 : N < nwg ? N : nwg;
+  const int w = blockIdx.x;
+  const int v = N == nwg && nwg % 8 == 0 ? (w % 8) * (nwg / 8) + w / 8 : w;
+  const int64_t p_lo = v < N ? (v * U + N - 1) / N : U;
+  const int64_t p_hi = v < N ? ((v + 1) * U + N - 1) / N : U;
+  CutItem cut{0, 0, 0, 0};
+  if (p_lo < p_hi) {
+    const LaneOffsets off = lane_offsets(a, lane);
+    int kvh = static_cast<int>(p_lo / H);
+    int e = __builtin_amdgcn_readfirstlane(last_at_most(s_pos, E, p_lo - kvh * H));
+    while (true) {
+      const int64_t P = kvh * H + uniform64(s_pos[e]);  // the item's position
+      if (P >= p_hi) break;
+      const int b = __builtin_amdgcn_readfirstlane(last_at_most(s_first, a.B, e));
+      const int mt = e - __builtin_amdgcn_readfirstlane(s_first[b]);
+      const Seq s = seq_at(a, b);
+      const int tiles = (keys_of(a, s, (mt + 1) * kRows) + kBN - 1) / kBN;
+      // tile j's midpoint: P + kItemUnits + kUnits j + kUnits / 2; an item without
+      // tiles belongs to the range that holds its position
+      const int64_t base = P + kItemUnits + kUnits / 2;
+      auto first_at = [&](int64_t p) {
+        const int64_t j = p <= base ? 0 : (p - base + kUnits - 1) / kUnits;
+        return static_cast<int>(j < tiles ? j : tiles);
+      };
+      const int j0 = first_at(p_lo), j1 = first_at(p_hi);
+      if (j0 < j1 || (tiles == 0 && P >= p_lo)) {
+        const WaveRows wr = wave_rows(a, s, mt, wave, lane);
+        float m_run, l_run;
+        q3::f32x16 acc[4];
+        run_tiles(a, off, s, wr, kvh, j0, j1, tb, lane, wave, m_run, l_run, acc);
+        l_run = cross_half_sum(l_run);
+        if (j0 == 0 && j1 == tiles) {
+          if (wr.active) store_output(a, s, wr, kvh, lane, l_run, acc, stage_of(tb, wave));
+        } else {
+          const int slot = j0 == 0 ? 2 * v + 1 : 2 * v;
+          if (wr.active) {
+            const int64_t row = static_cast<int64_t>(slot) * kRows + wave * 32 + (lane & 31);
+            float* po = a.po + row * kD + 4 * (lane >> 5);
+#pragma unroll
+            for (int db = 0; db < 4; ++db)
+#pragma unroll
+              for (int r4 = 0; r4 < 4; ++r4)
+                *reinterpret_cast<q3::f32x4*>(po + 32 * db + 8 * r4) =
+                    q3::f32x4{acc[db][4 * r4], acc[db][4 * r4 + 1], acc[db][4 * r4 + 2],
+                              acc[db][4 * r4 + 3]};
+            if (lane < 32) a.pml[row] = float2{m_run, l_run};
+          }
+          if (j0 == 0) {
+            const int64_t last = base + static_cast<int64_t>(kUnits) * (tiles - 1);
+            cut = CutItem{static_cast<int32_t>(last * N / U) - v + 1, b, kvh, mt};
+          }
+        }
+        __syncthreads();  // the staging buffers are read before the next loads refill them
+      }
+      if (++e == E) {
+        e = 0;
+        if (++kvh == a.Hkv) break;
+      }
+    }
+  }
+  if (tid == 0) a.cuts[v] = cut;
+}
+
+// Joins the parts of the cut items: a workgroup takes kMergeRows rows of the item
+// noted by range blockIdx.x, a wave a row at a time, a lane two of its elements.
+constexpr int kMergeRows = 16;
+
+__global__ __launch_bounds__(kWaves * 64) void paged_chunk_join_kernel(ChunkArgs a) {
+  const int v = blockIdx.x;
+  const CutItem c = a.cuts[v];
+  if (c.parts == 0) return;
+  const Seq s = seq_at(a, c.b);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (int i = wave; i < kMergeRows; i += kWaves) {
+    const int row = blockIdx.y * kMergeRows + i;
+    const int r = c.mt * kRows + row;
+    if (r >= s.n * a.G) return;
+    auto slot_row = [&](int p) {
+      return static_cast<int64_t>(p == 0 ? 2 * v + 1 : 2 * (v + p)) * kRows + row;
+    };
+    float M = q3::kNegInf;
+    for (int p = lane; p < c.parts; p += 64) M = fmaxf(M, a.pml[slot_row(p)].x);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, q3::shfl_xor(M, o));
+    const float m = M == q3::kNegInf ? 0.f : M;
+    float l = 0.f, o0 = 0.f, o1 = 0.f;
+    for (int p0 = 0; p0 < c.parts; p0 += 64) {
+      float2 ml{q3::kNegInf, 0.f};
+      if (p0 + lane < c.parts) ml = a.pml[slot_row(p0 + lane)];
+      const float f = q3::fast_exp2(ml.x - m);
+      l += ml.y * f;
+      const int n = min(64, c.parts - p0);
+      for (int j = 0; j < n; j += 8) {
+        float2 x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          x[u] = *reinterpret_cast<const float2*>(a.po + slot_row(p0 + min(j + u, n - 1)) * kD +
+                                                  2 * lane);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float fu = j + u < n ? __uint_as_float(__builtin_amdgcn_readlane(
+                                           __float_as_uint(f), j + u)) : 0.f;
+          o0 += fu * x[u].x;
+          o1 += fu * x[u].y;
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) l += q3::shfl_xor(l, o);
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const int tok = r / a.G;
+    *reinterpret_cast<uint32_t*>(a.o + (s.q0 + tok) * a.o_st +
+                                 (static_cast<int64_t>(c.kvh) * a.G + (r - tok * a.G)) * a.o_sh +
+                                 2 * lane) = q3::pack_bf16x2(o0 * inv, o1 * inv);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+
+int cu_count() {
+  static int cached[64] = {0};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 0;
+  if (cached[dev] == 0) {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
+      return 0;
+    cached[dev] = n;
+  }
+  return cached[dev];
+}
+
+// Resident workgroups of the range schedule (two per CU), 512 where no device can be
+// asked.
+int range_workgroups() {
+  const int cus = cu_count();
+  return 2 * (cus > 0 ? cus : 256);
+}
+
+struct ChunkLayout {
+  int64_t po, pml, cuts, total;
+};
+ChunkLayout chunk_layout(int ranges) {
+  ChunkLayout l;
+  l.po = 0;
+  l.pml = l.po + int64_t(2) * ranges * kRows * kD * sizeof(float);
+  l.cuts = l.pml + int64_t(2) * ranges * kRows * sizeof(float2);
+  l.total = l.cuts + (ranges * sizeof(CutItem) + 255) / 256 * 256;
+  return l;
+}
+
+// Items that a launch has at most, and whether the range schedule takes it.
+int64_t entries_at_most(int B, int64_t total, int G) { return q3::cdiv(total * G, kRows) + B; }
+bool takes_ranges(int B, int64_t total, int G, int Hkv) {
+  const int64_t e = entries_at_most(B, total, G);
+  return e <= kMaxEntries && e * Hkv <= 4 * static_cast<int64_t>(range_workgroups());
+}
+
 }  // namespace
 
 extern "C" size_t qwen3_paged_chunk_workspace_bytes(int B, int max_chunk, int64_t total_tokens,
@@ -419,7 +686,9 @@ extern "C" size_t qwen3_paged_chunk_workspace_bytes(int B, int max_chunk, int64_
   if (B <= 0 || total_tokens <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
       num_heads / num_kv_heads > kMaxG || head_dim != kD || max_chunk <= 0)
     return 0;
-  return 256;
+  return takes_ranges(B, total_tokens, num_heads / num_kv_heads, num_kv_heads)
+             ? chunk_layout(range_workgroups()).total
+             : 256;
 }
 
 extern "C" int qwen3_paged_chunk_bf16(
@@ -508,14 +777,28 @@ extern "C" int qwen3_paged_chunk_bf16(
   a.G = num_heads / num_kv_heads;
   a.bs = block_size;
   a.scale_log2 = scale * q3::kLog2e;
+  q3::clear_error();
+  const auto s = static_cast<hipStream_t>(stream);
+  if (takes_ranges(B, total_tokens, a.G, a.Hkv)) {
+    const int wgs = range_workgroups();
+    const ChunkLayout l = chunk_layout(wgs);
+    char* ws = static_cast<char*>(workspace);
+    a.po = reinterpret_cast<float*>(ws + l.po);
+    a.pml = reinterpret_cast<float2*>(ws + l.pml);
+    a.cuts = reinterpret_cast<CutItem*>(ws + l.cuts);
+    hipLaunchKernelGGL(paged_chunk_range_kernel, dim3(wgs), dim3(kWaves * 64), 0, s, a);
+    if (const int rc = q3::launch_status(who)) return rc;
+    hipLaunchKernelGGL(paged_chunk_join_kernel, dim3(wgs, kRows / kMergeRows), dim3(kWaves * 64), 0,
+                       s, a);
+    return q3::launch_status(who);
+  }
   const int64_t longest = max_chunk < total_tokens ? max_chunk : total_tokens;
   a.n_mtiles = static_cast<int>(q3::cdiv(longest * a.G, kRows));
   const int64_t items = static_cast<int64_t>(a.Hkv) * B * a.n_mtiles;
   if (items > 0x7fffffff)
     return q3::fail(QWEN3_EINVAL, "%s: grid too large (KV heads %d, batch %d, max_chunk %d)", who,
                     num_kv_heads, B, max_chunk);
-  q3::clear_error();
   hipLaunchKernelGGL(paged_chunk_flat_kernel, dim3(static_cast<unsigned>(items)),
-                     dim3(kWaves * 64), 0, static_cast<hipStream_t>(stream), a);
+                     dim3(kWaves * 64), 0, s, a);
   return q3::launch_status(who);
 }
