@@ -11,38 +11,45 @@
 //
 //  * Query rows of one KV head are packed: row r is token r / G, head r % G of
 //    the group, so one staged K/V tile serves every head of the group whatever
-//    G is.  A work item is (sequence, KV head, 128 packed rows); each of the
-//    four waves of a workgroup owns 32 of them.
+//    G is.  A work item is (sequence, KV head, 128 or 256 packed rows); each of the
+//    four or eight waves of a workgroup owns 32 of them.
 //  * K/V tiles of 64 keys go from HBM into LDS by buffer loads that write LDS,
-//    16 keys a wave, so a wave reads one page per tile: its base is a scalar and
+//    16 or 8 keys a wave, so a wave reads one page per tile: its base is a scalar and
 //    the lanes' offsets never change.  The descriptor ends at the sequence's
 //    last key (or holds nothing where the table names no page of the pool), so
 //    slots behind it are never read.  Page ids come 64 at a time into a
 //    register (16 tiles' worth), the next 64 before they are needed.
+#include <cstdlib>
 #include "prefill_tile.hpp"
 
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kRows = 32 * kWaves;   // packed query rows of an item
+// Workgroups of W = 4 or 8 waves: packed query rows of an item.
+template <int W>
+constexpr int rows_of() { return 32 * W; }
 constexpr int kMaxG = 16;
 constexpr float kRescaleSlack = 8.f;  // log2 headroom before the running maximum is raised
 constexpr int kGroup = 16;           // keys a wave loads of a tile: inside one page
 
-// A cut item, noted by the range that holds its first tile: its parts lie in slot
-// 2 v + 1 of that range v and in slots 2 (v + 1), 2 (v + 2), ... of the next ones.
+// A cut item, noted by the range v that holds its first tile: its parts lie in slot
+// 2 v + 1 and in slots 2 (v + 1), 2 (v + 2), ... of the next ranges.
 struct CutItem {
   int32_t parts;  // 0: this range holds no cut item's first tile
-  int32_t b, kvh, mt;
+  int32_t rows;   // packed rows of the item
+  int32_t r0;     // the first one
+  int32_t kvh;
+  int64_t q0;     // first row of q of its sequence
 };
 
 struct ChunkArgs {
   const uint16_t* q;
   int64_t q_st, q_sh;
   const uint16_t* k;
-  int64_t k_blk, k_sh, k_slot;
+  int64_t k_blk, k_sh;
+  int k_slot;
   const uint16_t* v;
-  int64_t v_blk, v_sh, v_slot;
+  int64_t v_blk, v_sh;
+  int v_slot;
   int64_t num_blocks;
   const int32_t* bt;
   int64_t bt_stride, max_rows, max_pages;
@@ -52,7 +59,9 @@ struct ChunkArgs {
   uint16_t* o;
   int64_t o_st, o_sh;
   int64_t total;   // rows of q
-  int B, Hkv, G, bs;
+  int B, Hkv, G;
+  int gpb;         // groups of kGroup keys of a block
+  int reach;       // positions that a row of the table addresses
   int n_mtiles;    // items of the longest chunk of one KV head
   float scale_log2;
   // range schedule
@@ -70,19 +79,30 @@ struct Seq {
   int cap;      // keys that may be attended: at most what its tokens reach and a row holds
 };
 
-__device__ __forceinline__ Seq seq_at(const ChunkArgs& a, int b) {
-  Seq s;
-  const int64_t s0 = a.cu[b], s1 = a.cu[b + 1];
-  const bool ok = s0 >= 0 && s1 > s0 && s1 <= a.total;
-  s.q0 = ok ? s0 : 0;
-  s.n = ok ? static_cast<int>(s1 - s0) : 0;
-  const int64_t row = a.row_ids ? a.row_ids[b] : b;
-  s.row = row >= 0 && row < a.max_rows ? row : -1;
-  s.ctx = s.row >= 0 ? a.seq_lens[s.row] : 0;
-  const int64_t len = static_cast<int64_t>(s.ctx) + s.n, most = a.max_pages * a.bs;
-  const int64_t cap = len < most ? len : most;
-  s.cap = s.row >= 0 && cap > 0 ? static_cast<int>(cap) : 0;
+// The same, as a table keeps it.
+struct SeqEntry {
+  int32_t q0, n, row, ctx;
+};
+
+__device__ __forceinline__ Seq seq_of(const ChunkArgs& a, const SeqEntry& e) {
+  Seq s{e.q0, e.n, e.row, e.ctx, 0};
+  const int64_t len = static_cast<int64_t>(e.ctx) + e.n;
+  const int cap = static_cast<int>(len < a.reach ? len : a.reach);
+  s.cap = e.row >= 0 && cap > 0 ? cap : 0;
   return s;
+}
+
+__device__ __forceinline__ Seq seq_at(const ChunkArgs& a, int b) {
+  const int64_t s0 = a.cu[b], s1 = a.cu[b + 1];
+  const int64_t row = a.row_ids ? a.row_ids[b] : b;
+  const bool ok = s0 >= 0 && s1 > s0 && s1 <= a.total;
+  const bool listed = row >= 0 && row < a.max_rows;
+  SeqEntry e;
+  e.q0 = ok ? static_cast<int32_t>(s0) : 0;
+  e.n = ok ? static_cast<int32_t>(s1 - s0) : 0;
+  e.row = listed ? static_cast<int32_t>(row) : -1;
+  e.ctx = listed ? a.seq_lens[row] : 0;
+  return seq_of(a, e);
 }
 
 // Keys that packed rows r0 .. r1 - 1 of a sequence reach.
@@ -99,20 +119,25 @@ struct TileBufs {
   uint16_t* v1;
 };
 
-constexpr int kDma = kGroup * kRowBytes / (64 * 16);  // 16-byte loads a lane of a K or V tile
+// 16-byte loads a lane issues of a K or V tile.
+template <int W>
+constexpr int dma_per_wave() { return kBN * kRowBytes / (W * 64 * 16); }
+constexpr int kMaxDma = dma_per_wave<4>();
 
 struct LaneOffsets {
-  uint32_t kdma[kDma], vdma[kDma];  // source offsets within the wave's 16 keys
+  uint32_t kdma[kMaxDma], vdma[kMaxDma];  // source offsets within a group of 16 keys
   uint32_t kread, vread;
 };
 
-__device__ __forceinline__ LaneOffsets lane_offsets(const ChunkArgs& a, int lane) {
+template <int W>
+__device__ __forceinline__ LaneOffsets lane_offsets(const ChunkArgs& a, int lane, int wave) {
   LaneOffsets o;
-  // Load j of a wave fills rows 4 j .. 4 j + 3 of its 16; lane i writes slot
-  // i % 16 of row 4 j + i / 16, i.e. source chunk slot ^ swz(row).
+  // Load j of wave w fills LDS rows 4 n .. 4 n + 3, n = D w + j (D loads a wave);
+  // lane i writes slot i % 16 of row 4 n + i / 16, i.e. source chunk slot ^ swz(row).
+  constexpr int D = dma_per_wave<W>();
 #pragma unroll
-  for (int j = 0; j < kDma; ++j) {
-    const int row = 4 * j + (lane >> 4);
+  for (int j = 0; j < D; ++j) {
+    const int row = (4 * (D * wave + j) + (lane >> 4)) % kGroup;
     const int slot = lane & 15;
     o.kdma[j] = static_cast<uint32_t>(row * a.k_slot * 2) + ((slot ^ (row & 15)) << 4);
     o.vdma[j] = static_cast<uint32_t>(row * a.v_slot * 2) + ((slot ^ (4 * (row & 3))) << 4);
@@ -121,26 +146,29 @@ __device__ __forceinline__ LaneOffsets lane_offsets(const ChunkArgs& a, int lane
   return o;
 }
 
-// The pages of the item's next 64 groups of 16 keys (16 tiles), a lane each,
-// and of the 64 after them.
+// Where the item's next 64 groups of 16 keys (16 tiles) lie, a lane each, and the 64
+// after them: the page, and the group's place inside it.
 struct PageWindow {
-  int base;           // group of lane 0
-  int32_t cur, next;
-  uint64_t ok;        // groups of the window whose page is a block of the pool
+  int base;                // group of lane 0
+  int32_t page, next_page;
+  uint32_t sub, next_sub;
+  uint64_t ok;             // groups of the window whose page is a block of the pool
 };
 
-__device__ __forceinline__ int32_t page_of_group(const ChunkArgs& a, int64_t row, int group) {
-  const int64_t page = static_cast<int64_t>(group) * kGroup / a.bs;
-  return row >= 0 && page < a.max_pages ? a.bt[row * a.bt_stride + page] : -1;
+__device__ __forceinline__ void group_at(const ChunkArgs& a, int64_t row, int group, int32_t& page,
+                                         uint32_t& sub) {
+  const uint32_t p = static_cast<uint32_t>(group) / static_cast<uint32_t>(a.gpb);
+  sub = static_cast<uint32_t>(group) - p * a.gpb;
+  page = row >= 0 && p < a.max_pages ? a.bt[row * a.bt_stride + p] : -1;
 }
 __device__ __forceinline__ void window_check(PageWindow& w, const ChunkArgs& a) {
-  w.ok = __ballot(w.cur >= 0 && w.cur < a.num_blocks);
+  w.ok = __ballot(w.page >= 0 && w.page < a.num_blocks);
 }
 __device__ __forceinline__ void window_start(PageWindow& w, const ChunkArgs& a, int64_t row,
                                              int tile, int lane) {
   w.base = tile * (kBN / kGroup);
-  w.cur = page_of_group(a, row, w.base + lane);
-  w.next = page_of_group(a, row, w.base + 64 + lane);
+  group_at(a, row, w.base + lane, w.page, w.sub);
+  group_at(a, row, w.base + 64 + lane, w.next_page, w.next_sub);
   window_check(w, a);
 }
 // Moves on once `tile` lies behind the window (tiles come in order).
@@ -148,38 +176,50 @@ __device__ __forceinline__ void window_to(PageWindow& w, const ChunkArgs& a, int
                                           int lane) {
   if (tile * (kBN / kGroup) < w.base + 64) return;
   w.base += 64;
-  w.cur = w.next;
-  w.next = page_of_group(a, row, w.base + 64 + lane);
+  w.page = w.next_page;
+  w.sub = w.next_sub;
+  group_at(a, row, w.base + 64 + lane, w.next_page, w.next_sub);
   window_check(w, a);
 }
 
-// Issues this wave's share (16 keys) of the loads of key tile `tile` into (sk, sv).
-// Returns which of the tile's four groups lie in the pool's blocks.
+// An item's keys.
+struct ItemKeys {
+  const uint16_t* k;  // the KV head of block 0
+  const uint16_t* v;
+  int64_t row;        // of the block table
+  int cap;            // keys of the sequence
+};
+
+// Issues this wave's share of the loads of key tile `tile` into (sk, sv).  Returns
+// which of the tile's four groups lie in the pool's blocks.
+template <int W>
 __device__ __forceinline__ uint32_t tile_dma(const ChunkArgs& a, const LaneOffsets& off,
-                                             PageWindow& w, const Seq& s, int kvh, int tile,
+                                             PageWindow& w, const ItemKeys& ks, int tile,
                                              uint16_t* sk, uint16_t* sv, int wave, int lane) {
-  window_to(w, a, s.row, tile, lane);
+  window_to(w, a, ks.row, tile, lane);
   const int g0 = tile * (kBN / kGroup) - w.base;
-  const int64_t phys = __builtin_amdgcn_readlane(w.cur, g0 + wave);
+  const int g = wave * (kBN / kGroup) / W;  // this wave's group
+  const int64_t page = __builtin_amdgcn_readlane(w.page, g0 + g);
+  const int sub = __builtin_amdgcn_readlane(w.sub, g0 + g) * kGroup;
   const uint32_t ok = static_cast<uint32_t>(w.ok >> g0) & 15u;
-  const int key = tile * kBN + wave * kGroup;
-  const int rows = (ok >> wave) & 1u ? min(kGroup, s.cap - key) : 0;
-  const int64_t sub = key % a.bs;
-  const uint16_t* kb = a.k + kvh * a.k_sh;
-  const uint16_t* vb = a.v + kvh * a.v_sh;
+  const int rows = (ok >> g) & 1u ? min(kGroup, ks.cap - tile * kBN - g * kGroup) : 0;
+  const uint16_t* kb = ks.k;
+  const uint16_t* vb = ks.v;
   if (rows > 0) {
-    kb += phys * a.k_blk + sub * a.k_slot;
-    vb += phys * a.v_blk + sub * a.v_slot;
+    kb += page * a.k_blk + static_cast<int64_t>(sub) * a.k_slot;
+    vb += page * a.v_blk + static_cast<int64_t>(sub) * a.v_slot;
   }
-  const int k_bytes = rows > 0 ? static_cast<int>((rows - 1) * a.k_slot * 2) + kRowBytes : 0;
-  const int v_bytes = rows > 0 ? static_cast<int>((rows - 1) * a.v_slot * 2) + kRowBytes : 0;
+  // rows behind the last key lie outside the descriptor and read as zero
+  const int k_bytes = rows > 0 ? (rows - 1) * a.k_slot * 2 + kRowBytes : 0;
+  const int v_bytes = rows > 0 ? (rows - 1) * a.v_slot * 2 + kRowBytes : 0;
   const __amdgpu_buffer_rsrc_t kr =
       __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(kb), 0, k_bytes, 0x00020000);
   const __amdgpu_buffer_rsrc_t vr =
       __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(vb), 0, v_bytes, 0x00020000);
+  constexpr int D = dma_per_wave<W>();
 #pragma unroll
-  for (int j = 0; j < kDma; ++j) {
-    const int blk = (kDma * wave + j) * 512;  // elements: 1 KiB per load
+  for (int j = 0; j < D; ++j) {
+    const int blk = (D * wave + j) * 512;  // elements: 1 KiB per load
     __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void_t*)(sk + blk), 16, off.kdma[j], 0, 0, 0);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void_t*)(sv + blk), 16, off.vdma[j], 0, 0, 0);
   }
@@ -195,20 +235,21 @@ struct WaveRows {
   bool active;    // the wave has rows of the sequence
 };
 
+template <int W>
 __device__ __forceinline__ WaveRows wave_rows(const ChunkArgs& a, const Seq& s, int mt, int wave,
                                               int lane) {
   WaveRows w;
-  w.r0 = mt * kRows + wave * 32;
+  w.r0 = mt * rows_of<W>() + wave * 32;
   const int r = w.r0 + (lane & 31);
-  w.tok = r / a.G;
+  w.tok = static_cast<uint32_t>(r) / static_cast<uint32_t>(a.G);
   w.head = r - w.tok * a.G;
   auto last = [&](int tok) {
     const int64_t p = static_cast<int64_t>(s.ctx) + min(tok, s.n - 1);
     return static_cast<int>(p < s.cap - 1 ? (p < -1 ? -1 : p) : s.cap - 1);
   };
   w.last = last(w.tok);
-  w.lo = last(w.r0 / a.G);
-  w.hi = last((w.r0 + 31) / a.G);
+  w.lo = last(static_cast<uint32_t>(w.r0) / static_cast<uint32_t>(a.G));
+  w.hi = last(static_cast<uint32_t>(w.r0 + 31) / static_cast<uint32_t>(a.G));
   w.active = w.r0 < s.n * a.G;
   return w;
 }
@@ -312,6 +353,7 @@ __device__ __forceinline__ void tile_fold(const Off& off, float c, const Mask& m
 
 // Key tiles [t0, t1) of an item folded into a fresh state.  Every thread of the
 // workgroup calls it; the tile buffers are free when it returns.
+template <int W>
 __device__ __forceinline__ void run_tiles(const ChunkArgs& a, const LaneOffsets& off, const Seq& s,
                                           const WaveRows& w, int kvh, int t0, int t1,
                                           const TileBufs& tb, int lane, int wave, float& m_run,
@@ -325,14 +367,15 @@ __device__ __forceinline__ void run_tiles(const ChunkArgs& a, const LaneOffsets&
   if (t0 >= t1) return;
   PageWindow pw;
   window_start(pw, a, s.row, t0, lane);
-  uint32_t ok = tile_dma(a, off, pw, s, kvh, t0, tb.k0, tb.v0, wave, lane);
+  const ItemKeys ks{a.k + kvh * a.k_sh, a.v + kvh * a.v_sh, s.row, s.cap};
+  uint32_t ok = tile_dma<W>(a, off, pw, ks, t0, tb.k0, tb.v0, wave, lane);
   q3::bf16x8 qv[8];
   load_q(a, s, w, kvh, lane, qv);
   wait_loads();
   __syncthreads();
   auto tile = [&](int it, const uint16_t* kt, const uint16_t* vt, uint16_t* nk, uint16_t* nv) {
     const uint32_t here = ok;
-    if (it + 1 < t1) ok = tile_dma(a, off, pw, s, kvh, it + 1, nk, nv, wave, lane);
+    if (it + 1 < t1) ok = tile_dma<W>(a, off, pw, ks, it + 1, nk, nv, wave, lane);
     const int n0 = it * kBN;
     if (w.active && n0 <= w.hi) {
       auto mask = [&](q3::f32x16 (&x)[2]) {
@@ -382,7 +425,8 @@ __device__ __forceinline__ void store_output(const ChunkArgs& a, const Seq& s, c
     const int rr = 4 * j + (lane >> 4);
     const q3::u32x4 x =
         *reinterpret_cast<const q3::u32x4*>(stage + rr * 256 + ((oc ^ (rr & 15)) << 4));
-    const int r = w.r0 + rr, tok = r / a.G;
+    const int r = w.r0 + rr;
+    const int tok = static_cast<uint32_t>(r) / static_cast<uint32_t>(a.G);
     if (tok < s.n)
       q3::st16(a.o + (s.q0 + tok) * a.o_st +
                    (static_cast<int64_t>(kvh) * a.G + (r - tok * a.G)) * a.o_sh + 8 * oc,
@@ -392,7 +436,8 @@ __device__ __forceinline__ void store_output(const ChunkArgs& a, const Seq& s, c
 
 __device__ __forceinline__ char* stage_of(const TileBufs& tb, int wave) {
   const int sb = wave >> 1;
-  return reinterpret_cast<char*>(sb == 0 ? tb.k0 : tb.v0) + (wave & 1) * 8192;
+  return reinterpret_cast<char*>(sb == 0 ? tb.k0 : sb == 1 ? tb.v0 : sb == 2 ? tb.k1 : tb.v1) +
+         (wave & 1) * 8192;
 }
 
 #define Q3_CHUNK_TILE_BUFFERS                                          \
@@ -404,23 +449,25 @@ __device__ __forceinline__ char* stage_of(const TileBufs& tb, int wave) {
 
 // One workgroup per item, KV head fastest (neighbouring workgroups go to
 // different XCDs, and an XCD's L2 holds few heads), longest reach first.
-__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+template <int W>
+__global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_chunk_flat_kernel(ChunkArgs a) {
   Q3_CHUNK_TILE_BUFFERS;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int id = blockIdx.x;
-  const int kvh = id % a.Hkv;
-  const int b = id / a.Hkv % a.B;
-  const int mt = a.n_mtiles - 1 - id / a.Hkv / a.B;
+  const uint32_t id = blockIdx.x, per_tile = static_cast<uint32_t>(a.Hkv) * a.B;
+  const int mt = a.n_mtiles - 1 - static_cast<int>(id / per_tile);
+  const uint32_t rest = id % per_tile;
+  const int b = static_cast<int>(rest / a.Hkv);
+  const int kvh = static_cast<int>(rest % a.Hkv);
   const Seq s = seq_at(a, b);
-  if (mt * kRows >= static_cast<int64_t>(s.n) * a.G) return;
-  const LaneOffsets off = lane_offsets(a, lane);
-  const WaveRows w = wave_rows(a, s, mt, wave, lane);
-  const int tiles = (keys_of(a, s, (mt + 1) * kRows) + kBN - 1) / kBN;
+  if (mt * rows_of<W>() >= static_cast<int64_t>(s.n) * a.G) return;
+  const LaneOffsets off = lane_offsets<W>(a, lane, wave);
+  const WaveRows w = wave_rows<W>(a, s, mt, wave, lane);
+  const int tiles = (keys_of(a, s, (mt + 1) * rows_of<W>()) + kBN - 1) / kBN;
   float m_run, l_run;
   q3::f32x16 acc[4];
-  run_tiles(a, off, s, w, kvh, 0, tiles, tb, lane, wave, m_run, l_run, acc);
+  run_tiles<W>(a, off, s, w, kvh, 0, tiles, tb, lane, wave, m_run, l_run, acc);
   l_run = cross_half_sum(l_run);
   if (w.active) store_output(a, s, w, kvh, lane, l_run, acc, stage_of(tb, wave));
 }
@@ -436,13 +483,14 @@ void paged_chunk_flat_kernel(ChunkArgs a) {
 constexpr int kUnits = 16;
 constexpr int kItemUnits = 40;
 constexpr int kMinRangeTiles = 4;
-constexpr int kMaxEntries = 1024;   // (sequence, row tile) pairs tabulated in LDS
+constexpr int kMaxSeqs = 256;       // sequences and (sequence, row tile) pairs
+constexpr int kMaxEntries = 1024;   // tabulated in LDS
 
 // Exclusive prefix sum of v[0 .. n) in LDS, in place, n <= kMaxEntries; returns the
 // total.  Every thread of the workgroup calls it.
-template <typename T>
+template <int W, typename T>
 __device__ __forceinline__ T block_scan(T* v, int n, T* s_wsum) {
-  constexpr int kPer = kMaxEntries / (kWaves * 64);
+  constexpr int kPer = kMaxEntries / (W * 64);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   T x[kPer], sum = 0;
 #pragma unroll
@@ -460,7 +508,7 @@ __device__ __forceinline__ T block_scan(T* v, int n, T* s_wsum) {
   __syncthreads();
   T run = incl - sum, total = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < W; ++w) {
     run += w < wave ? s_wsum[w] : 0;
     total += s_wsum[w];
   }
@@ -490,51 +538,67 @@ __device__ __forceinline__ int64_t uniform64(int64_t x) {
   return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
 }
 
-__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+// floor(x / y) of integers below 2^52: a quotient that is no integer lies at least
+// 1 / y below the next one, more than the rounding of x / y < 2^52 / y.
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+  return static_cast<int64_t>(__builtin_floor(static_cast<double>(x) / static_cast<double>(y)));
+}
+
+template <int W>
+__global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_chunk_range_kernel(ChunkArgs a) {
   Q3_CHUNK_TILE_BUFFERS;
   __shared__ int64_t s_pos[kMaxEntries];  // weight before each (sequence, row tile)
-  __shared__ int s_first[kMaxEntries];    // row tiles before each sequence
-  __shared__ int64_t s_wsum[kWaves];
+  __shared__ int s_first[kMaxSeqs];       // row tiles before each sequence
+  __shared__ SeqEntry s_seq[kMaxSeqs];
+  __shared__ int64_t s_wsum[W];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  for (int b = tid; b < a.B; b += kWaves * 64) {
-    const int64_t s0 = a.cu[b], s1 = a.cu[b + 1];
-    const bool ok = s0 >= 0 && s1 > s0 && s1 <= a.total;
-    s_first[b] = ok ? static_cast<int>(((s1 - s0) * a.G + kRows - 1) / kRows) : 0;
+  // Every workgroup waits for this before its first K/V load: one chain of two
+  // memory round trips (row_ids, then seq_lens), the rest is in LDS.
+  for (int b = tid; b < a.B; b += W * 64) {
+    const Seq s = seq_at(a, b);
+    s_seq[b] = SeqEntry{static_cast<int32_t>(s.q0), s.n, static_cast<int32_t>(s.row), s.ctx};
+    s_first[b] = static_cast<int>((static_cast<int64_t>(s.n) * a.G + rows_of<W>() - 1) / rows_of<W>());
   }
   __syncthreads();
   // (the bound matters only where cu_seqlens is not ascending)
-  const int E = min(kMaxEntries, block_scan<int>(s_first, a.B, reinterpret_cast<int*>(s_wsum)));
-  for (int e = tid; e < E; e += kWaves * 64) {
+  const int E = min(kMaxEntries, block_scan<W, int>(s_first, a.B, reinterpret_cast<int*>(s_wsum)));
+  for (int e = tid; e < E; e += W * 64) {
     const int b = last_at_most(s_first, a.B, e);
-    const Seq s = seq_at(a, b);
-    const int tiles = (keys_of(a, s, (e - s_first[b] + 1) * kRows) + kBN - 1) / kBN;
+    const Seq s = seq_of(a, s_seq[b]);
+    const int tiles = (keys_of(a, s, (e - s_first[b] + 1) * rows_of<W>()) + kBN - 1) / kBN;
     s_pos[e] = static_cast<int64_t>(kUnits) * tiles + kItemUnits;
   }
   __syncthreads();
-  const int64_t H = block_scan<int64_t>(s_pos, E, s_wsum);
+  const int64_t H = block_scan<W, int64_t>(s_pos, E, s_wsum);
   const int nwg = gridDim.x;
   const int64_t U = H * a.Hkv;
-  int64_t N = U / (kMinRangeTiles * kUnits);
-  N = N < 1 ? 1 : N < nwg ? N : nwg;
+  // a range's width: every workgroup's share, at least kMinRangeTiles tiles
+  const int64_t share = U / static_cast<uint32_t>(nwg) + 1;
+  const int64_t width = share < kMinRangeTiles * kUnits ? kMinRangeTiles * kUnits : share;
   const int w = blockIdx.x;
-  const int v = N == nwg && nwg % 8 == 0 ? (w % 8) * (nwg / 8) + w / 8 : w;
-  const int64_t p_lo = v < N ? (v * U + N - 1) / N : U;
-  const int64_t p_hi = v < N ? ((v + 1) * U + N - 1) / N : U;
-  CutItem cut{0, 0, 0, 0};
+  const int v = width == share && nwg % 8 == 0 ? (w % 8) * (nwg / 8) + w / 8 : w;
+  const int64_t p_lo = v * width < U ? v * width : U;
+  const int64_t p_hi = p_lo + width < U ? p_lo + width : U;
+  CutItem cut{};
   if (p_lo < p_hi) {
-    const LaneOffsets off = lane_offsets(a, lane);
-    int kvh = static_cast<int>(p_lo / H);
+    const LaneOffsets off = lane_offsets<W>(a, lane, wave);
+    int kvh = static_cast<int>(quotient(p_lo, H));
     int e = __builtin_amdgcn_readfirstlane(last_at_most(s_pos, E, p_lo - kvh * H));
     while (true) {
       const int64_t P = kvh * H + uniform64(s_pos[e]);  // the item's position
       if (P >= p_hi) break;
       const int b = __builtin_amdgcn_readfirstlane(last_at_most(s_first, a.B, e));
       const int mt = e - __builtin_amdgcn_readfirstlane(s_first[b]);
-      const Seq s = seq_at(a, b);
-      const int tiles = (keys_of(a, s, (mt + 1) * kRows) + kBN - 1) / kBN;
+      SeqEntry se = s_seq[b];
+      se.q0 = __builtin_amdgcn_readfirstlane(se.q0);
+      se.n = __builtin_amdgcn_readfirstlane(se.n);
+      se.row = __builtin_amdgcn_readfirstlane(se.row);
+      se.ctx = __builtin_amdgcn_readfirstlane(se.ctx);
+      const Seq s = seq_of(a, se);
+      const int tiles = (keys_of(a, s, (mt + 1) * rows_of<W>()) + kBN - 1) / kBN;
       // tile j's midpoint: P + kItemUnits + kUnits j + kUnits / 2; an item without
       // tiles belongs to the range that holds its position
       const int64_t base = P + kItemUnits + kUnits / 2;
@@ -544,17 +608,17 @@ void paged_chunk_range_kernel(ChunkArgs a) {
       };
       const int j0 = first_at(p_lo), j1 = first_at(p_hi);
       if (j0 < j1 || (tiles == 0 && P >= p_lo)) {
-        const WaveRows wr = wave_rows(a, s, mt, wave, lane);
+        const WaveRows wr = wave_rows<W>(a, s, mt, wave, lane);
         float m_run, l_run;
         q3::f32x16 acc[4];
-        run_tiles(a, off, s, wr, kvh, j0, j1, tb, lane, wave, m_run, l_run, acc);
+        run_tiles<W>(a, off, s, wr, kvh, j0, j1, tb, lane, wave, m_run, l_run, acc);
         l_run = cross_half_sum(l_run);
         if (j0 == 0 && j1 == tiles) {
           if (wr.active) store_output(a, s, wr, kvh, lane, l_run, acc, stage_of(tb, wave));
         } else {
           const int slot = j0 == 0 ? 2 * v + 1 : 2 * v;
           if (wr.active) {
-            const int64_t row = static_cast<int64_t>(slot) * kRows + wave * 32 + (lane & 31);
+            const int64_t row = static_cast<int64_t>(slot) * rows_of<W>() + wave * 32 + (lane & 31);
             float* po = a.po + row * kD + 4 * (lane >> 5);
 #pragma unroll
             for (int db = 0; db < 4; ++db)
@@ -567,7 +631,11 @@ void paged_chunk_range_kernel(ChunkArgs a) {
           }
           if (j0 == 0) {
             const int64_t last = base + static_cast<int64_t>(kUnits) * (tiles - 1);
-            cut = CutItem{static_cast<int32_t>(last * N / U) - v + 1, b, kvh, mt};
+            cut.parts = static_cast<int32_t>(quotient(last, width)) - v + 1;
+            cut.r0 = mt * rows_of<W>();
+            cut.rows = min(rows_of<W>(), s.n * a.G - cut.r0);
+            cut.kvh = kvh;
+            cut.q0 = s.q0;
           }
         }
         __syncthreads();  // the staging buffers are read before the next loads refill them
@@ -581,58 +649,119 @@ void paged_chunk_range_kernel(ChunkArgs a) {
   if (tid == 0) a.cuts[v] = cut;
 }
 
-// Joins the parts of the cut items: a workgroup takes kMergeRows rows of the item
-// noted by range blockIdx.x, a wave a row at a time, a lane two of its elements.
-constexpr int kMergeRows = 16;
+// Joins the parts of the cut items: 16 lanes per row, eight elements each, the loads of
+// up to eight parts in flight at once.  A task is 16 rows of an item of up to three
+// parts (a wave takes four of them), or four rows of one with more, whose parts the
+// four waves share.  The workgroups deal the tasks among themselves from the list of
+// cut items: a workgroup for each possible task (ranges x rows) costs more in
+// workgroups that find nothing to do than the joins take.
+constexpr int kJoinParts = 8;
+constexpr int kJoinWaves = 4;
+constexpr int kJoinFew = 3;
 
-__global__ __launch_bounds__(kWaves * 64) void paged_chunk_join_kernel(ChunkArgs a) {
-  const int v = blockIdx.x;
-  const CutItem c = a.cuts[v];
-  if (c.parts == 0) return;
-  const Seq s = seq_at(a, c.b);
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  for (int i = wave; i < kMergeRows; i += kWaves) {
-    const int row = blockIdx.y * kMergeRows + i;
-    const int r = c.mt * kRows + row;
-    if (r >= s.n * a.G) return;
-    auto slot_row = [&](int p) {
-      return static_cast<int64_t>(p == 0 ? 2 * v + 1 : 2 * (v + p)) * kRows + row;
-    };
-    float M = q3::kNegInf;
-    for (int p = lane; p < c.parts; p += 64) M = fmaxf(M, a.pml[slot_row(p)].x);
+// A lane's eight elements of a row, joined so far.
+struct Joined {
+  float m, l, o[8];
+};
+
+// Joins the next K of n further parts, from slot `slot` on (slot0 in place of the first,
+// and read with weight 0 where there are fewer: other slots may hold anything).
+template <int K, int W>
+__device__ __forceinline__ void join_parts(const ChunkArgs& a, Joined& j, int slot0, int slot, int n,
+                                           int row, int e) {
+  float2 ml[K];
+  q3::f32x4 x[K][2];
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, q3::shfl_xor(M, o));
-    const float m = M == q3::kNegInf ? 0.f : M;
-    float l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int p0 = 0; p0 < c.parts; p0 += 64) {
-      float2 ml{q3::kNegInf, 0.f};
-      if (p0 + lane < c.parts) ml = a.pml[slot_row(p0 + lane)];
-      const float f = q3::fast_exp2(ml.x - m);
-      l += ml.y * f;
-      const int n = min(64, c.parts - p0);
-      for (int j = 0; j < n; j += 8) {
-        float2 x[8];
+  for (int u = 0; u < K; ++u) {
+    const int64_t at =
+        static_cast<int64_t>(u == 0 || u >= n ? slot0 : slot + 2 * u) * rows_of<W>() + row;
+    ml[u] = a.pml[at];
+    const q3::f32x4* src = reinterpret_cast<const q3::f32x4*>(a.po + at * kD + e);
+    x[u][0] = src[0];
+    x[u][1] = src[1];
+  }
+  __builtin_amdgcn_sched_barrier(0);  // every load is issued before the first is waited for
+  float m = j.m;
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          x[u] = *reinterpret_cast<const float2*>(a.po + slot_row(p0 + min(j + u, n - 1)) * kD +
-                                                  2 * lane);
+  for (int u = 0; u < K; ++u) m = fmaxf(m, ml[u].x);
+  const float use = m == q3::kNegInf ? 0.f : m;
+  const float f = q3::fast_exp2(j.m - use);
+  j.m = m;
+  j.l *= f;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const float fu = j + u < n ? __uint_as_float(__builtin_amdgcn_readlane(
-                                           __float_as_uint(f), j + u)) : 0.f;
-          o0 += fu * x[u].x;
-          o1 += fu * x[u].y;
-        }
-      }
+  for (int i = 0; i < 8; ++i) j.o[i] *= f;
+#pragma unroll
+  for (int u = 0; u < K; ++u) {
+    const float g = u < n ? q3::fast_exp2(ml[u].x - use) : 0.f;
+    j.l += g * ml[u].y;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) j.o[i] += g * x[u][i >> 2][i & 3];
+  }
+}
+
+__device__ __forceinline__ void store_joined(const ChunkArgs& a, const CutItem& c, const Joined& j,
+                                             int row, int e) {
+  const float inv = j.l > 0.f ? 1.f / j.l : 0.f;
+  const int r = c.r0 + row;
+  const int tok = static_cast<uint32_t>(r) / static_cast<uint32_t>(a.G);
+  q3::st16(a.o + (c.q0 + tok) * a.o_st +
+               (static_cast<int64_t>(c.kvh) * a.G + (r - tok * a.G)) * a.o_sh + e,
+           q3::u32x4{q3::pack_bf16x2(j.o[0] * inv, j.o[1] * inv),
+                     q3::pack_bf16x2(j.o[2] * inv, j.o[3] * inv),
+                     q3::pack_bf16x2(j.o[4] * inv, j.o[5] * inv),
+                     q3::pack_bf16x2(j.o[6] * inv, j.o[7] * inv)});
+}
+
+template <int W>
+__global__ __launch_bounds__(kJoinWaves * 64) void paged_chunk_join_kernel(ChunkArgs a, int ranges) {
+  __shared__ int s_task[kMaxEntries];  // tasks before each range's item
+  __shared__ int s_wsum[kJoinWaves];
+  __shared__ Joined s_j[kJoinWaves - 1][64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  for (int v = tid; v < ranges; v += kJoinWaves * 64) {
+    const CutItem c = a.cuts[v];
+    const int per = c.parts <= kJoinFew ? 4 * kJoinWaves : 4;
+    s_task[v] = c.parts > 0 ? (c.rows + per - 1) / per : 0;
+  }
+  __syncthreads();
+  const int tasks = block_scan<kJoinWaves, int>(s_task, ranges, s_wsum);
+  const int e = 8 * (lane & 15);
+  for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
+    const int v = __builtin_amdgcn_readfirstlane(last_at_most(s_task, ranges, task));
+    const CutItem c = a.cuts[v];
+    const int k = task - s_task[v];
+    Joined j{q3::kNegInf, 0.f, {}};
+    if (c.parts <= kJoinFew) {
+      const int row = 4 * (kJoinWaves * k + wave) + (lane >> 4);
+      if (row >= c.rows) continue;
+      join_parts<kJoinFew, W>(a, j, 2 * v + 1, 2 * v, c.parts, row, e);
+      store_joined(a, c, j, row, e);
+      continue;
     }
+    const int row = 4 * k + (lane >> 4);
+    const int each = (c.parts + kJoinWaves - 1) / kJoinWaves;
+    const int p1 = min(c.parts, (wave + 1) * each);
+    if (row < c.rows)
+      for (int p = wave * each; p < p1; p += kJoinParts)
+        join_parts<kJoinParts, W>(a, j, p == 0 ? 2 * v + 1 : 2 * (v + p), 2 * (v + p), p1 - p, row,
+                                  e);
+    if (wave > 0) s_j[wave - 1][lane] = j;
+    __syncthreads();
+    if (wave == 0 && row < c.rows) {
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) l += q3::shfl_xor(l, o);
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    const int tok = r / a.G;
-    *reinterpret_cast<uint32_t*>(a.o + (s.q0 + tok) * a.o_st +
-                                 (static_cast<int64_t>(c.kvh) * a.G + (r - tok * a.G)) * a.o_sh +
-                                 2 * lane) = q3::pack_bf16x2(o0 * inv, o1 * inv);
+      for (int s = 0; s < kJoinWaves - 1; ++s) {
+        const Joined& x = s_j[s][lane];
+        const float m = fmaxf(j.m, x.m), use = m == q3::kNegInf ? 0.f : m;
+        const float f = q3::fast_exp2(j.m - use), g = q3::fast_exp2(x.m - use);
+        j.m = m;
+        j.l = j.l * f + x.l * g;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) j.o[i] = j.o[i] * f + x.o[i] * g;
+      }
+      store_joined(a, c, j, row, e);
+    }
+    __syncthreads();  // s_j is read before the next task writes it
   }
 }
 
@@ -652,30 +781,68 @@ int cu_count() {
   return cached[dev];
 }
 
-// Resident workgroups of the range schedule (two per CU), 512 where no device can be
-// asked.
-int range_workgroups() {
+// Resident workgroups of the range schedule (two waves a SIMD); 256 CUs where no device
+// can be asked.
+int range_workgroups(int W) {
   const int cus = cu_count();
-  return 2 * (cus > 0 ? cus : 256);
+  const int wgs = (cus > 0 ? cus : 256) * 8 / W;
+  return wgs < kMaxEntries ? wgs : kMaxEntries;
 }
 
 struct ChunkLayout {
   int64_t po, pml, cuts, total;
 };
-ChunkLayout chunk_layout(int ranges) {
+ChunkLayout chunk_layout(int W) {
+  const int64_t ranges = range_workgroups(W), rows = 2 * ranges * 32 * W;
   ChunkLayout l;
   l.po = 0;
-  l.pml = l.po + int64_t(2) * ranges * kRows * kD * sizeof(float);
-  l.cuts = l.pml + int64_t(2) * ranges * kRows * sizeof(float2);
+  l.pml = l.po + rows * kD * sizeof(float);
+  l.cuts = l.pml + rows * sizeof(float2);
   l.total = l.cuts + (ranges * sizeof(CutItem) + 255) / 256 * 256;
   return l;
 }
 
-// Items that a launch has at most, and whether the range schedule takes it.
-int64_t entries_at_most(int B, int64_t total, int G) { return q3::cdiv(total * G, kRows) + B; }
-bool takes_ranges(int B, int64_t total, int G, int Hkv) {
-  const int64_t e = entries_at_most(B, total, G);
-  return e <= kMaxEntries && e * Hkv <= 4 * static_cast<int64_t>(range_workgroups());
+// How a call runs: waves of a workgroup, and by ranges or whole items.
+struct Variant {
+  int waves;
+  bool ranges;
+};
+Variant variant_of(int B, int max_chunk, int64_t total, int G, int Hkv) {
+  static const char* e = getenv("Q3_W");
+  static const char* f = getenv("Q3_R");
+  Variant v{e ? atoi(e) : 4, false};
+  const int64_t entries = q3::cdiv(total * G, 32 * v.waves) + B;
+  v.ranges = B <= kMaxSeqs && entries <= kMaxEntries &&
+             entries * Hkv <= (f ? atoi(f) : 4) * static_cast<int64_t>(range_workgroups(v.waves));
+  return v;
+}
+
+template <int W>
+int launch_tiles(ChunkArgs a, const Variant& var, int max_chunk, void* workspace, hipStream_t s,
+                 const char* who) {
+  q3::clear_error();
+  if (var.ranges) {
+    const int wgs = range_workgroups(W);
+    const ChunkLayout l = chunk_layout(W);
+    char* ws = static_cast<char*>(workspace);
+    a.po = reinterpret_cast<float*>(ws + l.po);
+    a.pml = reinterpret_cast<float2*>(ws + l.pml);
+    a.cuts = reinterpret_cast<CutItem*>(ws + l.cuts);
+    hipLaunchKernelGGL(paged_chunk_range_kernel<W>, dim3(wgs), dim3(W * 64), 0, s, a);
+    if (const int rc = q3::launch_status(who)) return rc;
+    hipLaunchKernelGGL(paged_chunk_join_kernel<W>, dim3(4 * (wgs * W / 8)), dim3(kJoinWaves * 64), 0,
+                       s, a, wgs);
+    return q3::launch_status(who);
+  }
+  const int64_t longest = max_chunk < a.total ? max_chunk : a.total;
+  a.n_mtiles = static_cast<int>(q3::cdiv(longest * a.G, rows_of<W>()));
+  const int64_t items = static_cast<int64_t>(a.Hkv) * a.B * a.n_mtiles;
+  if (items > 0x7fffffff)
+    return q3::fail(QWEN3_EINVAL, "%s: grid too large (KV heads %d, batch %d, max_chunk %d)", who,
+                    a.Hkv, a.B, max_chunk);
+  hipLaunchKernelGGL(paged_chunk_flat_kernel<W>, dim3(static_cast<unsigned>(items)), dim3(W * 64), 0,
+                     s, a);
+  return q3::launch_status(who);
 }
 
 }  // namespace
@@ -686,9 +853,9 @@ extern "C" size_t qwen3_paged_chunk_workspace_bytes(int B, int max_chunk, int64_
   if (B <= 0 || total_tokens <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
       num_heads / num_kv_heads > kMaxG || head_dim != kD || max_chunk <= 0)
     return 0;
-  return takes_ranges(B, total_tokens, num_heads / num_kv_heads, num_kv_heads)
-             ? chunk_layout(range_workgroups()).total
-             : 256;
+  const Variant v =
+      variant_of(B, max_chunk, total_tokens, num_heads / num_kv_heads, num_kv_heads);
+  return v.ranges ? chunk_layout(v.waves).total : 256;
 }
 
 extern "C" int qwen3_paged_chunk_bf16(
@@ -738,7 +905,7 @@ extern "C" int qwen3_paged_chunk_bf16(
       return q3::fail(QWEN3_EUNSUPPORTED, "%s: slot stride %lld outside %d..2^24", who,
                       (long long)st, kD);
   const int64_t total_rows = total_tokens * (num_heads / num_kv_heads);
-  if (total_rows > 0x7fffffff - kRows)
+  if (total_rows > 0x7fffffff - 256)
     return q3::fail(QWEN3_EINVAL, "%s: too many tokens", who);
   if (B == 0 || max_chunk == 0 || total_tokens == 0) return QWEN3_OK;
   const size_t need = qwen3_paged_chunk_workspace_bytes(B, max_chunk, total_tokens, num_heads,
@@ -755,11 +922,11 @@ extern "C" int qwen3_paged_chunk_bf16(
   a.k = static_cast<const uint16_t*>(k_cache);
   a.k_blk = k_strides[0];
   a.k_sh = k_strides[1];
-  a.k_slot = k_strides[2];
+  a.k_slot = static_cast<int>(k_strides[2]);
   a.v = static_cast<const uint16_t*>(v_cache);
   a.v_blk = v_strides[0];
   a.v_sh = v_strides[1];
-  a.v_slot = v_strides[2];
+  a.v_slot = static_cast<int>(v_strides[2]);
   a.num_blocks = num_blocks;
   a.bt = block_table;
   a.bt_stride = bt_row_stride;
@@ -775,30 +942,11 @@ extern "C" int qwen3_paged_chunk_bf16(
   a.B = B;
   a.Hkv = num_kv_heads;
   a.G = num_heads / num_kv_heads;
-  a.bs = block_size;
+  a.gpb = block_size / kGroup;
+  a.reach = static_cast<int>(max_pages * block_size);
   a.scale_log2 = scale * q3::kLog2e;
-  q3::clear_error();
+  const Variant var = variant_of(B, max_chunk, total_tokens, a.G, a.Hkv);
   const auto s = static_cast<hipStream_t>(stream);
-  if (takes_ranges(B, total_tokens, a.G, a.Hkv)) {
-    const int wgs = range_workgroups();
-    const ChunkLayout l = chunk_layout(wgs);
-    char* ws = static_cast<char*>(workspace);
-    a.po = reinterpret_cast<float*>(ws + l.po);
-    a.pml = reinterpret_cast<float2*>(ws + l.pml);
-    a.cuts = reinterpret_cast<CutItem*>(ws + l.cuts);
-    hipLaunchKernelGGL(paged_chunk_range_kernel, dim3(wgs), dim3(kWaves * 64), 0, s, a);
-    if (const int rc = q3::launch_status(who)) return rc;
-    hipLaunchKernelGGL(paged_chunk_join_kernel, dim3(wgs, kRows / kMergeRows), dim3(kWaves * 64), 0,
-                       s, a);
-    return q3::launch_status(who);
-  }
-  const int64_t longest = max_chunk < total_tokens ? max_chunk : total_tokens;
-  a.n_mtiles = static_cast<int>(q3::cdiv(longest * a.G, kRows));
-  const int64_t items = static_cast<int64_t>(a.Hkv) * B * a.n_mtiles;
-  if (items > 0x7fffffff)
-    return q3::fail(QWEN3_EINVAL, "%s: grid too large (KV heads %d, batch %d, max_chunk %d)", who,
-                    num_kv_heads, B, max_chunk);
-  hipLaunchKernelGGL(paged_chunk_flat_kernel, dim3(static_cast<unsigned>(items)),
-                     dim3(kWaves * 64), 0, s, a);
-  return q3::launch_status(who);
+  return var.waves == 8 ? launch_tiles<8>(a, var, max_chunk, workspace, s, who)
+                        : launch_tiles<4>(a, var, max_chunk, workspace, s, who);
 }
