@@ -19,7 +19,9 @@
 //    last key (or holds nothing where the table names no page of the pool), so
 //    slots behind it are never read.  Page ids come 64 at a time into a
 //    register (16 tiles' worth), the next 64 before they are needed.
-#include <cstdlib>
+#include <algorithm>
+
+#include "paged_chunk_stream.hpp"
 #include "prefill_tile.hpp"
 
 namespace {
@@ -483,6 +485,8 @@ void paged_chunk_flat_kernel(ChunkArgs a) {
 constexpr int kUnits = 16;
 constexpr int kItemUnits = 40;
 constexpr int kMinRangeTiles = 4;
+constexpr int kWholeSlack = 20;     // an uncut item: one part in 20, and six tiles, above
+constexpr int kWholeUnits = 96;     // an equal share
 constexpr int kMaxSeqs = 256;       // sequences and (sequence, row tile) pairs
 constexpr int kMaxEntries = 1024;   // tabulated in LDS
 
@@ -552,9 +556,11 @@ void paged_chunk_range_kernel(ChunkArgs a) {
   __shared__ int s_first[kMaxSeqs];       // row tiles before each sequence
   __shared__ SeqEntry s_seq[kMaxSeqs];
   __shared__ int64_t s_wsum[W];
+  __shared__ int s_most;                  // key tiles of the longest item
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (tid == 0) s_most = 0;
   // Every workgroup waits for this before its first K/V load: one chain of two
   // memory round trips (row_ids, then seq_lens), the rest is in LDS.
   for (int b = tid; b < a.B; b += W * 64) {
@@ -570,6 +576,7 @@ void paged_chunk_range_kernel(ChunkArgs a) {
     const Seq s = seq_of(a, s_seq[b]);
     const int tiles = (keys_of(a, s, (e - s_first[b] + 1) * rows_of<W>()) + kBN - 1) / kBN;
     s_pos[e] = static_cast<int64_t>(kUnits) * tiles + kItemUnits;
+    atomicMax(&s_most, tiles);
   }
   __syncthreads();
   const int64_t H = block_scan<W, int64_t>(s_pos, E, s_wsum);
@@ -579,9 +586,20 @@ void paged_chunk_range_kernel(ChunkArgs a) {
   const int64_t share = U / static_cast<uint32_t>(nwg) + 1;
   const int64_t width = share < kMinRangeTiles * kUnits ? kMinRangeTiles * kUnits : share;
   const int w = blockIdx.x;
-  const int v = width == share && nwg % 8 == 0 ? (w % 8) * (nwg / 8) + w / 8 : w;
-  const int64_t p_lo = v * width < U ? v * width : U;
-  const int64_t p_hi = p_lo + width < U ? p_lo + width : U;
+  // Items that are no more than the workgroups and nearly as long as each other are not
+  // cut: the longest takes little more than an equal share, and a cut costs its saves
+  // and the second launch's reads (2,048 tokens behind 64,000: 1.92 ms against 2.04).
+  const int64_t longest = static_cast<int64_t>(kUnits) * s_most + kItemUnits;
+  const bool whole = static_cast<int64_t>(E) * a.Hkv <= nwg &&
+                     longest <= share + share / kWholeSlack + kWholeUnits;
+  const int v = (whole || width == share) && nwg % 8 == 0 ? (w % 8) * (nwg / 8) + w / 8 : w;
+  int64_t p_lo = v * width < U ? v * width : U;
+  int64_t p_hi = p_lo + width < U ? p_lo + width : U;
+  if (whole) {
+    const int kvh = E > 0 ? v / E : a.Hkv, e = E > 0 ? v - kvh * E : 0;
+    p_lo = kvh < a.Hkv ? kvh * H + uniform64(s_pos[e]) : U;
+    p_hi = kvh >= a.Hkv ? U : (e + 1 < E ? kvh * H + uniform64(s_pos[e + 1]) : (kvh + 1) * H);
+  }
   CutItem cut{};
   if (p_lo < p_hi) {
     const LaneOffsets off = lane_offsets<W>(a, lane, wave);
@@ -802,18 +820,26 @@ ChunkLayout chunk_layout(int W) {
   return l;
 }
 
-// How a call runs: waves of a workgroup, and by ranges or whole items.
+// How a call runs; a rule on its launch shape, so that a captured call stays valid.
+//  - few packed rows a KV head: the streaming kernel (paged_chunk_stream.hip);
+//  - chunks of more than four waves' rows: eight-wave workgroups, which stage each K/V
+//    tile once for twice the rows (2,048 tokens behind 64,000, 32/8 heads: 1.92 ms
+//    against 2.03; eight chunks of 100-500 behind 100-9,000: 313 us against 318; 16
+//    single tokens behind 4,000 in the same kernels: 54 against 51);
+//  - ranges, unless the items are so many that whole ones finish together: at 1.4
+//    items a workgroup 313 us against 431 (eight ragged chunks), at 2 (one prompt of
+//    4,096, whose items pair up heavy with light) 181 against 153.
 struct Variant {
+  bool stream;
   int waves;
   bool ranges;
 };
 Variant variant_of(int B, int max_chunk, int64_t total, int G, int Hkv) {
-  static const char* e = getenv("Q3_W");
-  static const char* f = getenv("Q3_R");
-  Variant v{e ? atoi(e) : 4, false};
+  const int64_t rows = std::min<int64_t>(max_chunk, total) * G;
+  Variant v{q3::chunk_streams(B, rows), rows > rows_of<4>() ? 8 : 4, false};
   const int64_t entries = q3::cdiv(total * G, 32 * v.waves) + B;
   v.ranges = B <= kMaxSeqs && entries <= kMaxEntries &&
-             entries * Hkv <= (f ? atoi(f) : 4) * static_cast<int64_t>(range_workgroups(v.waves));
+             4 * entries * Hkv <= 7 * static_cast<int64_t>(range_workgroups(v.waves));
   return v;
 }
 
@@ -855,6 +881,9 @@ extern "C" size_t qwen3_paged_chunk_workspace_bytes(int B, int max_chunk, int64_
     return 0;
   const Variant v =
       variant_of(B, max_chunk, total_tokens, num_heads / num_kv_heads, num_kv_heads);
+  if (v.stream)
+    return q3::chunk_stream_workspace(
+        B, static_cast<int>(std::min<int64_t>(max_chunk, total_tokens) * (num_heads / num_kv_heads)));
   return v.ranges ? chunk_layout(v.waves).total : 256;
 }
 
@@ -947,6 +976,14 @@ extern "C" int qwen3_paged_chunk_bf16(
   a.scale_log2 = scale * q3::kLog2e;
   const Variant var = variant_of(B, max_chunk, total_tokens, a.G, a.Hkv);
   const auto s = static_cast<hipStream_t>(stream);
+  if (var.stream) {
+    const q3::ChunkStreamCall call{
+        a.q, a.q_st, a.q_sh, a.k, a.k_blk, a.k_sh, a.k_slot, a.v, a.v_blk, a.v_sh, a.v_slot,
+        a.num_blocks, a.bt, a.bt_stride, a.max_rows, a.max_pages, a.seq_lens, a.row_ids, a.cu,
+        a.o, a.o_st, a.o_sh, a.total, a.B, a.Hkv, a.G, block_size,
+        static_cast<int>(std::min<int64_t>(max_chunk, total_tokens) * a.G), a.scale_log2};
+    return q3::launch_chunk_stream(call, workspace, s, who);
+  }
   return var.waves == 8 ? launch_tiles<8>(a, var, max_chunk, workspace, s, who)
                         : launch_tiles<4>(a, var, max_chunk, workspace, s, who);
 }
