@@ -9,6 +9,7 @@ qwen3/PagedKVcache.py:16) resolve unchanged.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -184,8 +185,13 @@ def paged_chunk_workspace_bytes(batch: int, max_chunk: int, total_tokens: int, n
                                 num_kv_heads: int, head_dim: int) -> int:
     """Workspace size of paged_attention_chunk_hip on the current device; depends
     only on the launch shape, so a captured call stays valid for any lengths."""
-    return int(_lib.load().qwen3_paged_chunk_workspace_bytes(
-        batch, max_chunk, total_tokens, num_heads, num_kv_heads, head_dim))
+    return _chunk_workspace(torch.cuda.current_device() if torch.cuda.is_initialized() else -1,
+                            batch, max_chunk, total_tokens, num_heads, num_kv_heads, head_dim)
+
+
+@functools.lru_cache(maxsize=1024)
+def _chunk_workspace(device: int, *shape) -> int:
+    return int(_lib.load().qwen3_paged_chunk_workspace_bytes(*shape))
 
 
 def paged_attention_chunk_hip(q, k_buffer, v_buffer, block_table_2d, seq_lens_full, row_ids,
@@ -211,25 +217,27 @@ def paged_attention_chunk_hip(q, k_buffer, v_buffer, block_table_2d, seq_lens_fu
     1/sqrt(head_dim) unless given.  workspace: paged_chunk_workspace_bytes(...)
     bytes, a fresh one per call by default.
     """
+    bf16, i32 = torch.bfloat16, torch.int32
     assert q.dim() == 3
     T, num_heads, head_dim = q.shape
     num_blocks, num_kv_heads, block_size_check, head_dim_check = k_buffer.shape
     assert block_size_check == block_size and head_dim_check == head_dim
     assert v_buffer.shape == k_buffer.shape
-    assert q.dtype == torch.bfloat16 and k_buffer.dtype == torch.bfloat16 \
-        and v_buffer.dtype == torch.bfloat16, "HIP chunk kernel is bf16 only"
-    assert block_table_2d.dtype == torch.int32 and seq_lens_full.dtype == torch.int32
+    assert q.dtype is bf16 and k_buffer.dtype is bf16 and v_buffer.dtype is bf16, \
+        "HIP chunk kernel is bf16 only"
+    assert block_table_2d.dtype is i32 and seq_lens_full.dtype is i32
     assert block_table_2d.dim() == 2 and block_table_2d.stride(1) == 1, \
         "block_table_2d rows must be contiguous"
-    assert seq_lens_full.dim() == 1 and seq_lens_full.shape[0] >= block_table_2d.shape[0]
-    assert cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1
+    table_rows, table_pages = block_table_2d.shape
+    assert seq_lens_full.dim() == 1 and seq_lens_full.shape[0] >= table_rows
+    assert cu_seqlens.dtype is i32 and cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1
     assert k_buffer.stride(3) == 1 and v_buffer.stride(3) == 1
-    B = cu_seqlens.numel() - 1
+    B = cu_seqlens.shape[0] - 1
     if row_ids is not None:
-        assert row_ids.dtype == torch.int32 and row_ids.numel() == B
+        assert row_ids.dtype is i32 and row_ids.numel() == B
         row_ids = row_ids.contiguous()
     else:
-        assert B <= block_table_2d.shape[0], "more sequences than rows of the block table"
+        assert B <= table_rows, "more sequences than rows of the block table"
     dev = _lib.require_hip(q, k_buffer, v_buffer, block_table_2d, seq_lens_full, row_ids,
                            cu_seqlens, out, workspace)
     cu_seqlens = cu_seqlens.contiguous()
@@ -237,30 +245,28 @@ def paged_attention_chunk_hip(q, k_buffer, v_buffer, block_table_2d, seq_lens_fu
     if q.stride(2) != 1:
         q = q.contiguous()
     if max_chunk is None:
-        lens = cu_seqlens.cpu().diff()
-        max_chunk = int(lens.max()) if B else 0
+        max_chunk = int(cu_seqlens.cpu().diff().max()) if B else 0
     if scale is None:
         scale = 1.0 / math.sqrt(head_dim)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty(q.shape, dtype=bf16, device=dev)
     else:
-        assert out.shape == q.shape and out.dtype == torch.bfloat16 and out.stride(2) == 1, \
+        assert out.shape == q.shape and out.dtype is bf16 and out.stride(2) == 1, \
             "out must be a bf16 (total_tokens, num_heads, head_dim) tensor with unit last stride"
     if T == 0 or B == 0:
         return out
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        need = paged_chunk_workspace_bytes(B, max_chunk, T, num_heads, num_kv_heads, head_dim)
+    strides = _lib.outer_strides
+    with _lib.on_device(dev):
+        need = _chunk_workspace(dev.index, B, max_chunk, T, num_heads, num_kv_heads, head_dim)
         if workspace is None or workspace.numel() * workspace.element_size() < need:
             workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
-        rc = lib.qwen3_paged_chunk_bf16(
-            q.data_ptr(), _lib.strides(q, (0, 1)),
-            k_buffer.data_ptr(), _lib.strides(k_buffer, (0, 1, 2)),
-            v_buffer.data_ptr(), _lib.strides(v_buffer, (0, 1, 2)), num_blocks,
-            block_table_2d.data_ptr(), block_table_2d.stride(0), *block_table_2d.shape,
+        rc = _lib.load().qwen3_paged_chunk_bf16(
+            q.data_ptr(), strides(q), k_buffer.data_ptr(), strides(k_buffer),
+            v_buffer.data_ptr(), strides(v_buffer), num_blocks,
+            block_table_2d.data_ptr(), block_table_2d.stride(0), table_rows, table_pages,
             seq_lens_full.data_ptr(), _lib.ptr(row_ids), cu_seqlens.data_ptr(),
-            out.data_ptr(), _lib.strides(out, (0, 1)),
-            B, int(max_chunk), T, num_heads, num_kv_heads, head_dim, block_size, float(scale),
+            out.data_ptr(), strides(out),
+            B, max_chunk, T, num_heads, num_kv_heads, head_dim, block_size, scale,
             workspace.data_ptr(), workspace.numel() * workspace.element_size(),
             _lib.stream_of(dev))
     _lib.check(rc, "qwen3_paged_chunk_bf16")

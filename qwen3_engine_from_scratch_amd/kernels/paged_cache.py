@@ -21,7 +21,7 @@ __all__ = ["copy_pages_hip", "fork_pages_hip", "move_pages_hip"]
 
 
 def _list(values, n: int, what: str):
-    values = [operator.index(x) for x in values]
+    values = list(map(operator.index, values))
     if len(values) != n:
         raise ValueError(f"{what} has {len(values)} entries, expected {n}")
     if n and not -2 ** 31 <= min(values) <= max(values) < 2 ** 31:
@@ -55,7 +55,7 @@ def copy_pages_hip(k_buffer: torch.Tensor, v_buffer: torch.Tensor, src, dst, tok
     s, d = _list(src, n, "src"), _list(dst, n, "dst")
     t = None if tokens is None else _list(tokens, n, "tokens")
     dev = _lib.require_hip(k_buffer, v_buffer)
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         rc = _lib.load().qwen3_page_copy_bf16(*pool, s, d, t, n, _lib.stream_of(dev))
     _lib.check(rc, "qwen3_page_copy_bf16")
 
@@ -75,7 +75,7 @@ def fork_pages_hip(k_buffer: torch.Tensor, v_buffer: torch.Tensor, block_table_2
     lists = (_list(src_rows, n, "src_rows"), _list(dst_rows, n, "dst_rows"),
              _list(tokens, n, "tokens"), _list(new_blocks, n, "new_blocks"))
     dev = _lib.require_hip(k_buffer, v_buffer, block_table_2d, seq_lens)
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         rc = _lib.load().qwen3_page_fork_bf16(*pool, *table, seq_lens.data_ptr(), *lists, n,
                                               _lib.stream_of(dev))
     _lib.check(rc, "qwen3_page_fork_bf16")
@@ -90,6 +90,6 @@ def move_pages_hip(k_buffer: torch.Tensor, v_buffer: torch.Tensor, block_table_2
     pool, table = _pool(k_buffer, v_buffer), _table(block_table_2d)
     s, d = _list(src, n, "src"), _list(dst, n, "dst")
     dev = _lib.require_hip(k_buffer, v_buffer, block_table_2d)
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         rc = _lib.load().qwen3_page_move_bf16(*pool, *table, s, d, n, _lib.stream_of(dev))
     _lib.check(rc, "qwen3_page_move_bf16")

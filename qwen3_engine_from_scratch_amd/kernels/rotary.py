@@ -130,7 +130,7 @@ def _check(q, k, rotary, q_out, k_out):
 
 def _positions(positions, T):
     assert positions.dtype == torch.int64 and positions.numel() == T
-    return positions.reshape(-1).contiguous()
+    return positions.contiguous()
 
 
 def _new(x):
@@ -154,12 +154,12 @@ def rotary_embedding_hip(q: torch.Tensor, k: torch.Tensor | None, positions: tor
         k_out = _new(k)
     if T == 0:
         return q_out, k_out
-    st = _lib.strides
-    with torch.cuda.device(dev):
+    st = _lib.outer_strides
+    with _lib.on_device(dev):
         rc = _lib.load().qwen3_rotary(
-            q.data_ptr(), st(q, (0, 1)), _lib.ptr(k), None if k is None else st(k, (0, 1)),
-            q_out.data_ptr(), st(q_out, (0, 1)), _lib.ptr(k_out),
-            None if k is None else st(k_out, (0, 1)), _DTYPES[q.dtype],
+            q.data_ptr(), st(q), _lib.ptr(k), None if k is None else st(k),
+            q_out.data_ptr(), st(q_out), _lib.ptr(k_out),
+            None if k is None else st(k_out), _DTYPES[q.dtype],
             rotary.inv_freq.data_ptr(), float(rotary.attention_factor), _LAYOUTS[rotary.layout],
             1 if inverse else 0, positions.data_ptr(), T, Hq, 0 if k is None else k.shape[1], D,
             rotary.rotary_dim, _lib.stream_of(dev))
@@ -195,15 +195,15 @@ def rotary_embedding_prefill_hip(q: torch.Tensor, k: torch.Tensor, v: torch.Tens
     k_out = _new(k) if k_out is None else k_out
     if T == 0:
         return q_out, k_out
-    st = _lib.strides
-    with torch.cuda.device(dev):
+    st = _lib.outer_strides
+    with _lib.on_device(dev):
         rc = _lib.load().qwen3_rotary_slots_bf16(
-            q.data_ptr(), st(q, (0, 1)), k.data_ptr(), st(k, (0, 1)), v.data_ptr(),
-            st(v, (0, 1)), q_out.data_ptr(), st(q_out, (0, 1)), k_out.data_ptr(),
-            st(k_out, (0, 1)), rotary.inv_freq.data_ptr(), float(rotary.attention_factor),
+            q.data_ptr(), st(q), k.data_ptr(), st(k), v.data_ptr(),
+            st(v), q_out.data_ptr(), st(q_out), k_out.data_ptr(),
+            st(k_out), rotary.inv_freq.data_ptr(), float(rotary.attention_factor),
             _LAYOUTS[rotary.layout], positions.data_ptr(), slot_mapping.data_ptr(),
-            k_buffer.data_ptr(), st(k_buffer, (0, 1, 2, 3)), v_buffer.data_ptr(),
-            st(v_buffer, (0, 1, 2, 3)), k_buffer.shape[0], int(layer_idx), k_buffer.shape[1], T,
+            k_buffer.data_ptr(), st(k_buffer), v_buffer.data_ptr(),
+            st(v_buffer), k_buffer.shape[0], int(layer_idx), k_buffer.shape[1], T,
             Hq, k.shape[1], D, rotary.rotary_dim, k_buffer.shape[3], _lib.stream_of(dev))
     _lib.check(rc, "qwen3_rotary_slots_bf16")
     return q_out, k_out
@@ -231,13 +231,13 @@ def rotary_embedding_decode_hip(q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
     q_out = _new(q) if q_out is None else q_out
     if B == 0:
         return q_out
-    st = _lib.strides
-    with torch.cuda.device(dev):
+    st = _lib.outer_strides
+    with _lib.on_device(dev):
         rc = _lib.load().qwen3_rotary_decode_bf16(
-            q.data_ptr(), st(q, (0, 1)), k.data_ptr(), st(k, (0, 1)), v.data_ptr(),
-            st(v, (0, 1)), q_out.data_ptr(), st(q_out, (0, 1)), rotary.inv_freq.data_ptr(),
+            q.data_ptr(), st(q), k.data_ptr(), st(k), v.data_ptr(),
+            st(v), q_out.data_ptr(), st(q_out), rotary.inv_freq.data_ptr(),
             float(rotary.attention_factor), _LAYOUTS[rotary.layout], kb.data_ptr(),
-            st(kb, (0, 1, 2, 3)), vb.data_ptr(), st(vb, (0, 1, 2, 3)), kb.shape[0],
+            st(kb), vb.data_ptr(), st(vb), kb.shape[0],
             int(layer_idx), kb.shape[1], pool.seq_lens.data_ptr(), bt.data_ptr(), bt.stride(0),
             bt.shape[0], bt.shape[1], _lib.ptr(row_ids), _lib.ptr(positions), B, Hq, k.shape[1],
             D, rotary.rotary_dim, kb.shape[3], _lib.stream_of(dev))
