@@ -22,10 +22,12 @@ class Qwen3Config:
     rope_theta: float
     max_position_embeddings: int = 4096
     tie_word_embeddings: bool = False
+    rope_scaling: dict | None = None  # as in config.json (kernels/rotary.py: rotary_frequencies)
 
     @classmethod
-    def from_pretrained(cls, model_path: str) -> "Qwen3Config":
-        """Reads <model_path>/config.json (the HF layout, as the reference)."""
+    def from_pretrained(cls, model_path: str, use_rope_scaling: bool = False) -> "Qwen3Config":
+        """Reads <model_path>/config.json (the HF layout, as the reference, which does
+        not look at rope_scaling; use_rope_scaling takes it over)."""
         with open(os.path.join(model_path, "config.json")) as f:
             d = json.load(f)
         return cls(
@@ -40,6 +42,7 @@ class Qwen3Config:
             rope_theta=d["rope_theta"],
             max_position_embeddings=d.get("max_position_embeddings", 4096),
             tie_word_embeddings=d.get("tie_word_embeddings", False),
+            rope_scaling=d.get("rope_scaling") if use_rope_scaling else None,
         )
 
 

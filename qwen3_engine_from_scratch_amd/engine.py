@@ -23,6 +23,11 @@ the per-step state lives:
     is known without the read-back; an eos seen one step late drops the one
     token computed past it (its page writes land beyond its final length).
 Greedy decoding only (temperature 0), as the reference's benchmark runs.
+
+Prompts may also follow a prefix that is cached already (Engine.cache_prefix,
+GenRequest.prefix: its pages are shared, not computed again), and long ones may be
+prefilled in pieces (prefill_chunk: bounds a step's activations); both attend the
+pages through the chunk kernel.
 """
 from __future__ import annotations
 
@@ -33,7 +38,7 @@ from dataclasses import dataclass, field
 import numpy as np
 import torch
 
-from .PagedKVcache import PageIn, PagedKVCache, set_seq_lens_bulk
+from .PagedKVcache import PageIn, PagedKVCache, fork_caches, set_seq_lens_bulk
 from .graph_runner import GraphRunner, pow2_buckets
 from .kernels.model_ops import argmax
 
@@ -47,6 +52,7 @@ class GenRequest:
     prompt: list
     max_new_tokens: int
     eos_token_id: int | None = None
+    prefix: PagedKVCache | None = None  # tokens before the prompt; forked, stays the caller's
     output_ids: list = field(default_factory=list)
     cache: PagedKVCache | None = None
     finished: bool = False
@@ -67,14 +73,18 @@ class GenRequest:
 
 class Engine:
     def __init__(self, model, pool, max_batch: int = 64, use_graph: bool = True,
-                 batch_invariant: bool = False, max_prefill_batch: int | None = None):
+                 batch_invariant: bool = False, max_prefill_batch: int | None = None,
+                 prefill_chunk: int | None = None):
         """batch_invariant: decode attention on the batch-invariant kernel,
         so a request's decode tokens do not depend on what else is batched
         with it.  max_prefill_batch: prompts per prefill step (None: as many
         as there are free rows); 1 prefills every prompt alone, as a
         request running by itself would be (the library GEMMs of the
         prefill pick kernels by row count, so a prompt's prefill bits depend
-        on the rows batched with it)."""
+        on the rows batched with it).  prefill_chunk: tokens of a prompt per
+        prefill step (None: whole prompts)."""
+        assert prefill_chunk is None or prefill_chunk > 0
+        self.prefill_chunk = prefill_chunk
         self.model = model
         self.pool = pool
         self.max_batch = max_batch
@@ -102,7 +112,73 @@ class Engine:
 
     # ---- steps -------------------------------------------------------------
 
+    def _run_chunk(self, caches, tokens, want_logits):
+        """One chunk step: tokens[i] (a list, not empty) behind what caches[i] holds.
+        Returns the greedy next token of each handle, or None."""
+        dev = self.device
+        starts, lens = [c.seq_len for c in caches], [len(t) for t in tokens]
+        self._pages.reserve(caches, [a + n for a, n in zip(starts, lens)])
+        n, T = len(caches), sum(lens)
+        cu = np.zeros(n + 1, dtype=np.int64)
+        cu[1:] = np.cumsum(lens)
+        bs = self.pool.block_size
+        # one host buffer, one copy: ids | positions | slots | last rows | cu | rows
+        buf = np.empty(3 * T + 3 * n + 1, dtype=np.int64)
+        buf[:T] = np.concatenate([np.asarray(t, dtype=np.int64) for t in tokens])
+        for c, i, a, m in zip(caches, cu[:-1], starts, lens):
+            p = np.arange(a, a + m, dtype=np.int64)
+            table = np.asarray(c.block_table, dtype=np.int64)
+            buf[T + i:T + i + m] = p
+            buf[2 * T + i:2 * T + i + m] = table[p // bs] * bs + p % bs
+        buf[3 * T:3 * T + n] = cu[1:] - 1
+        buf[3 * T + n:3 * T + 2 * n + 1] = cu
+        buf[3 * T + 2 * n + 1:] = [c.row_id for c in caches]
+        d = torch.from_numpy(buf).to(dev)
+        small = d[3 * T + n:].to(torch.int32)
+        rows = d[3 * T:3 * T + n] if want_logits else d[3 * T:3 * T + 1]
+        logits = self.model.chunk_logits(d[:T], small[:n + 1], max(lens), small[n + 1:],
+                                         d[T:2 * T], d[2 * T:3 * T], self.pool, rows)
+        toks = argmax(logits).cpu().tolist() if want_logits else None
+        for c, m in zip(caches, lens):
+            c.seq_len += m
+        set_seq_lens_bulk(caches)
+        return toks
+
+    @torch.no_grad()
+    def cache_prefix(self, tokens: list) -> PagedKVCache:
+        """Computes the K/V of tokens that several requests begin with; pass the handle
+        as their `prefix` and free() it when no request needs it any more (what running
+        requests still share stays)."""
+        c = PagedKVCache(self.pool)
+        step = self.prefill_chunk or max(len(tokens), 1)
+        for i in range(0, len(tokens), step):
+            self._run_chunk([c], [tokens[i:i + step]], False)
+        return c
+
+    def _prefill_pieces(self, reqs) -> None:
+        """Prefill behind prefixes and in pieces."""
+        behind = [r for r in reqs if r.prefix is not None]
+        for r, c in zip(behind, fork_caches([r.prefix for r in behind])):
+            r.cache = c
+        for r in reqs:
+            if r.prefix is None:
+                r.cache = PagedKVCache(self.pool)
+        step = self.prefill_chunk or max(len(r.prompt) for r in reqs)
+        done = {id(r): 0 for r in reqs}
+        left = list(reqs)
+        while left:
+            toks = self._run_chunk([r.cache for r in left],
+                                   [r.prompt[done[id(r)]:done[id(r)] + step] for r in left], True)
+            for r, tok in zip(left, toks):
+                done[id(r)] += step
+                if done[id(r)] >= len(r.prompt):
+                    self._take(r, int(tok))
+            left = [r for r in left if done[id(r)] < len(r.prompt)]
+
     def _prefill(self, reqs) -> None:
+        if any(r.prefix is not None or len(r.prompt) > (self.prefill_chunk or len(r.prompt))
+               for r in reqs):
+            return self._prefill_pieces(reqs)
         dev = self.device
         lens = [len(r.prompt) for r in reqs]
         for r in reqs:

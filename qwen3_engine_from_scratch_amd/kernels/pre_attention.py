@@ -14,16 +14,24 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
+from .rotary import rotary_frequencies
 
 __all__ = ["qk_norm_rope_decode", "qk_norm_rope_prefill", "rope_tables"]
 
 
-def rope_tables(head_dim: int, base: float = 1e6, max_seq_len: int = 4096, device=None):
+def rope_tables(head_dim: int, base: float = 1e6, max_seq_len: int = 4096, device=None,
+                scaling: dict | None = None):
     """The model's fp32 cos/sin tables (max_seq_len, head_dim), as
     RotaryEmbedding builds them (qwen3/rope.py:42-58): inverse frequencies
     base^(-2i/head_dim), their outer product with the positions, repeated
     for both halves.  Computed on the CPU (like the reference's buffers) and
-    moved to `device`."""
+    moved to `device`.  scaling: a rope_scaling dict (rotary_frequencies); its angles are
+    formed in 64 bits, its factor goes into the tables."""
+    if scaling is not None and scaling.get("rope_type", scaling.get("type")) != "default":
+        freq, gain = rotary_frequencies(head_dim, base, scaling, seq_len=max_seq_len)
+        angle = torch.outer(torch.arange(max_seq_len, dtype=torch.float64), freq)
+        cos, sin = ((f(angle) * gain).float().repeat(1, 2) for f in (torch.cos, torch.sin))
+        return cos.to(device), sin.to(device)
     inv_freq = 1.0 / (base ** (torch.arange(0, head_dim, 2, dtype=torch.float32,
                                             device="cpu") / head_dim))
     positions = torch.arange(max_seq_len, dtype=torch.float32, device="cpu")

@@ -21,6 +21,8 @@ Entry points:
       capture-friendly decode step (qwen3/model.py:243-251 with :186-217)
   decode_logits / prefill_logits                    the same steps on packed
       device inputs, used by the batching engine and the graph runner.
+  extend / chunk_logits                             new tokens behind what the
+      caches hold already (the reference prefills a prompt whole or decodes).
 """
 from __future__ import annotations
 
@@ -38,7 +40,7 @@ from .kernels.model_ops import (DECODE_LINEAR_MAX_ROWS, add_rms_norm, argmax, de
                                 decode_qkv_rope, embed_rms_norm, embed_ss, lm_head_argmax,
                                 lm_head_argmax_ok, silu_mul)
 from . import _lib
-from .kernels.paged_attention import (paged_attention_decode_hip,
+from .kernels.paged_attention import (paged_attention_chunk_hip, paged_attention_decode_hip,
                                       paged_attention_decode_partials_hip,
                                       paged_decode_workspace_bytes)
 from .kernels.pre_attention import qk_norm_rope_decode, qk_norm_rope_prefill, rope_tables
@@ -62,10 +64,11 @@ class RotaryEmbedding(nn.Module):
     leaves them alone: the kernels round cos/sin to bf16 themselves, as the
     reference's cast to q.dtype does."""
 
-    def __init__(self, head_dim: int, base: float = 1e6, max_seq_len: int = 4096):
+    def __init__(self, head_dim: int, base: float = 1e6, max_seq_len: int = 4096,
+                 scaling: dict | None = None):
         super().__init__()
         self.head_dim, self.base, self.max_seq_len = head_dim, base, max_seq_len
-        self._cpu = rope_tables(head_dim, base, max_seq_len)
+        self._cpu = rope_tables(head_dim, base, max_seq_len, scaling=scaling)
         self._dev = {}
 
     def tables(self, device: torch.device):
@@ -125,7 +128,8 @@ class Qwen3Model(nn.Module):
             [Qwen3DecoderLayer(config, i) for i in range(config.num_hidden_layers)])
         self.norm = RMSNorm(config.hidden_size, config.rms_norm_eps)
         self.rotary_emb = RotaryEmbedding(config.head_dim, config.rope_theta,
-                                          max_seq_len=config.max_position_embeddings)
+                                          max_seq_len=config.max_position_embeddings,
+                                          scaling=config.rope_scaling)
 
 
 class Qwen3ForCausalLM(nn.Module):
@@ -380,6 +384,70 @@ class Qwen3ForCausalLM(nn.Module):
             return o.view(T, Hq * D)
 
         return self._run(ids.reshape(-1), attend, logit_rows)
+
+    # ---- chunks behind a cache ---------------------------------------------
+
+    @torch.no_grad()
+    def chunk_logits(self, ids: torch.Tensor, cu_seqlens: torch.Tensor, max_chunk: int,
+                     row_ids: torch.Tensor, positions: torch.Tensor,
+                     slot_mapping: torch.Tensor, pool,
+                     logit_rows: torch.Tensor | None) -> torch.Tensor:
+        """New tokens of n sequences behind what their caches hold: packed ids (T,)
+        int64, cu_seqlens (n+1,) int32, row_ids (n,) int32 rows of the block table,
+        positions (T,) int64 and slot_mapping (T,) int64 of the tokens (from each row's
+        seq_lens on; pages reserved).  A sequence may bring one token (decoding) or
+        many (a piece of its prompt, draft tokens).  Writes their K/V, leaves seq_lens
+        to the caller, returns the logits of the rows in logit_rows (int64; None:
+        every token)."""
+        cfg = self.config
+        cos, sin = self.model.rotary_emb.tables(ids.device)
+        T = ids.numel()
+        kb, vb = pool.k_buffer, pool.v_buffer
+
+        def attend(i, at, qkv):
+            q, k, v = at.split(qkv)
+            qr, _ = qk_norm_rope_prefill(q, k, v, at.q_norm.weight, at.k_norm.weight,
+                                         cfg.rms_norm_eps, cos, sin, positions, slot_mapping,
+                                         kb, vb, i)
+            o = paged_attention_chunk_hip(qr, kb[:, i], vb[:, i], pool.block_table_2d,
+                                          pool.seq_lens, row_ids, cu_seqlens, pool.block_size,
+                                          max_chunk=max_chunk)
+            return o.view(T, -1)
+
+        return self._run(ids.reshape(-1), attend, logit_rows)
+
+    @torch.no_grad()
+    def extend(self, input_ids: torch.Tensor, kv_cache,
+               input_lens: list[int] | None = None) -> torch.Tensor:
+        """forward for tokens that follow what each handle holds (any number of
+        tokens, none included): input_ids (B, S), right-padded, input_lens the new
+        tokens of each row (0: the row's handle is left alone).  Reserves pages, writes
+        K/V, attends over the cached and the new tokens and advances each handle.
+        Returns logits (B, S, V), pad positions zero."""
+        B, S = input_ids.shape
+        dev = input_ids.device
+        caches = list(kv_cache) if isinstance(kv_cache, (list, tuple)) else [kv_cache]
+        assert len(caches) == B, "one kv cache handle per batch row"
+        lens = list(input_lens) if input_lens is not None else [S] * B
+        assert len(lens) == B and all(0 <= n <= S for n in lens)
+        out = torch.zeros(B, S, self.config.vocab_size, dtype=self.lm_head.weight.dtype, device=dev)
+        if sum(lens) == 0:
+            return out
+        pool = caches[0]._pool
+        slots = np.concatenate([c.reserve_slots(n) for c, n in zip(caches, lens)])
+        pos = np.concatenate([np.arange(c.seq_len, c.seq_len + n, dtype=np.int64)
+                              for c, n in zip(caches, lens)])
+        cu = np.zeros(B + 1, dtype=np.int32)
+        cu[1:] = np.cumsum(lens)
+        valid = (torch.arange(S)[None, :] < torch.tensor(lens)[:, None]).to(dev)
+        out[valid] = self.chunk_logits(
+            input_ids[valid], torch.from_numpy(cu).to(dev), max(lens),
+            torch.tensor([c.row_id for c in caches], dtype=torch.int32, device=dev),
+            torch.from_numpy(pos).to(dev), torch.from_numpy(slots).to(dev), pool, None)
+        for c, n in zip(caches, lens):
+            if n:
+                c.advance_seq_len(n)
+        return out
 
     # ---- drop-in forward ---------------------------------------------------
 

@@ -174,3 +174,27 @@ def test_wrappers_refuse():
                                                       kb[:, :, :1], 0)):
         with pytest.raises(AssertionError):
             call()
+
+
+def test_tables_and_config_take_scalings(tmp_path):
+    import json
+
+    from qwen3_engine_from_scratch_amd.config import Qwen3Config
+    from qwen3_engine_from_scratch_amd.kernels.pre_attention import rope_tables
+
+    plain = rope_tables(64, 1e4, 300)
+    for none in (None, {"rope_type": "default"}):
+        for a, b in zip(rope_tables(64, 1e4, 300, scaling=none), plain):
+            assert torch.equal(a, b)
+    cos, sin = rope_tables(128, 1e6, 5000, scaling=YARN)
+    f, m = rotary_frequencies(128, 1e6, YARN)
+    t = 4999 * f
+    assert cos.shape == sin.shape == (5000, 128) and cos.dtype == torch.float32
+    for table, fn in ((cos, torch.cos), (sin, torch.sin)):
+        assert torch.equal(table[4999], (fn(t) * m).float().repeat(2))
+    d = dict(hidden_size=64, num_attention_heads=2, num_key_value_heads=1, head_dim=32,
+             num_hidden_layers=1, vocab_size=10, intermediate_size=64, rms_norm_eps=1e-6,
+             rope_theta=1e4, rope_scaling=YARN)
+    (tmp_path / "config.json").write_text(json.dumps(d))
+    assert Qwen3Config.from_pretrained(str(tmp_path)).rope_scaling is None
+    assert Qwen3Config.from_pretrained(str(tmp_path), use_rope_scaling=True).rope_scaling == YARN
