@@ -7,6 +7,7 @@ call raises, so a test or benchmark can never silently measure something else.
 from __future__ import annotations
 
 import ctypes
+import functools
 from pathlib import Path
 
 import torch
@@ -244,10 +245,15 @@ def strides(t: torch.Tensor, dims) -> ctypes.Array:
     return _stride_array[len(dims)](*[st[d] for d in dims])
 
 
-def outer_strides(t: torch.Tensor) -> ctypes.Array:
-    """The strides of every dimension but the innermost."""
-    st = t.stride()
+@functools.lru_cache(maxsize=4096)
+def _outer_strides(st: tuple) -> ctypes.Array:
     return _stride_array[len(st) - 1](*st[:-1])
+
+
+def outer_strides(t: torch.Tensor) -> ctypes.Array:
+    """The strides of every dimension but the innermost, as an array that is only read
+    (and so kept by its values: making one costs a microsecond)."""
+    return _outer_strides(t.stride())
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
@@ -256,6 +262,9 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def require_hip(*tensors: torch.Tensor) -> torch.device:
     """All tensors must live on one HIP device; returns it."""
+    index = tensors[0].get_device() if tensors[0] is not None else -1
+    if index >= 0 and all(t is None or t.get_device() == index for t in tensors):
+        return tensors[0].device
     dev = None
     for t in tensors:
         if t is None:
