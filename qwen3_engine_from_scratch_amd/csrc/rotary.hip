@@ -12,17 +12,20 @@
 // one turn in 64 bits (at position 2^31 still exact to 2^-22 of a turn and better
 // below), then cos and sin in 32.  Everything else is fp32, rounded once at the end.
 //
-// Bound by HBM: each q, k (and v) element is read once and written once.  A
-// workgroup takes a few tokens, computes their cos and sin once into LDS for all
-// their heads, and moves rows in 16-byte chunks; a lane of the half layout holds
-// both chunks of its pairs, so nothing crosses lanes.
+// Bound by HBM: each q, k (and v) element is read once and written once.  The rows of
+// all tokens are one list of work units, 16-byte chunks or (half layout) the two chunks
+// of eight pairs, so that nothing crosses lanes; a workgroup takes kThreads x
+// units_of units of it, all loaded before the angles of the tokens they belong to are
+// formed, once each, in LDS.  MEASURED
 #include "common.hpp"
 
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxPairs = 256;      // rotary_dim up to 512
-constexpr int kMaxTokens = 16;      // tokens of a workgroup
+// Units a thread has in flight: 64 bytes.
+template <bool kHalf>
+constexpr int units_of() { return kHalf ? 2 : 4; }
 
 enum class Addr { None, Slots, Decode };
 
@@ -53,8 +56,18 @@ struct RotaryArgs {
   const int32_t* row_ids;
   int64_t n_tokens;
   int Hq, Hkv, D, r, bs;
-  int tokens;   // of a workgroup
+  // Work units of a head row: a pair of chunks (half layout) or one chunk of the
+  // rotated part, then one chunk each of what passes through.
+  int rot_units, row_units;
+  int units;           // of a token
+  uint32_t row_magic, unit_magic;  // ceil(2^32 / row_units), ceil(2^32 / units)
+  int span;            // tokens that a workgroup's units belong to, at most
 };
+
+// x / d for the magic ceil(2^32 / d), where x d < 2^32 (d = 1: the magic is 0).
+__device__ __forceinline__ int divide(int x, uint32_t magic) {
+  return magic == 0 ? x : static_cast<int>(__umulhi(static_cast<uint32_t>(x), magic));
+}
 
 // 16 bytes of T as floats and back.
 template <typename T>
@@ -149,89 +162,114 @@ __device__ __forceinline__ Where where(const RotaryArgs& a, int64_t t) {
 
 template <typename T, bool kHalf, Addr A>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
-  extern __shared__ float2 s_cs[];  // [tokens][r / 2]
-  __shared__ Where s_where[kMaxTokens];
+  extern __shared__ float2 s_cs[];  // [span][r / 2], then the tokens' places in the pool
   constexpr int kN = Vec<T>::n;  // elements of a chunk
+  constexpr int kU = units_of<kHalf>();
   const int tid = threadIdx.x;
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tokens;
-  const int nt = static_cast<int>(min(static_cast<int64_t>(a.tokens), a.n_tokens - t0));
   const int pairs = a.r / 2;
-  if (tid < nt) s_where[tid] = where<A>(a, t0 + tid);
+  const int heads = a.Hq + (a.k ? a.Hkv : 0);
+  const int64_t g0 = static_cast<int64_t>(blockIdx.x) * (kThreads * kU);
+  const int64_t t0 = g0 / a.units;  // the first unit's token
+  const int rest = static_cast<int>(g0 - t0 * a.units);
+  const int left = static_cast<int>(min(a.n_tokens - t0, static_cast<int64_t>(a.span)));
+
+  struct Unit {
+    int tok, row, e;   // token (from t0 on), head row (q, then k, then v), first element
+    bool rot;
+    q3::u32x4 x1, x2;  // x2: the half layout's other chunk, e + r / 2
+  };
+  Unit n[kU];
+#pragma unroll
+  for (int b = 0; b < kU; ++b) {
+    const int l = rest + b * kThreads + tid;
+    n[b].tok = divide(l, a.unit_magic);
+    if (n[b].tok >= left) continue;
+    const int i = l - n[b].tok * a.units;
+    n[b].row = divide(i, a.row_magic);
+    const int u = i - n[b].row * a.row_units;
+    n[b].rot = u < a.rot_units;
+    n[b].e = n[b].rot ? u * kN : a.r + (u - a.rot_units) * kN;
+    const int64_t tok = t0 + n[b].tok;
+    const T* src =
+        n[b].row < a.Hq
+            ? reinterpret_cast<const T*>(a.q) + tok * a.q_s0 + n[b].row * a.q_s1
+        : n[b].row < heads
+            ? reinterpret_cast<const T*>(a.k) + tok * a.k_s0 + (n[b].row - a.Hq) * a.k_s1
+            : reinterpret_cast<const T*>(a.v) + tok * a.v_s0 + (n[b].row - heads) * a.v_s1;
+    n[b].x1 = q3::ld16(src + n[b].e);
+    if (kHalf && n[b].rot) n[b].x2 = q3::ld16(src + n[b].e + pairs);
+  }
+
+  int64_t* s_kc = reinterpret_cast<int64_t*>(s_cs + a.span * pairs);  // pool offsets, -1: none
+  int64_t* s_vc = s_kc + a.span;
+  double* s_pos = reinterpret_cast<double*>(s_vc + a.span);
+  for (int i = tid; i < left; i += kThreads) {
+    const Where w = where<A>(a, t0 + i);
+    s_kc[i] = w.kc;
+    s_vc[i] = w.vc;
+    s_pos[i] = static_cast<double>(w.pos);
+  }
   __syncthreads();
-  for (int i = tid; i < nt * pairs; i += kThreads) {
+  for (int i = tid; i < left * pairs; i += kThreads) {
     const int t = i / pairs, p = i - t * pairs;
     constexpr double kInvTwoPi = 0.15915494309189533577;
-    double turn = static_cast<double>(s_where[t].pos) * (a.inv_freq[p] * kInvTwoPi);
+    double turn = s_pos[t] * (a.inv_freq[p] * kInvTwoPi);
     turn -= __builtin_rint(turn);
     float s, c;
     sincospif(2.f * static_cast<float>(turn), &s, &c);
     s_cs[i] = float2{c * a.factor, s * a.factor * a.sign};
   }
   __syncthreads();
-  // Work units of a head row: a pair of chunks (half layout) or one chunk of the
-  // rotated part, then one chunk each of what passes through.
-  const int rot_units = kHalf ? pairs / kN : a.r / kN;
-  const int pass = (a.D - a.r) / kN;
-  const int upr = rot_units + pass;
-  const int heads = a.Hq + (a.k ? a.Hkv : 0);
-  const int rows = A == Addr::None ? heads : heads + a.Hkv;
-  const int per_token = rows * upr;
-  const int vsteps = a.D / kN;  // a v row is copied chunk by chunk
-  for (int i = tid; i < nt * per_token; i += kThreads) {
-    const int t = i / per_token, j = i - t * per_token;
-    const int row = j / upr, u = j - row * upr;
-    const int64_t tok = t0 + t;
-    const Where w = s_where[t];
-    if (A != Addr::None && row >= heads) {  // v: bits into the pool
-      if (w.vc < 0) continue;
-      const int h = row - heads;
-      for (int c = u; c < vsteps; c += upr)
-        q3::st16(a.v_cache + w.vc + h * a.vc[2] + c * kN,
-                 q3::ld16(a.v + tok * a.v_s0 + h * a.v_s1 + c * kN));
-      continue;
-    }
-    const bool is_q = row < a.Hq;
-    const int h = is_q ? row : row - a.Hq;
-    const T* src = is_q ? reinterpret_cast<const T*>(a.q) + tok * a.q_s0 + h * a.q_s1
-                        : reinterpret_cast<const T*>(a.k) + tok * a.k_s0 + h * a.k_s1;
-    T* out = is_q ? reinterpret_cast<T*>(a.q_out) + tok * a.qo_s0 + h * a.qo_s1
-             : a.k_out ? reinterpret_cast<T*>(a.k_out) + tok * a.ko_s0 + h * a.ko_s1 : nullptr;
+
+#pragma unroll
+  for (int b = 0; b < kU; ++b) {
+    const Unit& x = n[b];
+    if (x.tok >= left) continue;
+    const int64_t tok = t0 + x.tok;
+    T* out = nullptr;
     uint16_t* pool = nullptr;
-    if (A != Addr::None && !is_q && w.kc >= 0) pool = a.k_cache + w.kc + h * a.kc[2];
-    auto store = [&](int e, q3::u32x4 x) {
-      if (out) q3::st16(out + e, x);
-      if (A != Addr::None && pool) q3::st16(pool + e, x);
-    };
-    const float2* cs = s_cs + t * pairs;
-    if (u >= rot_units) {
-      const int e = a.r + (u - rot_units) * kN;
-      store(e, q3::ld16(src + e));
-    } else if constexpr (kHalf) {
-      const int e = u * kN;
-      float x1[kN], x2[kN], y1[kN], y2[kN];
-      const q3::u32x4 w1 = q3::ld16(src + e), w2 = q3::ld16(src + e + pairs);
-      Vec<T>::get(w1, x1);
-      Vec<T>::get(w2, x2);
-#pragma unroll
-      for (int n = 0; n < kN; ++n) {
-        const float2 f = cs[e + n];
-        y1[n] = x1[n] * f.x - x2[n] * f.y;
-        y2[n] = x2[n] * f.x + x1[n] * f.y;
-      }
-      store(e, Vec<T>::put(y1));
-      store(e + pairs, Vec<T>::put(y2));
-    } else {
-      const int e = u * kN;
-      float x[kN], y[kN];
-      Vec<T>::get(q3::ld16(src + e), x);
-#pragma unroll
-      for (int n = 0; n < kN / 2; ++n) {
-        const float2 f = cs[e / 2 + n];
-        y[2 * n] = x[2 * n] * f.x - x[2 * n + 1] * f.y;
-        y[2 * n + 1] = x[2 * n + 1] * f.x + x[2 * n] * f.y;
-      }
-      store(e, Vec<T>::put(y));
+    bool rot = x.rot;
+    if (x.row < a.Hq) {
+      out = reinterpret_cast<T*>(a.q_out) + tok * a.qo_s0 + x.row * a.qo_s1;
+    } else if (x.row < heads) {
+      const int h = x.row - a.Hq;
+      if (a.k_out) out = reinterpret_cast<T*>(a.k_out) + tok * a.ko_s0 + h * a.ko_s1;
+      if (A != Addr::None && s_kc[x.tok] >= 0) pool = a.k_cache + s_kc[x.tok] + h * a.kc[2];
+    } else {  // v: bits into the pool
+      rot = false;
+      if (s_vc[x.tok] >= 0) pool = a.v_cache + s_vc[x.tok] + (x.row - heads) * a.vc[2];
     }
+    auto store = [&](int e, q3::u32x4 y) {
+      if (out) q3::st16(out + e, y);
+      if (A != Addr::None && pool) q3::st16(pool + e, y);
+    };
+    q3::u32x4 y1 = x.x1, y2 = x.x2;
+    if (rot) {
+      const float2* cs = s_cs + x.tok * pairs;
+      float x1[kN], o1[kN];
+      Vec<T>::get(x.x1, x1);
+      if constexpr (kHalf) {
+        float x2[kN], o2[kN];
+        Vec<T>::get(x.x2, x2);
+#pragma unroll
+        for (int m = 0; m < kN; ++m) {
+          const float2 f = cs[x.e + m];
+          o1[m] = x1[m] * f.x - x2[m] * f.y;
+          o2[m] = x2[m] * f.x + x1[m] * f.y;
+        }
+        y2 = Vec<T>::put(o2);
+      } else {
+#pragma unroll
+        for (int m = 0; m < kN / 2; ++m) {
+          const float2 f = cs[x.e / 2 + m];
+          o1[2 * m] = x1[2 * m] * f.x - x1[2 * m + 1] * f.y;
+          o1[2 * m + 1] = x1[2 * m + 1] * f.x + x1[2 * m] * f.y;
+        }
+      }
+      y1 = Vec<T>::put(o1);
+    }
+    store(x.e, y1);
+    if (kHalf && x.rot) store(x.e + pairs, y2);
   }
 }
 
@@ -282,10 +320,24 @@ int run(RotaryArgs a, int dtype, int layout, int inverse, int num_layers, void* 
                     n);
   if (a.n_tokens == 0) return QWEN3_OK;
   a.sign = inverse ? -1.f : 1.f;
-  a.tokens = 4;
-  const int64_t blocks = q3::cdiv(a.n_tokens, a.tokens);
-  if (blocks > 0x7fffffff) return q3::fail(QWEN3_EINVAL, "%s: too many tokens", who);
-  const size_t lds = static_cast<size_t>(a.tokens) * (a.r / 2) * sizeof(float2);
+  a.rot_units = layout == 0 ? a.r / 2 / n : a.r / n;
+  a.row_units = a.rot_units + (a.D - a.r) / n;
+  a.units = (a.Hq + (a.k ? a.Hkv : 0) + (A != Addr::None ? a.Hkv : 0)) * a.row_units;
+  const int group = kThreads * (layout == 0 ? units_of<true>() : units_of<false>());
+  // the kernel's divisions: of at most units + group by units, of units by row_units
+  if (static_cast<int64_t>(a.units + group) * a.units >= (int64_t(1) << 32))
+    return q3::fail(QWEN3_EINVAL, "%s: bad sizes", who);
+  auto magic = [](int d) {
+    return d == 1 ? 0u : static_cast<uint32_t>(((uint64_t(1) << 32) + d - 1) / d);
+  };
+  a.row_magic = magic(a.row_units);
+  a.unit_magic = magic(a.units);
+  a.span = (group - 1) / a.units + 2;
+  const int64_t blocks = q3::cdiv(a.n_tokens * a.units, group);
+  if (a.n_tokens > (int64_t(1) << 40) / a.units || blocks > 0x7fffffff)
+    return q3::fail(QWEN3_EINVAL, "%s: too many tokens", who);
+  const size_t lds =
+      static_cast<size_t>(a.span) * (static_cast<size_t>(a.r / 2) * sizeof(float2) + 24);
   q3::clear_error();
   const auto s = static_cast<hipStream_t>(stream);
   const auto g = static_cast<unsigned>(blocks);
