@@ -19,7 +19,7 @@ _c_i32p = ctypes.c_void_p  # device pointers travel as void*
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
-_i32p = ctypes.POINTER(ctypes.c_int32)  # host arrays
+_i32p = ctypes.c_void_p  # host arrays of int32
 
 
 class DecodeChainArgs(ctypes.Structure):

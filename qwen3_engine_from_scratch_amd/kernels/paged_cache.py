@@ -10,8 +10,7 @@ truncate and compact.
 """
 from __future__ import annotations
 
-import ctypes
-import operator
+from array import array
 
 import torch
 
@@ -20,13 +19,19 @@ from .. import _lib
 __all__ = ["copy_pages_hip", "fork_pages_hip", "move_pages_hip"]
 
 
-def _list(values, n: int, what: str):
-    values = list(map(operator.index, values))
-    if len(values) != n:
-        raise ValueError(f"{what} has {len(values)} entries, expected {n}")
-    if n and not -2 ** 31 <= min(values) <= max(values) < 2 ** 31:
-        raise ValueError(f"{what} does not fit 32 bits")
-    return (ctypes.c_int32 * n)(*values)
+def _list(values, n: int, what: str) -> array:
+    """A host list as 32-bit integers."""
+    try:
+        a = array("i", values)
+    except OverflowError:
+        raise ValueError(f"{what} does not fit 32 bits") from None
+    if len(a) != n:
+        raise ValueError(f"{what} has {len(a)} entries, expected {n}")
+    return a
+
+
+def _at(a: array) -> int:
+    return a.buffer_info()[0]
 
 
 def _pool(k_buffer, v_buffer):
@@ -56,7 +61,8 @@ def copy_pages_hip(k_buffer: torch.Tensor, v_buffer: torch.Tensor, src, dst, tok
     t = None if tokens is None else _list(tokens, n, "tokens")
     dev = _lib.require_hip(k_buffer, v_buffer)
     with _lib.on_device(dev):
-        rc = _lib.load().qwen3_page_copy_bf16(*pool, s, d, t, n, _lib.stream_of(dev))
+        rc = _lib.load().qwen3_page_copy_bf16(
+            *pool, _at(s), _at(d), None if t is None else _at(t), n, _lib.stream_of(dev))
     _lib.check(rc, "qwen3_page_copy_bf16")
 
 
@@ -76,8 +82,8 @@ def fork_pages_hip(k_buffer: torch.Tensor, v_buffer: torch.Tensor, block_table_2
              _list(tokens, n, "tokens"), _list(new_blocks, n, "new_blocks"))
     dev = _lib.require_hip(k_buffer, v_buffer, block_table_2d, seq_lens)
     with _lib.on_device(dev):
-        rc = _lib.load().qwen3_page_fork_bf16(*pool, *table, seq_lens.data_ptr(), *lists, n,
-                                              _lib.stream_of(dev))
+        rc = _lib.load().qwen3_page_fork_bf16(*pool, *table, seq_lens.data_ptr(),
+                                              *map(_at, lists), n, _lib.stream_of(dev))
     _lib.check(rc, "qwen3_page_fork_bf16")
 
 
@@ -91,5 +97,6 @@ def move_pages_hip(k_buffer: torch.Tensor, v_buffer: torch.Tensor, block_table_2
     s, d = _list(src, n, "src"), _list(dst, n, "dst")
     dev = _lib.require_hip(k_buffer, v_buffer, block_table_2d)
     with _lib.on_device(dev):
-        rc = _lib.load().qwen3_page_move_bf16(*pool, *table, s, d, n, _lib.stream_of(dev))
+        rc = _lib.load().qwen3_page_move_bf16(*pool, *table, _at(s), _at(d), n,
+                                              _lib.stream_of(dev))
     _lib.check(rc, "qwen3_page_move_bf16")
