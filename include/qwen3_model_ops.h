@@ -241,7 +241,7 @@ int qwen3_page_in_bf16(int32_t* block_table, int64_t bt_row_stride, int64_t max_
  * entries, read before the call returns; the plan travels in the launch (several
  * launches above 240 entries).  Refused before anything is launched: an id outside
  * the pool or the table, a destination named twice, one that is also a source (the
- * copies of a call run at the same time). */
+ * copies of a call run at the same time).  Blocks of up to 2^31 elements. */
 
 /* Block dst[i] becomes a copy of block src[i], K and V, all layers: of its first
  * tokens[i] slots, the others zero (NULL: of all slots). */
@@ -254,7 +254,7 @@ int qwen3_page_copy_bf16(void* k_cache, void* v_cache, int64_t block_elems, int 
  * becomes a copy of its first slots (the others zero) and takes its place.  The
  * row's other entries become -1, seq_lens[dst_rows[i]] = tokens[i].  new_blocks[i]
  * is not read where the tokens fill whole pages.  A last page whose entry is no
- * block of the pool is not copied. */
+ * block of the pool is not copied.  A new block must be one that no row names. */
 int qwen3_page_fork_bf16(void* k_cache, void* v_cache, int64_t block_elems, int slot_elems,
                          int block_size, int64_t num_blocks, int32_t* block_table,
                          int64_t bt_row_stride, int64_t max_rows, int64_t max_pages,

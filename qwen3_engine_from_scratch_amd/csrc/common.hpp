@@ -133,6 +133,9 @@ __host__ __device__ __forceinline__ int64_t cdiv(int64_t a, int64_t b) {
   return (a + b - 1) / b;
 }
 
+// Threads of one launch along a dimension: a grid's size is 32 bits, in threads.
+constexpr int64_t kMaxThreads = 0xffffffff;
+
 inline bool aligned16(const void* p) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
 }

@@ -147,7 +147,7 @@ int check_pool(Pool& p, void* k_cache, void* v_cache, int64_t block_elems, int s
     return q3::fail(QWEN3_EINVAL, "%s: bad sizes", who);
   if (slot_elems % 8 != 0 || !q3::aligned16(k_cache) || !q3::aligned16(v_cache))
     return q3::fail(QWEN3_EALIGN, "%s: slots must be whole 16-byte chunks", who);
-  if (block_elems > (int64_t(1) << 34))
+  if (block_elems > (int64_t(1) << 31))
     return q3::fail(QWEN3_EUNSUPPORTED, "%s: blocks of %lld elements", who, (long long)block_elems);
   p.k = static_cast<uint16_t*>(k_cache);
   p.v = static_cast<uint16_t*>(v_cache);
@@ -165,10 +165,12 @@ struct Plan {
 
 int check_plan(Plan& plan, const int32_t* src, const int32_t* dst, int n, int64_t num_blocks,
                bool src_once, const char* who) {
+  if (n > num_blocks)
+    return q3::fail(QWEN3_EINVAL, "%s: %d destinations among %lld", who, n, (long long)num_blocks);
   for (int i = 0; i < n; ++i)
     if (src[i] < 0 || src[i] >= num_blocks || dst[i] < 0 || dst[i] >= num_blocks)
-      return q3::fail(QWEN3_EINVAL, "%s: copy %d (%d -> %d) outside the pool's %lld blocks", who, i,
-                      src[i], dst[i], (long long)num_blocks);
+      return q3::fail(QWEN3_EINVAL, "%s: entry %d (%d -> %d) outside 0 .. %lld", who, i,
+                      src[i], dst[i], (long long)num_blocks - 1);
   std::unique_ptr<int64_t[]> pairs(new (std::nothrow) int64_t[n]);
   plan.src.reset(new (std::nothrow) int32_t[n]);
   plan.dst.reset(new (std::nothrow) int32_t[n]);
@@ -177,17 +179,17 @@ int check_plan(Plan& plan, const int32_t* src, const int32_t* dst, int n, int64_
   std::sort(plan.dst.get(), plan.dst.get() + n);
   for (int i = 1; i < n; ++i)
     if (plan.dst[i] == plan.dst[i - 1])
-      return q3::fail(QWEN3_EINVAL, "%s: block %d is written twice", who, plan.dst[i]);
+      return q3::fail(QWEN3_EINVAL, "%s: %d is written twice", who, plan.dst[i]);
   for (int i = 0; i < n; ++i)
     if (std::binary_search(plan.dst.get(), plan.dst.get() + n, src[i]))
-      return q3::fail(QWEN3_EINVAL, "%s: block %d is read and written", who, src[i]);
+      return q3::fail(QWEN3_EINVAL, "%s: %d is read and written", who, src[i]);
   for (int i = 0; i < n; ++i) pairs[i] = (static_cast<int64_t>(src[i]) << 32) | dst[i];
   std::sort(pairs.get(), pairs.get() + n);
   for (int i = 0; i < n; ++i) {
     plan.src[i] = static_cast<int32_t>(pairs[i] >> 32);
     plan.dst[i] = static_cast<int32_t>(pairs[i] & 0xffffffff);
     if (src_once && i > 0 && plan.src[i] == plan.src[i - 1])
-      return q3::fail(QWEN3_EINVAL, "%s: block %d moves twice", who, plan.src[i]);
+      return q3::fail(QWEN3_EINVAL, "%s: %d moves twice", who, plan.src[i]);
   }
   return QWEN3_OK;
 }
@@ -320,7 +322,7 @@ extern "C" int qwen3_page_move_bf16(void* k_cache, void* v_cache, int64_t block_
   const int64_t pieces = q3::cdiv(p.block_chunks, kPiece);
   const int64_t scans = q3::cdiv(max_rows * max_pages, kThreads);
   const int64_t most = scans + 2 * pieces * std::min(n, kMaxJobs);
-  if (most > 0x7fffffff) return q3::fail(QWEN3_EINVAL, "%s: table or blocks too large", who);
+  if (most > q3::kMaxThreads / kThreads) return q3::fail(QWEN3_EINVAL, "%s: table or blocks too large", who);
   q3::clear_error();
   for (int at = 0; at < n; at += kMaxJobs) {
     const int m = std::min(kMaxJobs, n - at);

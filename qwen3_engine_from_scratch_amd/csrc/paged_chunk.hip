@@ -67,8 +67,8 @@ struct ChunkArgs {
   int n_mtiles;    // items of the longest chunk of one KV head
   float scale_log2;
   // range schedule
-  float* po;       // [2 ranges][kRows][kD] partial outputs, not normalised
-  float2* pml;     // [2 ranges][kRows] their running maximum (log2 domain) and sum
+  float* po;       // [2 ranges][rows][kD] partial outputs, not normalised, 32 rows mixed
+  float2* pml;     // [2 ranges][rows] their running maximum (log2 domain) and sum
   CutItem* cuts;   // [ranges]
 };
 
@@ -166,12 +166,12 @@ __device__ __forceinline__ void group_at(const ChunkArgs& a, int64_t row, int gr
 __device__ __forceinline__ void window_check(PageWindow& w, const ChunkArgs& a) {
   w.ok = __ballot(w.page >= 0 && w.page < a.num_blocks);
 }
+// (window_check before its first use: the loads may be on their way until then.)
 __device__ __forceinline__ void window_start(PageWindow& w, const ChunkArgs& a, int64_t row,
                                              int tile, int lane) {
   w.base = tile * (kBN / kGroup);
   group_at(a, row, w.base + lane, w.page, w.sub);
   group_at(a, row, w.base + 64 + lane, w.next_page, w.next_sub);
-  window_check(w, a);
 }
 // Moves on once `tile` lies behind the window (tiles come in order).
 __device__ __forceinline__ void window_to(PageWindow& w, const ChunkArgs& a, int64_t row, int tile,
@@ -353,13 +353,13 @@ __device__ __forceinline__ void tile_fold(const Off& off, float c, const Mask& m
   l_run += (psum[0] + psum[1]) + (psum[2] + psum[3]);
 }
 
-// Key tiles [t0, t1) of an item folded into a fresh state.  Every thread of the
-// workgroup calls it; the tile buffers are free when it returns.
+// Key tiles [t0, t1) of an item folded into a fresh state; pw: window_start of t0.  Every
+// thread of the workgroup calls it; the tile buffers are free when it returns.
 template <int W>
 __device__ __forceinline__ void run_tiles(const ChunkArgs& a, const LaneOffsets& off, const Seq& s,
                                           const WaveRows& w, int kvh, int t0, int t1,
-                                          const TileBufs& tb, int lane, int wave, float& m_run,
-                                          float& l_run, q3::f32x16 (&acc)[4]) {
+                                          PageWindow pw, const TileBufs& tb, int lane, int wave,
+                                          float& m_run, float& l_run, q3::f32x16 (&acc)[4]) {
   m_run = q3::kNegInf;
   l_run = 0.f;
 #pragma unroll
@@ -367,8 +367,7 @@ __device__ __forceinline__ void run_tiles(const ChunkArgs& a, const LaneOffsets&
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[db][r] = 0.f;
   if (t0 >= t1) return;
-  PageWindow pw;
-  window_start(pw, a, s.row, t0, lane);
+  window_check(pw, a);
   const ItemKeys ks{a.k + kvh * a.k_sh, a.v + kvh * a.v_sh, s.row, s.cap};
   uint32_t ok = tile_dma<W>(a, off, pw, ks, t0, tb.k0, tb.v0, wave, lane);
   q3::bf16x8 qv[8];
@@ -469,7 +468,9 @@ void paged_chunk_flat_kernel(ChunkArgs a) {
   const int tiles = (keys_of(a, s, (mt + 1) * rows_of<W>()) + kBN - 1) / kBN;
   float m_run, l_run;
   q3::f32x16 acc[4];
-  run_tiles<W>(a, off, s, w, kvh, 0, tiles, tb, lane, wave, m_run, l_run, acc);
+  PageWindow pw;
+  window_start(pw, a, s.row, 0, lane);
+  run_tiles<W>(a, off, s, w, kvh, 0, tiles, pw, tb, lane, wave, m_run, l_run, acc);
   l_run = cross_half_sum(l_run);
   if (w.active) store_output(a, s, w, kvh, lane, l_run, acc, stage_of(tb, wave));
 }
@@ -482,13 +483,20 @@ void paged_chunk_flat_kernel(ChunkArgs a) {
 // tile belongs to the range that holds its midpoint.  An item cut by a border leaves
 // a partial state per part, which a second launch joins, a wave per row: with up to
 // 64 parts to a row, joining inside one workgroup would take as long as the tiles.
-constexpr int kUnits = 16;
+constexpr int kUnits = 16;          // a tile with more than four waves' rows, or of W = 4
+constexpr int kFewUnits = 12;       // a tile of W = 8 that no SIMD computes two waves of
 constexpr int kItemUnits = 40;
 constexpr int kMinRangeTiles = 4;
 constexpr int kWholeSlack = 20;     // an uncut item: one part in 20, and six tiles, above
 constexpr int kWholeUnits = 96;     // an equal share
 constexpr int kMaxSeqs = 256;       // sequences and (sequence, row tile) pairs
 constexpr int kMaxEntries = 1024;   // tabulated in LDS
+
+// A key tile's weight in an item of `rows` packed rows.
+template <int W>
+__device__ __forceinline__ int tile_units(int rows) {
+  return W == 8 && rows <= rows_of<4>() ? kFewUnits : kUnits;
+}
 
 // Exclusive prefix sum of v[0 .. n) in LDS, in place, n <= kMaxEntries; returns the
 // total.  Every thread of the workgroup calls it.
@@ -574,8 +582,9 @@ void paged_chunk_range_kernel(ChunkArgs a) {
   for (int e = tid; e < E; e += W * 64) {
     const int b = last_at_most(s_first, a.B, e);
     const Seq s = seq_of(a, s_seq[b]);
-    const int tiles = (keys_of(a, s, (e - s_first[b] + 1) * rows_of<W>()) + kBN - 1) / kBN;
-    s_pos[e] = static_cast<int64_t>(kUnits) * tiles + kItemUnits;
+    const int mt = e - s_first[b];
+    const int tiles = (keys_of(a, s, (mt + 1) * rows_of<W>()) + kBN - 1) / kBN;
+    s_pos[e] = static_cast<int64_t>(tile_units<W>(s.n * a.G - mt * rows_of<W>())) * tiles + kItemUnits;
     atomicMax(&s_most, tiles);
   }
   __syncthreads();
@@ -605,23 +614,30 @@ void paged_chunk_range_kernel(ChunkArgs a) {
     const LaneOffsets off = lane_offsets<W>(a, lane, wave);
     int kvh = static_cast<int>(quotient(p_lo, H));
     int e = __builtin_amdgcn_readfirstlane(last_at_most(s_pos, E, p_lo - kvh * H));
-    while (true) {
-      const int64_t P = kvh * H + uniform64(s_pos[e]);  // the item's position
-      if (P >= p_hi) break;
-      const int b = __builtin_amdgcn_readfirstlane(last_at_most(s_first, a.B, e));
-      const int mt = e - __builtin_amdgcn_readfirstlane(s_first[b]);
+    auto item_at = [&](int entry, int& mt) {  // its sequence and row tile
+      const int b = __builtin_amdgcn_readfirstlane(last_at_most(s_first, a.B, entry));
+      mt = entry - __builtin_amdgcn_readfirstlane(s_first[b]);
       SeqEntry se = s_seq[b];
       se.q0 = __builtin_amdgcn_readfirstlane(se.q0);
       se.n = __builtin_amdgcn_readfirstlane(se.n);
       se.row = __builtin_amdgcn_readfirstlane(se.row);
       se.ctx = __builtin_amdgcn_readfirstlane(se.ctx);
-      const Seq s = seq_of(a, se);
+      return seq_of(a, se);
+    };
+    int mt;
+    Seq s = item_at(e, mt);
+    PageWindow ahead;
+    bool have = false;  // `ahead` is this item's first window
+    while (true) {
+      const int64_t P = kvh * H + uniform64(s_pos[e]);  // the item's position
+      if (P >= p_hi) break;
+      const int units = tile_units<W>(s.n * a.G - mt * rows_of<W>());
       const int tiles = (keys_of(a, s, (mt + 1) * rows_of<W>()) + kBN - 1) / kBN;
-      // tile j's midpoint: P + kItemUnits + kUnits j + kUnits / 2; an item without
-      // tiles belongs to the range that holds its position
-      const int64_t base = P + kItemUnits + kUnits / 2;
+      // tile j's midpoint: P + kItemUnits + units j + units / 2; an item without tiles
+      // belongs to the range that holds its position
+      const int64_t base = P + kItemUnits + units / 2;
       auto first_at = [&](int64_t p) {
-        const int64_t j = p <= base ? 0 : (p - base + kUnits - 1) / kUnits;
+        const int64_t j = p <= base ? 0 : quotient(p - base + units - 1, units);
         return static_cast<int>(j < tiles ? j : tiles);
       };
       const int j0 = first_at(p_lo), j1 = first_at(p_hi);
@@ -629,26 +645,31 @@ void paged_chunk_range_kernel(ChunkArgs a) {
         const WaveRows wr = wave_rows<W>(a, s, mt, wave, lane);
         float m_run, l_run;
         q3::f32x16 acc[4];
-        run_tiles<W>(a, off, s, wr, kvh, j0, j1, tb, lane, wave, m_run, l_run, acc);
+        PageWindow pw = ahead;
+        if (!have) window_start(pw, a, s.row, j0, lane);
+        // the next item's first window, on its way while this one's tiles run
+        int next_mt;
+        const int64_t next_row = item_at(e + 1 == E ? 0 : e + 1, next_mt).row;
+        window_start(ahead, a, next_row, 0, lane);
+        have = true;
+        run_tiles<W>(a, off, s, wr, kvh, j0, j1, pw, tb, lane, wave, m_run, l_run, acc);
         l_run = cross_half_sum(l_run);
         if (j0 == 0 && j1 == tiles) {
           if (wr.active) store_output(a, s, wr, kvh, lane, l_run, acc, stage_of(tb, wave));
         } else {
           const int slot = j0 == 0 ? 2 * v + 1 : 2 * v;
           if (wr.active) {
-            const int64_t row = static_cast<int64_t>(slot) * rows_of<W>() + wave * 32 + (lane & 31);
-            float* po = a.po + row * kD + 4 * (lane >> 5);
+            // [wave][16 chunks of 8 elements][2 halves][32 rows][4]: every store whole lines
+            const int64_t row = static_cast<int64_t>(slot) * rows_of<W>() + wave * 32;
+            q3::f32x4* po = reinterpret_cast<q3::f32x4*>(a.po + row * kD) + lane;
 #pragma unroll
-            for (int db = 0; db < 4; ++db)
-#pragma unroll
-              for (int r4 = 0; r4 < 4; ++r4)
-                *reinterpret_cast<q3::f32x4*>(po + 32 * db + 8 * r4) =
-                    q3::f32x4{acc[db][4 * r4], acc[db][4 * r4 + 1], acc[db][4 * r4 + 2],
-                              acc[db][4 * r4 + 3]};
-            if (lane < 32) a.pml[row] = float2{m_run, l_run};
+            for (int i = 0; i < 16; ++i)
+              po[64 * i] = q3::f32x4{acc[i >> 2][4 * (i & 3)], acc[i >> 2][4 * (i & 3) + 1],
+                                     acc[i >> 2][4 * (i & 3) + 2], acc[i >> 2][4 * (i & 3) + 3]};
+            if (lane < 32) a.pml[row + lane] = float2{m_run, l_run};
           }
           if (j0 == 0) {
-            const int64_t last = base + static_cast<int64_t>(kUnits) * (tiles - 1);
+            const int64_t last = base + static_cast<int64_t>(units) * (tiles - 1);
             cut.parts = static_cast<int32_t>(quotient(last, width)) - v + 1;
             cut.r0 = mt * rows_of<W>();
             cut.rows = min(rows_of<W>(), s.n * a.G - cut.r0);
@@ -662,17 +683,18 @@ void paged_chunk_range_kernel(ChunkArgs a) {
         e = 0;
         if (++kvh == a.Hkv) break;
       }
+      s = item_at(e, mt);
     }
   }
   if (tid == 0) a.cuts[v] = cut;
 }
 
-// Joins the parts of the cut items: 16 lanes per row, eight elements each, the loads of
-// up to eight parts in flight at once.  A task is 16 rows of an item of up to three
-// parts (a wave takes four of them), or four rows of one with more, whose parts the
-// four waves share.  The workgroups deal the tasks among themselves from the list of
-// cut items: a workgroup for each possible task (ranges x rows) costs more in
-// workgroups that find nothing to do than the joins take.
+// Joins the parts of the cut items: a lane takes eight elements of a row, the loads of
+// up to eight parts in flight at once.  A task is 32 rows of an item of up to three parts
+// (a wave takes a quarter of their elements), or 32 rows by a quarter of the elements of
+// one with more, whose parts the four waves share.  The workgroups deal the tasks among
+// themselves from the list of cut items: a workgroup for each possible task (ranges x
+// rows) costs more in workgroups that find nothing to do than the joins take.
 constexpr int kJoinParts = 8;
 constexpr int kJoinWaves = 4;
 constexpr int kJoinFew = 3;
@@ -691,12 +713,13 @@ __device__ __forceinline__ void join_parts(const ChunkArgs& a, Joined& j, int sl
   q3::f32x4 x[K][2];
 #pragma unroll
   for (int u = 0; u < K; ++u) {
-    const int64_t at =
-        static_cast<int64_t>(u == 0 || u >= n ? slot0 : slot + 2 * u) * rows_of<W>() + row;
-    ml[u] = a.pml[at];
-    const q3::f32x4* src = reinterpret_cast<const q3::f32x4*>(a.po + at * kD + e);
+    const int64_t first =
+        static_cast<int64_t>(u == 0 || u >= n ? slot0 : slot + 2 * u) * rows_of<W>() + (row & ~31);
+    ml[u] = a.pml[first + (row & 31)];
+    // elements e .. e + 3 of 32 rows, then e + 4 .. e + 7 of them
+    const q3::f32x4* src = reinterpret_cast<const q3::f32x4*>(a.po + first * kD) + 8 * e + (row & 31);
     x[u][0] = src[0];
-    x[u][1] = src[1];
+    x[u][1] = src[32];
   }
   __builtin_amdgcn_sched_barrier(0);  // every load is issued before the first is waited for
   float m = j.m;
@@ -739,47 +762,55 @@ __global__ __launch_bounds__(kJoinWaves * 64) void paged_chunk_join_kernel(Chunk
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   for (int v = tid; v < ranges; v += kJoinWaves * 64) {
     const CutItem c = a.cuts[v];
-    const int per = c.parts <= kJoinFew ? 4 * kJoinWaves : 4;
-    s_task[v] = c.parts > 0 ? (c.rows + per - 1) / per : 0;
+    const int blocks = (c.rows + 31) / 32;
+    s_task[v] = c.parts == 0 ? 0 : c.parts <= kJoinFew ? blocks : 4 * blocks;
   }
   __syncthreads();
   const int tasks = block_scan<kJoinWaves, int>(s_task, ranges, s_wsum);
-  const int e = 8 * (lane & 15);
   for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
     const int v = __builtin_amdgcn_readfirstlane(last_at_most(s_task, ranges, task));
     const CutItem c = a.cuts[v];
     const int k = task - s_task[v];
-    Joined j{q3::kNegInf, 0.f, {}};
     if (c.parts <= kJoinFew) {
-      const int row = 4 * (kJoinWaves * k + wave) + (lane >> 4);
+      const int row = 32 * k + (lane & 31);
       if (row >= c.rows) continue;
-      join_parts<kJoinFew, W>(a, j, 2 * v + 1, 2 * v, c.parts, row, e);
-      store_joined(a, c, j, row, e);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int e = 32 * wave + 16 * i + 8 * (lane >> 5);
+        Joined j{q3::kNegInf, 0.f, {}};
+        join_parts<kJoinFew, W>(a, j, 2 * v + 1, 2 * v, c.parts, row, e);
+        store_joined(a, c, j, row, e);
+      }
       continue;
     }
-    const int row = 4 * k + (lane >> 4);
+    const int row = 32 * (k >> 2) + (lane & 31);
     const int each = (c.parts + kJoinWaves - 1) / kJoinWaves;
     const int p1 = min(c.parts, (wave + 1) * each);
-    if (row < c.rows)
-      for (int p = wave * each; p < p1; p += kJoinParts)
-        join_parts<kJoinParts, W>(a, j, p == 0 ? 2 * v + 1 : 2 * (v + p), 2 * (v + p), p1 - p, row,
-                                  e);
-    if (wave > 0) s_j[wave - 1][lane] = j;
-    __syncthreads();
-    if (wave == 0 && row < c.rows) {
 #pragma unroll
-      for (int s = 0; s < kJoinWaves - 1; ++s) {
-        const Joined& x = s_j[s][lane];
-        const float m = fmaxf(j.m, x.m), use = m == q3::kNegInf ? 0.f : m;
-        const float f = q3::fast_exp2(j.m - use), g = q3::fast_exp2(x.m - use);
-        j.m = m;
-        j.l = j.l * f + x.l * g;
+    for (int i = 0; i < 2; ++i) {
+      const int e = 32 * (k & 3) + 16 * i + 8 * (lane >> 5);
+      Joined j{q3::kNegInf, 0.f, {}};
+      if (row < c.rows)
+        for (int p = wave * each; p < p1; p += kJoinParts)
+          join_parts<kJoinParts, W>(a, j, p == 0 ? 2 * v + 1 : 2 * (v + p), 2 * (v + p), p1 - p, row,
+                                    e);
+      if (wave > 0) s_j[wave - 1][lane] = j;
+      __syncthreads();
+      if (wave == 0 && row < c.rows) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) j.o[i] = j.o[i] * f + x.o[i] * g;
+        for (int s = 0; s < kJoinWaves - 1; ++s) {
+          const Joined& x = s_j[s][lane];
+          const float m = fmaxf(j.m, x.m), use = m == q3::kNegInf ? 0.f : m;
+          const float f = q3::fast_exp2(j.m - use), g = q3::fast_exp2(x.m - use);
+          j.m = m;
+          j.l = j.l * f + x.l * g;
+#pragma unroll
+          for (int o = 0; o < 8; ++o) j.o[o] = j.o[o] * f + x.o[o] * g;
+        }
+        store_joined(a, c, j, row, e);
       }
-      store_joined(a, c, j, row, e);
+      __syncthreads();  // s_j is read before it is written again
     }
-    __syncthreads();  // s_j is read before the next task writes it
   }
 }
 
@@ -863,7 +894,7 @@ int launch_tiles(ChunkArgs a, const Variant& var, int max_chunk, void* workspace
   const int64_t longest = max_chunk < a.total ? max_chunk : a.total;
   a.n_mtiles = static_cast<int>(q3::cdiv(longest * a.G, rows_of<W>()));
   const int64_t items = static_cast<int64_t>(a.Hkv) * a.B * a.n_mtiles;
-  if (items > 0x7fffffff)
+  if (items > q3::kMaxThreads / (W * 64))
     return q3::fail(QWEN3_EINVAL, "%s: grid too large (KV heads %d, batch %d, max_chunk %d)", who,
                     a.Hkv, a.B, max_chunk);
   hipLaunchKernelGGL(paged_chunk_flat_kernel<W>, dim3(static_cast<unsigned>(items)), dim3(W * 64), 0,

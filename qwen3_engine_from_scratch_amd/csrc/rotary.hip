@@ -353,7 +353,7 @@ int run(RotaryArgs a, int dtype, int layout, int inverse, int num_layers, void* 
   a.span = (group - 1) / a.units + 2;
   const bool streams = a.n_tokens * (a.Hq + static_cast<int64_t>(a.Hkv)) * a.D * size > kStreamBytes;
   const int64_t blocks = q3::cdiv(a.n_tokens * a.units, group);
-  if (a.n_tokens > (int64_t(1) << 40) / a.units || blocks > 0x7fffffff)
+  if (a.n_tokens > (int64_t(1) << 40) / a.units || blocks > q3::kMaxThreads / kThreads)
     return q3::fail(QWEN3_EINVAL, "%s: too many tokens", who);
   const size_t lds =
       static_cast<size_t>(a.span) * (static_cast<size_t>(a.r / 2) * sizeof(float2) + 24);

@@ -116,3 +116,8 @@ def test_wrapper_refuses():
                  dict(v=torch.zeros(3, 4, 16, 128, dtype=torch.bfloat16))):
         with pytest.raises(AssertionError):
             call(**over)
+
+
+def test_a_grid_beyond_32_bits_is_refused():
+    assert _call(B=100000, mc=1 << 20, T=1 << 20, rows=100000) == -1
+    assert b"grid too large" in _lib.load().qwen3_attn_last_error()

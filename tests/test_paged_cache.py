@@ -26,7 +26,7 @@ def _copy(src=(1, 2), dst=(3, 4), tokens=None, n=2, k=FAKE, v=FAKE, be=65536, se
     (-1, dict(src=(1, 8))), (-1, dict(src=(-1, 2))), (-1, dict(dst=(3, 8))),
     (-1, dict(dst=(3, -2))), (-1, dict(dst=(3, 3))), (-1, dict(dst=(2, 4))),
     (-1, dict(src=(1, 1), dst=(1, 4))), (-1, dict(tokens=(16, 17))), (-1, dict(tokens=(-1, 3))),
-    (0, dict(n=0)),
+    (0, dict(n=0)), (-1, dict(n=9)), (-3, dict(be=1 << 32)),
 ])
 def test_copy_refuses(code, over):
     assert _copy(**over) == code, _lib.load().qwen3_attn_last_error()

@@ -198,3 +198,8 @@ def test_tables_and_config_take_scalings(tmp_path):
     (tmp_path / "config.json").write_text(json.dumps(d))
     assert Qwen3Config.from_pretrained(str(tmp_path)).rope_scaling is None
     assert Qwen3Config.from_pretrained(str(tmp_path), use_rope_scaling=True).rope_scaling == YARN
+
+
+def test_a_grid_beyond_32_bits_is_refused():
+    assert _rot(T=1 << 33) == -1
+    assert b"too many tokens" in _lib.load().qwen3_attn_last_error()
