@@ -16,10 +16,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxJobs = 240;   // copies of one launch: their plan is a launch argument
-// 16-byte chunks a thread copies.  200 moves of 1.8 MB, cold: 136 us with one, 139 with
-// two, 151 with four, 185 with eight (a plain copy of as many bytes: 137); with cached
-// loads and stores 153 with four: nothing reads a moved page before the caches have
-// turned over.
+// 16-byte chunks a thread copies.  200 moves of 1.8 MB: 130 us with one, 135 with two, 140
+// with four (a plain copy of as many bytes: 137); with cached loads and stores 139, 141
+// and 148: nothing reads a moved page before the caches have turned over.
 constexpr int kUnroll = 1;
 constexpr int kPiece = kThreads * kUnroll;  // chunks of a block that one workgroup copies
 
@@ -37,7 +36,9 @@ struct Pool {
   int block_size;
 };
 
-// One piece of one block of K or of V.
+// One piece of one block of K or of V.  kOnce: no other copy of the call reads the source
+// (forks of one request do: 24 forks of eight, 17.7 us with streaming loads, 10.8 without).
+template <bool kOnce>
 __device__ __forceinline__ void copy_piece(const Pool& p, int64_t piece, int which, int64_t src,
                                            int64_t dst, int tokens) {
   uint16_t* base = which ? p.v : p.k;
@@ -53,7 +54,7 @@ __device__ __forceinline__ void copy_piece(const Pool& p, int64_t piece, int whi
     if (c < p.block_chunks &&
         (whole || static_cast<uint32_t>(c) / p.slot_chunks % p.block_size <
                       static_cast<uint32_t>(tokens)))
-      x[i] = q3::ld16_nt(s + 8 * c);
+      x[i] = kOnce ? q3::ld16_nt(s + 8 * c) : q3::ld16(s + 8 * c);
   }
 #pragma unroll
   for (int i = 0; i < kUnroll; ++i) {
@@ -65,7 +66,7 @@ __device__ __forceinline__ void copy_piece(const Pool& p, int64_t piece, int whi
 
 __global__ __launch_bounds__(kThreads) void page_copy_kernel(Pool p, CopyJobs jobs) {
   const int j = blockIdx.y;
-  copy_piece(p, blockIdx.x, blockIdx.z, jobs.src[j], jobs.dst[j], jobs.tokens[j]);
+  copy_piece<false>(p, blockIdx.x, blockIdx.z, jobs.src[j], jobs.dst[j], jobs.tokens[j]);
 }
 
 // Forks: row dst takes over the entries of row src for the first tokens[j] tokens.
@@ -93,7 +94,7 @@ __global__ __launch_bounds__(kThreads) void page_fork_kernel(Pool p, Table t, Fo
     if (rest == 0) return;
     const int32_t from = t.bt[src * t.stride + full];
     if (from < 0 || from >= t.num_blocks) return;
-    copy_piece(p, blockIdx.x >> 1, blockIdx.x & 1, from, jobs.block[j], rest);
+    copy_piece<false>(p, blockIdx.x >> 1, blockIdx.x & 1, from, jobs.block[j], rest);
     return;
   }
   // the table row, one workgroup
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(kThreads) void page_move_kernel(Pool p, Table t, Mo
     const int64_t i = blockIdx.x - scans;  // (job, K or V, piece)
     const int piece = static_cast<int>(i % pieces);
     const int j = static_cast<int>(i / pieces);
-    copy_piece(p, piece, j & 1, jobs.src[j >> 1], jobs.dst[j >> 1], p.block_size);
+    copy_piece<true>(p, piece, j & 1, jobs.src[j >> 1], jobs.dst[j >> 1], p.block_size);
     return;
   }
   __shared__ int32_t s_src[kMaxJobs], s_dst[kMaxJobs];
