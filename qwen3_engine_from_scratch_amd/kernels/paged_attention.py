@@ -249,7 +249,7 @@ def paged_attention_chunk_hip(q, k_buffer, v_buffer, block_table_2d, seq_lens_fu
     if scale is None:
         scale = 1.0 / math.sqrt(head_dim)
     if out is None:
-        out = torch.empty(q.shape, dtype=bf16, device=dev)
+        out = torch.empty_like(q)
     else:
         assert out.shape == q.shape and out.dtype is bf16 and out.stride(2) == 1, \
             "out must be a bf16 (total_tokens, num_heads, head_dim) tensor with unit last stride"

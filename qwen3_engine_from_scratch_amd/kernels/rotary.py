@@ -133,10 +133,6 @@ def _positions(positions, T):
     return positions.contiguous()
 
 
-def _new(x):
-    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
-
-
 def rotary_embedding_hip(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
                          rotary: Rotary, *, inverse: bool = False,
                          q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
@@ -149,9 +145,9 @@ def rotary_embedding_hip(q: torch.Tensor, k: torch.Tensor | None, positions: tor
     T, Hq, D = q.shape
     positions = _positions(positions, T)
     dev = _lib.require_hip(q, k, positions, rotary.inv_freq, q_out, k_out)
-    q_out = _new(q) if q_out is None else q_out
+    q_out = torch.empty_like(q) if q_out is None else q_out
     if k is not None and k_out is None:
-        k_out = _new(k)
+        k_out = torch.empty_like(k)
     if T == 0:
         return q_out, k_out
     st = _lib.outer_strides
@@ -191,8 +187,8 @@ def rotary_embedding_prefill_hip(q: torch.Tensor, k: torch.Tensor, v: torch.Tens
     slot_mapping = _positions(slot_mapping, T)
     dev = _lib.require_hip(q, k, v, positions, slot_mapping, rotary.inv_freq, k_buffer, v_buffer,
                            q_out, k_out)
-    q_out = _new(q) if q_out is None else q_out
-    k_out = _new(k) if k_out is None else k_out
+    q_out = torch.empty_like(q) if q_out is None else q_out
+    k_out = torch.empty_like(k) if k_out is None else k_out
     if T == 0:
         return q_out, k_out
     st = _lib.outer_strides
@@ -228,7 +224,7 @@ def rotary_embedding_decode_hip(q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
         positions = _positions(positions, B)
     bt = pool.block_table_2d
     dev = _lib.require_hip(q, k, v, rotary.inv_freq, kb, bt, row_ids, positions, q_out)
-    q_out = _new(q) if q_out is None else q_out
+    q_out = torch.empty_like(q) if q_out is None else q_out
     if B == 0:
         return q_out
     st = _lib.outer_strides
