@@ -481,12 +481,15 @@ void paged_chunk_flat_kernel(ChunkArgs a) {
 // end to end, KV head by KV head; they are cut into equal ranges, one per resident
 // workgroup.  Neighbouring ranges run on one XCD, so its L2 serves one KV head.  A
 // tile belongs to the range that holds its midpoint.  An item cut by a border leaves
-// a partial state per part, which a second launch joins, a wave per row: with up to
-// 64 parts to a row, joining inside one workgroup would take as long as the tiles.
+// a partial state per part, which a second launch joins: with up to a part for each
+// workgroup, joining inside one of them would take as long as the tiles.
+// A range is at least kMinRangeTiles long, where few rows meet few keys: 202 tokens
+// behind 53 take 21.1 us with four tiles, 17.7 with two, 17.1 with one, seven sequences
+// of 6 tokens behind 300 keys 19.7, 18.6 and 23.7.
 constexpr int kUnits = 16;          // a tile with more than four waves' rows, or of W = 4
 constexpr int kFewUnits = 12;       // a tile of W = 8 that no SIMD computes two waves of
 constexpr int kItemUnits = 40;
-constexpr int kMinRangeTiles = 4;
+constexpr int kMinRangeTiles = 2;
 constexpr int kWholeSlack = 20;     // an uncut item: one part in 20, and six tiles, above
 constexpr int kWholeUnits = 96;     // an equal share
 constexpr int kMaxSeqs = 256;       // sequences and (sequence, row tile) pairs
@@ -689,15 +692,17 @@ void paged_chunk_range_kernel(ChunkArgs a) {
   if (tid == 0) a.cuts[v] = cut;
 }
 
-// Joins the parts of the cut items: a lane takes eight elements of a row, the loads of
-// up to eight parts in flight at once.  A task is 32 rows of an item of up to three parts
-// (a wave takes a quarter of their elements), or 32 rows by a quarter of the elements of
-// one with more, whose parts the four waves share.  The workgroups deal the tasks among
-// themselves from the list of cut items: a workgroup for each possible task (ranges x
-// rows) costs more in workgroups that find nothing to do than the joins take.
+// Joins the parts of the cut items: a lane takes eight elements of a row.  A task is 32
+// rows of an item of up to six parts by half their elements (a wave takes an eighth, all
+// parts' loads in flight at once), or 32 rows by a quarter of the elements of an item
+// with more parts, which the four waves share.  (Items of four to six parts on the second
+// path: 1,001 tokens behind 650 take 45.5 us instead of 38.9, 509 behind 20,000 take 132
+// instead of 125.)  The workgroups deal the tasks among themselves from the list of cut
+// items: a workgroup for each possible task (ranges x rows) costs more in workgroups that
+// find nothing to do than the joins take.
 constexpr int kJoinParts = 8;
 constexpr int kJoinWaves = 4;
-constexpr int kJoinFew = 3;
+constexpr int kJoinFew = 6;
 
 // A lane's eight elements of a row, joined so far.
 struct Joined {
@@ -763,7 +768,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void paged_chunk_join_kernel(Chunk
   for (int v = tid; v < ranges; v += kJoinWaves * 64) {
     const CutItem c = a.cuts[v];
     const int blocks = (c.rows + 31) / 32;
-    s_task[v] = c.parts == 0 ? 0 : c.parts <= kJoinFew ? blocks : 4 * blocks;
+    s_task[v] = c.parts == 0 ? 0 : c.parts <= kJoinFew ? 2 * blocks : 4 * blocks;
   }
   __syncthreads();
   const int tasks = block_scan<kJoinWaves, int>(s_task, ranges, s_wsum);
@@ -772,15 +777,15 @@ __global__ __launch_bounds__(kJoinWaves * 64) void paged_chunk_join_kernel(Chunk
     const CutItem c = a.cuts[v];
     const int k = task - s_task[v];
     if (c.parts <= kJoinFew) {
-      const int row = 32 * k + (lane & 31);
+      const int row = 32 * (k >> 1) + (lane & 31);
       if (row >= c.rows) continue;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int e = 32 * wave + 16 * i + 8 * (lane >> 5);
-        Joined j{q3::kNegInf, 0.f, {}};
+      const int e = 64 * (k & 1) + 16 * wave + 8 * (lane >> 5);
+      Joined j{q3::kNegInf, 0.f, {}};
+      if (c.parts <= 3)
+        join_parts<3, W>(a, j, 2 * v + 1, 2 * v, c.parts, row, e);
+      else
         join_parts<kJoinFew, W>(a, j, 2 * v + 1, 2 * v, c.parts, row, e);
-        store_joined(a, c, j, row, e);
-      }
+      store_joined(a, c, j, row, e);
       continue;
     }
     const int row = 32 * (k >> 2) + (lane & 31);
