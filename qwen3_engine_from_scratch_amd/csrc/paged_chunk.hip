@@ -448,8 +448,9 @@ __device__ __forceinline__ char* stage_of(const TileBufs& tb, int wave) {
   __shared__ __attribute__((aligned(1024))) uint16_t s_v1[kTileElems]; \
   const TileBufs tb{s_k0, s_v0, s_k1, s_v1}
 
-// One workgroup per item, KV head fastest (neighbouring workgroups go to
-// different XCDs, and an XCD's L2 holds few heads), longest reach first.
+// Batches that no workgroup can tabulate: one workgroup per item, KV head fastest
+// (neighbouring workgroups go to different XCDs, and an XCD's L2 holds few heads), the
+// last row tiles first.
 template <int W>
 __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_chunk_flat_kernel(ChunkArgs a) {
@@ -559,6 +560,35 @@ __device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
   return static_cast<int64_t>(__builtin_floor(static_cast<double>(x) / static_cast<double>(y)));
 }
 
+// Tabulates the batch, its sequences and the row tiles before each; returns the row tiles
+// of all.  Every workgroup waits for this before its first K/V load: one chain of two
+// memory round trips (row_ids, then seq_lens), the rest is in LDS.
+template <int W>
+__device__ __forceinline__ int tabulate(const ChunkArgs& a, int* s_first, SeqEntry* s_seq,
+                                        int* s_wsum) {
+  for (int b = threadIdx.x; b < a.B; b += W * 64) {
+    const Seq s = seq_at(a, b);
+    s_seq[b] = SeqEntry{static_cast<int32_t>(s.q0), s.n, static_cast<int32_t>(s.row), s.ctx};
+    s_first[b] = static_cast<int>((static_cast<int64_t>(s.n) * a.G + rows_of<W>() - 1) / rows_of<W>());
+  }
+  __syncthreads();
+  // (the bound matters only where cu_seqlens is not ascending)
+  return min(kMaxEntries, block_scan<W, int>(s_first, a.B, s_wsum));
+}
+
+// The sequence and row tile of a tabulated (sequence, row tile) pair.
+__device__ __forceinline__ Seq item_at(const ChunkArgs& a, const int* s_first,
+                                       const SeqEntry* s_seq, int entry, int& mt) {
+  const int b = __builtin_amdgcn_readfirstlane(last_at_most(s_first, a.B, entry));
+  mt = entry - __builtin_amdgcn_readfirstlane(s_first[b]);
+  SeqEntry se = s_seq[b];
+  se.q0 = __builtin_amdgcn_readfirstlane(se.q0);
+  se.n = __builtin_amdgcn_readfirstlane(se.n);
+  se.row = __builtin_amdgcn_readfirstlane(se.row);
+  se.ctx = __builtin_amdgcn_readfirstlane(se.ctx);
+  return seq_of(a, se);
+}
+
 template <int W>
 __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_chunk_range_kernel(ChunkArgs a) {
@@ -572,16 +602,7 @@ void paged_chunk_range_kernel(ChunkArgs a) {
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (tid == 0) s_most = 0;
-  // Every workgroup waits for this before its first K/V load: one chain of two
-  // memory round trips (row_ids, then seq_lens), the rest is in LDS.
-  for (int b = tid; b < a.B; b += W * 64) {
-    const Seq s = seq_at(a, b);
-    s_seq[b] = SeqEntry{static_cast<int32_t>(s.q0), s.n, static_cast<int32_t>(s.row), s.ctx};
-    s_first[b] = static_cast<int>((static_cast<int64_t>(s.n) * a.G + rows_of<W>() - 1) / rows_of<W>());
-  }
-  __syncthreads();
-  // (the bound matters only where cu_seqlens is not ascending)
-  const int E = min(kMaxEntries, block_scan<W, int>(s_first, a.B, reinterpret_cast<int*>(s_wsum)));
+  const int E = tabulate<W>(a, s_first, s_seq, reinterpret_cast<int*>(s_wsum));
   for (int e = tid; e < E; e += W * 64) {
     const int b = last_at_most(s_first, a.B, e);
     const Seq s = seq_of(a, s_seq[b]);
@@ -617,18 +638,8 @@ void paged_chunk_range_kernel(ChunkArgs a) {
     const LaneOffsets off = lane_offsets<W>(a, lane, wave);
     int kvh = static_cast<int>(quotient(p_lo, H));
     int e = __builtin_amdgcn_readfirstlane(last_at_most(s_pos, E, p_lo - kvh * H));
-    auto item_at = [&](int entry, int& mt) {  // its sequence and row tile
-      const int b = __builtin_amdgcn_readfirstlane(last_at_most(s_first, a.B, entry));
-      mt = entry - __builtin_amdgcn_readfirstlane(s_first[b]);
-      SeqEntry se = s_seq[b];
-      se.q0 = __builtin_amdgcn_readfirstlane(se.q0);
-      se.n = __builtin_amdgcn_readfirstlane(se.n);
-      se.row = __builtin_amdgcn_readfirstlane(se.row);
-      se.ctx = __builtin_amdgcn_readfirstlane(se.ctx);
-      return seq_of(a, se);
-    };
     int mt;
-    Seq s = item_at(e, mt);
+    Seq s = item_at(a, s_first, s_seq, e, mt);
     PageWindow ahead;
     bool have = false;  // `ahead` is this item's first window
     while (true) {
@@ -652,7 +663,7 @@ void paged_chunk_range_kernel(ChunkArgs a) {
         if (!have) window_start(pw, a, s.row, j0, lane);
         // the next item's first window, on its way while this one's tiles run
         int next_mt;
-        const int64_t next_row = item_at(e + 1 == E ? 0 : e + 1, next_mt).row;
+        const int64_t next_row = item_at(a, s_first, s_seq, e + 1 == E ? 0 : e + 1, next_mt).row;
         window_start(ahead, a, next_row, 0, lane);
         have = true;
         run_tiles<W>(a, off, s, wr, kvh, j0, j1, pw, tb, lane, wave, m_run, l_run, acc);
@@ -686,10 +697,106 @@ void paged_chunk_range_kernel(ChunkArgs a) {
         e = 0;
         if (++kvh == a.Hkv) break;
       }
-      s = item_at(e, mt);
+      s = item_at(a, s_first, s_seq, e, mt);
     }
   }
   if (tid == 0) a.cuts[v] = cut;
+}
+
+// ---------------------------------------------------------------------------
+// Dealt schedule: more items than cutting pays for.  Every workgroup sorts the (sequence,
+// row tile) pairs by their weight, the longest first, and takes one item of each round of
+// as many items as there are workgroups, in the rounds' order to and fro: who had the
+// longest of one round has the shortest of the next.  The sort is by 64 classes of
+// weight, by counting and stable, so every workgroup has the same order.
+template <int W>
+__global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void paged_chunk_deal_kernel(ChunkArgs a) {
+  Q3_CHUNK_TILE_BUFFERS;
+  __shared__ int s_first[kMaxSeqs];  // row tiles before each sequence
+  __shared__ SeqEntry s_seq[kMaxSeqs];
+  __shared__ int s_slot[kMaxEntries];  // [class][64 pairs]: those of the class, then the ones before
+  __shared__ uint16_t s_order[kMaxEntries];
+  __shared__ int s_wsum[W];
+  __shared__ int s_most;               // weight of the longest
+  constexpr int kGroups = kMaxEntries / 64, kPer = kGroups / W;
+  constexpr int kClasses = 64;
+  static_assert(kClasses * kGroups == kMaxEntries, "the counts fill s_slot");
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (tid == 0) s_most = 0;
+  for (int i = tid; i < kMaxEntries; i += W * 64) s_slot[i] = 0;
+  const int E = tabulate<W>(a, s_first, s_seq, s_wsum);
+  int weight[kPer], rank[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = (wave + W * i) * 64 + lane;
+    weight[i] = 0;
+    if (e < E) {
+      const int b = last_at_most(s_first, a.B, e);
+      const Seq s = seq_of(a, s_seq[b]);
+      const int mt = e - s_first[b];
+      const int tiles = (keys_of(a, s, (mt + 1) * rows_of<W>()) + kBN - 1) / kBN;
+      weight[i] = tile_units<W>(s.n * a.G - mt * rows_of<W>()) * tiles + kItemUnits;
+      atomicMax(&s_most, weight[i]);
+    }
+  }
+  __syncthreads();
+  const float per_class = (kClasses - 1) / static_cast<float>(max(s_most, 1));
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = (wave + W * i) * 64 + lane;
+    const int c = kClasses - 1 -
+                  min(kClasses - 1, static_cast<int>(static_cast<float>(weight[i]) * per_class));
+    uint64_t same = __ballot(e < E);
+#pragma unroll
+    for (int bit = 1; bit < kClasses; bit <<= 1) {
+      const uint64_t set = __ballot((c & bit) != 0);
+      same &= (c & bit) != 0 ? set : ~set;
+    }
+    rank[i] = __popcll(same & ((uint64_t{1} << lane) - 1));
+    weight[i] = c * kGroups + wave + W * i;
+    if (e < E && rank[i] == 0) s_slot[weight[i]] = __popcll(same);
+  }
+  __syncthreads();
+  block_scan<W, int>(s_slot, kMaxEntries, s_wsum);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = (wave + W * i) * 64 + lane;
+    if (e < E) s_order[s_slot[weight[i]] + rank[i]] = static_cast<uint16_t>(e);
+  }
+  __syncthreads();
+
+  const LaneOffsets off = lane_offsets<W>(a, lane, wave);
+  const int nwg = gridDim.x, w = blockIdx.x;
+  const int items = E * a.Hkv;
+  // an XCD's neighbours share KV heads where their number allows it, else sequences
+  const int p = a.Hkv % 8 != 0 && nwg % 8 == 0 ? (w % 8) * (nwg / 8) + w / 8 : w;
+  auto item_of = [&](int round) { return round * nwg + ((round & 1) ? nwg - 1 - p : p); };
+  auto entry_of = [&](int item) {
+    return __builtin_amdgcn_readfirstlane(static_cast<int>(s_order[item / a.Hkv]));
+  };
+  PageWindow ahead;
+  for (int round = 0, item = item_of(0); item < items; ++round) {
+    int mt, next_mt;
+    const Seq s = item_at(a, s_first, s_seq, entry_of(item), mt);
+    const int kvh = item % a.Hkv;
+    const WaveRows wr = wave_rows<W>(a, s, mt, wave, lane);
+    const int tiles = (keys_of(a, s, (mt + 1) * rows_of<W>()) + kBN - 1) / kBN;
+    float m_run, l_run;
+    q3::f32x16 acc[4];
+    PageWindow pw = ahead;
+    if (round == 0) window_start(pw, a, s.row, 0, lane);
+    // the next item's first window, on its way while this one's tiles run
+    item = item_of(round + 1);
+    const int next = item < items ? item : item_of(round);
+    window_start(ahead, a, item_at(a, s_first, s_seq, entry_of(next), next_mt).row, 0, lane);
+    run_tiles<W>(a, off, s, wr, kvh, 0, tiles, pw, tb, lane, wave, m_run, l_run, acc);
+    l_run = cross_half_sum(l_run);
+    if (wr.active) store_output(a, s, wr, kvh, lane, l_run, acc, stage_of(tb, wave));
+    __syncthreads();  // the staging buffers are read before the next loads refill them
+  }
 }
 
 // Joins the parts of the cut items: a lane takes eight elements of a row.  A task is 32
@@ -862,20 +969,26 @@ ChunkLayout chunk_layout(int W) {
 //    tile once for twice the rows (2,048 tokens behind 64,000, 32/8 heads: 1.92 ms
 //    against 2.03; eight chunks of 100-500 behind 100-9,000: 313 us against 318; 16
 //    single tokens behind 4,000 in the same kernels: 54 against 51);
-//  - ranges, unless the items are so many that whole ones finish together: at 1.4
-//    items a workgroup 313 us against 431 (eight ragged chunks), at 2 (one prompt of
-//    4,096, whose items pair up heavy with light) 181 against 153.
+//  - ranges for up to 1.75 items a workgroup, dealt items above: one prompt of 4,096 (2.03
+//    items) 141 us dealt, 165 in ranges; eight chunks of about 1,000 (2.2) 71 and 77;
+//    eight of 200-800 behind 1,000-8,000 (2.2) 309 and 300; below it, by how unequal the
+//    items are, twelve turns of 20-700 behind 0-6,000 (1.44) 186 and 165, six chunks
+//    with groups of five heads (1.31) 205 and 218;
+//  - items in order where the batch is too large to be tabulated in LDS.  (Where it is
+//    not, order alone costs: 16 chunks of 200-800 behind 1,000-8,000 825 us, dealt 658;
+//    100 of 30-100 behind 200-2,000 213 and 196; one prompt of 4,096 146 and 141.)
 struct Variant {
   bool stream;
   int waves;
-  bool ranges;
+  bool ranges, dealt;
 };
 Variant variant_of(int B, int max_chunk, int64_t total, int G, int Hkv) {
   const int64_t rows = std::min<int64_t>(max_chunk, total) * G;
-  Variant v{q3::chunk_streams(B, rows), rows > rows_of<4>() ? 8 : 4, false};
+  Variant v{q3::chunk_streams(B, rows), rows > rows_of<4>() ? 8 : 4, false, false};
   const int64_t entries = q3::cdiv(total * G, 32 * v.waves) + B;
-  v.ranges = B <= kMaxSeqs && entries <= kMaxEntries &&
-             4 * entries * Hkv <= 7 * static_cast<int64_t>(range_workgroups(v.waves));
+  const bool listed = B <= kMaxSeqs && entries <= kMaxEntries && Hkv <= (1 << 20);
+  v.ranges = listed && 4 * entries * Hkv <= 7 * static_cast<int64_t>(range_workgroups(v.waves));
+  v.dealt = listed && !v.ranges;
   return v;
 }
 
@@ -894,6 +1007,10 @@ int launch_tiles(ChunkArgs a, const Variant& var, int max_chunk, void* workspace
     if (const int rc = q3::launch_status(who)) return rc;
     hipLaunchKernelGGL(paged_chunk_join_kernel<W>, dim3(4 * (wgs * W / 8)), dim3(kJoinWaves * 64), 0,
                        s, a, wgs);
+    return q3::launch_status(who);
+  }
+  if (var.dealt) {
+    hipLaunchKernelGGL(paged_chunk_deal_kernel<W>, dim3(range_workgroups(W)), dim3(W * 64), 0, s, a);
     return q3::launch_status(who);
   }
   const int64_t longest = max_chunk < a.total ? max_chunk : a.total;

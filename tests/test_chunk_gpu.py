@@ -294,3 +294,69 @@ def test_nothing_to_do(gpu):
     out = torch.full_like(t["q"], 2.0)
     assert (run(t, gpu, out=out) == 2.0).all()
     assert (run(t, gpu, out=out, max_chunk=None) == 2.0).all()
+
+
+def _lengths(seed, B, most, far):
+    """B chunks of up to `most` tokens, two empty, behind contexts of very unequal lengths."""
+    g = torch.Generator().manual_seed(seed)
+    chunks = torch.randint(1, most + 1, (B,), generator=g)
+    chunks[0], chunks[B // 2], chunks[-1] = most, 0, 0
+    ctxs = (torch.rand(B, generator=g) ** 4 * far).int()
+    return chunks.tolist(), ctxs.tolist()
+
+
+@pytest.mark.parametrize("B,most,far,hq,hkv,bs", [
+    (24, 600, 5000, 32, 8, 16),     # eight waves, a few items a workgroup
+    (100, 30, 3000, 32, 8, 16),     # four waves
+    (60, 150, 900, 40, 5, 32),      # KV heads that no round divides by
+    (256, 20, 200, 32, 2, 16),      # two KV heads, as many sequences as are tabulated
+    (90, 200, 1, 16, 2, 16),        # prompts
+    (257, 20, 200, 16, 8, 16),      # one sequence more: items in order
+    (25, 800, 1, 16, 1, 16),        # few sequences of one KV head
+    (40, 1000, 1, 16, 1, 16),       # more row tiles than are tabulated
+])
+def test_more_items_than_workgroups(gpu, B, most, far, hq, hkv, bs):
+    announce(f"{B} chunks of up to {most}, contexts up to {far}, heads {hq}/{hkv}")
+    t = make_case(*_lengths(B, B, most, far), hq, hkv, bs, gpu, seed=B, tail=3)
+    t["row_ids"][1] = -1  # no row of the table: zeros
+    out = torch.full_like(t["q"], 7.0)
+    run(t, gpu, out=out)
+    torch.cuda.synchronize()
+    check(out, t, f"{B} chunks")
+    assert (out[-3:] == 7.0).all()
+    again = run(t, gpu)
+    assert torch.equal(again[:-3], out[:-3]), "the same call gave other bits"
+
+
+def test_many_items_of_one_length(gpu):
+    announce("chunk: 64 chunks of 64 tokens behind 100 each")
+    t = make_case([64] * 64, [100] * 64, 32, 8, 16, gpu, seed=14)
+    check(run(t, gpu), t, "one length")
+
+
+def test_replay_of_many_items_with_other_lengths(gpu):
+    announce("chunk: many items, captured and replayed with other lengths")
+    t = make_case(*_lengths(15, 30, 300, 2000), 32, 8, 16, gpu, seed=15)
+    dev = {k: t[k].to(gpu) for k in ("table", "seq_lens", "row_ids", "cu")}
+    from qwen3_engine_from_scratch_amd.kernels.paged_attention import paged_attention_chunk_hip
+
+    out = torch.empty_like(t["q"])
+
+    def call():
+        paged_attention_chunk_hip(t["q"], t["k"], t["v"], dev["table"], dev["seq_lens"],
+                                  dev["row_ids"], dev["cu"], 16, max_chunk=t["most"], out=out)
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for i in range(3):
+        for b in range(i, 30, 3):
+            r = int(t["row_ids"][b])
+            t["seq_lens"][r] = int(t["seq_lens"][r]) // 2
+        dev["seq_lens"].copy_(t["seq_lens"])
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out, t, f"replay {i}")
