@@ -172,6 +172,8 @@ class PagedKVCache:
     """Per-request handle over the shared pool (reference:
     qwen3/PagedKVcache.py:117-228)."""
 
+    freed = False  # its row is another request's by now
+
     def __init__(self, pool: KVCachePool):
         self._pool = pool
         self.seq_len = 0
@@ -266,7 +268,7 @@ class PagedKVCache:
         """Gives back everything behind the first `tokens` tokens (draft tokens that
         were not accepted): pages that hold nothing of the rest are freed, and one
         that is left partly filled and has other holders is replaced by a copy."""
-        if not 0 <= tokens <= self.seq_len:
+        if self.freed or not 0 <= tokens <= self.seq_len:
             raise ValueError(f"cannot keep {tokens} of {self.seq_len} tokens")
         pool = self._pool
         bs = pool.block_size
@@ -296,6 +298,7 @@ class PagedKVCache:
             self.block_table = []
             self.num_pages = 0
         self.seq_len = 0
+        self.freed = True
         self._pool.free_row(self.row_id)
 
 
@@ -316,6 +319,8 @@ def fork_caches(parents: list, tokens: list | None = None) -> list:
     for p, n in zip(parents, tokens):
         if p._pool is not pool:
             raise ValueError("forks of several pools in one call")
+        if p.freed:
+            raise ValueError("a fork of a handle that was freed")
         if not 0 <= n <= p.seq_len:
             raise ValueError(f"cannot fork {n} of {p.seq_len} tokens")
     if len(pool._free_rows) < len(parents):

@@ -157,6 +157,10 @@ class Engine:
 
     def _prefill_pieces(self, reqs) -> None:
         """Prefill behind prefixes and in pieces."""
+        if not all(len(r.prompt) for r in reqs):
+            raise ValueError("a prompt behind a prefix needs a token of its own")
+        if any(r.prefix is not None and r.prefix._pool is not self.pool for r in reqs):
+            raise ValueError("a prefix in another pool than the engine's")
         behind = [r for r in reqs if r.prefix is not None]
         for r, c in zip(behind, fork_caches([r.prefix for r in behind])):
             r.cache = c

@@ -213,7 +213,8 @@ def paged_attention_chunk_hip(q, k_buffer, v_buffer, block_table_2d, seq_lens_fu
     max_chunk:      host bound of the chunk lengths (None: read from cu_seqlens,
                     which synchronises and cannot be captured)
     Returns out (total_tokens, num_heads, head_dim) bf16.  Rows behind
-    cu_seqlens[-1] are left as they are; a token without keys is zero.  scale:
+    cu_seqlens[-1] are left as they are; a token without keys is zero.  A value of a
+    new token that is not finite reaches the tokens before it in its chunk too.  scale:
     1/sqrt(head_dim) unless given.  workspace: paged_chunk_workspace_bytes(...)
     bytes, a fresh one per call by default.
     """
@@ -246,6 +247,7 @@ def paged_attention_chunk_hip(q, k_buffer, v_buffer, block_table_2d, seq_lens_fu
         q = q.contiguous()
     if max_chunk is None:
         max_chunk = int(cu_seqlens.cpu().diff().max()) if B else 0
+    max_chunk = min(max_chunk, T)
     if scale is None:
         scale = 1.0 / math.sqrt(head_dim)
     if out is None:

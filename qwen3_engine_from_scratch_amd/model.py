@@ -430,6 +430,8 @@ class Qwen3ForCausalLM(nn.Module):
         assert len(caches) == B, "one kv cache handle per batch row"
         lens = list(input_lens) if input_lens is not None else [S] * B
         assert len(lens) == B and all(0 <= n <= S for n in lens)
+        if len({id(c) for c in caches}) != B or any(c._pool is not caches[0]._pool for c in caches):
+            raise ValueError("extend needs a handle of its own for each row, all of one pool")
         out = torch.zeros(B, S, self.config.vocab_size, dtype=self.lm_head.weight.dtype, device=dev)
         if sum(lens) == 0:
             return out

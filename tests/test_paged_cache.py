@@ -110,3 +110,45 @@ def test_holders_are_counted():
     assert pool.free_count == 5 and pool.is_shared(a[0]) is False
     pool.free(a[:1])
     assert sorted(pool.free_block_ids) == list(range(6))
+
+
+def test_freed_handles_and_mixed_pools_are_refused():
+    from qwen3_engine_from_scratch_amd.PagedKVcache import KVCachePool, PagedKVCache, fork_caches
+
+    pools = [KVCachePool(6, 1, 16, 1, 128, device="cpu", dtype=torch.bfloat16, max_seq_len=64,
+                         max_requests=4) for _ in range(2)]
+    a, b = (PagedKVCache(p) for p in pools)
+    with pytest.raises(ValueError, match="several pools"):
+        fork_caches([a, b])
+    with pytest.raises(ValueError, match="another pool"):
+        pools[0].compact([b])
+    with pytest.raises(ValueError, match="cannot fork"):
+        a.fork(1)
+    a.free()
+    with pytest.raises(ValueError, match="freed"):
+        a.fork()
+    with pytest.raises(ValueError, match="cannot keep"):
+        a.truncate(0)
+    assert all(p.free_count == 6 for p in pools)
+
+
+def test_rows_and_requests_that_cannot_be_extended_are_refused():
+    from types import SimpleNamespace
+
+    from qwen3_engine_from_scratch_amd.PagedKVcache import KVCachePool, PagedKVCache
+    from qwen3_engine_from_scratch_amd.engine import Engine, GenRequest
+    from qwen3_engine_from_scratch_amd.model import Qwen3ForCausalLM
+
+    pools = [KVCachePool(6, 1, 16, 1, 128, device="cpu", dtype=torch.bfloat16, max_seq_len=64,
+                         max_requests=4) for _ in range(2)]
+    a, b = (PagedKVCache(p) for p in pools)
+    ids = torch.zeros(2, 3, dtype=torch.long)
+    for caches in ([a, a], [a, b]):
+        with pytest.raises(ValueError, match="handle of its own"):
+            Qwen3ForCausalLM.extend(SimpleNamespace(), ids, caches)
+    engine = SimpleNamespace(pool=pools[0], prefill_chunk=None)
+    with pytest.raises(ValueError, match="token of its own"):
+        Engine._prefill_pieces(engine, [GenRequest(0, [], 4, prefix=a)])
+    with pytest.raises(ValueError, match="another pool"):
+        Engine._prefill_pieces(engine, [GenRequest(0, [1], 4, prefix=b)])
+    assert all(p.free_count == 6 for p in pools)
