@@ -33,5 +33,8 @@ live in tests/test_oracle.py):
                                pair; position 0 is the identity exactly;
                                adjacent pairing, a flipped sign, an off-by-one
                                position and norm-after-RoPE are rejected.
+  chunk.paged_chunk_ref        chunks of one token equal the fp64 decode, chunks with
+                               nothing cached the fp64 varlen form, to 1e-9
+                               (tests/test_chunk_refusals.py).
 No function of this package is "parity unpinned".
 """

@@ -803,7 +803,7 @@ void paged_chunk_deal_kernel(ChunkArgs a) {
 // rows of an item of up to six parts by half their elements (a wave takes an eighth, all
 // parts' loads in flight at once), or 32 rows by a quarter of the elements of an item
 // with more parts, which the four waves share.  (Items of four to six parts on the second
-// path: 1,001 tokens behind 650 take 45.5 us instead of 38.9, 509 behind 20,000 take 132
+// path: 1,001 tokens behind 650 take 45.5 us instead of 38.9, 509 behind 12,000 take 132
 // instead of 125.)  The workgroups deal the tasks among themselves from the list of cut
 // items: a workgroup for each possible task (ranges x rows) costs more in workgroups that
 // find nothing to do than the joins take.
