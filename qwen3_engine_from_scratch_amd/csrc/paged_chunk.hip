@@ -67,6 +67,7 @@ struct ChunkArgs {
   int n_mtiles;    // items of the longest chunk of one KV head
   float scale_log2;
   // range schedule
+  double per_range;  // 1 / ranges
   float* po;       // [2 ranges][rows][kD] partial outputs, not normalised, 32 rows mixed
   float2* pml;     // [2 ranges][rows] their running maximum (log2 domain) and sum
   CutItem* cuts;   // [ranges]
@@ -514,12 +515,12 @@ __device__ __forceinline__ T block_scan(T* v, int n, T* s_wsum) {
     x[i] = tid * kPer + i < n ? v[tid * kPer + i] : 0;
     sum += x[i];
   }
-  T incl = sum;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const T y = __shfl_up(incl, o, 64);
-    if (lane >= o) incl += y;
-  }
+  T incl;
+  if constexpr (sizeof(T) == 8)  // a thread's weights are below 2^31, a wave's in two halves
+    incl = (static_cast<int64_t>(q3::wave_prefix_sum(static_cast<int>(sum >> 16))) << 16) +
+           q3::wave_prefix_sum(static_cast<int>(sum & 0xffff));
+  else
+    incl = q3::wave_prefix_sum(sum);
   if (lane == 63) s_wsum[wave] = incl;
   __syncthreads();
   T run = incl - sum, total = 0;
@@ -554,10 +555,12 @@ __device__ __forceinline__ int64_t uniform64(int64_t x) {
   return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
 }
 
-// floor(x / y) of integers below 2^52: a quotient that is no integer lies at least
-// 1 / y below the next one, more than the rounding of x / y < 2^52 / y.
-__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
-  return static_cast<int64_t>(__builtin_floor(static_cast<double>(x) / static_cast<double>(y)));
+// floor(x / y) below 2^20, x >= 0: an estimate in 32 bits, less than one off, put right.
+__device__ __forceinline__ int quotient(int64_t x, int64_t y) {
+  int q = static_cast<int>(static_cast<float>(x) * __builtin_amdgcn_rcpf(static_cast<float>(y)));
+  if (q * y > x) --q;
+  if ((q + 1) * y <= x) ++q;
+  return __builtin_amdgcn_readfirstlane(q);
 }
 
 // Tabulates the batch, its sequences and the row tiles before each; returns the row tiles
@@ -576,12 +579,8 @@ __device__ __forceinline__ int tabulate(const ChunkArgs& a, int* s_first, SeqEnt
   return min(kMaxEntries, block_scan<W, int>(s_first, a.B, s_wsum));
 }
 
-// The sequence and row tile of a tabulated (sequence, row tile) pair.
-__device__ __forceinline__ Seq item_at(const ChunkArgs& a, const int* s_first,
-                                       const SeqEntry* s_seq, int entry, int& mt) {
-  const int b = __builtin_amdgcn_readfirstlane(last_at_most(s_first, a.B, entry));
-  mt = entry - __builtin_amdgcn_readfirstlane(s_first[b]);
-  SeqEntry se = s_seq[b];
+// A tabulated sequence, in scalar registers.
+__device__ __forceinline__ Seq tabulated(const ChunkArgs& a, SeqEntry se) {
   se.q0 = __builtin_amdgcn_readfirstlane(se.q0);
   se.n = __builtin_amdgcn_readfirstlane(se.n);
   se.row = __builtin_amdgcn_readfirstlane(se.row);
@@ -596,6 +595,8 @@ void paged_chunk_range_kernel(ChunkArgs a) {
   __shared__ int64_t s_pos[kMaxEntries];  // weight before each (sequence, row tile)
   __shared__ int s_first[kMaxSeqs];       // row tiles before each sequence
   __shared__ SeqEntry s_seq[kMaxSeqs];
+  __shared__ uint8_t s_of[kMaxEntries];   // a pair's sequence
+  static_assert(kMaxSeqs <= 256, "s_of holds a sequence");
   __shared__ int64_t s_wsum[W];
   __shared__ int s_most;                  // key tiles of the longest item
   const int tid = threadIdx.x;
@@ -608,6 +609,7 @@ void paged_chunk_range_kernel(ChunkArgs a) {
     const Seq s = seq_of(a, s_seq[b]);
     const int mt = e - s_first[b];
     const int tiles = (keys_of(a, s, (mt + 1) * rows_of<W>()) + kBN - 1) / kBN;
+    s_of[e] = static_cast<uint8_t>(b);
     s_pos[e] = static_cast<int64_t>(tile_units<W>(s.n * a.G - mt * rows_of<W>())) * tiles + kItemUnits;
     atomicMax(&s_most, tiles);
   }
@@ -615,8 +617,10 @@ void paged_chunk_range_kernel(ChunkArgs a) {
   const int64_t H = block_scan<W, int64_t>(s_pos, E, s_wsum);
   const int nwg = gridDim.x;
   const int64_t U = H * a.Hkv;
-  // a range's width: every workgroup's share, at least kMinRangeTiles tiles
-  const int64_t share = U / static_cast<uint32_t>(nwg) + 1;
+  // a range's width: every workgroup's share (its product with the workgroups is U or more:
+  // the rounding below is far less than the step to the next multiple), at least
+  // kMinRangeTiles tiles
+  const int64_t share = static_cast<int64_t>(static_cast<double>(U) * a.per_range) + 1;
   const int64_t width = share < kMinRangeTiles * kUnits ? kMinRangeTiles * kUnits : share;
   const int w = blockIdx.x;
   // Items that are no more than the workgroups and nearly as long as each other are not
@@ -636,10 +640,15 @@ void paged_chunk_range_kernel(ChunkArgs a) {
   CutItem cut{};
   if (p_lo < p_hi) {
     const LaneOffsets off = lane_offsets<W>(a, lane, wave);
-    int kvh = static_cast<int>(quotient(p_lo, H));
+    int kvh = quotient(p_lo, H);
     int e = __builtin_amdgcn_readfirstlane(last_at_most(s_pos, E, p_lo - kvh * H));
+    auto seq_of_pair = [&](int entry, int& tile) {
+      const int b = __builtin_amdgcn_readfirstlane(static_cast<int>(s_of[entry]));
+      tile = entry - __builtin_amdgcn_readfirstlane(s_first[b]);
+      return tabulated(a, s_seq[b]);
+    };
     int mt;
-    Seq s = item_at(a, s_first, s_seq, e, mt);
+    Seq s = seq_of_pair(e, mt);
     PageWindow ahead;
     bool have = false;  // `ahead` is this item's first window
     while (true) {
@@ -651,8 +660,11 @@ void paged_chunk_range_kernel(ChunkArgs a) {
       // belongs to the range that holds its position
       const int64_t base = P + kItemUnits + units / 2;
       auto first_at = [&](int64_t p) {
-        const int64_t j = p <= base ? 0 : quotient(p - base + units - 1, units);
-        return static_cast<int>(j < tiles ? j : tiles);
+        const int64_t d = p - base;
+        if (d <= 0) return 0;
+        if (d > static_cast<int64_t>(units) * (tiles - 1)) return tiles;
+        const uint32_t x = static_cast<uint32_t>(d) + units - 1;
+        return static_cast<int>(units == kUnits ? x / kUnits : x / kFewUnits);
       };
       const int j0 = first_at(p_lo), j1 = first_at(p_hi);
       if (j0 < j1 || (tiles == 0 && P >= p_lo)) {
@@ -662,9 +674,8 @@ void paged_chunk_range_kernel(ChunkArgs a) {
         PageWindow pw = ahead;
         if (!have) window_start(pw, a, s.row, j0, lane);
         // the next item's first window, on its way while this one's tiles run
-        int next_mt;
-        const int64_t next_row = item_at(a, s_first, s_seq, e + 1 == E ? 0 : e + 1, next_mt).row;
-        window_start(ahead, a, next_row, 0, lane);
+        const int next = e + 1 == E ? 0 : e + 1;
+        window_start(ahead, a, __builtin_amdgcn_readfirstlane(s_seq[s_of[next]].row), 0, lane);
         have = true;
         run_tiles<W>(a, off, s, wr, kvh, j0, j1, pw, tb, lane, wave, m_run, l_run, acc);
         l_run = cross_half_sum(l_run);
@@ -684,7 +695,7 @@ void paged_chunk_range_kernel(ChunkArgs a) {
           }
           if (j0 == 0) {
             const int64_t last = base + static_cast<int64_t>(units) * (tiles - 1);
-            cut.parts = static_cast<int32_t>(quotient(last, width)) - v + 1;
+            cut.parts = quotient(last, width) - v + 1;
             cut.r0 = mt * rows_of<W>();
             cut.rows = min(rows_of<W>(), s.n * a.G - cut.r0);
             cut.kvh = kvh;
@@ -697,7 +708,7 @@ void paged_chunk_range_kernel(ChunkArgs a) {
         e = 0;
         if (++kvh == a.Hkv) break;
       }
-      s = item_at(a, s_first, s_seq, e, mt);
+      s = seq_of_pair(e, mt);
     }
   }
   if (tid == 0) a.cuts[v] = cut;
@@ -716,7 +727,7 @@ void paged_chunk_deal_kernel(ChunkArgs a) {
   __shared__ int s_first[kMaxSeqs];  // row tiles before each sequence
   __shared__ SeqEntry s_seq[kMaxSeqs];
   __shared__ int s_slot[kMaxEntries];  // [class][64 pairs]: those of the class, then the ones before
-  __shared__ uint16_t s_order[kMaxEntries];
+  __shared__ uint32_t s_order[kMaxEntries];  // the sequence, and 16 bits of its row tile
   __shared__ int s_wsum[W];
   __shared__ int s_most;               // weight of the longest
   constexpr int kGroups = kMaxEntries / 64, kPer = kGroups / W;
@@ -729,14 +740,17 @@ void paged_chunk_deal_kernel(ChunkArgs a) {
   for (int i = tid; i < kMaxEntries; i += W * 64) s_slot[i] = 0;
   const int E = tabulate<W>(a, s_first, s_seq, s_wsum);
   int weight[kPer], rank[kPer];
+  uint32_t pair[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int e = (wave + W * i) * 64 + lane;
     weight[i] = 0;
+    pair[i] = 0;
     if (e < E) {
       const int b = last_at_most(s_first, a.B, e);
       const Seq s = seq_of(a, s_seq[b]);
       const int mt = e - s_first[b];
+      pair[i] = static_cast<uint32_t>(b) << 16 | static_cast<uint32_t>(mt);
       const int tiles = (keys_of(a, s, (mt + 1) * rows_of<W>()) + kBN - 1) / kBN;
       weight[i] = tile_units<W>(s.n * a.G - mt * rows_of<W>()) * tiles + kItemUnits;
       atomicMax(&s_most, weight[i]);
@@ -764,7 +778,7 @@ void paged_chunk_deal_kernel(ChunkArgs a) {
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int e = (wave + W * i) * 64 + lane;
-    if (e < E) s_order[s_slot[weight[i]] + rank[i]] = static_cast<uint16_t>(e);
+    if (e < E) s_order[s_slot[weight[i]] + rank[i]] = pair[i];
   }
   __syncthreads();
 
@@ -774,13 +788,14 @@ void paged_chunk_deal_kernel(ChunkArgs a) {
   // an XCD's neighbours share KV heads where their number allows it, else sequences
   const int p = a.Hkv % 8 != 0 && nwg % 8 == 0 ? (w % 8) * (nwg / 8) + w / 8 : w;
   auto item_of = [&](int round) { return round * nwg + ((round & 1) ? nwg - 1 - p : p); };
-  auto entry_of = [&](int item) {
-    return __builtin_amdgcn_readfirstlane(static_cast<int>(s_order[item / a.Hkv]));
+  auto pair_of = [&](int item) {
+    return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(s_order[item / a.Hkv])));
   };
   PageWindow ahead;
   for (int round = 0, item = item_of(0); item < items; ++round) {
-    int mt, next_mt;
-    const Seq s = item_at(a, s_first, s_seq, entry_of(item), mt);
+    const uint32_t pr = pair_of(item);
+    const Seq s = tabulated(a, s_seq[pr >> 16]);
+    const int mt = pr & 0xffff;
     const int kvh = item % a.Hkv;
     const WaveRows wr = wave_rows<W>(a, s, mt, wave, lane);
     const int tiles = (keys_of(a, s, (mt + 1) * rows_of<W>()) + kBN - 1) / kBN;
@@ -791,7 +806,7 @@ void paged_chunk_deal_kernel(ChunkArgs a) {
     // the next item's first window, on its way while this one's tiles run
     item = item_of(round + 1);
     const int next = item < items ? item : item_of(round);
-    window_start(ahead, a, item_at(a, s_first, s_seq, entry_of(next), next_mt).row, 0, lane);
+    window_start(ahead, a, __builtin_amdgcn_readfirstlane(s_seq[pair_of(next) >> 16].row), 0, lane);
     run_tiles<W>(a, off, s, wr, kvh, 0, tiles, pw, tb, lane, wave, m_run, l_run, acc);
     l_run = cross_half_sum(l_run);
     if (wr.active) store_output(a, s, wr, kvh, lane, l_run, acc, stage_of(tb, wave));
@@ -1003,6 +1018,7 @@ int launch_tiles(ChunkArgs a, const Variant& var, int max_chunk, void* workspace
     a.po = reinterpret_cast<float*>(ws + l.po);
     a.pml = reinterpret_cast<float2*>(ws + l.pml);
     a.cuts = reinterpret_cast<CutItem*>(ws + l.cuts);
+    a.per_range = 1. / wgs;
     hipLaunchKernelGGL(paged_chunk_range_kernel<W>, dim3(wgs), dim3(W * 64), 0, s, a);
     if (const int rc = q3::launch_status(who)) return rc;
     hipLaunchKernelGGL(paged_chunk_join_kernel<W>, dim3(4 * (wgs * W / 8)), dim3(kJoinWaves * 64), 0,

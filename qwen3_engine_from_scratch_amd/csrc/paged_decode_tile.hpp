@@ -75,17 +75,7 @@ __device__ __forceinline__ int64_t clamp_len(const DecodeArgs& a, int32_t seq_le
   return L > 0 ? L : 0;
 }
 
-// Inclusive prefix sum over the 64 lanes of a wave: four shifted adds inside
-// each 16-lane DPP row, then the row totals broadcast into the rows above.
-__device__ __forceinline__ int wave_prefix_sum(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // row_shr:1
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);   // row_shr:2
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);   // row_shr:4
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);   // row_shr:8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31
-  return v;
-}
+using q3::wave_prefix_sum;
 
 // Tabulates the batch in LDS for a persistent workgroup (kWaves waves): each
 // sequence's row and length, and the exclusive prefix of its tiles
