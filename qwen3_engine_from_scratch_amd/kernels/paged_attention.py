@@ -194,6 +194,29 @@ def _chunk_workspace(device: int, *shape) -> int:
     return int(_lib.load().qwen3_paged_chunk_workspace_bytes(*shape))
 
 
+@functools.lru_cache(maxsize=1024)
+def _chunk_layout(q, k, v, table, lens, cu, k_stride, v_stride, table_stride, q_type, k_type,
+                  v_type, table_type, lens_type, cu_type, block_size, own_rows):
+    """The checks of paged_attention_chunk_hip that go by shapes, strides and types alone
+    (kept by those: they cost more than a launch), and what it takes from them."""
+    bf16, i32 = torch.bfloat16, torch.int32
+    assert len(q) == 3
+    T, num_heads, head_dim = q
+    num_blocks, num_kv_heads, block_size_check, head_dim_check = k
+    assert block_size_check == block_size and head_dim_check == head_dim
+    assert v == k
+    assert q_type is bf16 and k_type is bf16 and v_type is bf16, "HIP chunk kernel is bf16 only"
+    assert table_type is i32 and lens_type is i32
+    assert len(table) == 2 and table_stride[1] == 1, "block_table_2d rows must be contiguous"
+    assert len(lens) == 1 and lens[0] >= table[0]
+    assert cu_type is i32 and len(cu) == 1 and cu[0] >= 1
+    assert k_stride[3] == 1 and v_stride[3] == 1
+    B = cu[0] - 1
+    if own_rows:
+        assert B <= table[0], "more sequences than rows of the block table"
+    return T, B, num_heads, num_kv_heads, head_dim, num_blocks, (table_stride[0], *table)
+
+
 def paged_attention_chunk_hip(q, k_buffer, v_buffer, block_table_2d, seq_lens_full, row_ids,
                               cu_seqlens, block_size, *, max_chunk: int | None = None,
                               scale: float | None = None, out: torch.Tensor | None = None,
@@ -218,27 +241,14 @@ def paged_attention_chunk_hip(q, k_buffer, v_buffer, block_table_2d, seq_lens_fu
     1/sqrt(head_dim) unless given.  workspace: paged_chunk_workspace_bytes(...)
     bytes, a fresh one per call by default.
     """
-    bf16, i32 = torch.bfloat16, torch.int32
-    assert q.dim() == 3
-    T, num_heads, head_dim = q.shape
-    num_blocks, num_kv_heads, block_size_check, head_dim_check = k_buffer.shape
-    assert block_size_check == block_size and head_dim_check == head_dim
-    assert v_buffer.shape == k_buffer.shape
-    assert q.dtype is bf16 and k_buffer.dtype is bf16 and v_buffer.dtype is bf16, \
-        "HIP chunk kernel is bf16 only"
-    assert block_table_2d.dtype is i32 and seq_lens_full.dtype is i32
-    assert block_table_2d.dim() == 2 and block_table_2d.stride(1) == 1, \
-        "block_table_2d rows must be contiguous"
-    table_rows, table_pages = block_table_2d.shape
-    assert seq_lens_full.dim() == 1 and seq_lens_full.shape[0] >= table_rows
-    assert cu_seqlens.dtype is i32 and cu_seqlens.dim() == 1 and cu_seqlens.shape[0] >= 1
-    assert k_buffer.stride(3) == 1 and v_buffer.stride(3) == 1
-    B = cu_seqlens.shape[0] - 1
+    T, B, num_heads, num_kv_heads, head_dim, num_blocks, table = _chunk_layout(
+        q.shape, k_buffer.shape, v_buffer.shape, block_table_2d.shape, seq_lens_full.shape,
+        cu_seqlens.shape, k_buffer.stride(), v_buffer.stride(), block_table_2d.stride(), q.dtype,
+        k_buffer.dtype, v_buffer.dtype, block_table_2d.dtype, seq_lens_full.dtype,
+        cu_seqlens.dtype, block_size, row_ids is None)
     if row_ids is not None:
-        assert row_ids.dtype is i32 and row_ids.numel() == B
+        assert row_ids.dtype is torch.int32 and row_ids.numel() == B
         row_ids = row_ids.contiguous()
-    else:
-        assert B <= table_rows, "more sequences than rows of the block table"
     dev = _lib.require_hip(q, k_buffer, v_buffer, block_table_2d, seq_lens_full, row_ids,
                            cu_seqlens, out, workspace)
     cu_seqlens = cu_seqlens.contiguous()
@@ -253,7 +263,7 @@ def paged_attention_chunk_hip(q, k_buffer, v_buffer, block_table_2d, seq_lens_fu
     if out is None:
         out = torch.empty_like(q)
     else:
-        assert out.shape == q.shape and out.dtype is bf16 and out.stride(2) == 1, \
+        assert out.shape == q.shape and out.dtype is torch.bfloat16 and out.stride(2) == 1, \
             "out must be a bf16 (total_tokens, num_heads, head_dim) tensor with unit last stride"
     if T == 0 or B == 0:
         return out
@@ -265,12 +275,10 @@ def paged_attention_chunk_hip(q, k_buffer, v_buffer, block_table_2d, seq_lens_fu
         rc = _lib.load().qwen3_paged_chunk_bf16(
             q.data_ptr(), strides(q), k_buffer.data_ptr(), strides(k_buffer),
             v_buffer.data_ptr(), strides(v_buffer), num_blocks,
-            block_table_2d.data_ptr(), block_table_2d.stride(0), table_rows, table_pages,
-            seq_lens_full.data_ptr(), _lib.ptr(row_ids), cu_seqlens.data_ptr(),
-            out.data_ptr(), strides(out),
+            block_table_2d.data_ptr(), *table, seq_lens_full.data_ptr(), _lib.ptr(row_ids),
+            cu_seqlens.data_ptr(), out.data_ptr(), strides(out),
             B, max_chunk, T, num_heads, num_kv_heads, head_dim, block_size, scale,
-            workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-            _lib.stream_of(dev))
+            workspace.data_ptr(), need, _lib.stream_of(dev))
     _lib.check(rc, "qwen3_paged_chunk_bf16")
     return out
 

@@ -9,6 +9,7 @@ needs no table and a far one loses nothing.
 """
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 
@@ -102,7 +103,7 @@ class Rotary:
                 or not self.inv_freq.is_contiguous():
             raise ValueError("inv_freq must be a contiguous float64 vector")
 
-    @property
+    @functools.cached_property
     def rotary_dim(self) -> int:
         return 2 * self.inv_freq.numel()
 
@@ -114,18 +115,34 @@ def make_rotary(rotary_dim: int, base: float = 1e6, *, layout: str = "half",
     return Rotary(freq.to(device), layout, gain)
 
 
-def _check(q, k, rotary, q_out, k_out):
-    assert q.dim() == 3 and q.stride(2) == 1, "q must be (tokens, heads, head_dim) rows"
-    assert q.dtype in _DTYPES, f"dtype {q.dtype} not supported"
-    T, _, D = q.shape
+@functools.lru_cache(maxsize=1024)
+def _layout(q, q_stride, q_type, k, k_stride, k_type, rotary_dim):
+    """The checks that go by shapes, strides and types alone (kept by those); returns
+    (tokens, query heads, KV heads, head_dim)."""
+    assert len(q) == 3 and q_stride[2] == 1, "q must be (tokens, heads, head_dim) rows"
+    assert q_type in _DTYPES, f"dtype {q_type} not supported"
+    T, Hq, D = q
     if k is not None:
-        assert k.dim() == 3 and k.stride(2) == 1 and k.dtype == q.dtype
-        assert k.shape[0] == T and k.shape[2] == D
-    assert rotary.rotary_dim <= D, f"rotary_dim {rotary.rotary_dim} of head_dim {D}"
-    for x, y in ((q, q_out), (k, k_out)):
-        if y is not None:
-            assert x is not None and y.shape == x.shape and y.dtype == x.dtype \
-                and y.stride(2) == 1, "an output must have its input's shape and type"
+        assert len(k) == 3 and k_stride[2] == 1 and k_type == q_type
+        assert k[0] == T and k[2] == D
+    assert rotary_dim <= D, f"rotary_dim {rotary_dim} of head_dim {D}"
+    return T, Hq, 0 if k is None else k[1], D
+
+
+def _check(q, k, rotary, q_out, k_out):
+    if k is None:
+        assert k_out is None
+        sizes = _layout(q.shape, q.stride(), q.dtype, None, None, None, rotary.rotary_dim)
+    else:
+        sizes = _layout(q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype,
+                        rotary.rotary_dim)
+        assert k_out is None or _like(k, k_out), "an output must have its input's shape and type"
+    assert q_out is None or _like(q, q_out), "an output must have its input's shape and type"
+    return sizes
+
+
+def _like(x, y):
+    return y.shape == x.shape and y.dtype == x.dtype and y.stride(2) == 1
 
 
 def _positions(positions, T):
@@ -141,8 +158,7 @@ def rotary_embedding_hip(q: torch.Tensor, k: torch.Tensor | None, positions: tor
     fused projection).  Returns (q_out, k_out); they may be given, also as q and k
     themselves.  inverse: the transposed map, which takes the gradient of the outputs to
     that of the inputs."""
-    _check(q, k, rotary, q_out, k_out)
-    T, Hq, D = q.shape
+    T, Hq, Hkv, D = _check(q, k, rotary, q_out, k_out)
     positions = _positions(positions, T)
     dev = _lib.require_hip(q, k, positions, rotary.inv_freq, q_out, k_out)
     q_out = torch.empty_like(q) if q_out is None else q_out
@@ -157,7 +173,7 @@ def rotary_embedding_hip(q: torch.Tensor, k: torch.Tensor | None, positions: tor
             q_out.data_ptr(), st(q_out), _lib.ptr(k_out),
             None if k is None else st(k_out), _DTYPES[q.dtype],
             rotary.inv_freq.data_ptr(), float(rotary.attention_factor), _LAYOUTS[rotary.layout],
-            1 if inverse else 0, positions.data_ptr(), T, Hq, 0 if k is None else k.shape[1], D,
+            1 if inverse else 0, positions.data_ptr(), T, Hq, Hkv, D,
             rotary.rotary_dim, _lib.stream_of(dev))
     _lib.check(rc, "qwen3_rotary")
     return q_out, k_out
@@ -180,9 +196,8 @@ def rotary_embedding_prefill_hip(q: torch.Tensor, k: torch.Tensor, v: torch.Tens
     """rotary_embedding_hip of T packed tokens that also writes the rotated k and v
     into layer layer_idx of the pool at slot_mapping (T,) (int64 block * block_size +
     offset; negative: not written).  bf16.  Returns (q_out, k_out)."""
-    _check(q, k, rotary, q_out, k_out)
+    T, Hq, Hkv, D = _check(q, k, rotary, q_out, k_out)
     _check_pool(q, k, v, k_buffer, v_buffer)
-    T, Hq, D = q.shape
     positions = _positions(positions, T)
     slot_mapping = _positions(slot_mapping, T)
     dev = _lib.require_hip(q, k, v, positions, slot_mapping, rotary.inv_freq, k_buffer, v_buffer,
@@ -200,7 +215,7 @@ def rotary_embedding_prefill_hip(q: torch.Tensor, k: torch.Tensor, v: torch.Tens
             _LAYOUTS[rotary.layout], positions.data_ptr(), slot_mapping.data_ptr(),
             k_buffer.data_ptr(), st(k_buffer), v_buffer.data_ptr(),
             st(v_buffer), k_buffer.shape[0], int(layer_idx), k_buffer.shape[1], T,
-            Hq, k.shape[1], D, rotary.rotary_dim, k_buffer.shape[3], _lib.stream_of(dev))
+            Hq, Hkv, D, rotary.rotary_dim, k_buffer.shape[3], _lib.stream_of(dev))
     _lib.check(rc, "qwen3_rotary_slots_bf16")
     return q_out, k_out
 
@@ -213,10 +228,9 @@ def rotary_embedding_decode_hip(q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
     and v into `pool` (a KVCachePool) at position seq_lens[row], whose page must be
     reserved; rotated there too, or at positions (B,) int64.  row_ids: int32 (B,) rows of
     the block table (None: row b for token b).  bf16."""
-    _check(q, k, rotary, q_out, None)
+    B, Hq, Hkv, D = _check(q, k, rotary, q_out, None)
     kb, vb = pool.k_buffer, pool.v_buffer
     _check_pool(q, k, v, kb, vb)
-    B, Hq, D = q.shape
     if row_ids is not None:
         assert row_ids.dtype == torch.int32 and row_ids.numel() == B
         row_ids = row_ids.contiguous()
@@ -235,7 +249,7 @@ def rotary_embedding_decode_hip(q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
             float(rotary.attention_factor), _LAYOUTS[rotary.layout], kb.data_ptr(),
             st(kb), vb.data_ptr(), st(vb), kb.shape[0],
             int(layer_idx), kb.shape[1], pool.seq_lens.data_ptr(), bt.data_ptr(), bt.stride(0),
-            bt.shape[0], bt.shape[1], _lib.ptr(row_ids), _lib.ptr(positions), B, Hq, k.shape[1],
+            bt.shape[0], bt.shape[1], _lib.ptr(row_ids), _lib.ptr(positions), B, Hq, Hkv,
             D, rotary.rotary_dim, kb.shape[3], _lib.stream_of(dev))
     _lib.check(rc, "qwen3_rotary_decode_bf16")
     return q_out
