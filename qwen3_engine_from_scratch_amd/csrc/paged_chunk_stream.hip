@@ -137,7 +137,8 @@ __device__ __forceinline__ void fold_chunk(Chunk& c, float scale_log2, int hi, C
   const float m_use = m_new == q3::kNegInf ? 0.f : m_new;
   const float alpha = q3::fast_exp2(st.m - m_use);
   st.m = m_new;
-  q3::bf16x4 p[kChunk];
+  // P as two bf16 terms, p = hi + lo, as the decode carries it: 16 significant bits
+  q3::bf16x4 p[kChunk], pl[kChunk];
   float psum = 0.f;
 #pragma unroll
   for (int i = 0; i < kChunk; ++i) {
@@ -147,7 +148,7 @@ __device__ __forceinline__ void fold_chunk(Chunk& c, float scale_log2, int hi, C
       e[r] = q3::fast_exp2(s[i][r] - m_use);
       psum += e[r];
     }
-    p[i] = q3::as_bf16x4(q3::u32x2{q3::pack_bf16x2(e[0], e[1]), q3::pack_bf16x2(e[2], e[3])});
+    split_p(e, p[i], pl[i]);
   }
   st.l = st.l * alpha + psum;
 #pragma unroll
@@ -162,6 +163,7 @@ __device__ __forceinline__ void fold_chunk(Chunk& c, float scale_log2, int hi, C
         const q3::u32x2 av = {q3::pick_halves(c.v[i][0][w], c.v[i][1][w], h),
                               q3::pick_halves(c.v[i][2][w], c.v[i][3][w], h)};
         st.acc[j] = q3::mfma16x16x16(q3::as_bf16x4(av), p[i], st.acc[j]);
+        st.acc[j] = q3::mfma16x16x16(q3::as_bf16x4(av), pl[i], st.acc[j]);
       }
     }
   }

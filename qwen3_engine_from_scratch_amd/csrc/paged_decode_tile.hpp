@@ -231,6 +231,17 @@ __device__ __forceinline__ void load_q(q3::bf16x8 (&qv)[4], const DecodeArgs& a,
   }
 }
 
+// e as two bf16 terms: hi = bf16(e), lo = bf16(e - hi).
+__device__ __forceinline__ void split_p(const float (&e)[4], q3::bf16x4& hi, q3::bf16x4& lo) {
+  const q3::u32x2 pk = {q3::pack_bf16x2(e[0], e[1]), q3::pack_bf16x2(e[2], e[3])};
+  hi = q3::as_bf16x4(pk);
+  // the rounded terms back in fp32: a bf16's bits are the top half of a float's
+  const float h0 = __uint_as_float(pk[0] << 16), h1 = __uint_as_float(pk[0] & 0xffff0000u);
+  const float h2 = __uint_as_float(pk[1] << 16), h3 = __uint_as_float(pk[1] & 0xffff0000u);
+  lo = q3::as_bf16x4(q3::u32x2{q3::pack_bf16x2(e[0] - h0, e[1] - h1),
+                               q3::pack_bf16x2(e[2] - h2, e[3] - h3)});
+}
+
 // Folds c.n tiles (first tile c.t0) into the online softmax state.
 __device__ __forceinline__ void compute_chunk(Chunk& c, float scale_log2, int hi,
                                               const q3::bf16x8 (&qv)[4], SoftmaxState& st) {
@@ -280,14 +291,7 @@ __device__ __forceinline__ void compute_chunk(Chunk& c, float scale_log2, int hi
       e[r] = q3::fast_exp2(s[i][r] - m_use);
       psum += e[r];
     }
-    const q3::u32x2 pk = {q3::pack_bf16x2(e[0], e[1]), q3::pack_bf16x2(e[2], e[3])};
-    p[i] = q3::as_bf16x4(pk);
-    // the rounded terms back in fp32: a bf16's bits are the top half of a float's
-    const float h0 = __uint_as_float(pk[0] << 16), h1 = __uint_as_float(pk[0] & 0xffff0000u);
-    const float h2 = __uint_as_float(pk[1] << 16), h3 = __uint_as_float(pk[1] & 0xffff0000u);
-    const q3::u32x2 lk = {q3::pack_bf16x2(e[0] - h0, e[1] - h1),
-                          q3::pack_bf16x2(e[2] - h2, e[3] - h3)};
-    pl[i] = q3::as_bf16x4(lk);
+    split_p(e, p[i], pl[i]);
   }
   st.l = st.l * alpha + psum;
 #pragma unroll
