@@ -182,7 +182,13 @@ class PagedKVCache:
         self.block_table_tensor = pool.block_table_2d[self.row_id]
         self.num_pages = 0
 
+    def check_live(self):
+        """Refuses a handle that was freed: what it would write into is another's."""
+        if self.freed:
+            raise ValueError("the handle was freed: its row may be another request's by now")
+
     def _allocate_block(self):
+        self.check_live()
         max_pages = self.block_table_tensor.shape[0]
         assert self.num_pages < max_pages, \
             f"request exceeds max_seq_len ({self._pool.max_seq_len} tokens / {max_pages} pages)"
@@ -193,6 +199,7 @@ class PagedKVCache:
 
     def reserve_next(self):
         """Reserves the page the next decode token lands in (:152-162)."""
+        self.check_live()
         need = (self.seq_len + 1 + self._pool.block_size - 1) // self._pool.block_size
         if need > self.num_pages:
             self._allocate_block()
@@ -213,6 +220,7 @@ class PagedKVCache:
         k_new, v_new: (B, num_kv_heads, S_new, head_dim); as in the reference
         only batch row 0 is written.  Pages are reserved first.
         """
+        self.check_live()
         _, _, S_new, _ = k_new.shape
         pool = self._pool
         end_pos = self.seq_len + S_new
@@ -245,7 +253,7 @@ class PagedKVCache:
         """Reserves the pages of positions seq_len .. seq_len + n - 1 (as
         update does, :186-190) and returns their pool slots, block *
         block_size + offset, as an int64 numpy array."""
-
+        self.check_live()
         bs = self._pool.block_size
         end = self.seq_len + n
         while len(self.block_table) < (end + bs - 1) // bs:
@@ -255,6 +263,7 @@ class PagedKVCache:
         return table[p // bs] * bs + p % bs
 
     def advance_seq_len(self, n: int = 1):
+        self.check_live()
         self.seq_len += n
         self._pool.seq_lens[self.row_id] = self.seq_len
 
@@ -378,6 +387,7 @@ class PageIn:
         max_pages = pool.block_table_2d.shape[1]
         want = []
         for c, n in zip(caches, tokens):
+            c.check_live()
             k = (int(n) + bs - 1) // bs - c.num_pages
             if k > 0:
                 assert c.num_pages + k <= max_pages, \
@@ -425,6 +435,7 @@ def reserve_pages_bulk(caches, tokens: list) -> None:
     max_pages = pool.block_table_2d.shape[1]
     want = []
     for c, n in zip(caches, tokens):
+        c.check_live()
         k = (int(n) + bs - 1) // bs - c.num_pages
         if k > 0:
             assert c.num_pages + k <= max_pages, \
@@ -450,6 +461,8 @@ def set_seq_lens_bulk(caches) -> None:
     """Writes every handle's host seq_len into the resident seq_lens table
     with one copy (the batched form of advance_seq_len's device write)."""
     pool = caches[0]._pool
+    for c in caches:
+        c.check_live()
     idx = torch.tensor([[c.row_id for c in caches], [c.seq_len for c in caches]],
                        dtype=torch.int64).to(pool.seq_lens.device)
     pool.seq_lens.index_put_((idx[0],), idx[1].to(torch.int32))
@@ -464,6 +477,7 @@ def prefill_slot_mapping(caches, S: int, device) -> torch.Tensor:
     slots = np.empty((len(caches), S), dtype=np.int64)
     pos = np.arange(S, dtype=np.int64)
     for i, c in enumerate(caches):
+        c.check_live()
         end_pos = c.seq_len + S
         need = (end_pos + bs - 1) // bs
         while len(c.block_table) < need:

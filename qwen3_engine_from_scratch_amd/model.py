@@ -422,7 +422,8 @@ class Qwen3ForCausalLM(nn.Module):
         """forward for tokens that follow what each handle holds (any number of
         tokens, none included): input_ids (B, S), right-padded, input_lens the new
         tokens of each row (0: the row's handle is left alone).  Reserves pages, writes
-        K/V, attends over the cached and the new tokens and advances each handle.
+        K/V, attends over the cached and the new tokens and advances each handle (a freed
+        one is refused).
         Returns logits (B, S, V), pad positions zero."""
         B, S = input_ids.shape
         dev = input_ids.device
@@ -432,6 +433,8 @@ class Qwen3ForCausalLM(nn.Module):
         assert len(lens) == B and all(0 <= n <= S for n in lens)
         if len({id(c) for c in caches}) != B or any(c._pool is not caches[0]._pool for c in caches):
             raise ValueError("extend needs a handle of its own for each row, all of one pool")
+        for c in caches:
+            c.check_live()
         out = torch.zeros(B, S, self.config.vocab_size, dtype=self.lm_head.weight.dtype, device=dev)
         if sum(lens) == 0:
             return out

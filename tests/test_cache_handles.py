@@ -1,0 +1,64 @@
+"""Handles of the paged cache that may not be used any more, and pools that run out: what is
+refused, and that nothing of another request's changes (CPU; the few device writes of the
+host bookkeeping run on CPU tensors)."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from qwen3_engine_from_scratch_amd import PagedKVcache as pc
+from qwen3_engine_from_scratch_amd.PagedKVcache import KVCachePool, PagedKVCache
+
+
+def _pool(blocks=6, rows=4):
+    return KVCachePool(blocks, 1, 16, 1, 128, device="cpu", dtype=torch.bfloat16, max_seq_len=96,
+                       max_requests=rows)
+
+
+def _state(pool):
+    return (list(pool.free_block_ids), list(pool._free_rows), dict(pool._extra_holders),
+            pool.block_table_2d.tolist(), pool.seq_lens.tolist())
+
+
+def _freed_and_its_heir():
+    """A freed handle, and the request that has its row now."""
+    pool = _pool()
+    a = PagedKVCache(pool)
+    a.reserve_slots(20)
+    a.advance_seq_len(20)
+    a.free()
+    b = PagedKVCache(pool)
+    assert b.row_id == a.row_id
+    b.reserve_slots(16)
+    b.advance_seq_len(5)
+    return pool, a, b
+
+
+def test_extend_refuses_a_freed_handle():
+    from qwen3_engine_from_scratch_amd.model import Qwen3ForCausalLM
+
+    pool, a, b = _freed_and_its_heir()
+    c = PagedKVCache(pool)
+    before = _state(pool)
+    ids = torch.zeros(2, 3, dtype=torch.long)
+    for caches in ([c, a], [a, c]):
+        for lens in (None, [1, 0], [0, 0]):
+            with pytest.raises(ValueError, match="freed"):
+                Qwen3ForCausalLM.extend(SimpleNamespace(), ids, caches, lens)
+    assert _state(pool) == before and b.block_table == [int(pool.block_table_2d[b.row_id, 0])]
+
+
+@pytest.mark.parametrize("use", [
+    lambda c: c.reserve_slots(3), lambda c: c.reserve_next(), lambda c: c.advance_seq_len(3),
+    lambda c: c._allocate_block(),
+    lambda c: c.update(0, torch.zeros(1, 1, 3, 128), torch.zeros(1, 1, 3, 128)),
+    lambda c: pc.reserve_pages_bulk([c], [3]), lambda c: pc.set_seq_lens_bulk([c]),
+    lambda c: pc.prefill_slot_mapping([c], 3, "cpu"),
+    lambda c: pc.PageIn.reserve(SimpleNamespace(pool=c._pool, cap=8), [c], [3]),
+])
+def test_a_freed_handle_writes_into_no_row(use):
+    pool, a, b = _freed_and_its_heir()
+    before = _state(pool)
+    with pytest.raises(ValueError, match="freed"):
+        use(a)
+    assert _state(pool) == before and a.block_table == [] and a.seq_len == 0
