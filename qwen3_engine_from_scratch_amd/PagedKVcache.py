@@ -302,6 +302,9 @@ class PagedKVCache:
         pool.seq_lens[self.row_id] = tokens
 
     def free(self):
+        """Gives back the row and the pages; once: a second call finds nothing left."""
+        if self.freed:
+            return
         if self.block_table:
             self._pool.free(self.block_table)
             self.block_table = []

@@ -62,3 +62,18 @@ def test_a_freed_handle_writes_into_no_row(use):
     with pytest.raises(ValueError, match="freed"):
         use(a)
     assert _state(pool) == before and a.block_table == [] and a.seq_len == 0
+
+
+def test_a_second_free_gives_nothing_back_twice():
+    pool = _pool()
+    a, b = PagedKVCache(pool), PagedKVCache(pool)
+    a.reserve_slots(20)
+    b.reserve_slots(5)
+    a.free()
+    before = _state(pool)
+    a.free()
+    assert _state(pool) == before
+    c, d = PagedKVCache(pool), PagedKVCache(pool)
+    assert len({b.row_id, c.row_id, d.row_id}) == 3
+    a.free()  # its row is c's or d's by now
+    assert len(pool._free_rows) == 1
