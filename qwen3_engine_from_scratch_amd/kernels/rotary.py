@@ -36,7 +36,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 1e6, scaling: dict | None 
                base * (factor seq_len / L - factor + 1)^(d / (d - 2))
       yarn     pairs that turn more than beta_fast times within L keep f_i, those that
                turn less than beta_slow times take f_i / factor, linear in i between;
-               cos and sin times attention_factor (default 0.1 ln(factor) + 1)
+               cos and sin times attention_factor (default m(1), or m(mscale) /
+               m(mscale_all_dim) where both are given, m(k) = 0.1 k ln(factor) + 1)
       llama3   by wave length: f_i from L / high_freq_factor down, f_i / factor from
                L / low_freq_factor up, linear in L / wave length between
     """
@@ -75,9 +76,7 @@ def rotary_frequencies(rotary_dim: int, base: float = 1e6, scaling: dict | None 
             low, high = math.floor(low), math.ceil(high)
         low, high = max(low, 0), min(high, d - 1)
         slow = ((i - low) / max(high - low, 0.001)).clamp(0, 1)
-        gain = scaling.get("attention_factor")
-        gain = 0.1 * math.log(factor) + 1.0 if gain is None else float(gain)
-        return freq * (1 - slow) + freq / factor * slow, gain
+        return freq * (1 - slow) + freq / factor * slow, _yarn_factor(scaling, factor)
     if kind == "llama3":
         lo, hi = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
         if not 0 < lo < hi:
@@ -85,6 +84,23 @@ def rotary_frequencies(rotary_dim: int, base: float = 1e6, scaling: dict | None 
         keep = ((L * freq / (2 * math.pi) - lo) / (hi - lo)).clamp(0, 1)
         return freq * keep + freq / factor * (1 - keep), 1.0
     raise ValueError(f"rope_scaling type {kind!r} not supported")
+
+
+def _yarn_factor(scaling: dict, factor: float) -> float:
+    """yarn's factor on cos and sin."""
+    if scaling.get("attention_factor") is not None:
+        return float(scaling["attention_factor"])
+
+    def m(k):
+        return 0.1 * k * math.log(factor) + 1.0
+
+    scales = [scaling.get("mscale"), scaling.get("mscale_all_dim")]
+    if scales == [None, None]:
+        return m(1.0)
+    # one without the other, or a zero, means different things to different libraries
+    if None in scales or not all(float(x) > 0 for x in scales):
+        raise ValueError("yarn scaling takes mscale and mscale_all_dim together, both positive")
+    return m(float(scales[0])) / m(float(scales[1]))
 
 
 @dataclass(frozen=True)
