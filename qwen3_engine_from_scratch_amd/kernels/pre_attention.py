@@ -27,8 +27,9 @@ def rope_tables(head_dim: int, base: float = 1e6, max_seq_len: int = 4096, devic
     for both halves.  Computed on the CPU (like the reference's buffers) and
     moved to `device`.  scaling: a rope_scaling dict (rotary_frequencies); its angles are
     formed in 64 bits, its factor goes into the tables."""
-    if scaling is not None and scaling.get("rope_type", scaling.get("type")) != "default":
+    if scaling is not None:
         freq, gain = rotary_frequencies(head_dim, base, scaling, seq_len=max_seq_len)
+    if scaling is not None and scaling.get("rope_type", scaling.get("type")) != "default":
         angle = torch.outer(torch.arange(max_seq_len, dtype=torch.float64), freq)
         cos, sin = ((f(angle) * gain).float().repeat(1, 2) for f in (torch.cos, torch.sin))
         return cos.to(device), sin.to(device)

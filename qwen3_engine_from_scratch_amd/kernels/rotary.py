@@ -40,6 +40,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 1e6, scaling: dict | None 
                m(mscale_all_dim) where both are given, m(k) = 0.1 k ln(factor) + 1)
       llama3   by wave length: f_i from L / high_freq_factor down, f_i / factor from
                L / low_freq_factor up, linear in L / wave length between
+
+    A key that its type does not know is refused: it would ask for other angles.
     """
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f"rotary_dim {rotary_dim} must be positive and even")
@@ -48,6 +50,7 @@ def rotary_frequencies(rotary_dim: int, base: float = 1e6, scaling: dict | None 
     freq = torch.pow(torch.tensor(float(base), dtype=torch.float64), -2 * i / d)
     scaling = dict(scaling or {})
     kind = scaling.get("rope_type", scaling.get("type", "default"))
+    _check_keys(scaling, kind, base)
     if kind == "default":
         return freq, 1.0
     factor = float(scaling["factor"])
@@ -77,13 +80,37 @@ def rotary_frequencies(rotary_dim: int, base: float = 1e6, scaling: dict | None 
         low, high = max(low, 0), min(high, d - 1)
         slow = ((i - low) / max(high - low, 0.001)).clamp(0, 1)
         return freq * (1 - slow) + freq / factor * slow, _yarn_factor(scaling, factor)
-    if kind == "llama3":
-        lo, hi = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
-        if not 0 < lo < hi:
-            raise ValueError("llama3 scaling needs 0 < low_freq_factor < high_freq_factor")
-        keep = ((L * freq / (2 * math.pi) - lo) / (hi - lo)).clamp(0, 1)
-        return freq * keep + freq / factor * (1 - keep), 1.0
-    raise ValueError(f"rope_scaling type {kind!r} not supported")
+    # llama3
+    lo, hi = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+    if not 0 < lo < hi:
+        raise ValueError("llama3 scaling needs 0 < low_freq_factor < high_freq_factor")
+    keep = ((L * freq / (2 * math.pi) - lo) / (hi - lo)).clamp(0, 1)
+    return freq * keep + freq / factor * (1 - keep), 1.0
+
+
+# What a rope_scaling dict of each type may say, beside the keys of all of them.
+_SCALING_KEYS = {
+    "default": set(),
+    "linear": {"factor"},
+    "dynamic": {"factor"},
+    "yarn": {"factor", "beta_fast", "beta_slow", "truncate", "attention_factor", "mscale",
+             "mscale_all_dim"},
+    "llama3": {"factor", "low_freq_factor", "high_freq_factor"},
+}
+
+
+def _check_keys(scaling: dict, kind, base: float) -> None:
+    if kind not in _SCALING_KEYS:
+        raise ValueError(f"rope_scaling type {kind!r} not supported")
+    # these may come along, where they agree with what the caller says
+    same = {"rope_type": kind, "type": kind, "rope_theta": base, "partial_rotary_factor": 1.0}
+    for key, value in scaling.items():
+        if value is None or key in _SCALING_KEYS[kind] or key == "original_max_position_embeddings":
+            continue
+        if key not in same:
+            raise ValueError(f"rope_scaling key {key!r} is not one of type {kind!r}")
+        if value != same[key]:
+            raise ValueError(f"rope_scaling {key} {value!r} where {same[key]!r} is asked for")
 
 
 def _yarn_factor(scaling: dict, factor: float) -> float:

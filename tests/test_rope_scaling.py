@@ -49,3 +49,41 @@ def test_yarn_factor_against_transformers(mscale, mscale_all_dim):
 def test_one_scale_alone_is_refused(over):
     with pytest.raises(ValueError, match="mscale"):
         rotary_frequencies(64, 1e4, dict(YARN, **over))
+
+
+LLAMA3 = {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+          "original_max_position_embeddings": 8192}
+
+
+@pytest.mark.parametrize("bad", [
+    {"rope_type": "default", "mrope_section": [16, 24, 24]},
+    {"mrope_section": [16, 24, 24]},
+    {"factor": 4.0},                                    # a factor of no type
+    {"rope_type": "linear", "factor": 2.0, "beta_fast": 32},
+    {"rope_type": "linear", "factor": 2.0, "attention_factor": 1.1},
+    dict(YARN, long_factor=[1.0] * 32),
+    dict(YARN, low_freq_factor=1.0),
+    dict(LLAMA3, mscale=1.0, mscale_all_dim=1.0),
+    dict(YARN, rope_theta=5e5),                         # another base than the one given
+    dict(YARN, partial_rotary_factor=0.5),
+    dict(YARN, type="linear"),                          # two types
+])
+def test_keys_that_are_not_understood_are_refused(bad):
+    from qwen3_engine_from_scratch_amd.kernels.pre_attention import rope_tables
+
+    with pytest.raises(ValueError, match="rope_scaling"):
+        rotary_frequencies(128, 1e4, bad)
+    with pytest.raises(ValueError, match="rope_scaling"):
+        rope_tables(128, 1e4, 64, scaling=bad)
+
+
+def test_keys_that_say_nothing_new_are_taken():
+    for kind, d in (("linear", {"factor": 2.0, "original_max_position_embeddings": 4096}),
+                    ("default", {}), ("dynamic", {"factor": 2.0,
+                                                  "original_max_position_embeddings": 4096})):
+        want = rotary_frequencies(64, 1e4, {"rope_type": kind, **d})
+        for more in ({"type": kind}, {"rope_theta": 1e4}, {"partial_rotary_factor": 1.0},
+                     {"beta_fast": None}):
+            got = rotary_frequencies(64, 1e4, {"rope_type": kind, **d, **more})
+            assert torch.equal(got[0], want[0]) and got[1] == want[1]
+    assert torch.equal(rotary_frequencies(64, 1e4, {})[0], rotary_frequencies(64, 1e4)[0])
