@@ -26,10 +26,16 @@ def rope_tables(head_dim: int, base: float = 1e6, max_seq_len: int = 4096, devic
     base^(-2i/head_dim), their outer product with the positions, repeated
     for both halves.  Computed on the CPU (like the reference's buffers) and
     moved to `device`.  scaling: a rope_scaling dict (rotary_frequencies); its angles are
-    formed in 64 bits, its factor goes into the tables."""
+    formed in 64 bits, its factor goes into the tables.  Dynamic scaling is refused beyond
+    the length it keeps: there the angles depend on each sequence's own length."""
+    kind = None if scaling is None else scaling.get("rope_type", scaling.get("type"))
     if scaling is not None:
-        freq, gain = rotary_frequencies(head_dim, base, scaling, seq_len=max_seq_len)
-    if scaling is not None and scaling.get("rope_type", scaling.get("type")) != "default":
+        freq, gain = rotary_frequencies(head_dim, base, scaling)
+        if kind == "dynamic" and max_seq_len > scaling["original_max_position_embeddings"]:
+            raise ValueError(
+                f"a table of {max_seq_len} positions cannot hold dynamic scaling, whose base "
+                f"grows with a sequence beyond {scaling['original_max_position_embeddings']} tokens")
+    if scaling is not None and kind != "default":
         angle = torch.outer(torch.arange(max_seq_len, dtype=torch.float64), freq)
         cos, sin = ((f(angle) * gain).float().repeat(1, 2) for f in (torch.cos, torch.sin))
         return cos.to(device), sin.to(device)

@@ -87,3 +87,21 @@ def test_keys_that_say_nothing_new_are_taken():
             got = rotary_frequencies(64, 1e4, {"rope_type": kind, **d, **more})
             assert torch.equal(got[0], want[0]) and got[1] == want[1]
     assert torch.equal(rotary_frequencies(64, 1e4, {})[0], rotary_frequencies(64, 1e4)[0])
+
+
+def test_a_table_of_fixed_length_holds_no_growing_base():
+    """dynamic turns a sequence of up to L tokens by the plain frequencies and a longer one
+    by others: a table beyond L would be wrong for one of them."""
+    from qwen3_engine_from_scratch_amd.kernels.pre_attention import rope_tables
+    from qwen3_engine_from_scratch_amd.model import RotaryEmbedding
+
+    d = {"rope_type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 4096}
+    plain = rope_tables(64, 1e4, 4096, scaling={"rope_type": "linear", "factor": 1.0})
+    for n in (1000, 4096):
+        for a, b in zip(rope_tables(64, 1e4, n, scaling=d), plain):
+            assert torch.equal(a, b[:n])
+    for n in (4097, 16384):
+        with pytest.raises(ValueError, match="dynamic"):
+            rope_tables(64, 1e4, n, scaling=d)
+        with pytest.raises(ValueError, match="dynamic"):
+            RotaryEmbedding(64, 1e4, n, scaling=d)
