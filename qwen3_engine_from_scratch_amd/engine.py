@@ -144,11 +144,18 @@ class Engine:
         set_seq_lens_bulk(caches)
         return toks
 
+    def _check_positions(self, tokens: int) -> None:
+        """The rotary tables end; a token behind them would be computed wrongly."""
+        most = self.model.config.max_position_embeddings
+        if tokens > most:
+            raise ValueError(f"{tokens} tokens, but the rotary tables hold {most} positions")
+
     @torch.no_grad()
     def cache_prefix(self, tokens: list) -> PagedKVCache:
         """Computes the K/V of tokens that several requests begin with; pass the handle
         as their `prefix` and free() it when no request needs it any more (what running
         requests still share stays)."""
+        self._check_positions(len(tokens))
         c = PagedKVCache(self.pool)
         step = self.prefill_chunk or max(len(tokens), 1)
         for i in range(0, len(tokens), step):
@@ -161,6 +168,8 @@ class Engine:
             raise ValueError("a prompt behind a prefix needs a token of its own")
         if any(r.prefix is not None and r.prefix._pool is not self.pool for r in reqs):
             raise ValueError("a prefix in another pool than the engine's")
+        for r in reqs:
+            self._check_positions((r.prefix.seq_len if r.prefix is not None else 0) + len(r.prompt))
         behind = [r for r in reqs if r.prefix is not None]
         for r, c in zip(behind, fork_caches([r.prefix for r in behind])):
             r.cache = c

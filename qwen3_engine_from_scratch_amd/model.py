@@ -395,7 +395,7 @@ class Qwen3ForCausalLM(nn.Module):
         """New tokens of n sequences behind what their caches hold: packed ids (T,)
         int64, cu_seqlens (n+1,) int32, row_ids (n,) int32 rows of the block table,
         positions (T,) int64 and slot_mapping (T,) int64 of the tokens (from each row's
-        seq_lens on; pages reserved).  A sequence may bring one token (decoding) or
+        seq_lens on, below config.max_position_embeddings; pages reserved).  A sequence may bring one token (decoding) or
         many (a piece of its prompt, draft tokens).  Writes their K/V, leaves seq_lens
         to the caller, returns the logits of the rows in logit_rows (int64; None:
         every token)."""
@@ -422,8 +422,8 @@ class Qwen3ForCausalLM(nn.Module):
         """forward for tokens that follow what each handle holds (any number of
         tokens, none included): input_ids (B, S), right-padded, input_lens the new
         tokens of each row (0: the row's handle is left alone).  Reserves pages, writes
-        K/V, attends over the cached and the new tokens and advances each handle (a freed
-        one is refused).
+        K/V, attends over the cached and the new tokens and advances each handle.  Refuses a
+        freed handle, and tokens behind config.max_position_embeddings.
         Returns logits (B, S, V), pad positions zero."""
         B, S = input_ids.shape
         dev = input_ids.device
@@ -435,6 +435,10 @@ class Qwen3ForCausalLM(nn.Module):
             raise ValueError("extend needs a handle of its own for each row, all of one pool")
         for c in caches:
             c.check_live()
+        most = max((c.seq_len + n for c, n in zip(caches, lens) if n), default=0)
+        if most > self.config.max_position_embeddings:
+            raise ValueError(f"{most} tokens, but the rotary tables hold "
+                             f"{self.config.max_position_embeddings} positions")
         out = torch.zeros(B, S, self.config.vocab_size, dtype=self.lm_head.weight.dtype, device=dev)
         if sum(lens) == 0:
             return out

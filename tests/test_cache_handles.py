@@ -77,3 +77,49 @@ def test_a_second_free_gives_nothing_back_twice():
     assert len({b.row_id, c.row_id, d.row_id}) == 3
     a.free()  # its row is c's or d's by now
     assert len(pool._free_rows) == 1
+
+
+def _model(positions):
+    return SimpleNamespace(config=SimpleNamespace(max_position_embeddings=positions, vocab_size=8),
+                           lm_head=SimpleNamespace(weight=torch.zeros(1)))
+
+
+def test_extend_refuses_positions_behind_the_tables():
+    """The step that rotates knows no angle there: it would leave q and the slot unwritten."""
+    from qwen3_engine_from_scratch_amd.model import Qwen3ForCausalLM
+
+    pool = _pool()
+    a, b = PagedKVCache(pool), PagedKVCache(pool)
+    a.reserve_slots(38)
+    a.advance_seq_len(38)
+    before = _state(pool)
+    ids = torch.zeros(2, 3, dtype=torch.long)
+    for caches, lens in (([a, b], None), ([a, b], [3, 0]), ([b, a], [1, 3])):
+        with pytest.raises(ValueError, match="positions"):
+            Qwen3ForCausalLM.extend(_model(40), ids, caches, lens)
+    assert _state(pool) == before
+    out = Qwen3ForCausalLM.extend(_model(40), ids, [a, b], [0, 0])  # nothing to place
+    assert out.shape == (2, 3, 8) and not out.any()
+
+
+def test_the_engine_refuses_prompts_behind_the_tables():
+    from qwen3_engine_from_scratch_amd.engine import Engine, GenRequest
+
+    pool = _pool()
+    prefix = PagedKVCache(pool)
+    prefix.reserve_slots(30)
+    prefix.advance_seq_len(30)
+    before = _state(pool)
+
+    def no_step(*args):
+        raise AssertionError("a step was run")
+
+    engine = SimpleNamespace(pool=pool, prefill_chunk=8, model=_model(40), _run_chunk=no_step,
+                             _check_positions=lambda n: Engine._check_positions(engine, n))
+    for reqs in ([GenRequest(0, [1] * 5, 4, prefix=prefix), GenRequest(1, [1] * 11, 4, prefix=prefix)],
+                 [GenRequest(0, [1] * 41, 4)]):
+        with pytest.raises(ValueError, match="positions"):
+            Engine._prefill_pieces(engine, reqs)
+    with pytest.raises(ValueError, match="positions"):
+        Engine.cache_prefix(engine, [1] * 41)
+    assert _state(pool) == before
