@@ -158,8 +158,12 @@ class Engine:
         self._check_positions(len(tokens))
         c = PagedKVCache(self.pool)
         step = self.prefill_chunk or max(len(tokens), 1)
-        for i in range(0, len(tokens), step):
-            self._run_chunk([c], [tokens[i:i + step]], False)
+        try:
+            for i in range(0, len(tokens), step):
+                self._run_chunk([c], [tokens[i:i + step]], False)
+        except BaseException:
+            c.free()  # nobody else knows it
+            raise
         return c
 
     def _prefill_pieces(self, reqs) -> None:

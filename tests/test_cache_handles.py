@@ -123,3 +123,35 @@ def test_the_engine_refuses_prompts_behind_the_tables():
     with pytest.raises(ValueError, match="positions"):
         Engine.cache_prefix(engine, [1] * 41)
     assert _state(pool) == before
+
+
+def _engine(pool, fail_at):
+    """An engine whose chunk step number `fail_at` finds no memory."""
+    from qwen3_engine_from_scratch_amd.engine import Engine
+
+    steps = []
+
+    def step(caches, tokens, want_logits):
+        steps.append(1)
+        for c, t in zip(caches, tokens):
+            c.reserve_slots(len(t))
+            c.seq_len += len(t)
+        if len(steps) == fail_at:
+            raise RuntimeError("OOM: a step")
+        return [7] * len(caches)
+
+    return SimpleNamespace(pool=pool, prefill_chunk=8, model=_model(96), _run_chunk=step,
+                           _take=Engine._take, _check_positions=lambda n: None)
+
+
+@pytest.mark.parametrize("fail_at", [1, 3])
+def test_a_prefix_that_fails_gives_its_row_and_pages_back(fail_at):
+    from qwen3_engine_from_scratch_amd.engine import Engine
+
+    pool = _pool()
+    free, rows = sorted(pool.free_block_ids), sorted(pool._free_rows)
+    with pytest.raises(RuntimeError, match="a step"):
+        Engine.cache_prefix(_engine(pool, fail_at), [1] * 30)
+    assert sorted(pool.free_block_ids) == free and sorted(pool._free_rows) == rows
+    c = Engine.cache_prefix(_engine(pool, 9), [1] * 30)
+    assert c.seq_len == 30 and not c.freed
