@@ -193,9 +193,25 @@ class Engine:
             left = [r for r in left if done[id(r)] < len(r.prompt)]
 
     def _prefill(self, reqs) -> None:
-        if any(r.prefix is not None or len(r.prompt) > (self.prefill_chunk or len(r.prompt))
-               for r in reqs):
-            return self._prefill_pieces(reqs)
+        """Prefills the requests' prompts and takes their first tokens.  A failure (no
+        rows, no pages) leaves the requests and the pool as they were."""
+        before = [(r.cache, len(r.output_ids), r.eos_hit) for r in reqs]
+        try:
+            if any(r.prefix is not None or len(r.prompt) > (self.prefill_chunk or len(r.prompt))
+                   for r in reqs):
+                self._prefill_pieces(reqs)
+            else:
+                self._prefill_whole(reqs)
+        except BaseException:
+            for r, (cache, told, eos_hit) in zip(reqs, before):
+                if r.cache is not cache:
+                    r.cache.free()
+                    r.cache = cache
+                del r.output_ids[told:]
+                r.eos_hit = eos_hit
+            raise
+
+    def _prefill_whole(self, reqs) -> None:
         dev = self.device
         lens = [len(r.prompt) for r in reqs]
         for r in reqs:

@@ -155,3 +155,43 @@ def test_a_prefix_that_fails_gives_its_row_and_pages_back(fail_at):
     assert sorted(pool.free_block_ids) == free and sorted(pool._free_rows) == rows
     c = Engine.cache_prefix(_engine(pool, 9), [1] * 30)
     assert c.seq_len == 30 and not c.freed
+
+
+@pytest.mark.parametrize("fail_at", [1, 2, 3])
+def test_a_prefill_that_fails_leaves_nothing_behind(fail_at, monkeypatch):
+    """Rows, pages, holders and tokens as before: the requests can be submitted again."""
+    from qwen3_engine_from_scratch_amd.engine import Engine, GenRequest
+
+    monkeypatch.setattr(pc, "fork_pages_hip", lambda *args: None)  # the launch: bookkeeping only
+    pool = _pool(blocks=12, rows=6)
+    prefix = PagedKVCache(pool)
+    prefix.reserve_slots(40)
+    prefix.advance_seq_len(40)
+    free, rows = sorted(pool.free_block_ids), sorted(pool._free_rows)
+    reqs = [GenRequest(0, [1] * 5, 4, prefix=prefix), GenRequest(1, [1] * 20, 4),
+            GenRequest(2, [2] * 9, 4, prefix=prefix, eos_token_id=7)]
+    engine = _engine(pool, fail_at)
+    engine._prefill_pieces = lambda r: Engine._prefill_pieces(engine, r)
+    with pytest.raises(RuntimeError, match="a step"):
+        Engine._prefill(engine, reqs)
+    assert sorted(pool.free_block_ids) == free and sorted(pool._free_rows) == rows
+    assert not pool._extra_holders and not prefix.freed and prefix.num_pages == 3
+    assert all(r.cache is None and r.output_ids == [] and not r.eos_hit for r in reqs)
+    engine._run_chunk = _engine(pool, 99)._run_chunk
+    Engine._prefill(engine, reqs)
+    assert [r.output_ids for r in reqs] == [[7], [7], [7]] and reqs[2].eos_hit
+
+
+def test_too_few_rows_for_a_prefill_leave_nothing_behind():
+    from qwen3_engine_from_scratch_amd.engine import Engine, GenRequest
+
+    pool = _pool(blocks=12, rows=2)
+    for prefill_chunk, n in ((8, 20), (None, 5)):  # in pieces, whole
+        engine = _engine(pool, 99)
+        engine.prefill_chunk, engine.device = prefill_chunk, torch.device("cpu")
+        engine._prefill_pieces = lambda r: Engine._prefill_pieces(engine, r)
+        engine._prefill_whole = lambda r: Engine._prefill_whole(engine, r)
+        reqs = [GenRequest(i, [1] * n, 4) for i in range(3)]
+        with pytest.raises(RuntimeError, match="rows exhausted"):
+            Engine._prefill(engine, reqs)
+        assert len(pool._free_rows) == 2 and all(r.cache is None for r in reqs)
