@@ -276,25 +276,32 @@ class PagedKVCache:
     def truncate(self, tokens: int):
         """Gives back everything behind the first `tokens` tokens (draft tokens that
         were not accepted): pages that hold nothing of the rest are freed, and one
-        that is left partly filled and has other holders is replaced by a copy."""
+        that is left partly filled and has other holders is replaced by a copy (which
+        takes a free block, or one of those that are given back)."""
         if self.freed or not 0 <= tokens <= self.seq_len:
             raise ValueError(f"cannot keep {tokens} of {self.seq_len} tokens")
         pool = self._pool
         bs = pool.block_size
         keep, rest = -(-tokens // bs), tokens % bs
+        back = self.block_table[keep:]
         if rest and pool.is_shared(self.block_table[keep - 1]):
             old = self.block_table[keep - 1]
-            new = pool.take_blocks(1)[0]
+            own = [b for b in back if not pool.is_shared(b)]
+            reuse = own and not pool.free_count  # in a full pool: one that is given back anyway
+            new = own[0] if reuse else pool.take_blocks(1)[0]
             try:
                 copy_pages_hip(pool.k_buffer, pool.v_buffer, [old], [new], [rest])
             except Exception:
-                pool.free([new])
+                if not reuse:
+                    pool.free([new])
                 raise
+            if reuse:
+                back.remove(new)
             self.block_table[keep - 1] = new
             self.block_table_tensor[keep - 1] = new
             pool.free([old])
         if keep < self.num_pages:
-            pool.free(self.block_table[keep:])
+            pool.free(back)
             del self.block_table[keep:]
             self.block_table_tensor[keep:self.num_pages] = -1
             self.num_pages = keep

@@ -195,3 +195,60 @@ def test_too_few_rows_for_a_prefill_leave_nothing_behind():
         with pytest.raises(RuntimeError, match="rows exhausted"):
             Engine._prefill(engine, reqs)
         assert len(pool._free_rows) == 2 and all(r.cache is None for r in reqs)
+
+
+def _fork_rows(k, v, table, seq_lens, src, dst, tokens, blocks):
+    """The fork launch's part in the table, in blocks of 16."""
+    for a, b, n, new in zip(src, dst, tokens, blocks):
+        table[b] = -1
+        table[b, :n // 16] = table[a, :n // 16]
+        if n % 16:
+            table[b, n // 16] = new
+        seq_lens[b] = n
+
+
+def _shared_and_full(monkeypatch, own_tail):
+    """A handle of five (or three) pages, the first three shared, in a pool without a free
+    block; and the page copies that are launched."""
+    copies = []
+    monkeypatch.setattr(pc, "fork_pages_hip", _fork_rows)
+    monkeypatch.setattr(pc, "copy_pages_hip", lambda k, v, src, dst, tokens: copies.append((src, dst, tokens)))
+    pool = _pool(blocks=5 if own_tail else 3)
+    a = PagedKVCache(pool)
+    a.reserve_slots(48)
+    a.advance_seq_len(48)
+    b = a.fork()
+    if own_tail:
+        b.reserve_slots(30)
+        b.advance_seq_len(30)
+    assert pool.free_count == 0
+    return pool, a, b, copies
+
+
+def test_truncate_in_a_full_pool_takes_a_page_it_gives_back(monkeypatch):
+    pool, a, b, copies = _shared_and_full(monkeypatch, True)
+    old, tail = list(b.block_table), b.block_table[3:]
+    b.truncate(40)
+    (src, dst, tokens), = copies
+    assert src == [old[2]] and tokens == [8] and dst[0] in tail
+    assert b.block_table == old[:2] + dst and b.num_pages == 3 and b.seq_len == 40
+    assert pool.block_table_2d[b.row_id, :5].tolist() == b.block_table + [-1, -1]
+    assert pool.free_block_ids == [x for x in tail if x not in dst]
+    assert not pool.is_shared(old[2]) and pool.is_shared(old[1])
+    a.free()
+    b.free()
+    assert sorted(pool.free_block_ids) == list(range(5)) and not pool._extra_holders
+
+
+def test_truncate_without_a_page_to_copy_into_changes_nothing(monkeypatch):
+    pool, a, b, copies = _shared_and_full(monkeypatch, False)
+    before, pages = _state(pool), list(b.block_table)
+    with pytest.raises(RuntimeError, match="OOM"):
+        b.truncate(40)
+    assert _state(pool) == before and b.block_table == pages and b.seq_len == 48 and not copies
+    c = b.fork()  # a tail that others hold gives no page either
+    c.truncate(16)
+    before = _state(pool)
+    with pytest.raises(RuntimeError, match="OOM"):
+        b.truncate(10)
+    assert _state(pool) == before and b.block_table == pages
