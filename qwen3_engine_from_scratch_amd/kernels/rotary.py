@@ -200,7 +200,49 @@ def rotary_embedding_hip(q: torch.Tensor, k: torch.Tensor | None, positions: tor
     magnitude below 2^31; bf16, fp16 or fp32, views with strides welcome (slices of a
     fused projection).  Returns (q_out, k_out); they may be given, also as q and k
     themselves.  inverse: the transposed map, which takes the gradient of the outputs to
-    that of the inputs."""
+    that of the inputs; inputs that require a gradient get it (into outputs of the call's
+    own)."""
+    if _wants_grad(q, k):
+        if q_out is not None or k_out is not None:
+            raise RuntimeError("outputs that are given would lose the gradient of q and k: "
+                               "leave them out, or call under torch.no_grad()")
+        return _Rotated.apply(q, k, positions, rotary, inverse)
+    return _rotate(q, k, positions, rotary, inverse, q_out, k_out)
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+class _Rotated(torch.autograd.Function):
+    """The map is linear and its transpose the inverse form: that is its gradient."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, rotary, inverse):
+        ctx.rotary, ctx.inverse = rotary, inverse
+        ctx.save_for_backward(positions)
+        return _rotate(q, k, positions, rotary, inverse, None, None)
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        positions, = ctx.saved_tensors
+        grads = [_rows(g) if need else None for g, need in zip((gq, gk), ctx.needs_input_grad)]
+        if grads[0] is None:  # k's alone
+            dk, dq = rotary_embedding_hip(grads[1], None, positions, ctx.rotary,
+                                          inverse=not ctx.inverse)
+        else:
+            dq, dk = rotary_embedding_hip(*grads, positions, ctx.rotary, inverse=not ctx.inverse)
+        return dq, dk, None, None, None
+
+
+def _rows(g: torch.Tensor) -> torch.Tensor:
+    """A gradient as the kernel reads it: rows of 16-byte chunks, whatever it was."""
+    chunk = 16 // g.element_size()
+    ok = g.stride(2) == 1 and g.data_ptr() % 16 == 0 and all(s % chunk == 0 for s in g.stride()[:2])
+    return g if ok else g.clone(memory_format=torch.contiguous_format)
+
+
+def _rotate(q, k, positions, rotary, inverse, q_out, k_out):
     T, Hq, Hkv, D = _check(q, k, rotary, q_out, k_out)
     positions = _positions(positions, T)
     dev = _lib.require_hip(q, k, positions, rotary.inv_freq, q_out, k_out)
@@ -223,6 +265,9 @@ def rotary_embedding_hip(q: torch.Tensor, k: torch.Tensor | None, positions: tor
 
 
 def _check_pool(q, k, v, k_buffer, v_buffer):
+    if _wants_grad(q, k, v):
+        raise RuntimeError("what is written into the pool has no gradient: call under "
+                           "torch.no_grad(), or rotate with rotary_embedding_hip")
     assert v.dim() == 3 and v.stride(2) == 1 and v.shape == k.shape
     assert q.dtype == v.dtype == k_buffer.dtype == v_buffer.dtype == torch.bfloat16, "bf16 only"
     assert k_buffer.dim() == 5 and v_buffer.shape == k_buffer.shape
