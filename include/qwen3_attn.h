@@ -371,7 +371,9 @@ int qwen3_padded_prefill_bf16(const void* q, const int64_t q_strides[3], const v
  * Positions behind what a table row addresses, and pages whose id is no block of
  * the pool, are not attended.  Slots behind a sequence's last token are not read.
  * The new tokens' values must be finite: a value that is not reaches the chunk's
- * earlier tokens too.
+ * earlier tokens too.  Scores and sums are fp32; probabilities meet the values in 16 bits
+ * where max_chunk * num_heads / num_kv_heads is at most 16 (and B at most 2,048), rounded
+ * to bf16 otherwise.
  * Supported: head_dim 128; block_size a multiple of 16; num_heads / num_kv_heads up
  * to 16; slot strides from head_dim to 2^24 elements; 16-byte aligned rows.
  * ---------------------------------------------------------------------- */

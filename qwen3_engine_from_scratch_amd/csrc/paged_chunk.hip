@@ -5,9 +5,13 @@
 // in its pages already.  Token i attends the keys j <= c_s + i of its row of the
 // block table:
 //   o_i = sum_j exp(scale q_i k_j) v_j / sum_j exp(scale q_i k_j),
-// in one pass with a running maximum and sum in fp32; P is rounded to bf16 for
-// the PV product (a relative error of at most 2^-8 per term of a weighted mean),
-// the output once to bf16.  A row without keys is zero.
+// in one pass with a running maximum and sum in fp32; here P is rounded to bf16 for
+// the PV product, as in the prefill (a relative error of at most 2^-8 per term of a
+// weighted mean), the output once to bf16.  A row without keys is zero.  P as two bf16
+// terms, as paged_chunk_stream.hip carries it where loads are the bound, is a second PV
+// product here: 2,048 tokens behind 64,000 2.00 -> 2.69 ms, 509 behind 12,000 115 -> 149 us,
+// 40 behind 100,000 113 -> 138, twelve turns 160 -> 197.  One term: outputs 0.0023 off 64 bits
+// (root mean square, relative), of which 0.0017 are their own rounding.
 //
 //  * Query rows of one KV head are packed: row r is token r / G, head r % G of
 //    the group, so one staged K/V tile serves every head of the group whatever
@@ -1001,9 +1005,10 @@ ChunkLayout chunk_layout(int W) {
 //    single tokens behind 4,000 in the same kernels: 54 against 51);
 //  - ranges for up to 1.75 items a workgroup, dealt items above: one prompt of 4,096 (2.03
 //    items) 141 us dealt, 165 in ranges; eight chunks of about 1,000 (2.2) 71 and 77;
-//    eight of 200-800 behind 1,000-8,000 (2.2) 309 and 300; below it, by how unequal the
-//    items are, twelve turns of 20-700 behind 0-6,000 (1.44) 186 and 165, six chunks
-//    with groups of five heads (1.31) 205 and 218;
+//    twelve turns of 20-700 behind 0-6,000 (1.44) 186 and 165.  How unequal the items are
+//    decides too, and the lengths lie on the device: by the count alone, eight of 200-800
+//    behind 1,000-8,000 (2.2) take 309 where ranges take 300, and six chunks with groups of
+//    five heads (1.31) 218 where dealt items take 205;
 //  - items in order where the batch is too large to be tabulated in LDS.  (Where it is
 //    not, order alone costs: 16 chunks of 200-800 behind 1,000-8,000 825 us, dealt 658;
 //    100 of 30-100 behind 200-2,000 213 and 196; one prompt of 4,096 146 and 141.)

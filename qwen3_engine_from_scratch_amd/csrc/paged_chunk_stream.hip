@@ -5,16 +5,18 @@
 // are cut into equal ranges, one per resident wave; K and V go from HBM straight into
 // MFMA operands, two batches of tiles in flight per wave; a sequence-head that straddles
 // ranges is joined by a second launch.  Here the 16 columns of a product are the packed
-// rows of a sequence, each with its own last key.
+// rows of a sequence, each with its own last key.  P meets V as two bf16 terms, as in the
+// decode: 16 bits, for a second product that the loads hide (48 sequences of four tokens
+// 156 us with one term and with two).
 //
 // Bound by HBM: K and V are read once for all rows of a sequence (48 sequences of four
-// tokens behind 1,024-8,192, 32/8 heads: 862 MB algorithmic, 873 MB fetched, 152 us and 8
+// tokens behind 1,024-8,192, 32/8 heads: 862 MB algorithmic, 872 MB fetched, 153 us and 8
 // of merge, 5.5 TB/s).  The same batch in the tile kernels, whose loads
 // pass through LDS: 193 us.  Two column groups a wave, to 32 rows: 78 us against 55 for 16
 // sequences of eight tokens behind 4,000 (registers for one batch of tiles less in
 // flight), so 17 rows and more go to the tile kernels.  A few rows behind little are
 // latency: a dependent load each for rows, lengths, page ids, keys and the queries, then
-// code that no cache holds yet (one sequence of five tokens behind 900: 13.3 us in all).
+// code that no cache holds yet (one sequence of five tokens behind 900: 9.5 us, and 5 of merge).
 #include "paged_chunk_stream.hpp"
 #include "paged_decode_merge.hpp"
 #include "paged_decode_tile.hpp"

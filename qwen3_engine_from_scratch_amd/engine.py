@@ -26,8 +26,9 @@ Greedy decoding only (temperature 0), as the reference's benchmark runs.
 
 Prompts may also follow a prefix that is cached already (Engine.cache_prefix,
 GenRequest.prefix: its pages are shared, not computed again), and long ones may be
-prefilled in pieces (prefill_chunk: bounds a step's activations); both attend the
-pages through the chunk kernel.
+prefilled in pieces (prefill_chunk: bounds what each prompt adds to a step; with
+max_prefill_batch it bounds the step's activations); both attend the pages through the
+chunk kernel.
 """
 from __future__ import annotations
 
