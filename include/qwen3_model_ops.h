@@ -304,6 +304,44 @@ int qwen3_sample_ws_bf16(const void* logits, int64_t row_stride, int64_t rows, i
                          uint64_t seed, int64_t* out, void* workspace, size_t workspace_bytes,
                          void* stream);
 
+/* Log probabilities of given tokens, the entropy of their distribution and the most
+ * likely tokens (no counterpart in the reference engine: answers that are ranked,
+ * prompts that are scored, a policy's training step).  With z = logits[r] /
+ * temperature and log p = z - log(sum exp z):
+ *   logprobs[r, k]      log p of tokens[r, k] (int64, rows x given, at most 64 a row).
+ *                       A negative id is no token: 0.  One of vocab or more: NaN
+ *   entropy[r]          -sum p log p (nullable)
+ *   top_ids[r, j], top_logprobs[r, j]   the top_n (at most 64 and vocab) largest logits,
+ *                       descending, the lower index first among equal ones (-0 is 0;
+ *                       NaN ranks above every number)
+ *   stats[r, 0..1]      what the gradient needs of the row (nullable)
+ * Sums in fp32 over fp32 exponentials.  Logits of -inf have no mass; a row of
+ * nothing else, and one with NaN or +inf, is NaN (its ranking is still by the rule).
+ *   logits      dtype 0: bf16, 1: fp16, 2: fp32; rows of vocab values, row_stride
+ *               elements apart (aligned to their type only)
+ *   workspace   qwen3_token_logprobs_workspace_bytes(...) bytes, 16-byte aligned, no
+ *               initialisation; calls that share one must not overlap.  0: none
+ * Rows too few for the device are cut into parts, which a second launch joins. */
+size_t qwen3_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int dtype, int top_n);
+int qwen3_token_logprobs(const void* logits, int64_t row_stride, int dtype, int64_t rows,
+                         int64_t vocab, const int64_t* tokens, int given, float temperature,
+                         float* logprobs, float* entropy, int top_n, int64_t* top_ids,
+                         float* top_logprobs, float* stats, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* Its gradient: grad[r, i] (the logits' type, rows grad_row_stride apart) =
+ *   (sum_k g_logprobs[r, k] 1[i = tokens[r, k]] + sum_j g_top[r, j] 1[i = top_ids[r, j]]
+ *    - p_i (sum g_logprobs + sum g_top + g_entropy[r] (log p_i + entropy[r]))) / temperature
+ * rounded once.  g_* are fp32 and nullable (zero); ids that are no token add nothing;
+ * stats and entropy (needed with g_entropy) as the call above gave them. */
+int qwen3_token_logprobs_grad(const void* logits, int64_t row_stride, int dtype, int64_t rows,
+                              int64_t vocab, const int64_t* tokens, int given,
+                              float temperature, const float* entropy, int top_n,
+                              const int64_t* top_ids, const float* stats,
+                              const float* g_logprobs, const float* g_entropy,
+                              const float* g_top, void* grad, int64_t grad_row_stride,
+                              void* stream);
+
 /* seq_lens[row_ids[i]] += delta for i < n, except rows equal to skip_row
  * (a captured batch's padding row) and rows outside [0, max_rows).  Rows
  * other than skip_row must be distinct.  The host keeps its own copy of the

@@ -179,6 +179,17 @@ _SIGNATURES = {
     "qwen3_sample_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
     "qwen3_sample_ws_bf16": (_i, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, ctypes.c_uint64, _vp, _vp,
                                   ctypes.c_size_t, _vp]),
+    "qwen3_token_logprobs_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i, _i]),
+    "qwen3_token_logprobs": (
+        _i,
+        [_vp, _i64, _i, _i64, _i64, _vp, _i, ctypes.c_float, _vp, _vp, _i, _vp, _vp, _vp,
+         _vp, ctypes.c_size_t, _vp],
+    ),
+    "qwen3_token_logprobs_grad": (
+        _i,
+        [_vp, _i64, _i, _i64, _i64, _vp, _i, ctypes.c_float, _vp, _i, _vp, _vp, _vp, _vp, _vp,
+         _vp, _i64, _vp],
+    ),
     "qwen3_lm_head_argmax_workspace_bytes": (ctypes.c_size_t, []),
     "qwen3_lm_head_argmax_bf16": (_i, [_vp, _i64, _vp, _i, _vp, ctypes.c_float, _vp, _i64, _i,
                                        _i, _i, _vp, ctypes.c_size_t, _vp, _vp]),
@@ -202,7 +213,7 @@ _SIGNATURES = {
     ),
 }
 
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 _lib = None
 
