@@ -100,77 +100,6 @@ __device__ __forceinline__ int tabulate_chunks(const StreamArgs& a, int32_t* s_p
   return run;
 }
 
-// The 16 packed rows of a sequence-head: columns of the products, a lane's is lo.
-struct Columns {
-  q3::bf16x8 q[4];
-  int last;         // last key of this lane's column
-  SoftmaxState st;
-};
-
-// Folds c.n tiles (first tile c.t0) into the columns' state.
-__device__ __forceinline__ void fold_chunk(Chunk& c, float scale_log2, int hi, Columns& col) {
-  SoftmaxState& st = col.st;
-  q3::f32x4 s[kChunk];
-#pragma unroll
-  for (int i = 0; i < kChunk; ++i) {
-    s[i] = q3::f32x4{0.f, 0.f, 0.f, 0.f};
-    if (i < c.n) {
-#pragma unroll
-      for (int cc = 0; cc < 4; ++cc)
-        s[i] = q3::mfma16x16x32(q3::as_bf16x8(c.k[i][cc]), col.q[cc], s[i]);
-    }
-  }
-  float mx = q3::kNegInf;
-#pragma unroll
-  for (int i = 0; i < kChunk; ++i) {
-    const int tokb = (c.t0 + i) * kTile + 4 * hi;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const bool there = i < c.n && c.valid[i];
-      const bool ok = there && tokb + r <= col.last;
-      s[i][r] = ok ? s[i][r] * scale_log2 : q3::kNegInf;
-      mx = fmaxf(mx, s[i][r]);
-      // a slot at or behind L may hold anything; P is 0 there, but 0 * NaN is not
-      if (!(there && tokb + r < c.L)) c.v[i][r] = q3::u32x4{0u, 0u, 0u, 0u};
-    }
-  }
-  mx = q3::max_xor32(q3::max_xor16(mx));
-  const float m_new = fmaxf(st.m, mx);
-  const float m_use = m_new == q3::kNegInf ? 0.f : m_new;
-  const float alpha = q3::fast_exp2(st.m - m_use);
-  st.m = m_new;
-  // P as two bf16 terms, p = hi + lo, as the decode carries it: 16 significant bits
-  q3::bf16x4 p[kChunk], pl[kChunk];
-  float psum = 0.f;
-#pragma unroll
-  for (int i = 0; i < kChunk; ++i) {
-    float e[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      e[r] = q3::fast_exp2(s[i][r] - m_use);
-      psum += e[r];
-    }
-    split_p(e, p[i], pl[i]);
-  }
-  st.l = st.l * alpha + psum;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) st.acc[j] *= alpha;
-  // O^T += V^T P^T, as the decode's compute_chunk
-#pragma unroll
-  for (int i = 0; i < kChunk; ++i) {
-    if (i < c.n) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int w = j >> 1, h = j & 1;
-        const q3::u32x2 av = {q3::pick_halves(c.v[i][0][w], c.v[i][1][w], h),
-                              q3::pick_halves(c.v[i][2][w], c.v[i][3][w], h)};
-        st.acc[j] = q3::mfma16x16x16(q3::as_bf16x4(av), p[i], st.acc[j]);
-        st.acc[j] = q3::mfma16x16x16(q3::as_bf16x4(av), pl[i], st.acc[j]);
-      }
-    }
-  }
-}
-
 // Load-side cursor of a wave.
 struct ChunkCursor {
   int64_t g, g1;

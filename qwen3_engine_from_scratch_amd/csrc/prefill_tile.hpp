@@ -9,10 +9,10 @@
 #pragma once
 
 #include "common.hpp"
+#include "head_dim.hpp"
 
 namespace {
 
-constexpr int kD = 128;
 constexpr int kBN = 64;                   // keys per staged K/V tile
 constexpr int kRowBytes = kD * 2;         // one staged key row (256 B)
 constexpr int kTileElems = kBN * kD;      // one staged K or V tile (16 KiB)
