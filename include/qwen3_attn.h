@@ -393,6 +393,43 @@ int qwen3_paged_chunk_bf16(const void* q, const int64_t q_strides[2],
                            size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Decode attention of a batch whose groups of sequences share a prefix (no
+ * counterpart in the reference engine, whose requests share no page): samples of one
+ * prompt, requests behind one system prompt.  The attention of
+ * qwen3_paged_decode_bf16, with a group's prefix read once for all of its sequences.
+ *
+ * Group g is the batch entries cu_groups[g] .. cu_groups[g + 1] - 1 (device int32,
+ * num_groups + 1, ascending); the first shared_lens[g] positions of each of its
+ * sequences must lie in the same pages (those that the table names for the group's
+ * first sequence are read).  A prefix counts as far as the first sequence's length and
+ * in whole multiples of 16; entries of no group, and groups of one, attend alone.
+ * Sequences of a group may be shorter than its prefix; the values of shared positions
+ * behind such a sequence must be finite.
+ *   q .. out    as qwen3_paged_decode_bf16; scale positive and finite
+ *   workspace   qwen3_paged_decode_shared_workspace_bytes(...) bytes, 16-byte aligned,
+ *               no initialisation; calls that share one must not overlap.  Depends on
+ *               the launch shape only, so that a captured call stays valid for any
+ *               lengths and groups
+ * Supported: as qwen3_paged_decode_bf16, up to 1,024 sequences, slot strides from
+ * head_dim to 2^24 elements.  Two launches.
+ * ---------------------------------------------------------------------- */
+size_t qwen3_paged_decode_shared_workspace_bytes(int B, int num_heads, int num_kv_heads,
+                                                 int head_dim);
+
+int qwen3_paged_decode_shared_bf16(const void* q, const int64_t q_strides[2],
+                                   const void* k_cache, const int64_t k_strides[3],
+                                   const void* v_cache, const int64_t v_strides[3],
+                                   int64_t num_blocks, const int32_t* block_table,
+                                   int64_t bt_row_stride, int64_t max_rows,
+                                   int64_t max_pages, const int32_t* seq_lens,
+                                   int seq_len_bias, const int32_t* row_ids,
+                                   const int32_t* cu_groups, const int32_t* shared_lens,
+                                   int num_groups, void* out, const int64_t out_strides[2],
+                                   int B, int num_heads, int num_kv_heads, int head_dim,
+                                   int block_size, float scale, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Fused pre-attention step: QK-RMSNorm + RoPE + K/V pool write.
  *
  * Replaces, in one launch, q_norm / k_norm (qwen3/attention.py:91-92 with

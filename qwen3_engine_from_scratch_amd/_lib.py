@@ -120,6 +120,14 @@ _SIGNATURES = {
          ctypes.POINTER(ctypes.c_int32), _i, _i,
          _i, _i, _i, ctypes.c_float, _i, _vp, ctypes.c_size_t, _vp],
     ),
+    "qwen3_paged_decode_shared_workspace_bytes": (ctypes.c_size_t, [_i, _i, _i, _i]),
+    "qwen3_paged_decode_shared_bf16": (
+        _i,
+        [_vp, _c_i64p, _vp, _c_i64p, _vp, _c_i64p, _i64,
+         _vp, _i64, _i64, _i64, _vp, _i, _vp, _vp, _vp, _i,
+         _vp, _c_i64p,
+         _i, _i, _i, _i, _i, ctypes.c_float, _vp, ctypes.c_size_t, _vp],
+    ),
     "qwen3_paged_chunk_workspace_bytes": (ctypes.c_size_t, [_i, _i, _i64, _i, _i, _i]),
     "qwen3_paged_chunk_bf16": (
         _i,

@@ -1,0 +1,842 @@
+// Paged decode attention of a batch whose groups of sequences share a prefix, for gfx950
+// (GQA, one query token a sequence).
+//
+// Sequence b attends the keys j < L_b of its row of the block table; the first P of them
+// lie in the same pages for all sequences of a group.  With m, l, o the running maximum,
+// sum and weighted mean of some keys,
+//   (m, l, o)[0, L_b) = join((m, l, o)[0, P), (m, l, o)[P, L_b)),
+// so the prefix is attended once, by the rows (sequence, head) of all of the group's
+// sequences packed together, and its K and V are read once instead of once a sequence.
+//
+// One launch attends, a second joins.  In the first, a workgroup does one of two things:
+//  * prefixes of more than 16 rows: K/V tiles of 64 keys staged in LDS (paged_kv_tile.hpp),
+//    three stages, so that the loads of two tiles are on their way while one is computed;
+//    eight waves of 32 rows, 256 rows an item.  The items' tiles lie end to end and are cut
+//    into equal ranges, a workgroup each;
+//  * what each sequence has of its own, and prefixes of up to 16 rows: the streaming
+//    decode's loop (paged_decode.hip), K and V straight into MFMA operands, the 16-key
+//    tiles of all items end to end, cut into equal ranges, a wave each.
+// The workgroups are divided by the tiles' weights.  Parts of cut items, and whole ones
+// that have another half, are left in the workspace (normalised, with the log2 of their
+// sum), and the second launch joins each row's.  P is floored to whole tiles of 16 keys
+// and bounded by what the group's first sequence holds; the rest counts as each
+// sequence's own.  P meets V as two bf16 terms, as in the decode.
+#include <algorithm>
+
+#include "paged_decode_merge.hpp"
+#include "paged_decode_tile.hpp"
+#include "paged_kv_tile.hpp"
+
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kShWaves = kThreads / 64;
+constexpr int kMaxSeqs = 1024;        // sequences, and groups, tabulated in LDS
+constexpr int kRounds = kMaxSeqs / kThreads;
+constexpr int kRowsT = 32 * kShWaves; // rows of an item whose tiles are staged
+constexpr int kRowsS = 16;            // rows of one that is streamed
+constexpr int kMaxWgs = 512;
+// Weights, in streamed tiles of 16 keys, of a staged tile of 64; tiles that a range takes
+// at least.
+constexpr int kStagedUnits = 4;
+constexpr int kMinStaged = 2;
+constexpr int kMinStreamed = 2 * kChunk;
+
+// What the second launch needs of a sequence.
+struct SeqMeta {
+  int32_t own_at, own_n;  // its own tiles of one head: before them in the list, their number
+  int32_t pre_at, pre_n;  // its prefix's, in the list that `kind` says
+  int32_t pre_row;        // first row of the sequence in its group
+  int32_t kind;           // 0: no prefix, 1: streamed, 2: staged
+};
+struct CallMeta {
+  int32_t pw;       // tiles of a wave's range
+  int32_t pt;       // tiles of a workgroup's range
+  int32_t all_t;    // staged tiles of one KV head
+  int32_t pad;
+};
+
+struct SharedArgs {
+  DecodeArgs d;
+  // as the staged tiles' code calls them
+  const uint16_t* k;
+  int64_t k_blk, k_sh;
+  int k_slot;
+  const uint16_t* v;
+  int64_t v_blk, v_sh;
+  int v_slot;
+  int64_t num_blocks;
+  const int32_t* bt;
+  int64_t bt_stride, max_pages;
+  int gpb;
+  double per_group, per_head;
+  // groups
+  const int32_t* cu;      // (groups + 1)
+  const int32_t* shared;  // (groups)
+  int groups;
+  // workspace
+  float* po_s;      // [waves][2][kRowsS][kD] streamed parts
+  float* lse_s;
+  float* po_t;      // [workgroups][2][rows_t][kD] staged parts
+  float* lse_t;
+  float* po_own;    // [B][Hq][kD] whole items that have a prefix
+  float* lse_own;
+  float* po_pre;    // [B][Hq][kD] whole prefixes
+  float* lse_pre;
+  SeqMeta* seqs;
+  CallMeta* call;
+  int rows_t;       // rows of a staged part: kRowsT, or all of a smaller batch
+};
+
+struct Tables {
+  int32_t own[kMaxSeqs + 1];   // own tiles before each sequence
+  int32_t row[kMaxSeqs];
+  int32_t len[kMaxSeqs];
+  int32_t skip[kMaxSeqs];      // tiles of the shared prefix
+  int32_t gs[kMaxSeqs + 1];    // streamed prefix tiles before each group
+  int32_t gt[kMaxSeqs + 1];    // staged ones (of all its row tiles)
+  int32_t g0[kMaxSeqs + 1];    // first sequence
+  int32_t gp[kMaxSeqs];        // tiles of 16 keys of the prefix
+  int32_t wsum[3][kRounds][kShWaves];
+};
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Last index i < n with v[i] <= p (v ascending); -1: none.
+__device__ __forceinline__ int last_at_most(const int32_t* v, int n, int p) {
+  int lo = -1, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (v[mid] <= p) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Sequences of group g (0: not a range of the batch).
+__device__ __forceinline__ int members(const Tables& t, int g, int B) {
+  const int s0 = t.g0[g], s1 = t.g0[g + 1];
+  return s0 >= 0 && s1 > s0 && s1 <= B ? s1 - s0 : 0;
+}
+__device__ __forceinline__ int staged_tiles(int gp) { return (gp * kTile + kBN - 1) / kBN; }
+
+// Tabulates the batch; returns streamed own tiles, streamed prefix tiles and staged tiles
+// of one head.
+template <int R>
+__device__ __forceinline__ void tabulate_shared(const SharedArgs& a, Tables& t, int& all_own,
+                                                int& all_gs, int& all_gt) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int B = a.d.B, NG = a.groups;
+  int64_t row[R];
+  int32_t cap[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int b = i * kThreads + tid;
+    row[i] = row_of(a.d, min(b, B - 1));
+    if (b <= NG) t.g0[b] = a.cu[b];
+    cap[i] = b < NG ? a.shared[b] : 0;
+  }
+  if (R * kThreads == NG && tid == 0) t.g0[NG] = a.cu[NG];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int b = i * kThreads + tid;
+    const int32_t len = a.d.seq_lens[row[i] >= 0 ? row[i] : 0];
+    if (b < B) {
+      t.row[b] = static_cast<int32_t>(row[i]);
+      t.len[b] = static_cast<int32_t>(row[i] >= 0 ? clamp_len(a.d, len) : 0);
+    }
+  }
+  __syncthreads();
+  // a group's prefix: whole tiles of what its first sequence holds
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int g = i * kThreads + tid;
+    if (g < NG) {
+      const int n = members(t, g, B);
+      const int most = n > 1 ? min(cap[i], t.len[t.g0[g]]) : 0;
+      t.gp[g] = most > 0 ? most / kTile : 0;
+    }
+  }
+  __syncthreads();
+  int own[R], gs[R], gt[R], own_i[R], gs_i[R], gt_i[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int b = i * kThreads + tid;
+    int skip = 0;
+    own[i] = gs[i] = gt[i] = 0;
+    if (b < B) {
+      const int g = NG > 0 ? last_at_most(t.g0, NG, b) : -1;
+      if (g >= 0 && b < t.g0[g] + members(t, g, B)) skip = t.gp[g];
+      t.skip[b] = skip;
+      const int tiles = (t.len[b] + kTile - 1) / kTile;
+      own[i] = tiles > skip ? tiles - skip : 0;
+    }
+    if (b < NG) {
+      const int rows = members(t, b, B) * a.d.G, gp = t.gp[b];
+      if (rows > kRowsS) gt[i] = staged_tiles(gp) * ((rows + kRowsT - 1) / kRowsT);
+      else gs[i] = gp;
+    }
+    own_i[i] = wave_prefix_sum(own[i]);
+    gs_i[i] = wave_prefix_sum(gs[i]);
+    gt_i[i] = wave_prefix_sum(gt[i]);
+    if (lane == 63) {
+      t.wsum[0][i][wave] = own_i[i];
+      t.wsum[1][i][wave] = gs_i[i];
+      t.wsum[2][i][wave] = gt_i[i];
+    }
+  }
+  __syncthreads();
+  int run[3] = {0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    int before[3] = {run[0], run[1], run[2]};
+#pragma unroll
+    for (int x = 0; x < 3; ++x)
+#pragma unroll
+      for (int w = 0; w < kShWaves; ++w) {
+        const int s = t.wsum[x][i][w];
+        before[x] += w < wave ? s : 0;
+        run[x] += s;
+      }
+    const int b = i * kThreads + tid;
+    if (b < B) t.own[b] = before[0] + own_i[i] - own[i];
+    if (b < NG) {
+      t.gs[b] = before[1] + gs_i[i] - gs[i];
+      t.gt[b] = before[2] + gt_i[i] - gt[i];
+    }
+  }
+  if (tid == 0) {
+    t.own[B] = run[0];
+    t.gs[NG] = run[1];
+    t.gt[NG] = run[2];
+  }
+  __syncthreads();
+  all_own = uniform(run[0]);
+  all_gs = uniform(run[1]);
+  all_gt = uniform(run[2]);
+}
+
+// How the tiles are divided among the workgroups and waves.
+struct Plan {
+  int64_t streamed, staged;  // tiles of all KV heads
+  int wgs_t;                 // workgroups of staged tiles, the grid's first ones
+  int64_t pw, pt;
+};
+__device__ __forceinline__ Plan plan_of(const SharedArgs& a, int all_s, int all_t) {
+  Plan p;
+  const int N = gridDim.x;
+  p.streamed = static_cast<int64_t>(all_s) * a.d.Hkv;
+  p.staged = static_cast<int64_t>(all_t) * a.d.Hkv;
+  const float wt = static_cast<float>(p.staged) * kStagedUnits, ws = static_cast<float>(p.streamed);
+  int n = all_t == 0 ? 0 : static_cast<int>(N * (wt / (wt + ws)) + 0.5f);
+  if (all_t > 0) n = n < 1 ? 1 : n;
+  if (all_s > 0) n = n > N - 1 ? N - 1 : n;
+  p.wgs_t = uniform(n);
+  p.pt = n > 0 ? q3::cdiv(p.staged, n) : kMinStaged;
+  p.pt = p.pt < kMinStaged ? kMinStaged : p.pt;
+  const int64_t waves = static_cast<int64_t>(N - n) * kShWaves;
+  p.pw = waves > 0 ? q3::cdiv(p.streamed, waves) : kMinStreamed;
+  p.pw = p.pw < kMinStreamed ? kMinStreamed : p.pw;
+  return p;
+}
+
+// The normalised state of column lo (dims 32 hi ..) into a part's row.
+__device__ __forceinline__ void store_part(float* po, const q3::f32x4 (&acc)[8], float inv, int hi) {
+  po += 32 * hi;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    *reinterpret_cast<q3::f32x4*>(po + 8 * r) =
+        q3::f32x4{acc[0][r] * inv, acc[1][r] * inv, acc[2][r] * inv, acc[3][r] * inv};
+    *reinterpret_cast<q3::f32x4*>(po + 8 * r + 4) =
+        q3::f32x4{acc[4][r] * inv, acc[5][r] * inv, acc[6][r] * inv, acc[7][r] * inv};
+  }
+}
+
+// ---- streamed tiles: one wave --------------------------------------------------------
+
+// An item of the streamed list: a sequence's own keys, or a group's prefix.
+struct StreamItem {
+  int e;       // sequence, or B + group
+  int n;       // tiles
+  int t0;      // first tile of the sequence
+  int L;       // end of its keys
+  int row;     // of the block table
+};
+
+__device__ __forceinline__ StreamItem stream_item(const SharedArgs& a, const Tables& t, int e) {
+  const int B = a.d.B;
+  StreamItem s;
+  s.e = e;
+  if (e < B) {
+    s.n = uniform(t.own[e + 1] - t.own[e]);
+    s.t0 = uniform(t.skip[e]);
+    s.L = uniform(t.len[e]);
+    s.row = uniform(t.row[e]);
+  } else {
+    const int g = e - B;
+    s.n = uniform(t.gs[g + 1] - t.gs[g]);
+    s.t0 = 0;
+    s.L = s.n * kTile;
+    s.row = s.n > 0 ? uniform(t.row[t.g0[g]]) : -1;
+  }
+  return s;
+}
+
+__device__ __forceinline__ void stream_range(const SharedArgs& a, const Tables& t, int all_own, int64_t w,
+                             int64_t g0, int64_t g1) {
+  const DecodeArgs& d = a.d;
+  const int lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
+  const int B = d.B, entries = B + a.groups;
+  const int64_t own_end = static_cast<int64_t>(d.Hkv) * all_own;
+
+  StreamItem cur;
+  int hkv, at;  // the next tile to load: its KV head and place in the item
+  int64_t g = g0;
+  {
+    int e, before;
+    if (g0 < own_end) {
+      e = uniform(last_at_most(t.own, B, static_cast<int>(g0 / d.Hkv)));
+      // (heads lie inside a sequence: its tiles begin at Hkv * own)
+      before = uniform(t.own[e]);
+    } else {
+      const int p = static_cast<int>((g0 - own_end) / d.Hkv);
+      e = uniform(last_at_most(t.gs, a.groups, p));
+      before = all_own + uniform(t.gs[e]);
+      e += B;
+    }
+    cur = stream_item(a, t, e);
+    const int64_t off = g0 - static_cast<int64_t>(d.Hkv) * before;
+    hkv = static_cast<int>(off / cur.n);
+    at = static_cast<int>(off % cur.n);
+  }
+  TableWindow tw;
+  window_load(tw, d, cur.row, ((cur.t0 + at) * kTile) / d.bs, lane);
+
+  StreamItem load = cur;
+  auto issue = [&](Chunk& c) {
+    c.n = 0;
+    if (g >= g1) return;
+    if (at >= load.n) {  // the next item
+      if (++hkv == d.Hkv) {
+        hkv = 0;
+        int e = load.e;
+        do {
+          ++e;
+          load = stream_item(a, t, e);
+        } while (load.n == 0 && e + 1 < entries);
+      }
+      at = 0;
+      window_load(tw, d, load.row, (load.t0 * kTile) / d.bs, lane);
+    }
+    const int64_t left = g1 - g;
+    int n = load.n - at;
+    n = n < kChunk ? n : kChunk;
+    n = left < n ? static_cast<int>(left) : n;
+    c.n = n;
+    c.t0 = load.t0 + at;
+    c.seg = load.e * d.Hkv + hkv;
+    c.ntiles = load.n;
+    c.L = load.L;
+    const uint16_t* kbase = d.k + static_cast<int64_t>(hkv) * d.k_sh;
+    const uint16_t* vbase = d.v + static_cast<int64_t>(hkv) * d.v_sh;
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) {
+      int64_t phys = -1;
+      int sub = 0;
+      if (i < n) {
+        const int tok0 = (c.t0 + i) * kTile;
+        phys = window_phys(tw, d, tok0 / d.bs, lane);
+        sub = tok0 % d.bs;
+      }
+      load_tile(c, i, d, kbase, vbase, phys, sub, lo, hi);
+    }
+    at += n;
+    g += n;
+  };
+
+  // the item being accumulated
+  int cseg = -1, ce = 0, chkv = 0, ct_lo = 0, ct_hi = 0, cn = 0, cskip = 0;
+  int cb = 0, chead = 0;     // this lane's sequence and query head
+  bool clane = false;        // the lane's column is a row of the item
+  bool cfirst = true;
+  Columns col;
+
+  auto begin = [&](const Chunk& c) {
+    ce = c.seg / d.Hkv;
+    chkv = c.seg % d.Hkv;
+    ct_lo = c.t0;
+    cn = c.ntiles;
+    int s = 0, head = lo;
+    if (ce < B) {
+      cb = ce;
+      clane = lo < d.G;
+      cskip = uniform(t.skip[ce]);
+    } else {
+      const int grp = ce - B;
+      s = divide(lo, a.per_head);
+      head = lo - s * d.G;
+      clane = s < uniform(t.g0[grp + 1] - t.g0[grp]);
+      cb = uniform(t.g0[grp]) + (clane ? s : 0);
+      cskip = 0;
+    }
+    chead = chkv * d.G + (clane ? head : 0);
+    col.last = min(c.L, t.len[cb]) - 1;
+    reset(col.st);
+    const uint16_t* qp = d.q + cb * d.q_sb + static_cast<int64_t>(chead) * d.q_sh + hi * 8;
+#pragma unroll
+    for (int cc = 0; cc < 4; ++cc)
+      col.q[cc] = q3::as_bf16x8(clane ? q3::ld16(qp + cc * 32) : q3::u32x4{0u, 0u, 0u, 0u});
+  };
+
+  auto finish = [&]() {
+    const float l = q3::sum_xor32(q3::sum_xor16(col.st.l));
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    if (!clane) return;
+    const bool whole = ct_hi - ct_lo == cn;
+    if (whole && ce < B && cskip == 0) {
+      store_out_bf16(d, cb, chead, col.st.acc, inv, hi);
+      return;
+    }
+    const float lse = l > 0.f ? col.st.m + __builtin_log2f(l) : q3::kNegInf;
+    float* po;
+    float* pl;
+    if (whole) {
+      const int64_t row = static_cast<int64_t>(cb) * d.Hq + chead;
+      po = (ce < B ? a.po_own : a.po_pre) + row * kD;
+      pl = (ce < B ? a.lse_own : a.lse_pre) + row;
+    } else {
+      const int64_t slot = (w * 2 + (cfirst ? 0 : 1)) * kRowsS + lo;
+      po = a.po_s + slot * kD;
+      pl = a.lse_s + slot;
+    }
+    store_part(po, col.st.acc, inv, hi);
+    if (hi == 0) *pl = lse;
+  };
+
+  auto process = [&](Chunk& c) {
+    if (c.seg != cseg) {
+      if (cseg >= 0) {
+        finish();
+        cfirst = false;
+      }
+      cseg = c.seg;
+      begin(c);
+    }
+    fold_chunk(c, d.scale_log2, hi, col);
+    ct_hi = c.t0 + c.n;
+  };
+
+  Chunk ca, cbuf;
+  issue(ca);
+  issue(cbuf);
+  while (true) {
+    if (ca.n == 0) break;
+    process(ca);
+    issue(ca);
+    if (cbuf.n == 0) break;
+    process(cbuf);
+    issue(cbuf);
+  }
+  if (cseg >= 0) finish();
+}
+
+// ---- staged tiles: one workgroup ------------------------------------------------------
+
+struct Stage {
+  uint16_t* k;
+  uint16_t* v;
+};
+
+__device__ __forceinline__ void staged_range(const SharedArgs& a, const Tables& t, int all_t, int v, int64_t p0,
+                             int64_t p1, const Stage (&st)[3]) {
+  const DecodeArgs& d = a.d;
+  constexpr int W = kShWaves;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = uniform(tid >> 6);
+  const LaneOffsets off = lane_offsets<W>(a, lane, wave);
+  int64_t p = p0;
+  while (p < p1) {
+    const int kvh = uniform(static_cast<int>(p / all_t));
+    const int in = static_cast<int>(p - static_cast<int64_t>(kvh) * all_t);
+    const int grp = uniform(last_at_most(t.gt, a.groups, in));
+    const int keys = uniform(t.gp[grp]) * kTile;
+    const int tiles = (keys + kBN - 1) / kBN;
+    const int s0 = uniform(t.g0[grp]), rows = uniform(t.g0[grp + 1] - t.g0[grp]) * d.G;
+    const int mt = uniform((in - t.gt[grp]) / tiles);
+    const int j0 = in - uniform(t.gt[grp]) - mt * tiles;
+    const int64_t left = p1 - p;
+    const int j1 = left < tiles - j0 ? j0 + static_cast<int>(left) : tiles;
+
+    // this wave's 32 rows: lane l holds row r0 + l % 32
+    const int r0 = mt * kRowsT + wave * 32, r = r0 + (lane & 31);
+    const bool active = r0 < rows, mine = r < rows;
+    const int s = divide(mine ? r : 0, a.per_head);
+    const int b = s0 + s, head = kvh * d.G + ((mine ? r : 0) - s * d.G);
+    const int last = (mine ? min(t.len[b], keys) : keys) - 1;
+    int lo_last = last;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) lo_last = min(lo_last, __shfl_xor(lo_last, o, 64));
+    lo_last = uniform(lo_last);
+
+    PageWindow pw;
+    window_start(pw, a, uniform(t.row[s0]), j0, lane);
+    window_check(pw, a);
+    const ItemKeys ks{a.k + kvh * a.k_sh, a.v + kvh * a.v_sh, uniform(t.row[s0]), keys};
+    uint32_t ok[3];
+    ok[0] = tile_dma<W>(a, off, pw, ks, j0, st[0].k, st[0].v, wave, lane);
+    if (j0 + 1 < j1) ok[1] = tile_dma<W>(a, off, pw, ks, j0 + 1, st[1].k, st[1].v, wave, lane);
+    q3::bf16x8 qv[8];
+    {
+      const uint16_t* qp = d.q + b * d.q_sb + static_cast<int64_t>(head) * d.q_sh + 8 * (lane >> 5);
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        qv[c] = q3::as_bf16x8(mine ? q3::ld16(qp + 16 * c) : q3::u32x4{0u, 0u, 0u, 0u});
+    }
+    float m_run = q3::kNegInf, l_run = 0.f;
+    q3::f32x16 acc[4];
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) acc[db][x] = 0.f;
+
+    auto step = [&](int j, const Stage& here, uint32_t okh, const Stage& next, uint32_t& okn) {
+      wait_loads();
+      __syncthreads();
+      if (j + 2 < j1) okn = tile_dma<W>(a, off, pw, ks, j + 2, next.k, next.v, wave, lane);
+      if (!active) return;
+      const int n0 = j * kBN;
+      auto mask = [&](q3::f32x16 (&x)[2]) {
+        if (n0 + kBN - 1 > lo_last || okh != 15u) {
+          const int lim = last - n0 - 4 * (lane >> 5);
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int kr = kb * 32 + 8 * (i / 4) + (i % 4);
+              const int l = (okh >> (2 * kb + i / 8)) & 1u ? lim : -1;
+              x[kb][i] = kr <= l ? x[kb][i] : q3::kNegInf;
+            }
+        }
+      };
+      tile_fold<true>(off, d.scale_log2, mask, here.k, here.v, qv, m_run, l_run, acc);
+    };
+    for (int j = j0; j < j1; j += 3) {
+      step(j, st[0], ok[0], st[2], ok[2]);
+      if (j + 1 < j1) step(j + 1, st[1], ok[1], st[0], ok[0]);
+      if (j + 2 < j1) step(j + 2, st[2], ok[2], st[1], ok[1]);
+    }
+    l_run = cross_half_sum(l_run);
+    if (mine) {
+      const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+      float* po;
+      float* pl;
+      if (j1 - j0 == tiles) {
+        const int64_t row = static_cast<int64_t>(b) * d.Hq + head;
+        po = a.po_pre + row * kD;
+        pl = a.lse_pre + row;
+      } else {
+        const int64_t row = (2 * static_cast<int64_t>(v) + (j0 == 0 ? 1 : 0)) * a.rows_t + (r - mt * kRowsT);
+        po = a.po_t + row * kD;
+        pl = a.lse_t + row;
+      }
+      po += 4 * (lane >> 5);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        *reinterpret_cast<q3::f32x4*>(po + 8 * i) =
+            q3::f32x4{acc[i >> 2][4 * (i & 3)] * inv, acc[i >> 2][4 * (i & 3) + 1] * inv,
+                      acc[i >> 2][4 * (i & 3) + 2] * inv, acc[i >> 2][4 * (i & 3) + 3] * inv};
+      if (lane < 32) *pl = l_run > 0.f ? m_run + __builtin_log2f(l_run) : q3::kNegInf;
+    }
+    p += j1 - j0;
+    __syncthreads();  // the stages are read before the next item's loads refill them
+  }
+}
+
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void paged_shared_kernel(SharedArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint16_t s_k0[kTileElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t s_v0[kTileElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t s_k1[kTileElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t s_v1[kTileElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t s_k2[kTileElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t s_v2[kTileElems];
+  __shared__ Tables t;
+  const int tid = threadIdx.x, wave = uniform(tid >> 6);
+  int all_own, all_gs, all_t;
+  if (a.d.B <= kThreads && a.groups < kThreads)
+    tabulate_shared<1>(a, t, all_own, all_gs, all_t);
+  else
+    tabulate_shared<kRounds>(a, t, all_own, all_gs, all_t);
+  const Plan plan = plan_of(a, all_own + all_gs, all_t);
+  if (blockIdx.x == gridDim.x - 1) {
+    for (int b = tid; b < a.d.B; b += kThreads) {
+      SeqMeta m{};
+      m.own_at = t.own[b];
+      m.own_n = t.own[b + 1] - t.own[b];
+      if (t.skip[b] > 0) {
+        const int g = last_at_most(t.g0, a.groups, b);
+        const int rows = members(t, g, a.d.B) * a.d.G;
+        m.kind = rows > kRowsS ? 2 : 1;
+        m.pre_at = m.kind == 2 ? t.gt[g] : all_own + t.gs[g];
+        m.pre_n = m.kind == 2 ? staged_tiles(t.gp[g]) : t.gp[g];
+        m.pre_row = (b - t.g0[g]) * a.d.G;
+      }
+      a.seqs[b] = m;
+    }
+    if (tid == 0)
+      *a.call = CallMeta{static_cast<int32_t>(plan.pw), static_cast<int32_t>(plan.pt), all_t, 0};
+  }
+  const int v = blockIdx.x;
+  if (v < plan.wgs_t) {
+    const int64_t p0 = v * plan.pt, p1 = p0 + plan.pt;
+    const Stage st[3] = {{s_k0, s_v0}, {s_k1, s_v1}, {s_k2, s_v2}};
+    if (p0 < plan.staged)
+      staged_range(a, t, all_t, v, p0, p1 < plan.staged ? p1 : plan.staged, st);
+    return;
+  }
+  // a batch too small for every wave is dealt one wave a workgroup first
+  const int64_t N = gridDim.x - plan.wgs_t, at = v - plan.wgs_t;
+  const bool spread = plan.streamed <= (N * kShWaves - 1) * plan.pw;
+  const int64_t w = spread ? static_cast<int64_t>(wave) * N + at : at * kShWaves + wave;
+  const int64_t g0 = w * plan.pw, g1 = g0 + plan.pw;
+  if (g0 < plan.streamed)
+    stream_range(a, t, all_own, w, g0, g1 < plan.streamed ? g1 : plan.streamed);
+}
+
+// ---- the join ---------------------------------------------------------------------------
+
+// Parts of a row: `n` slots from `first` on, `step` apart; the first one may lie elsewhere.
+struct Parts {
+  const float* po;
+  const float* lse;
+  int64_t first, next;  // rows of po: of part 0, of part i > 0: next + i * step
+  int step, n;
+};
+
+// One workgroup per (KV head, sequence), one wave per query head of the group: lane i
+// fetches the sums of part i of up to 64 parts at once, then every lane owns two
+// dimensions and sums the weighted parts, kBatch loads in flight.
+__global__ __launch_bounds__(kMaxG * 64) void paged_shared_join_kernel(SharedArgs a) {
+  constexpr int kBatch = 8;
+  const DecodeArgs& d = a.d;
+  const int lane = threadIdx.x & 63;
+  const int g = uniform(threadIdx.x >> 6);
+  const int hkv = blockIdx.x, b = blockIdx.y;
+  const int hq = hkv * d.G + g;
+  const SeqMeta m = a.seqs[b];
+  const CallMeta call = *a.call;
+  const int64_t direct = static_cast<int64_t>(b) * d.Hq + hq;
+
+  Parts part[2];
+  part[0].n = part[1].n = 0;
+  // a streamed item's parts: `col` its column of this row
+  auto streamed = [&](Parts& x, const float* po, const float* lse, int before, int n, int col) {
+    if (n == 0) return;
+    const int64_t S = static_cast<int64_t>(d.Hkv) * before + static_cast<int64_t>(hkv) * n;
+    const int64_t wf = S / call.pw, wl = (S + n - 1) / call.pw;
+    x.n = static_cast<int>(wl - wf + 1);
+    if (wf == wl) {
+      x.po = po;
+      x.lse = lse;
+      x.first = x.next = direct;
+      x.step = 0;
+      return;
+    }
+    x.po = a.po_s;
+    x.lse = a.lse_s;
+    x.first = (2 * wf + (wf * call.pw != S ? 1 : 0)) * kRowsS + col;
+    x.step = 2 * kRowsS;
+    x.next = 2 * wf * kRowsS + col;
+  };
+  streamed(part[0], a.po_own, a.lse_own, m.own_at, m.own_n, g);
+  if (m.kind == 0 && part[0].n == 1) return;  // written whole
+  if (m.kind == 1) {
+    streamed(part[1], a.po_pre, a.lse_pre, m.pre_at, m.pre_n, m.pre_row + g);
+  } else if (m.kind == 2) {
+    const int r = m.pre_row + g, mt = r / kRowsT;
+    const int64_t S = static_cast<int64_t>(hkv) * call.all_t + m.pre_at + static_cast<int64_t>(mt) * m.pre_n;
+    const int64_t vf = S / call.pt, vl = (S + m.pre_n - 1) / call.pt;
+    Parts& x = part[1];
+    x.n = static_cast<int>(vl - vf + 1);
+    if (vf == vl) {
+      x.po = a.po_pre;
+      x.lse = a.lse_pre;
+      x.first = x.next = direct;
+      x.step = 0;
+    } else {
+      x.po = a.po_t;
+      x.lse = a.lse_t;
+      const int row = r - mt * kRowsT;
+      x.first = (2 * vf + 1) * a.rows_t + row;
+      x.step = 2 * a.rows_t;
+      x.next = 2 * vf * a.rows_t + row;
+    }
+  }
+  float M = q3::kNegInf, sw = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const Parts& x = part[h];
+    for (int i0 = 0; i0 < x.n; i0 += 64) {
+      const int i = i0 + lane;
+      const float lse = i < x.n ? x.lse[i == 0 ? x.first : x.next + static_cast<int64_t>(i) * x.step]
+                                : q3::kNegInf;
+      float top = lse;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, q3::shfl_xor(top, o));
+      const float m_new = fmaxf(M, top), use = m_new == q3::kNegInf ? 0.f : m_new;
+      const float f = q3::fast_exp2(M - use);
+      M = m_new;
+      const float wt = q3::fast_exp2(lse - use);
+      float wsum = wt;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) wsum += q3::shfl_xor(wsum, o);
+      sw = sw * f + wsum;
+      o0 *= f;
+      o1 *= f;
+      const int cnt = min(64, x.n - i0);
+      for (int j0 = 0; j0 < cnt; j0 += kBatch) {
+        float2 ov[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int i = min(i0 + j0 + j, x.n - 1);
+          const int64_t row = i == 0 ? x.first : x.next + static_cast<int64_t>(i) * x.step;
+          ov[j] = *reinterpret_cast<const float2*>(x.po + row * kD + 2 * lane);
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const float u = j0 + j < cnt ? __shfl(wt, j0 + j, 64) : 0.f;
+          o0 += u * ov[j].x;
+          o1 += u * ov[j].y;
+        }
+      }
+    }
+  }
+  const float inv = sw > 0.f ? 1.f / sw : 0.f;
+  *reinterpret_cast<uint32_t*>(d.out + b * d.o_sb + hq * d.o_sh + 2 * lane) =
+      q3::pack_bf16x2(o0 * inv, o1 * inv);
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+
+// One workgroup a CU (its LDS); 256 where no device can be asked.
+int shared_workgroups() {
+  const int cus = cu_count();
+  const int wgs = cus > 0 ? cus : 256;
+  return wgs < kMaxWgs ? wgs : kMaxWgs;
+}
+
+struct SharedLayout {
+  int64_t po_s, lse_s, po_t, lse_t, po_own, lse_own, po_pre, lse_pre, seqs, call, total;
+  int rows_t;
+};
+SharedLayout shared_layout(int B, int num_heads, int G) {
+  const int64_t wgs = shared_workgroups();
+  const int64_t slots = wgs * kShWaves * 2 * kRowsS, rows = static_cast<int64_t>(B) * num_heads;
+  SharedLayout l;
+  l.rows_t = static_cast<int>(std::min<int64_t>(kRowsT, static_cast<int64_t>(B) * G));
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += align256(bytes);
+    return here;
+  };
+  l.po_s = take(slots * kD * 4);
+  l.lse_s = take(slots * 4);
+  l.po_t = take(wgs * 2 * l.rows_t * kD * 4);
+  l.lse_t = take(wgs * 2 * l.rows_t * 4);
+  l.po_own = take(rows * kD * 4);
+  l.lse_own = take(rows * 4);
+  l.po_pre = take(rows * kD * 4);
+  l.lse_pre = take(rows * 4);
+  l.seqs = take(B * static_cast<int64_t>(sizeof(SeqMeta)));
+  l.call = take(sizeof(CallMeta));
+  l.total = at;
+  return l;
+}
+
+}  // namespace
+
+extern "C" size_t qwen3_paged_decode_shared_workspace_bytes(int B, int num_heads,
+                                                            int num_kv_heads, int head_dim) {
+  if (B <= 0 || B > kMaxSeqs || num_heads <= 0 || num_kv_heads <= 0 ||
+      num_heads % num_kv_heads != 0 || num_heads / num_kv_heads > kMaxG || head_dim != kD)
+    return 0;
+  return static_cast<size_t>(shared_layout(B, num_heads, num_heads / num_kv_heads).total);
+}
+
+extern "C" int qwen3_paged_decode_shared_bf16(
+    const void* q, const int64_t q_strides[2], const void* k_cache, const int64_t k_strides[3],
+    const void* v_cache, const int64_t v_strides[3], int64_t num_blocks,
+    const int32_t* block_table, int64_t bt_row_stride, int64_t max_rows, int64_t max_pages,
+    const int32_t* seq_lens, int seq_len_bias, const int32_t* row_ids, const int32_t* cu_groups,
+    const int32_t* shared_lens, int num_groups, void* out, const int64_t out_strides[2], int B,
+    int num_heads, int num_kv_heads, int head_dim, int block_size, float scale, void* workspace,
+    size_t workspace_bytes, void* stream) {
+  const char* who = "qwen3_paged_decode_shared_bf16";
+  SharedArgs a{};
+  if (int rc = prepare(a.d, who, q, q_strides, k_cache, k_strides, v_cache, v_strides, num_blocks,
+                       block_table, bt_row_stride, max_rows, max_pages, seq_lens,
+                       seq_len_bias, row_ids, out, out_strides, B, num_heads, num_kv_heads,
+                       head_dim, block_size, scale))
+    return rc;
+  if (!cu_groups || (num_groups > 0 && !shared_lens))
+    return q3::fail(QWEN3_EINVAL, "%s: null pointer argument", who);
+  if (num_groups < 0 || num_groups > B)
+    return q3::fail(QWEN3_EINVAL, "%s: %d groups of %d sequences", who, num_groups, B);
+  if (B > kMaxSeqs)
+    return q3::fail(QWEN3_EUNSUPPORTED, "%s: %d sequences (at most %d)", who, B, kMaxSeqs);
+  if (!(scale > 0.f) || !(scale < __builtin_inff()))
+    return q3::fail(QWEN3_EINVAL, "%s: scale must be positive and finite", who);
+  // Rows behind a descriptor's end must lie outside it, and 16 of them inside 32-bit offsets.
+  for (int64_t st : {k_strides[2], v_strides[2]})
+    if (st < kD || st > (int64_t(1) << 24))
+      return q3::fail(QWEN3_EUNSUPPORTED, "%s: slot stride %lld outside %d..2^24", who,
+                      (long long)st, kD);
+  // tiles are counted in 32 bits
+  if (static_cast<int64_t>(B) * 2 * max_pages * (block_size / kTile) > 0x7fffffff)
+    return q3::fail(QWEN3_EINVAL, "%s: batch %d times %lld pages too large", who, B,
+                    (long long)max_pages);
+  if (B == 0) return QWEN3_OK;
+  const SharedLayout l = shared_layout(B, num_heads, a.d.G);
+  if (!workspace || workspace_bytes < static_cast<size_t>(l.total))
+    return q3::fail(QWEN3_EWORKSPACE, "%s: workspace of %lld bytes needed, %zu given", who,
+                    (long long)l.total, workspace ? workspace_bytes : (size_t)0);
+  if (!q3::aligned16(workspace))
+    return q3::fail(QWEN3_EALIGN, "%s: workspace must be 16-byte aligned", who);
+  a.k = a.d.k;
+  a.k_blk = a.d.k_sblk;
+  a.k_sh = a.d.k_sh;
+  a.k_slot = static_cast<int>(a.d.k_sslot);
+  a.v = a.d.v;
+  a.v_blk = a.d.v_sblk;
+  a.v_sh = a.d.v_sh;
+  a.v_slot = static_cast<int>(a.d.v_sslot);
+  a.num_blocks = num_blocks;
+  a.bt = block_table;
+  a.bt_stride = bt_row_stride;
+  a.max_pages = max_pages;
+  a.gpb = block_size / kGroup;
+  a.per_group = 1. / a.gpb;
+  a.per_head = 1. / a.d.G;
+  a.cu = cu_groups;
+  a.shared = shared_lens;
+  a.groups = num_groups;
+  char* ws = static_cast<char*>(workspace);
+  a.po_s = reinterpret_cast<float*>(ws + l.po_s);
+  a.lse_s = reinterpret_cast<float*>(ws + l.lse_s);
+  a.po_t = reinterpret_cast<float*>(ws + l.po_t);
+  a.lse_t = reinterpret_cast<float*>(ws + l.lse_t);
+  a.po_own = reinterpret_cast<float*>(ws + l.po_own);
+  a.lse_own = reinterpret_cast<float*>(ws + l.lse_own);
+  a.po_pre = reinterpret_cast<float*>(ws + l.po_pre);
+  a.lse_pre = reinterpret_cast<float*>(ws + l.lse_pre);
+  a.seqs = reinterpret_cast<SeqMeta*>(ws + l.seqs);
+  a.call = reinterpret_cast<CallMeta*>(ws + l.call);
+  a.rows_t = l.rows_t;
+  const auto s = static_cast<hipStream_t>(stream);
+  q3::clear_error();
+  hipLaunchKernelGGL(paged_shared_kernel, dim3(shared_workgroups()), dim3(kThreads), 0, s, a);
+  if (const int rc = q3::launch_status(who)) return rc;
+  hipLaunchKernelGGL(paged_shared_join_kernel, dim3(num_kv_heads, B), dim3(64 * a.d.G), 0, s, a);
+  return q3::launch_status(who);
+}

@@ -19,11 +19,13 @@ from .. import _lib
 __all__ = [
     "paged_attention_decode_hip",
     "paged_attention_chunk_hip",
+    "paged_attention_decode_shared_hip",
     "hip_paged_attention_decode",
     "hip_paged_attention_decode_batch",
     "update_kv_batch_hip",
     "paged_decode_workspace_bytes",
     "paged_chunk_workspace_bytes",
+    "paged_decode_shared_workspace_bytes",
     # reference names
     "paged_attention_decode_triton",
     "triton_paged_attention_decode",
@@ -280,6 +282,104 @@ def paged_attention_chunk_hip(q, k_buffer, v_buffer, block_table_2d, seq_lens_fu
             B, max_chunk, T, num_heads, num_kv_heads, head_dim, block_size, scale,
             workspace.data_ptr(), need, _lib.stream_of(dev))
     _lib.check(rc, "qwen3_paged_chunk_bf16")
+    return out
+
+
+def paged_decode_shared_workspace_bytes(batch: int, num_heads: int, num_kv_heads: int,
+                                        head_dim: int) -> int:
+    """Workspace size of paged_attention_decode_shared_hip on the current device; depends
+    only on the launch shape, so a captured call stays valid for any lengths and groups."""
+    return _shared_workspace(torch.cuda.current_device() if torch.cuda.is_initialized() else -1,
+                             batch, num_heads, num_kv_heads, head_dim)
+
+
+@functools.lru_cache(maxsize=1024)
+def _shared_workspace(device: int, *shape) -> int:
+    return int(_lib.load().qwen3_paged_decode_shared_workspace_bytes(*shape))
+
+
+@functools.lru_cache(maxsize=1024)
+def _shared_layout(q, k, v, table, lens, cu, shared, k_stride, v_stride, table_stride, types,
+                   block_size, own_rows):
+    """The checks of paged_attention_decode_shared_hip that go by shapes, strides and types
+    alone (kept by those, as _chunk_layout's), and what it takes from them."""
+    bf16, i32 = torch.bfloat16, torch.int32
+    assert len(q) == 3
+    B, num_heads, head_dim = q
+    num_blocks, num_kv_heads, block_size_check, head_dim_check = k
+    assert block_size_check == block_size and head_dim_check == head_dim
+    assert v == k
+    assert types == (bf16, bf16, bf16, i32, i32, i32, i32), \
+        "HIP shared-prefix kernel is bf16 only; tables, lengths and groups are int32"
+    assert len(table) == 2 and table_stride[1] == 1, "block_table_2d rows must be contiguous"
+    assert len(lens) == 1 and lens[0] >= table[0]
+    assert len(cu) == 1 and len(shared) == 1 and cu[0] == shared[0] + 1, \
+        "cu_groups has one entry more than shared_lens"
+    assert shared[0] <= B, "more groups than sequences"
+    assert k_stride[3] == 1 and v_stride[3] == 1
+    if own_rows:
+        assert B <= table[0], "more sequences than rows of the block table"
+    return B, num_heads, num_kv_heads, head_dim, num_blocks, (table_stride[0], *table)
+
+
+def paged_attention_decode_shared_hip(q, k_buffer, v_buffer, block_table_2d, seq_lens_full,
+                                      row_ids, cu_groups, shared_lens, block_size, *,
+                                      seq_len_bias: int = 1, scale: float | None = None,
+                                      out: torch.Tensor | None = None,
+                                      workspace: torch.Tensor | None = None):
+    """paged_attention_decode_hip for a batch whose groups of sequences share a prefix
+    (forks of one handle): the prefix's pages are read once for all of a group.
+
+    q, k_buffer/v_buffer, block_table_2d, seq_lens_full, row_ids: as there; up to 1,024
+                    sequences, a group's sequences next to each other
+    cu_groups:      int32 (num_groups + 1,), ascending: group g is the batch entries
+                    cu_groups[g] .. cu_groups[g + 1] - 1
+    shared_lens:    int32 (num_groups,): the tokens that all of the group's sequences hold
+                    in the same pages (counted in whole multiples of 16, and as far as the
+                    group's first sequence goes).  PagedKVcache.shared_prefix_groups
+                    makes both from handles
+    Returns out (B, num_heads, head_dim) bf16.  Entries of no group attend alone.  Groups
+    and lengths are read on the device: a captured call follows them.  workspace:
+    paged_decode_shared_workspace_bytes(...) bytes, a fresh one per call by default.
+    """
+    B, num_heads, num_kv_heads, head_dim, num_blocks, table = _shared_layout(
+        q.shape, k_buffer.shape, v_buffer.shape, block_table_2d.shape, seq_lens_full.shape,
+        cu_groups.shape, shared_lens.shape, k_buffer.stride(), v_buffer.stride(),
+        block_table_2d.stride(),
+        (q.dtype, k_buffer.dtype, v_buffer.dtype, block_table_2d.dtype, seq_lens_full.dtype,
+         cu_groups.dtype, shared_lens.dtype), block_size, row_ids is None)
+    if row_ids is not None:
+        assert row_ids.dtype is torch.int32 and row_ids.numel() == B
+        row_ids = row_ids.contiguous()
+    dev = _lib.require_hip(q, k_buffer, v_buffer, block_table_2d, seq_lens_full, row_ids,
+                           cu_groups, shared_lens, out, workspace)
+    seq_lens_full = seq_lens_full.contiguous()
+    cu_groups = cu_groups.contiguous()
+    shared_lens = shared_lens.contiguous()
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    if scale is None:
+        scale = 1.0 / math.sqrt(head_dim)
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        assert out.shape == q.shape and out.dtype is torch.bfloat16 and out.stride(2) == 1, \
+            "out must be a bf16 (B, num_heads, head_dim) tensor with unit last stride"
+    if B == 0:
+        return out
+    strides = _lib.outer_strides
+    with _lib.on_device(dev):
+        need = _shared_workspace(dev.index, B, num_heads, num_kv_heads, head_dim)
+        if workspace is None or workspace.numel() * workspace.element_size() < need:
+            workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        rc = _lib.load().qwen3_paged_decode_shared_bf16(
+            q.data_ptr(), strides(q), k_buffer.data_ptr(), strides(k_buffer),
+            v_buffer.data_ptr(), strides(v_buffer), num_blocks,
+            block_table_2d.data_ptr(), *table, seq_lens_full.data_ptr(), seq_len_bias,
+            _lib.ptr(row_ids), cu_groups.data_ptr(), shared_lens.data_ptr(), shared_lens.shape[0],
+            out.data_ptr(), strides(out), B, num_heads, num_kv_heads, head_dim, block_size,
+            scale, workspace.data_ptr(), need, _lib.stream_of(dev))
+    _lib.check(rc, "qwen3_paged_decode_shared_bf16")
     return out
 
 
