@@ -10,8 +10,8 @@
 //
 // One launch attends, a second joins.  In the first, a workgroup does one of two things:
 //  * prefixes of more than 16 rows: K/V tiles of 64 keys staged in LDS (paged_kv_tile.hpp),
-//    three stages, so that the loads of two tiles are on their way while one is computed;
-//    eight waves of 32 rows, 256 rows an item.  The items' tiles lie end to end and are cut
+//    four stages, so that the loads of three tiles are on their way while one is computed;
+//    eight waves, 128 rows an item.  The items' tiles lie end to end and are cut
 //    into equal ranges, a workgroup each;
 //  * what each sequence has of its own, and prefixes of up to 16 rows: the streaming
 //    decode's loop (paged_decode.hip), K and V straight into MFMA operands, the 16-key
@@ -33,12 +33,14 @@ constexpr int kThreads = 512;
 constexpr int kShWaves = kThreads / 64;
 constexpr int kMaxSeqs = 1024;        // sequences, and groups, tabulated in LDS
 constexpr int kRounds = kMaxSeqs / kThreads;
-constexpr int kRowsT = 32 * kShWaves; // rows of an item whose tiles are staged
+constexpr int kRowsT = 128;           // rows of an item whose tiles are staged
 constexpr int kRowsS = 16;            // rows of one that is streamed
 constexpr int kMaxWgs = 512;
-// Weights, in streamed tiles of 16 keys, of a staged tile of 64; tiles that a range takes
-// at least.
-constexpr int kStagedUnits = 4;
+constexpr int kStages = 4;
+// Weight, in streamed tiles of 16 keys, of a staged tile of 64; what an item's start and
+// end weigh, in staged tiles; tiles that a range takes at least.
+constexpr int kStagedUnits = 6;
+constexpr int kItemTiles = 4;
 constexpr int kMinStaged = 2;
 constexpr int kMinStreamed = 2 * kChunk;
 
@@ -88,22 +90,24 @@ struct SharedArgs {
   int rows_t;       // rows of a staged part: kRowsT, or all of a smaller batch
 };
 
+constexpr int kNoGroup = 0xffff;
 struct Tables {
   int32_t own[kMaxSeqs + 1];   // own tiles before each sequence
   int32_t row[kMaxSeqs];
   int32_t len[kMaxSeqs];
-  int32_t skip[kMaxSeqs];      // tiles of the shared prefix
   int32_t gs[kMaxSeqs + 1];    // streamed prefix tiles before each group
-  int32_t gt[kMaxSeqs + 1];    // staged ones (of all its row tiles)
-  int32_t g0[kMaxSeqs + 1];    // first sequence
+  int32_t gt[kMaxSeqs + 1];    // staged ones, of all its items, with kItemTiles for each
   int32_t gp[kMaxSeqs];        // tiles of 16 keys of the prefix
+  uint16_t grp[kMaxSeqs];      // a sequence's group
+  int16_t g0[kMaxSeqs + 2];    // first sequence (-1, B + 1: outside the batch)
   int32_t wsum[3][kRounds][kShWaves];
 };
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // Last index i < n with v[i] <= p (v ascending); -1: none.
-__device__ __forceinline__ int last_at_most(const int32_t* v, int n, int p) {
+template <typename T>
+__device__ __forceinline__ int last_at_most(const T* v, int n, int p) {
   int lo = -1, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -116,6 +120,11 @@ __device__ __forceinline__ int last_at_most(const int32_t* v, int n, int p) {
 __device__ __forceinline__ int members(const Tables& t, int g, int B) {
   const int s0 = t.g0[g], s1 = t.g0[g + 1];
   return s0 >= 0 && s1 > s0 && s1 <= B ? s1 - s0 : 0;
+}
+// Tiles of the prefix that sequence b shares.
+__device__ __forceinline__ int skipped(const Tables& t, int b) {
+  const int g = t.grp[b];
+  return g == kNoGroup ? 0 : t.gp[g];
 }
 __device__ __forceinline__ int staged_tiles(int gp) { return (gp * kTile + kBN - 1) / kBN; }
 
@@ -132,10 +141,11 @@ __device__ __forceinline__ void tabulate_shared(const SharedArgs& a, Tables& t, 
   for (int i = 0; i < R; ++i) {
     const int b = i * kThreads + tid;
     row[i] = row_of(a.d, min(b, B - 1));
-    if (b <= NG) t.g0[b] = a.cu[b];
+    if (b <= NG) t.g0[b] = static_cast<int16_t>(max(-1, min(a.cu[b], B + 1)));
     cap[i] = b < NG ? a.shared[b] : 0;
   }
-  if (R * kThreads == NG && tid == 0) t.g0[NG] = a.cu[NG];
+  if (R * kThreads == NG && tid == 0)
+    t.g0[NG] = static_cast<int16_t>(max(-1, min(a.cu[NG], B + 1)));
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int b = i * kThreads + tid;
@@ -165,14 +175,15 @@ __device__ __forceinline__ void tabulate_shared(const SharedArgs& a, Tables& t, 
     own[i] = gs[i] = gt[i] = 0;
     if (b < B) {
       const int g = NG > 0 ? last_at_most(t.g0, NG, b) : -1;
-      if (g >= 0 && b < t.g0[g] + members(t, g, B)) skip = t.gp[g];
-      t.skip[b] = skip;
+      const bool in = g >= 0 && b < t.g0[g] + members(t, g, B);
+      if (in) skip = t.gp[g];
+      t.grp[b] = static_cast<uint16_t>(in ? g : kNoGroup);
       const int tiles = (t.len[b] + kTile - 1) / kTile;
       own[i] = tiles > skip ? tiles - skip : 0;
     }
     if (b < NG) {
       const int rows = members(t, b, B) * a.d.G, gp = t.gp[b];
-      if (rows > kRowsS) gt[i] = staged_tiles(gp) * ((rows + kRowsT - 1) / kRowsT);
+      if (rows > kRowsS) gt[i] = gp > 0 ? (staged_tiles(gp) + kItemTiles) * ((rows + kRowsT - 1) / kRowsT) : 0;
       else gs[i] = gp;
     }
     own_i[i] = wave_prefix_sum(own[i]);
@@ -215,26 +226,28 @@ __device__ __forceinline__ void tabulate_shared(const SharedArgs& a, Tables& t, 
   all_gt = uniform(run[2]);
 }
 
-// How the tiles are divided among the workgroups and waves.
+// How the tiles are divided among the workgroups and waves (all of it in scalar registers:
+// the compiler takes what LDS and floats give for a lane's own).
 struct Plan {
-  int64_t streamed, staged;  // tiles of all KV heads
-  int wgs_t;                 // workgroups of staged tiles, the grid's first ones
-  int64_t pw, pt;
+  int streamed, staged;  // tiles of all KV heads
+  int wgs_t;             // workgroups of staged tiles, the grid's first ones
+  int pw, pt;            // tiles of a wave's, of a workgroup's range
 };
 __device__ __forceinline__ Plan plan_of(const SharedArgs& a, int all_s, int all_t) {
   Plan p;
   const int N = gridDim.x;
-  p.streamed = static_cast<int64_t>(all_s) * a.d.Hkv;
-  p.staged = static_cast<int64_t>(all_t) * a.d.Hkv;
+  p.streamed = all_s * a.d.Hkv;
+  p.staged = all_t * a.d.Hkv;
   const float wt = static_cast<float>(p.staged) * kStagedUnits, ws = static_cast<float>(p.streamed);
   int n = all_t == 0 ? 0 : static_cast<int>(N * (wt / (wt + ws)) + 0.5f);
   if (all_t > 0) n = n < 1 ? 1 : n;
   if (all_s > 0) n = n > N - 1 ? N - 1 : n;
-  p.wgs_t = uniform(n);
-  p.pt = n > 0 ? q3::cdiv(p.staged, n) : kMinStaged;
+  n = uniform(n);
+  p.wgs_t = n;
+  p.pt = n > 0 ? uniform((p.staged + n - 1) / n) : kMinStaged;
   p.pt = p.pt < kMinStaged ? kMinStaged : p.pt;
-  const int64_t waves = static_cast<int64_t>(N - n) * kShWaves;
-  p.pw = waves > 0 ? q3::cdiv(p.streamed, waves) : kMinStreamed;
+  const int waves = (N - n) * kShWaves;
+  p.pw = waves > 0 ? uniform((p.streamed + waves - 1) / waves) : kMinStreamed;
   p.pw = p.pw < kMinStreamed ? kMinStreamed : p.pw;
   return p;
 }
@@ -268,7 +281,7 @@ __device__ __forceinline__ StreamItem stream_item(const SharedArgs& a, const Tab
   s.e = e;
   if (e < B) {
     s.n = uniform(t.own[e + 1] - t.own[e]);
-    s.t0 = uniform(t.skip[e]);
+    s.t0 = uniform(skipped(t, e));
     s.L = uniform(t.len[e]);
     s.row = uniform(t.row[e]);
   } else {
@@ -281,32 +294,32 @@ __device__ __forceinline__ StreamItem stream_item(const SharedArgs& a, const Tab
   return s;
 }
 
-__device__ __forceinline__ void stream_range(const SharedArgs& a, const Tables& t, int all_own, int64_t w,
-                             int64_t g0, int64_t g1) {
+__device__ __forceinline__ void stream_range(const SharedArgs& a, const Tables& t, int all_own, int w, int g0,
+                             int g1) {
   const DecodeArgs& d = a.d;
   const int lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
   const int B = d.B, entries = B + a.groups;
-  const int64_t own_end = static_cast<int64_t>(d.Hkv) * all_own;
+  const int own_end = d.Hkv * all_own;
 
   StreamItem cur;
   int hkv, at;  // the next tile to load: its KV head and place in the item
-  int64_t g = g0;
+  int g = g0;
   {
     int e, before;
     if (g0 < own_end) {
-      e = uniform(last_at_most(t.own, B, static_cast<int>(g0 / d.Hkv)));
+      e = uniform(last_at_most(t.own, B, g0 / d.Hkv));
       // (heads lie inside a sequence: its tiles begin at Hkv * own)
       before = uniform(t.own[e]);
     } else {
-      const int p = static_cast<int>((g0 - own_end) / d.Hkv);
+      const int p = (g0 - own_end) / d.Hkv;
       e = uniform(last_at_most(t.gs, a.groups, p));
       before = all_own + uniform(t.gs[e]);
       e += B;
     }
     cur = stream_item(a, t, e);
-    const int64_t off = g0 - static_cast<int64_t>(d.Hkv) * before;
-    hkv = static_cast<int>(off / cur.n);
-    at = static_cast<int>(off % cur.n);
+    const int off = g0 - d.Hkv * before;
+    hkv = uniform(off / cur.n);
+    at = off - hkv * cur.n;
   }
   TableWindow tw;
   window_load(tw, d, cur.row, ((cur.t0 + at) * kTile) / d.bs, lane);
@@ -327,10 +340,9 @@ __device__ __forceinline__ void stream_range(const SharedArgs& a, const Tables& 
       at = 0;
       window_load(tw, d, load.row, (load.t0 * kTile) / d.bs, lane);
     }
-    const int64_t left = g1 - g;
     int n = load.n - at;
     n = n < kChunk ? n : kChunk;
-    n = left < n ? static_cast<int>(left) : n;
+    n = g1 - g < n ? g1 - g : n;
     c.n = n;
     c.t0 = load.t0 + at;
     c.seg = load.e * d.Hkv + hkv;
@@ -369,7 +381,7 @@ __device__ __forceinline__ void stream_range(const SharedArgs& a, const Tables& 
     if (ce < B) {
       cb = ce;
       clane = lo < d.G;
-      cskip = uniform(t.skip[ce]);
+      cskip = uniform(skipped(t, ce));
     } else {
       const int grp = ce - B;
       s = divide(lo, a.per_head);
@@ -404,7 +416,7 @@ __device__ __forceinline__ void stream_range(const SharedArgs& a, const Tables& 
       po = (ce < B ? a.po_own : a.po_pre) + row * kD;
       pl = (ce < B ? a.lse_own : a.lse_pre) + row;
     } else {
-      const int64_t slot = (w * 2 + (cfirst ? 0 : 1)) * kRowsS + lo;
+      const int64_t slot = (static_cast<int64_t>(w) * 2 + (cfirst ? 0 : 1)) * kRowsS + lo;
       po = a.po_s + slot * kD;
       pl = a.lse_s + slot;
     }
@@ -446,44 +458,215 @@ struct Stage {
   uint16_t* v;
 };
 
-__device__ __forceinline__ void staged_range(const SharedArgs& a, const Tables& t, int all_t, int v, int64_t p0,
-                             int64_t p1, const Stage (&st)[3]) {
+// A buffer load that writes LDS, 16 bytes a lane from LDS byte `to` on.  In assembly: with
+// the builtin the compiler waits, before it reads one stage, for the loads into all of
+// them.  Whoever reads the stage waits for it by count (staged_range), and nothing else
+// here uses M0.
+__device__ __forceinline__ void load_lds16(q3::u32x4 rsrc, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(to), "v"(offset), "s"(rsrc)
+               : "memory");
+}
+__device__ __forceinline__ q3::u32x4 descriptor(const uint16_t* p, int bytes) {
+  const uint64_t at = reinterpret_cast<uint64_t>(p);
+  return q3::u32x4{static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32) & 0xffffu,
+                   static_cast<uint32_t>(bytes), 0x00020000u};
+}
+// LDS byte of a shared array's element.
+__device__ __forceinline__ uint32_t lds_byte(const uint16_t* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void_t*)const_cast<uint16_t*>(p)));
+}
+
+// Where a range's next tiles lie, in LDS: for each group of 16 keys the page (-1: the table
+// names no block of the pool) and the place in it, for each tile which of its groups have
+// one.  (Held in registers, as the chunk kernels have them, the wait for the next pages'
+// load would be a wait for the tiles ahead.)
+constexpr int kPageTiles = 64;
+constexpr int kTileGroups = kBN / kGroup;
+struct Pages {
+  int2 at[kPageTiles * kTileGroups];
+  uint32_t ok[kPageTiles];
+};
+
+__device__ __forceinline__ void fill_pages(const SharedArgs& a, Pages& pages, int64_t row, int tile,
+                                           int n) {
+  const int tid = threadIdx.x;
+  const int group = tile * kTileGroups + tid;
+  if (tid >= kPageTiles * kTileGroups) return;
+  const uint32_t p = divide(group, a.per_group);
+  int32_t id = tid < n * kTileGroups && p < a.max_pages ? a.bt[row * a.bt_stride + p] : -1;
+  id = id >= 0 && id < a.num_blocks ? id : -1;
+  pages.at[tid] = int2{id, (group - static_cast<int>(p) * a.gpb) * kGroup};
+  const uint64_t ok = __ballot(id >= 0);
+  if (tid % kTileGroups == 0) pages.ok[tid / kTileGroups] = static_cast<uint32_t>(ok >> (tid & 63)) & 15u;
+}
+
+// A wave's part of a tile's loads, as read from Pages before they are issued.
+struct Next {
+  int page, sub;
+  uint32_t ok;
+};
+__device__ __forceinline__ Next next_tile(const Pages& pages, int i, int wave) {
+  const int2 at = pages.at[i * kTileGroups + wave * kTileGroups / kShWaves];
+  return Next{at.x, at.y, pages.ok[i]};
+}
+
+// Issues this wave's share of a tile's loads: the keys from `first` on, `cap` keys in all.
+// Returns which of its groups lie in the pool.
+__device__ __forceinline__ uint32_t stage_tile(const SharedArgs& a, const LaneOffsets& off,
+                                               const uint16_t* kh, const uint16_t* vh, int first,
+                                               int cap, const Next& n, const Stage& st, int wave) {
+  const int g = wave * kTileGroups / kShWaves;  // this wave's group
+  const int page = uniform(n.page), sub = uniform(n.sub);
+  const int rows = page >= 0 ? min(kGroup, cap - first - g * kGroup) : 0;
+  const uint16_t* kb = kh;
+  const uint16_t* vb = vh;
+  if (rows > 0) {
+    kb += page * a.k_blk + static_cast<int64_t>(sub) * a.k_slot;
+    vb += page * a.v_blk + static_cast<int64_t>(sub) * a.v_slot;
+  }
+  // rows behind the last key lie outside the descriptor and read as zero
+  const q3::u32x4 kr = descriptor(kb, rows > 0 ? (rows - 1) * a.k_slot * 2 + kRowBytes : 0);
+  const q3::u32x4 vr = descriptor(vb, rows > 0 ? (rows - 1) * a.v_slot * 2 + kRowBytes : 0);
+  constexpr int D = dma_per_wave<kShWaves>();
+#pragma unroll
+  for (int j = 0; j < D; ++j) {
+    const uint32_t blk = (D * wave + j) * 1024;
+    load_lds16(kr, off.kdma[j], lds_byte(st.k) + blk);
+    load_lds16(vr, off.vdma[j], lds_byte(st.v) + blk);
+  }
+  return uniform(n.ok);
+}
+
+// Maximum of a lane's 16 scores (as max3_scores, of half a tile).
+__device__ __forceinline__ float max3_half(const q3::f32x16& a) {
+  float m, t;
+  asm volatile(
+      "v_max3_f32 %0, %2, %3, %4\n\t"
+      "v_max3_f32 %1, %10, %11, %12\n\t"
+      "v_max3_f32 %0, %0, %5, %6\n\t"
+      "v_max3_f32 %1, %1, %13, %14\n\t"
+      "v_max3_f32 %0, %0, %7, %8\n\t"
+      "v_max3_f32 %1, %1, %15, %16\n\t"
+      "v_max3_f32 %0, %0, %9, %17\n\t"
+      "v_max_f32 %0, %0, %1"
+      : "=&v"(m), "=&v"(t)
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7]),
+        "v"(a[8]), "v"(a[9]), "v"(a[10]), "v"(a[11]), "v"(a[12]), "v"(a[13]), "v"(a[14]),
+        "v"(a[15]));
+  return m;
+}
+
+// tile_fold of 32 keys, which kt and vt begin with, P in two terms.  s[r] of a lane is key
+// 8 (r / 4) + r % 4 + 4 (lane / 32) of them.
+template <typename Mask>
+__device__ __forceinline__ void half_fold(const LaneOffsets& off, float c, const Mask& mask,
+                                          const uint16_t* kt, const uint16_t* vt,
+                                          const q3::bf16x8 (&qv)[8], float& m_run, float& l_run,
+                                          q3::f32x16 (&acc)[4]) {
+  q3::f32x16 s, s2;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = s2[r] = 0.f;
+  {
+    q3::bf16x8 kf[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) kf[u] = lds_ld16(kt, off.kread ^ static_cast<uint32_t>(u << 5));
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < 8; u += 2) {  // (two sums, so that a product does not wait for the last)
+      s = q3::mfma32x32x16(kf[u], qv[u], s);
+      s2 = q3::mfma32x32x16(kf[u + 1], qv[u + 1], s2);
+    }
+    s += s2;
+  }
+  // (the values' first half on the way meanwhile)
+  q3::bf16x8 vf[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) vf[u] = lds_vt(vt, pv_operand(off, u));
+  __builtin_amdgcn_sched_barrier(0);
+  mask(s);
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7");  // the products before a read in assembly
+  const float m_cand = cross_half_max(max3_half(s)) * c;
+  const bool raise = m_cand > m_run + kRescaleSlack;
+  if (__any(raise)) {
+    const float m_new = raise ? m_cand : m_run;
+    const float alpha = raise ? q3::fast_exp2(m_run - m_new) : 1.f;
+    m_run = m_new;
+    l_run *= alpha;
+#pragma unroll
+    for (int db = 0; db < 4; ++db) acc[db] *= alpha;
+  }
+  const float m_use = m_run == q3::kNegInf ? 0.f : m_run;
+  q3::u32x4 pk[2], pl[2];
+  float psum[4] = {0.f, 0.f, 0.f, 0.f};
+  auto exp_pair = [&](int g, int h) {  // scores 2 h, 2 h + 1 of chunk g
+    const float e0 = q3::fast_exp2(__builtin_fmaf(s[8 * g + 2 * h], c, -m_use));
+    const float e1 = q3::fast_exp2(__builtin_fmaf(s[8 * g + 2 * h + 1], c, -m_use));
+    psum[(2 * h) & 3] += e0;
+    psum[(2 * h + 1) & 3] += e1;
+    pk[g][h] = q3::pack_bf16x2(e0, e1);
+    pl[g][h] = q3::pack_bf16x2(e0 - q3::bf16_lo(pk[g][h]), e1 - q3::bf16_hi(pk[g][h]));
+  };
+#pragma unroll
+  for (int h = 0; h < 4; ++h) exp_pair(0, h);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    // (the two terms' products of one accumulator lie four apart: the second would wait
+    // for the first)
+#pragma unroll
+    for (int db = 0; db < 4; ++db) {
+      acc[db] = q3::mfma32x32x16(vf[db], q3::as_bf16x8(pk[g]), acc[db]);
+      if (g == 0) exp_pair(1, db);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int db = 0; db < 4; ++db) {
+      acc[db] = q3::mfma32x32x16(vf[db], q3::as_bf16x8(pl[g]), acc[db]);
+      if (g == 0) vf[db] = lds_vt(vt, pv_operand(off, 4 + db));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  l_run += (psum[0] + psum[1]) + (psum[2] + psum[3]);
+}
+
+// Staged tiles [p0, p1) of the list, by one workgroup.  A wave takes 32 of an item's rows
+// and 32 of a tile's keys, so that each SIMD has work of up to 64 rows on; the two halves of
+// the keys are joined when the item ends.
+__device__ __forceinline__ void staged_range(const SharedArgs& a, const Tables& t, int all_t, int v,
+                                             int p0, int p1, const Stage (&st)[kStages],
+                                             Pages& pages) {
   const DecodeArgs& d = a.d;
-  constexpr int W = kShWaves;
+  constexpr int kShare = 2 * dma_per_wave<kShWaves>();  // a wave's loads of a tile
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = uniform(tid >> 6);
-  const LaneOffsets off = lane_offsets<W>(a, lane, wave);
-  int64_t p = p0;
+  const LaneOffsets off = lane_offsets<kShWaves>(a, lane, wave);
+  int p = p0;
   while (p < p1) {
-    const int kvh = uniform(static_cast<int>(p / all_t));
-    const int in = static_cast<int>(p - static_cast<int64_t>(kvh) * all_t);
+    const int kvh = uniform(p / all_t);
+    const int in = p - kvh * all_t;
     const int grp = uniform(last_at_most(t.gt, a.groups, in));
     const int keys = uniform(t.gp[grp]) * kTile;
     const int tiles = (keys + kBN - 1) / kBN;
     const int s0 = uniform(t.g0[grp]), rows = uniform(t.g0[grp + 1] - t.g0[grp]) * d.G;
-    const int mt = uniform((in - t.gt[grp]) / tiles);
-    const int j0 = in - uniform(t.gt[grp]) - mt * tiles;
-    const int64_t left = p1 - p;
-    const int j1 = left < tiles - j0 ? j0 + static_cast<int>(left) : tiles;
+    const int before = uniform(t.gt[grp]);
+    // (an item's tiles lie behind its kItemTiles)
+    const int mt = uniform((in - before) / (tiles + kItemTiles));
+    const int at0 = in - before - mt * (tiles + kItemTiles) - kItemTiles;
+    const int j0 = at0 > 0 ? at0 : 0, j1 = min(tiles, at0 + p1 - p);
+    p += tiles - at0;  // the next item
+    if (j0 >= j1) continue;
+    // waves 0 .. 3 lie on a SIMD each, 4 .. 7 on the same again
+    const bool few = rows - mt * kRowsT <= kRowsT / 2;
+    const int part = few ? wave & 1 : wave & 3;    // of the rows
+    const int half = few ? wave >> 1 : wave >> 2;  // of the keys
 
     // this wave's 32 rows: lane l holds row r0 + l % 32
-    const int r0 = mt * kRowsT + wave * 32, r = r0 + (lane & 31);
-    const bool active = r0 < rows, mine = r < rows;
+    const int r0 = mt * kRowsT + part * 32, r = r0 + (lane & 31);
+    const bool active = r0 < rows && half < 2, mine = r < rows;
     const int s = divide(mine ? r : 0, a.per_head);
     const int b = s0 + s, head = kvh * d.G + ((mine ? r : 0) - s * d.G);
-    const int last = (mine ? min(t.len[b], keys) : keys) - 1;
-    int lo_last = last;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) lo_last = min(lo_last, __shfl_xor(lo_last, o, 64));
-    lo_last = uniform(lo_last);
-
-    PageWindow pw;
-    window_start(pw, a, uniform(t.row[s0]), j0, lane);
-    window_check(pw, a);
-    const ItemKeys ks{a.k + kvh * a.k_sh, a.v + kvh * a.v_sh, uniform(t.row[s0]), keys};
-    uint32_t ok[3];
-    ok[0] = tile_dma<W>(a, off, pw, ks, j0, st[0].k, st[0].v, wave, lane);
-    if (j0 + 1 < j1) ok[1] = tile_dma<W>(a, off, pw, ks, j0 + 1, st[1].k, st[1].v, wave, lane);
     q3::bf16x8 qv[8];
     {
       const uint16_t* qp = d.q + b * d.q_sb + static_cast<int64_t>(head) * d.q_sh + 8 * (lane >> 5);
@@ -491,6 +674,14 @@ __device__ __forceinline__ void staged_range(const SharedArgs& a, const Tables& 
       for (int c = 0; c < 8; ++c)
         qv[c] = q3::as_bf16x8(mine ? q3::ld16(qp + 16 * c) : q3::u32x4{0u, 0u, 0u, 0u});
     }
+    const int last = (mine ? min(t.len[b], keys) : keys) - 1;
+    int lo_last = last;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) lo_last = min(lo_last, __shfl_xor(lo_last, o, 64));
+    lo_last = uniform(lo_last);
+    const int64_t row = uniform(t.row[s0]);
+    const uint16_t* kh = a.k + kvh * a.k_sh;
+    const uint16_t* vh = a.v + kvh * a.v_sh;
     float m_run = q3::kNegInf, l_run = 0.f;
     q3::f32x16 acc[4];
 #pragma unroll
@@ -498,55 +689,101 @@ __device__ __forceinline__ void staged_range(const SharedArgs& a, const Tables& 
 #pragma unroll
       for (int x = 0; x < 16; ++x) acc[db][x] = 0.f;
 
-    auto step = [&](int j, const Stage& here, uint32_t okh, const Stage& next, uint32_t& okn) {
-      wait_loads();
+    for (int ja = j0; ja < j1; ja += kPageTiles) {
+      const int je = min(ja + kPageTiles, j1);
+      fill_pages(a, pages, row, ja, je - ja);
       __syncthreads();
-      if (j + 2 < j1) okn = tile_dma<W>(a, off, pw, ks, j + 2, next.k, next.v, wave, lane);
-      if (!active) return;
-      const int n0 = j * kBN;
-      auto mask = [&](q3::f32x16 (&x)[2]) {
-        if (n0 + kBN - 1 > lo_last || okh != 15u) {
-          const int lim = last - n0 - 4 * (lane >> 5);
+      // (the queries too have arrived: that wait inside the loop would be one for the
+      // tiles ahead)
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
+      for (int c = 0; c < 8; ++c) asm volatile("" : "+v"(qv[c]));
+      uint32_t ok[kStages];
+      auto stage = [&](int j, const Next& n, int to) {
+        ok[to] = stage_tile(a, off, kh, vh, j * kBN, keys, n, st[to], wave);
+      };
+#pragma unroll
+      for (int u = 0; u < kStages - 1; ++u)
+        if (ja + u < je) stage(ja + u, next_tile(pages, u, wave), u);
+      Next ahead = next_tile(pages, min(kStages - 1, je - ja - 1), wave);
+
+      auto step = [&](int j, int u) {
+        // this wave's share of tile j has arrived (its loads of the next tiles are newer),
+        // then everybody's has, and nobody reads tile j - 1 any more
+        if (j + 2 < je) __builtin_amdgcn_s_waitcnt(0x0f70 | 2 * kShare);
+        else if (j + 1 < je) __builtin_amdgcn_s_waitcnt(0x0f70 | kShare);
+        else wait_loads();
+        __builtin_amdgcn_s_barrier();
+        const uint32_t here = ok[u];
+        if (j + kStages - 1 < je) {
+          stage(j + kStages - 1, ahead, (u + kStages - 1) % kStages);
+          ahead = next_tile(pages, min(j + kStages, je - 1) - ja, wave);
+        }
+        if (!active) return;
+        const int n0 = j * kBN + 32 * half;
+        auto mask = [&](q3::f32x16 (&x)) {
+          if (n0 + 31 > lo_last || here != 15u) {
+            // score i: key n0 + 4 (lane / 32) + kr of group 2 half + i / 8
+            const int lim = last - n0 - 4 * (lane >> 5);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const int kr = kb * 32 + 8 * (i / 4) + (i % 4);
-              const int l = (okh >> (2 * kb + i / 8)) & 1u ? lim : -1;
-              x[kb][i] = kr <= l ? x[kb][i] : q3::kNegInf;
+              const int kr = 8 * (i / 4) + (i % 4);
+              const int l = (here >> (2 * half + i / 8)) & 1u ? lim : -1;
+              x[i] = kr <= l ? x[i] : q3::kNegInf;
             }
-        }
+          }
+        };
+        half_fold(off, d.scale_log2, mask, st[u].k + half * 32 * kD, st[u].v + half * 32 * kD, qv,
+                  m_run, l_run, acc);
       };
-      tile_fold<true>(off, d.scale_log2, mask, here.k, here.v, qv, m_run, l_run, acc);
-    };
-    for (int j = j0; j < j1; j += 3) {
-      step(j, st[0], ok[0], st[2], ok[2]);
-      if (j + 1 < j1) step(j + 1, st[1], ok[1], st[0], ok[0]);
-      if (j + 2 < j1) step(j + 2, st[2], ok[2], st[1], ok[1]);
+      for (int j = ja; j < je; j += kStages) {
+        step(j, 0);
+        if (j + 1 < je) step(j + 1, 1);
+        if (j + 2 < je) step(j + 2, 2);
+        if (j + 3 < je) step(j + 3, 3);
+      }
+      __syncthreads();  // pages and stages are read before they are filled again
     }
-    l_run = cross_half_sum(l_run);
-    if (mine) {
-      const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+    // the second half's state, through the stages
+    q3::f32x4* hold = reinterpret_cast<q3::f32x4*>(part == 0 ? st[0].k : part == 1 ? st[0].v : part == 2 ? st[1].k : st[1].v) + lane;
+    float2* ml = reinterpret_cast<float2*>(st[2].k) + part * 64 + lane;
+    if (half == 1) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        hold[64 * i] = q3::f32x4{acc[i >> 2][4 * (i & 3)], acc[i >> 2][4 * (i & 3) + 1],
+                               acc[i >> 2][4 * (i & 3) + 2], acc[i >> 2][4 * (i & 3) + 3]};
+      *ml = float2{m_run, l_run};
+    }
+    __syncthreads();
+    if (half == 0) {
+      const float2 o = *ml;
+      const float m = fmaxf(m_run, o.x), use = m == q3::kNegInf ? 0.f : m;
+      const float f = q3::fast_exp2(m_run - use), g = q3::fast_exp2(o.x - use);
+      const float l = q3::sum_xor32(l_run * f + o.y * g), inv = l > 0.f ? 1.f / l : 0.f;
+      const float fi = f * inv, gi = g * inv;
       float* po;
       float* pl;
       if (j1 - j0 == tiles) {
-        const int64_t row = static_cast<int64_t>(b) * d.Hq + head;
-        po = a.po_pre + row * kD;
-        pl = a.lse_pre + row;
+        const int64_t to = static_cast<int64_t>(b) * d.Hq + head;
+        po = a.po_pre + to * kD;
+        pl = a.lse_pre + to;
       } else {
-        const int64_t row = (2 * static_cast<int64_t>(v) + (j0 == 0 ? 1 : 0)) * a.rows_t + (r - mt * kRowsT);
-        po = a.po_t + row * kD;
-        pl = a.lse_t + row;
+        const int64_t to = (2 * static_cast<int64_t>(v) + (j0 == 0 ? 1 : 0)) * a.rows_t + (r - mt * kRowsT);
+        po = a.po_t + to * kD;
+        pl = a.lse_t + to;
       }
       po += 4 * (lane >> 5);
+      if (mine) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        *reinterpret_cast<q3::f32x4*>(po + 8 * i) =
-            q3::f32x4{acc[i >> 2][4 * (i & 3)] * inv, acc[i >> 2][4 * (i & 3) + 1] * inv,
-                      acc[i >> 2][4 * (i & 3) + 2] * inv, acc[i >> 2][4 * (i & 3) + 3] * inv};
-      if (lane < 32) *pl = l_run > 0.f ? m_run + __builtin_log2f(l_run) : q3::kNegInf;
+        for (int i = 0; i < 16; ++i) {
+          const q3::f32x4 x = hold[64 * i];
+          q3::f32x4 y;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = acc[i >> 2][4 * (i & 3) + e] * fi + x[e] * gi;
+          *reinterpret_cast<q3::f32x4*>(po + 8 * i) = y;
+        }
+        if (lane < 32) *pl = l > 0.f ? m + __builtin_log2f(l) : q3::kNegInf;
+      }
     }
-    p += j1 - j0;
     __syncthreads();  // the stages are read before the next item's loads refill them
   }
 }
@@ -559,7 +796,10 @@ void paged_shared_kernel(SharedArgs a) {
   __shared__ __attribute__((aligned(1024))) uint16_t s_v1[kTileElems];
   __shared__ __attribute__((aligned(1024))) uint16_t s_k2[kTileElems];
   __shared__ __attribute__((aligned(1024))) uint16_t s_v2[kTileElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t s_k3[kTileElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t s_v3[kTileElems];
   __shared__ Tables t;
+  __shared__ Pages s_pages;
   const int tid = threadIdx.x, wave = uniform(tid >> 6);
   int all_own, all_gs, all_t;
   if (a.d.B <= kThreads && a.groups < kThreads)
@@ -572,8 +812,8 @@ void paged_shared_kernel(SharedArgs a) {
       SeqMeta m{};
       m.own_at = t.own[b];
       m.own_n = t.own[b + 1] - t.own[b];
-      if (t.skip[b] > 0) {
-        const int g = last_at_most(t.g0, a.groups, b);
+      if (skipped(t, b) > 0) {
+        const int g = t.grp[b];
         const int rows = members(t, g, a.d.B) * a.d.G;
         m.kind = rows > kRowsS ? 2 : 1;
         m.pre_at = m.kind == 2 ? t.gt[g] : all_own + t.gs[g];
@@ -583,23 +823,23 @@ void paged_shared_kernel(SharedArgs a) {
       a.seqs[b] = m;
     }
     if (tid == 0)
-      *a.call = CallMeta{static_cast<int32_t>(plan.pw), static_cast<int32_t>(plan.pt), all_t, 0};
+      *a.call = CallMeta{plan.pw, plan.pt, all_t, 0};
   }
   const int v = blockIdx.x;
   if (v < plan.wgs_t) {
-    const int64_t p0 = v * plan.pt, p1 = p0 + plan.pt;
-    const Stage st[3] = {{s_k0, s_v0}, {s_k1, s_v1}, {s_k2, s_v2}};
+    const int p0 = v * plan.pt;
+    const Stage st[kStages] = {{s_k0, s_v0}, {s_k1, s_v1}, {s_k2, s_v2}, {s_k3, s_v3}};
     if (p0 < plan.staged)
-      staged_range(a, t, all_t, v, p0, p1 < plan.staged ? p1 : plan.staged, st);
+      staged_range(a, t, all_t, v, p0, min(p0 + plan.pt, plan.staged), st, s_pages);
     return;
   }
   // a batch too small for every wave is dealt one wave a workgroup first
-  const int64_t N = gridDim.x - plan.wgs_t, at = v - plan.wgs_t;
+  const int N = gridDim.x - plan.wgs_t, at = v - plan.wgs_t;
   const bool spread = plan.streamed <= (N * kShWaves - 1) * plan.pw;
-  const int64_t w = spread ? static_cast<int64_t>(wave) * N + at : at * kShWaves + wave;
-  const int64_t g0 = w * plan.pw, g1 = g0 + plan.pw;
+  const int w = spread ? wave * N + at : at * kShWaves + wave;
+  const int g0 = w * plan.pw;
   if (g0 < plan.streamed)
-    stream_range(a, t, all_own, w, g0, g1 < plan.streamed ? g1 : plan.streamed);
+    stream_range(a, t, all_own, w, g0, min(g0 + plan.pw, plan.streamed));
 }
 
 // ---- the join ---------------------------------------------------------------------------
@@ -631,7 +871,7 @@ __global__ __launch_bounds__(kMaxG * 64) void paged_shared_join_kernel(SharedArg
   // a streamed item's parts: `col` its column of this row
   auto streamed = [&](Parts& x, const float* po, const float* lse, int before, int n, int col) {
     if (n == 0) return;
-    const int64_t S = static_cast<int64_t>(d.Hkv) * before + static_cast<int64_t>(hkv) * n;
+    const int S = d.Hkv * before + hkv * n;
     const int64_t wf = S / call.pw, wl = (S + n - 1) / call.pw;
     x.n = static_cast<int>(wl - wf + 1);
     if (wf == wl) {
@@ -653,7 +893,7 @@ __global__ __launch_bounds__(kMaxG * 64) void paged_shared_join_kernel(SharedArg
     streamed(part[1], a.po_pre, a.lse_pre, m.pre_at, m.pre_n, m.pre_row + g);
   } else if (m.kind == 2) {
     const int r = m.pre_row + g, mt = r / kRowsT;
-    const int64_t S = static_cast<int64_t>(hkv) * call.all_t + m.pre_at + static_cast<int64_t>(mt) * m.pre_n;
+    const int S = hkv * call.all_t + m.pre_at + mt * (m.pre_n + kItemTiles) + kItemTiles;
     const int64_t vf = S / call.pt, vl = (S + m.pre_n - 1) / call.pt;
     Parts& x = part[1];
     x.n = static_cast<int>(vl - vf + 1);
@@ -792,10 +1032,10 @@ extern "C" int qwen3_paged_decode_shared_bf16(
     if (st < kD || st > (int64_t(1) << 24))
       return q3::fail(QWEN3_EUNSUPPORTED, "%s: slot stride %lld outside %d..2^24", who,
                       (long long)st, kD);
-  // tiles are counted in 32 bits
-  if (static_cast<int64_t>(B) * 2 * max_pages * (block_size / kTile) > 0x7fffffff)
-    return q3::fail(QWEN3_EINVAL, "%s: batch %d times %lld pages too large", who, B,
-                    (long long)max_pages);
+  // tiles are counted in 32 bits, and products of them with a range's width
+  if (static_cast<int64_t>(B) * 2 * max_pages * (block_size / kTile) * num_kv_heads > (1 << 30))
+    return q3::fail(QWEN3_EINVAL, "%s: batch %d times %lld pages, %d KV heads too large", who, B,
+                    (long long)max_pages, num_kv_heads);
   if (B == 0) return QWEN3_OK;
   const SharedLayout l = shared_layout(B, num_heads, a.d.G);
   if (!workspace || workspace_bytes < static_cast<size_t>(l.total))
