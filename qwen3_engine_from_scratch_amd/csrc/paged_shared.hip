@@ -38,9 +38,10 @@ constexpr int kRowsS = 16;            // rows of one that is streamed
 constexpr int kMaxWgs = 512;
 constexpr int kStages = 4;
 // Weight, in streamed tiles of 16 keys, of a staged tile of 64; what an item's start and
-// end weigh, in staged tiles; tiles that a range takes at least.
-constexpr int kStagedUnits = 6;
+// end weigh, in tiles of its kind; tiles that a range takes at least.
+constexpr int kStagedUnits = 5;
 constexpr int kItemTiles = 4;
+constexpr int kSegTiles = 1;
 constexpr int kMinStaged = 2;
 constexpr int kMinStreamed = 2 * kChunk;
 
@@ -92,11 +93,12 @@ struct SharedArgs {
 
 constexpr int kNoGroup = 0xffff;
 struct Tables {
-  int32_t own[kMaxSeqs + 1];   // own tiles before each sequence
+  // Tiles of one head before each, with kSegTiles (kItemTiles) for each item:
+  int32_t own[kMaxSeqs + 1];   // of sequences
   int32_t row[kMaxSeqs];
   int32_t len[kMaxSeqs];
-  int32_t gs[kMaxSeqs + 1];    // streamed prefix tiles before each group
-  int32_t gt[kMaxSeqs + 1];    // staged ones, of all its items, with kItemTiles for each
+  int32_t gs[kMaxSeqs + 1];    // of groups, streamed
+  int32_t gt[kMaxSeqs + 1];    // of groups, staged
   int32_t gp[kMaxSeqs];        // tiles of 16 keys of the prefix
   uint16_t grp[kMaxSeqs];      // a sequence's group
   int16_t g0[kMaxSeqs + 2];    // first sequence (-1, B + 1: outside the batch)
@@ -179,12 +181,12 @@ __device__ __forceinline__ void tabulate_shared(const SharedArgs& a, Tables& t, 
       if (in) skip = t.gp[g];
       t.grp[b] = static_cast<uint16_t>(in ? g : kNoGroup);
       const int tiles = (t.len[b] + kTile - 1) / kTile;
-      own[i] = tiles > skip ? tiles - skip : 0;
+      own[i] = tiles > skip ? tiles - skip + kSegTiles : 0;
     }
     if (b < NG) {
       const int rows = members(t, b, B) * a.d.G, gp = t.gp[b];
       if (rows > kRowsS) gt[i] = gp > 0 ? (staged_tiles(gp) + kItemTiles) * ((rows + kRowsT - 1) / kRowsT) : 0;
-      else gs[i] = gp;
+      else gs[i] = gp > 0 ? gp + kSegTiles : 0;
     }
     own_i[i] = wave_prefix_sum(own[i]);
     gs_i[i] = wave_prefix_sum(gs[i]);
@@ -269,7 +271,7 @@ __device__ __forceinline__ void store_part(float* po, const q3::f32x4 (&acc)[8],
 // An item of the streamed list: a sequence's own keys, or a group's prefix.
 struct StreamItem {
   int e;       // sequence, or B + group
-  int n;       // tiles
+  int n;       // tiles (below 1: none)
   int t0;      // first tile of the sequence
   int L;       // end of its keys
   int row;     // of the block table
@@ -280,13 +282,13 @@ __device__ __forceinline__ StreamItem stream_item(const SharedArgs& a, const Tab
   StreamItem s;
   s.e = e;
   if (e < B) {
-    s.n = uniform(t.own[e + 1] - t.own[e]);
+    s.n = uniform(t.own[e + 1] - t.own[e]) - kSegTiles;
     s.t0 = uniform(skipped(t, e));
     s.L = uniform(t.len[e]);
     s.row = uniform(t.row[e]);
   } else {
     const int g = e - B;
-    s.n = uniform(t.gs[g + 1] - t.gs[g]);
+    s.n = uniform(t.gs[g + 1] - t.gs[g]) - kSegTiles;
     s.t0 = 0;
     s.L = s.n * kTile;
     s.row = s.n > 0 ? uniform(t.row[t.g0[g]]) : -1;
@@ -301,14 +303,13 @@ __device__ __forceinline__ void stream_range(const SharedArgs& a, const Tables& 
   const int B = d.B, entries = B + a.groups;
   const int own_end = d.Hkv * all_own;
 
-  StreamItem cur;
-  int hkv, at;  // the next tile to load: its KV head and place in the item
-  int g = g0;
+  StreamItem load;  // the item of the next tile to load: its KV head, the tile's place in it
+  int hkv, at;
+  int g = g0;       // its place in the list (an item's tiles lie behind its kSegTiles)
   {
     int e, before;
     if (g0 < own_end) {
       e = uniform(last_at_most(t.own, B, g0 / d.Hkv));
-      // (heads lie inside a sequence: its tiles begin at Hkv * own)
       before = uniform(t.own[e]);
     } else {
       const int p = (g0 - own_end) / d.Hkv;
@@ -316,15 +317,18 @@ __device__ __forceinline__ void stream_range(const SharedArgs& a, const Tables& 
       before = all_own + uniform(t.gs[e]);
       e += B;
     }
-    cur = stream_item(a, t, e);
+    load = stream_item(a, t, e);
     const int off = g0 - d.Hkv * before;
-    hkv = uniform(off / cur.n);
-    at = off - hkv * cur.n;
+    hkv = uniform(off / (load.n + kSegTiles));
+    at = off - hkv * (load.n + kSegTiles) - kSegTiles;
+    if (at < 0) {
+      g -= at;
+      at = 0;
+    }
   }
   TableWindow tw;
-  window_load(tw, d, cur.row, ((cur.t0 + at) * kTile) / d.bs, lane);
+  window_load(tw, d, load.row, ((load.t0 + at) * kTile) / d.bs, lane);
 
-  StreamItem load = cur;
   auto issue = [&](Chunk& c) {
     c.n = 0;
     if (g >= g1) return;
@@ -335,9 +339,11 @@ __device__ __forceinline__ void stream_range(const SharedArgs& a, const Tables& 
         do {
           ++e;
           load = stream_item(a, t, e);
-        } while (load.n == 0 && e + 1 < entries);
+        } while (load.n <= 0 && e + 1 < entries);
       }
       at = 0;
+      g += kSegTiles;
+      if (g >= g1) return;
       window_load(tw, d, load.row, (load.t0 * kTile) / d.bs, lane);
     }
     int n = load.n - at;
@@ -366,45 +372,43 @@ __device__ __forceinline__ void stream_range(const SharedArgs& a, const Tables& 
   };
 
   // the item being accumulated
-  int cseg = -1, ce = 0, chkv = 0, ct_lo = 0, ct_hi = 0, cn = 0, cskip = 0;
+  int cseg = -1, ce = 0, ct_lo = 0, ct_hi = 0, cn = 0, first = 0;
   int cb = 0, chead = 0;     // this lane's sequence and query head
-  bool clane = false;        // the lane's column is a row of the item
-  bool cfirst = true;
+  bool mine = false;         // its column is a row of the item
   Columns col;
 
   auto begin = [&](const Chunk& c) {
     ce = c.seg / d.Hkv;
-    chkv = c.seg % d.Hkv;
+    const int kvh = c.seg - ce * d.Hkv;
     ct_lo = c.t0;
     cn = c.ntiles;
-    int s = 0, head = lo;
+    int head = lo;
     if (ce < B) {
       cb = ce;
-      clane = lo < d.G;
-      cskip = uniform(skipped(t, ce));
+      mine = lo < d.G;
+      first = uniform(skipped(t, ce));
     } else {
-      const int grp = ce - B;
-      s = divide(lo, a.per_head);
+      const int grp = ce - B, s = divide(lo, a.per_head);
       head = lo - s * d.G;
-      clane = s < uniform(t.g0[grp + 1] - t.g0[grp]);
-      cb = uniform(t.g0[grp]) + (clane ? s : 0);
-      cskip = 0;
+      mine = s < uniform(t.g0[grp + 1] - t.g0[grp]);
+      cb = uniform(t.g0[grp]) + (mine ? s : 0);
+      first = 0;
     }
-    chead = chkv * d.G + (clane ? head : 0);
+    chead = kvh * d.G + (mine ? head : 0);
     col.last = min(c.L, t.len[cb]) - 1;
     reset(col.st);
     const uint16_t* qp = d.q + cb * d.q_sb + static_cast<int64_t>(chead) * d.q_sh + hi * 8;
 #pragma unroll
     for (int cc = 0; cc < 4; ++cc)
-      col.q[cc] = q3::as_bf16x8(clane ? q3::ld16(qp + cc * 32) : q3::u32x4{0u, 0u, 0u, 0u});
+      col.q[cc] = q3::as_bf16x8(mine ? q3::ld16(qp + cc * 32) : q3::u32x4{0u, 0u, 0u, 0u});
   };
 
   auto finish = [&]() {
     const float l = q3::sum_xor32(q3::sum_xor16(col.st.l));
     const float inv = l > 0.f ? 1.f / l : 0.f;
-    if (!clane) return;
+    if (!mine) return;
     const bool whole = ct_hi - ct_lo == cn;
-    if (whole && ce < B && cskip == 0) {
+    if (whole && ce < B && first == 0) {
       store_out_bf16(d, cb, chead, col.st.acc, inv, hi);
       return;
     }
@@ -416,7 +420,8 @@ __device__ __forceinline__ void stream_range(const SharedArgs& a, const Tables& 
       po = (ce < B ? a.po_own : a.po_pre) + row * kD;
       pl = (ce < B ? a.lse_own : a.lse_pre) + row;
     } else {
-      const int64_t slot = (static_cast<int64_t>(w) * 2 + (cfirst ? 0 : 1)) * kRowsS + lo;
+      // a range's first item may go on from the one before, its last one into the next
+      const int64_t slot = (static_cast<int64_t>(w) * 2 + (ct_lo == first ? 1 : 0)) * kRowsS + lo;
       po = a.po_s + slot * kD;
       pl = a.lse_s + slot;
     }
@@ -426,10 +431,7 @@ __device__ __forceinline__ void stream_range(const SharedArgs& a, const Tables& 
 
   auto process = [&](Chunk& c) {
     if (c.seg != cseg) {
-      if (cseg >= 0) {
-        finish();
-        cfirst = false;
-      }
+      if (cseg >= 0) finish();
       cseg = c.seg;
       begin(c);
     }
@@ -453,10 +455,7 @@ __device__ __forceinline__ void stream_range(const SharedArgs& a, const Tables& 
 
 // ---- staged tiles: one workgroup ------------------------------------------------------
 
-struct Stage {
-  uint16_t* k;
-  uint16_t* v;
-};
+constexpr int kStageElems = 2 * kTileElems;  // a tile's keys, then its values
 
 // A buffer load that writes LDS, 16 bytes a lane from LDS byte `to` on.  In assembly: with
 // the builtin the compiler waits, before it reads one stage, for the loads into all of
@@ -507,35 +506,52 @@ struct Next {
   int page, sub;
   uint32_t ok;
 };
-__device__ __forceinline__ Next next_tile(const Pages& pages, int i, int wave) {
-  const int2 at = pages.at[i * kTileGroups + wave * kTileGroups / kShWaves];
+// What a wave loads: waves 0 .. 3 a group of keys each, waves 4 .. 7 of values.
+struct Loader {
+  const uint16_t* base;  // the KV head of block 0
+  int64_t blk;
+  int slot;
+  int group;             // of a tile
+  uint32_t from[4];      // a lane's source offsets within a group
+};
+constexpr int kShare = 4;  // a wave's loads of a tile
+
+__device__ __forceinline__ Loader loader_of(const SharedArgs& a, int lane, int wave) {
+  Loader l;
+  const bool keys = wave < 4;
+  l.base = keys ? a.k : a.v;
+  l.blk = keys ? a.k_blk : a.v_blk;
+  l.slot = keys ? a.k_slot : a.v_slot;
+  l.group = wave & 3;
+#pragma unroll
+  for (int j = 0; j < kShare; ++j) {
+    // load j fills LDS rows 4 j .. 4 j + 3 of the group, lane i slot i % 16 of row 4 j + i / 16
+    // (prefill_tile.hpp: the source chunk is slot ^ swz(row))
+    const int row = 4 * j + (lane >> 4), slot = lane & 15;
+    l.from[j] = static_cast<uint32_t>(row * l.slot * 2) +
+                ((slot ^ (keys ? row & 15 : 4 * (row & 3))) << 4);
+  }
+  return l;
+}
+
+__device__ __forceinline__ Next next_tile(const Pages& pages, int i, const Loader& l) {
+  const int2 at = pages.at[i * kTileGroups + l.group];
   return Next{at.x, at.y, pages.ok[i]};
 }
 
-// Issues this wave's share of a tile's loads: the keys from `first` on, `cap` keys in all.
-// Returns which of its groups lie in the pool.
-__device__ __forceinline__ uint32_t stage_tile(const SharedArgs& a, const LaneOffsets& off,
-                                               const uint16_t* kh, const uint16_t* vh, int first,
-                                               int cap, const Next& n, const Stage& st, int wave) {
-  const int g = wave * kTileGroups / kShWaves;  // this wave's group
+// Issues this wave's share of a tile's loads: `keys` keys from its first on, head: the KV
+// head's place.  Returns which of its groups lie in the pool.
+__device__ __forceinline__ uint32_t stage_tile(const Loader& l, const uint16_t* head, int keys,
+                                               const Next& n, const uint16_t* to) {
   const int page = uniform(n.page), sub = uniform(n.sub);
-  const int rows = page >= 0 ? min(kGroup, cap - first - g * kGroup) : 0;
-  const uint16_t* kb = kh;
-  const uint16_t* vb = vh;
-  if (rows > 0) {
-    kb += page * a.k_blk + static_cast<int64_t>(sub) * a.k_slot;
-    vb += page * a.v_blk + static_cast<int64_t>(sub) * a.v_slot;
-  }
+  const int rows = page >= 0 ? min(kGroup, keys - l.group * kGroup) : 0;
+  const uint16_t* p = head;
+  if (rows > 0) p += page * l.blk + static_cast<int64_t>(sub) * l.slot;
   // rows behind the last key lie outside the descriptor and read as zero
-  const q3::u32x4 kr = descriptor(kb, rows > 0 ? (rows - 1) * a.k_slot * 2 + kRowBytes : 0);
-  const q3::u32x4 vr = descriptor(vb, rows > 0 ? (rows - 1) * a.v_slot * 2 + kRowBytes : 0);
-  constexpr int D = dma_per_wave<kShWaves>();
+  const q3::u32x4 r = descriptor(p, rows > 0 ? (rows - 1) * l.slot * 2 + kRowBytes : 0);
+  const uint32_t at = lds_byte(to) + l.group * (kGroup * kRowBytes);
 #pragma unroll
-  for (int j = 0; j < D; ++j) {
-    const uint32_t blk = (D * wave + j) * 1024;
-    load_lds16(kr, off.kdma[j], lds_byte(st.k) + blk);
-    load_lds16(vr, off.vdma[j], lds_byte(st.v) + blk);
-  }
+  for (int j = 0; j < kShare; ++j) load_lds16(r, l.from[j], at + j * 1024);
   return uniform(n.ok);
 }
 
@@ -558,90 +574,90 @@ __device__ __forceinline__ float max3_half(const q3::f32x16& a) {
   return m;
 }
 
-// tile_fold of 32 keys, which kt and vt begin with, P in two terms.  s[r] of a lane is key
-// 8 (r / 4) + r % 4 + 4 (lane / 32) of them.
-template <typename Mask>
-__device__ __forceinline__ void half_fold(const LaneOffsets& off, float c, const Mask& mask,
-                                          const uint16_t* kt, const uint16_t* vt,
-                                          const q3::bf16x8 (&qv)[8], float& m_run, float& l_run,
-                                          q3::f32x16 (&acc)[4]) {
-  q3::f32x16 s, s2;
+// A wave's probabilities of 32 keys, in two bf16 terms, not yet met with their values.
+struct Probs {
+  q3::u32x4 hi[2], lo[2];
+};
+__device__ __forceinline__ void prob_pair(Probs& p, float (&sums)[4], const q3::f32x16& s, int i,
+                                          float c, float m) {
+  const int g = i >> 2, h = i & 3;  // scores 2 h, 2 h + 1 of the 16 keys g
+  const float e0 = q3::fast_exp2(__builtin_fmaf(s[8 * g + 2 * h], c, -m));
+  const float e1 = q3::fast_exp2(__builtin_fmaf(s[8 * g + 2 * h + 1], c, -m));
+  sums[(2 * h) & 3] += e0;
+  sums[(2 * h + 1) & 3] += e1;
+  uint32_t hi = q3::pack_bf16x2(e0, e1);
+  asm("" : "+v"(hi));  // (or each half is rounded once more instead of taken from the pair)
+  uint32_t lo = q3::pack_bf16x2(e0 - q3::bf16_lo(hi), e1 - q3::bf16_hi(hi));
+  asm volatile("" : "+v"(lo));  // (or it is put off until the products have ended)
+  p.hi[g][h] = hi;
+  p.lo[g][h] = lo;
+}
+
+// Scores of the 32 keys that kt begins with: s[r] of a lane is key 8 (r / 4) + r % 4 +
+// 4 (lane / 32).
+__device__ __forceinline__ q3::f32x16 score(const LaneOffsets& off, const uint16_t* kt,
+                                            const q3::bf16x8 (&qv)[8]) {
+  q3::bf16x8 kf[8];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) s[r] = s2[r] = 0.f;
-  {
-    q3::bf16x8 kf[8];
+  for (int u = 0; u < 8; ++u) kf[u] = lds_ld16(kt, off.kread ^ static_cast<uint32_t>(u << 5));
+  __builtin_amdgcn_sched_barrier(0);  // (all reads on their way, not one by one)
+  q3::f32x16 s;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) kf[u] = lds_ld16(kt, off.kread ^ static_cast<uint32_t>(u << 5));
-    __builtin_amdgcn_sched_barrier(0);
+  for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-    for (int u = 0; u < 8; u += 2) {  // (two sums, so that a product does not wait for the last)
-      s = q3::mfma32x32x16(kf[u], qv[u], s);
-      s2 = q3::mfma32x32x16(kf[u + 1], qv[u + 1], s2);
-    }
-    s += s2;
-  }
-  // (the values' first half on the way meanwhile)
+  for (int u = 0; u < 8; ++u) s = q3::mfma32x32x16(kf[u], qv[u], s);
+  return s;
+}
+
+// Raises the running maximum to what scores s reach where that is far above it; returns
+// the factor of what was summed under the old one.
+__device__ __forceinline__ float raise_max(const q3::f32x16& s, float c, float& m_run) {
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7");  // the products before a read in assembly
+  const float m_cand = cross_half_max(max3_half(s)) * c;
+  const bool raise = m_cand > m_run + kRescaleSlack;
+  const float m_new = raise ? m_cand : m_run;
+  const float alpha = raise ? q3::fast_exp2(m_run - m_new) : 1.f;
+  m_run = m_new;
+  return alpha;
+}
+__device__ __forceinline__ float finite_max(float m) { return m == q3::kNegInf ? 0.f : m; }
+
+// O^T += V^T P^T of the 32 keys whose values vt begins with; between(i) is called after
+// every second of the 16 products: work that runs beside them.
+template <typename Between>
+__device__ __forceinline__ void add_values(const LaneOffsets& off, const uint16_t* vt,
+                                           const Probs& p, const Between& between,
+                                           q3::f32x16 (&acc)[4]) {
   q3::bf16x8 vf[4];
 #pragma unroll
   for (int u = 0; u < 4; ++u) vf[u] = lds_vt(vt, pv_operand(off, u));
   __builtin_amdgcn_sched_barrier(0);
-  mask(s);
-  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7");  // the products before a read in assembly
-  const float m_cand = cross_half_max(max3_half(s)) * c;
-  const bool raise = m_cand > m_run + kRescaleSlack;
-  if (__any(raise)) {
-    const float m_new = raise ? m_cand : m_run;
-    const float alpha = raise ? q3::fast_exp2(m_run - m_new) : 1.f;
-    m_run = m_new;
-    l_run *= alpha;
 #pragma unroll
-    for (int db = 0; db < 4; ++db) acc[db] *= alpha;
-  }
-  const float m_use = m_run == q3::kNegInf ? 0.f : m_run;
-  q3::u32x4 pk[2], pl[2];
-  float psum[4] = {0.f, 0.f, 0.f, 0.f};
-  auto exp_pair = [&](int g, int h) {  // scores 2 h, 2 h + 1 of chunk g
-    const float e0 = q3::fast_exp2(__builtin_fmaf(s[8 * g + 2 * h], c, -m_use));
-    const float e1 = q3::fast_exp2(__builtin_fmaf(s[8 * g + 2 * h + 1], c, -m_use));
-    psum[(2 * h) & 3] += e0;
-    psum[(2 * h + 1) & 3] += e1;
-    pk[g][h] = q3::pack_bf16x2(e0, e1);
-    pl[g][h] = q3::pack_bf16x2(e0 - q3::bf16_lo(pk[g][h]), e1 - q3::bf16_hi(pk[g][h]));
-  };
+  for (int g = 0; g < 2; ++g)
 #pragma unroll
-  for (int h = 0; h < 4; ++h) exp_pair(0, h);
-  __builtin_amdgcn_sched_barrier(0);
+    for (int term = 0; term < 2; ++term)
 #pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    // (the two terms' products of one accumulator lie four apart: the second would wait
-    // for the first)
-#pragma unroll
-    for (int db = 0; db < 4; ++db) {
-      acc[db] = q3::mfma32x32x16(vf[db], q3::as_bf16x8(pk[g]), acc[db]);
-      if (g == 0) exp_pair(1, db);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-#pragma unroll
-    for (int db = 0; db < 4; ++db) {
-      acc[db] = q3::mfma32x32x16(vf[db], q3::as_bf16x8(pl[g]), acc[db]);
-      if (g == 0) vf[db] = lds_vt(vt, pv_operand(off, 4 + db));
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  }
-  l_run += (psum[0] + psum[1]) + (psum[2] + psum[3]);
+      for (int db = 0; db < 4; ++db) {
+        // (the two terms' products of one accumulator lie four apart: the second would
+        // wait for the first)
+        acc[db] = q3::mfma32x32x16(vf[db], q3::as_bf16x8(term == 0 ? p.hi[g] : p.lo[g]), acc[db]);
+        if (g == 0 && term == 1) vf[db] = lds_vt(vt, pv_operand(off, 4 + db));
+        if (db & 1) between(4 * g + 2 * term + (db >> 1));
+        __builtin_amdgcn_sched_barrier(0);
+      }
 }
 
 // Staged tiles [p0, p1) of the list, by one workgroup.  A wave takes 32 of an item's rows
 // and 32 of a tile's keys, so that each SIMD has work of up to 64 rows on; the two halves of
 // the keys are joined when the item ends.
 __device__ __forceinline__ void staged_range(const SharedArgs& a, const Tables& t, int all_t, int v,
-                                             int p0, int p1, const Stage (&st)[kStages],
-                                             Pages& pages) {
+                                             int p0, int p1, uint16_t* tiles_at, Pages& pages) {
   const DecodeArgs& d = a.d;
-  constexpr int kShare = 2 * dma_per_wave<kShWaves>();  // a wave's loads of a tile
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = uniform(tid >> 6);
-  const LaneOffsets off = lane_offsets<kShWaves>(a, lane, wave);
+  LaneOffsets off;
+  read_offsets(off, lane);
+  const Loader loader = loader_of(a, lane, wave);
   int p = p0;
   while (p < p1) {
     const int kvh = uniform(p / all_t);
@@ -680,8 +696,7 @@ __device__ __forceinline__ void staged_range(const SharedArgs& a, const Tables& 
     for (int o = 1; o < 32; o <<= 1) lo_last = min(lo_last, __shfl_xor(lo_last, o, 64));
     lo_last = uniform(lo_last);
     const int64_t row = uniform(t.row[s0]);
-    const uint16_t* kh = a.k + kvh * a.k_sh;
-    const uint16_t* vh = a.v + kvh * a.v_sh;
+    const uint16_t* kv = loader.base + kvh * (wave < 4 ? a.k_sh : a.v_sh);
     float m_run = q3::kNegInf, l_run = 0.f;
     q3::f32x16 acc[4];
 #pragma unroll
@@ -697,55 +712,95 @@ __device__ __forceinline__ void staged_range(const SharedArgs& a, const Tables& 
       // tiles ahead)
 #pragma unroll
       for (int c = 0; c < 8; ++c) asm volatile("" : "+v"(qv[c]));
-      uint32_t ok[kStages];
-      auto stage = [&](int j, const Next& n, int to) {
-        ok[to] = stage_tile(a, off, kh, vh, j * kBN, keys, n, st[to], wave);
+      // stage i: tile ja + i of this round, then every fourth
+      auto stage = [&](int j, const Next& n) {
+        const uint16_t* to = tiles_at + ((j - ja) % kStages) * kStageElems;
+        return stage_tile(loader, kv, keys - j * kBN, n, wave < 4 ? to : to + kTileElems);
       };
+      uint32_t ok[kStages - 1] = {0u, 0u, 0u};  // of the next tiles
 #pragma unroll
       for (int u = 0; u < kStages - 1; ++u)
-        if (ja + u < je) stage(ja + u, next_tile(pages, u, wave), u);
-      Next ahead = next_tile(pages, min(kStages - 1, je - ja - 1), wave);
+        if (ja + u < je) ok[u] = stage(ja + u, next_tile(pages, u, loader));
+      Next ahead = next_tile(pages, min(kStages - 1, je - ja - 1), loader);
 
-      auto step = [&](int j, int u) {
-        // this wave's share of tile j has arrived (its loads of the next tiles are newer),
+      // a tile's scores, masked: x[i] is key n0 + 4 (lane / 32) + kr of group 2 half + i / 8
+      auto mask = [&](q3::f32x16& x, int j, uint32_t okj) {
+        const int n0 = j * kBN + 32 * half;
+        if (n0 + 31 > lo_last || okj != 15u) {
+          const int lim = last - n0 - 4 * (lane >> 5);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int kr = 8 * (i / 4) + (i % 4);
+            const int l = (okj >> (2 * half + i / 8)) & 1u ? lim : -1;
+            x[i] = kr <= l ? x[i] : q3::kNegInf;
+          }
+        }
+      };
+      const int rest = half < 2 ? half * 32 * kD : 0;  // where a wave's keys begin in a tile
+      // the first tile has arrived (its loads are the oldest), at every wave's
+      if (ja + 2 < je) __builtin_amdgcn_s_waitcnt(0x0f70 | 2 * kShare);
+      else if (ja + 1 < je) __builtin_amdgcn_s_waitcnt(0x0f70 | kShare);
+      else wait_loads();
+      __builtin_amdgcn_s_barrier();
+      Probs probs;
+      if (active) {
+        q3::f32x16 x = score(off, tiles_at + rest, qv);
+        mask(x, ja, ok[0]);
+        const float alpha = raise_max(x, d.scale_log2, m_run), use = finite_max(m_run);
+        float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) prob_pair(probs, sums, x, i, d.scale_log2, use);
+        l_run = l_run * alpha + ((sums[0] + sums[1]) + (sums[2] + sums[3]));
+#pragma unroll
+        for (int db = 0; db < 4; ++db) acc[db] *= alpha;
+      }
+      const uint16_t* here = tiles_at;
+      // Tile j's values meet their probabilities while the next tile's are computed.
+      for (int j = ja; j + 1 < je; ++j) {
+        const uint16_t* next = tiles_at + ((j + 1 - ja) % kStages) * kStageElems;
+        // this wave's share of tile j + 1 has arrived (its loads of tile j + 2 are newer),
         // then everybody's has, and nobody reads tile j - 1 any more
-        if (j + 2 < je) __builtin_amdgcn_s_waitcnt(0x0f70 | 2 * kShare);
-        else if (j + 1 < je) __builtin_amdgcn_s_waitcnt(0x0f70 | kShare);
+        if (j + 2 < je) __builtin_amdgcn_s_waitcnt(0x0f70 | kShare);
         else wait_loads();
         __builtin_amdgcn_s_barrier();
-        const uint32_t here = ok[u];
+        const uint32_t ok1 = ok[1];
+        ok[1] = ok[2];
         if (j + kStages - 1 < je) {
-          stage(j + kStages - 1, ahead, (u + kStages - 1) % kStages);
-          ahead = next_tile(pages, min(j + kStages, je - 1) - ja, wave);
+          ok[2] = stage(j + kStages - 1, ahead);
+          ahead = next_tile(pages, min(j + kStages, je - 1) - ja, loader);
         }
-        if (!active) return;
-        const int n0 = j * kBN + 32 * half;
-        auto mask = [&](q3::f32x16 (&x)) {
-          if (n0 + 31 > lo_last || here != 15u) {
-            // score i: key n0 + 4 (lane / 32) + kr of group 2 half + i / 8
-            const int lim = last - n0 - 4 * (lane >> 5);
+        if (active) {
+          const uint16_t* vt = here + kTileElems + rest;
+          if (half == 1) add_values(off, vt, probs, [](int) {}, acc);
+          q3::f32x16 x = score(off, next + rest, qv);
+          mask(x, j + 1, ok1);
+          const float alpha = raise_max(x, d.scale_log2, m_run), use = finite_max(m_run);
+          Probs p;
+          float sums[4] = {0.f, 0.f, 0.f, 0.f};
+          auto pair = [&](int i) { prob_pair(p, sums, x, i, d.scale_log2, use); };
+          if (half == 0) {
+            add_values(off, vt, probs, pair, acc);
+          } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int kr = 8 * (i / 4) + (i % 4);
-              const int l = (here >> (2 * half + i / 8)) & 1u ? lim : -1;
-              x[i] = kr <= l ? x[i] : q3::kNegInf;
-            }
+            for (int i = 0; i < 8; ++i) pair(i);
           }
-        };
-        half_fold(off, d.scale_log2, mask, st[u].k + half * 32 * kD, st[u].v + half * 32 * kD, qv,
-                  m_run, l_run, acc);
-      };
-      for (int j = ja; j < je; j += kStages) {
-        step(j, 0);
-        if (j + 1 < je) step(j + 1, 1);
-        if (j + 2 < je) step(j + 2, 2);
-        if (j + 3 < je) step(j + 3, 3);
+          l_run = l_run * alpha + ((sums[0] + sums[1]) + (sums[2] + sums[3]));
+          if (__any(alpha != 1.f)) {
+#pragma unroll
+            for (int db = 0; db < 4; ++db) acc[db] *= alpha;
+          }
+          probs = p;
+        }
+        here = next;
+      }
+      if (active) {
+        add_values(off, here + kTileElems + rest, probs, [](int) {}, acc);
       }
       __syncthreads();  // pages and stages are read before they are filled again
     }
     // the second half's state, through the stages
-    q3::f32x4* hold = reinterpret_cast<q3::f32x4*>(part == 0 ? st[0].k : part == 1 ? st[0].v : part == 2 ? st[1].k : st[1].v) + lane;
-    float2* ml = reinterpret_cast<float2*>(st[2].k) + part * 64 + lane;
+    q3::f32x4* hold = reinterpret_cast<q3::f32x4*>(tiles_at + part * kTileElems) + lane;
+    float2* ml = reinterpret_cast<float2*>(tiles_at + 4 * kTileElems) + part * 64 + lane;
     if (half == 1) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
@@ -790,14 +845,7 @@ __device__ __forceinline__ void staged_range(const SharedArgs& a, const Tables& 
 
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_shared_kernel(SharedArgs a) {
-  __shared__ __attribute__((aligned(1024))) uint16_t s_k0[kTileElems];
-  __shared__ __attribute__((aligned(1024))) uint16_t s_v0[kTileElems];
-  __shared__ __attribute__((aligned(1024))) uint16_t s_k1[kTileElems];
-  __shared__ __attribute__((aligned(1024))) uint16_t s_v1[kTileElems];
-  __shared__ __attribute__((aligned(1024))) uint16_t s_k2[kTileElems];
-  __shared__ __attribute__((aligned(1024))) uint16_t s_v2[kTileElems];
-  __shared__ __attribute__((aligned(1024))) uint16_t s_k3[kTileElems];
-  __shared__ __attribute__((aligned(1024))) uint16_t s_v3[kTileElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t s_tiles[kStages * kStageElems];
   __shared__ Tables t;
   __shared__ Pages s_pages;
   const int tid = threadIdx.x, wave = uniform(tid >> 6);
@@ -811,7 +859,7 @@ void paged_shared_kernel(SharedArgs a) {
     for (int b = tid; b < a.d.B; b += kThreads) {
       SeqMeta m{};
       m.own_at = t.own[b];
-      m.own_n = t.own[b + 1] - t.own[b];
+      m.own_n = max(0, t.own[b + 1] - t.own[b] - kSegTiles);
       if (skipped(t, b) > 0) {
         const int g = t.grp[b];
         const int rows = members(t, g, a.d.B) * a.d.G;
@@ -828,9 +876,8 @@ void paged_shared_kernel(SharedArgs a) {
   const int v = blockIdx.x;
   if (v < plan.wgs_t) {
     const int p0 = v * plan.pt;
-    const Stage st[kStages] = {{s_k0, s_v0}, {s_k1, s_v1}, {s_k2, s_v2}, {s_k3, s_v3}};
     if (p0 < plan.staged)
-      staged_range(a, t, all_t, v, p0, min(p0 + plan.pt, plan.staged), st, s_pages);
+      staged_range(a, t, all_t, v, p0, min(p0 + plan.pt, plan.staged), s_tiles, s_pages);
     return;
   }
   // a batch too small for every wave is dealt one wave a workgroup first
@@ -871,7 +918,7 @@ __global__ __launch_bounds__(kMaxG * 64) void paged_shared_join_kernel(SharedArg
   // a streamed item's parts: `col` its column of this row
   auto streamed = [&](Parts& x, const float* po, const float* lse, int before, int n, int col) {
     if (n == 0) return;
-    const int S = d.Hkv * before + hkv * n;
+    const int S = d.Hkv * before + hkv * (n + kSegTiles) + kSegTiles;
     const int64_t wf = S / call.pw, wl = (S + n - 1) / call.pw;
     x.n = static_cast<int>(wl - wf + 1);
     if (wf == wl) {
@@ -883,7 +930,7 @@ __global__ __launch_bounds__(kMaxG * 64) void paged_shared_join_kernel(SharedArg
     }
     x.po = a.po_s;
     x.lse = a.lse_s;
-    x.first = (2 * wf + (wf * call.pw != S ? 1 : 0)) * kRowsS + col;
+    x.first = (2 * wf + 1) * kRowsS + col;
     x.step = 2 * kRowsS;
     x.next = 2 * wf * kRowsS + col;
   };
