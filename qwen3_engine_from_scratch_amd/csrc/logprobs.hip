@@ -29,9 +29,11 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kMaxTop = 64;      // most likely tokens a row
 constexpr int kMaxGiven = 64;    // given tokens a row
 constexpr int kMaxParts = 64;
+constexpr int kResident = 512;   // workgroups that run at once
 constexpr int kCap = 1024;       // candidates of a part
 constexpr int kFewThreads = 128; // threads that reach T and are read again one by one
-constexpr int kBatch = 4;        // 16-byte pieces a thread loads at once
+constexpr int kBatchTokens = 16; // a thread's tokens of a load
+constexpr int kFewPieces = 256;  // pieces that are read again for a bound looser than n needs
 constexpr float kFloor = -1e38f; // R of a state without finite terms
 constexpr float kExtreme = 1e38f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -272,10 +274,11 @@ __device__ __forceinline__ u64 block_max(u64 v, Shared& sh) {
   return v;
 }
 
-// Largest bound that at least n of the keys reach, 0 if there are fewer: bit by bit, by
-// one wave, kPer keys a lane.
+// A bound that n to `most` of the keys reach, or the n-th largest key itself where equal
+// ones leave no such bound (0: fewer than n keys).  Bit by bit, by one wave, kPer keys a
+// lane.
 template <int kPer>
-__device__ __forceinline__ uint32_t nth_bound(const uint32_t (&k)[kPer], int n) {
+__device__ __forceinline__ uint32_t nth_bound(const uint32_t (&k)[kPer], int n, int most) {
   uint32_t t = 0;
   for (int bit = 31; bit >= 0; --bit) {
     const uint32_t cand = t | 1u << bit;
@@ -283,8 +286,22 @@ __device__ __forceinline__ uint32_t nth_bound(const uint32_t (&k)[kPer], int n) 
 #pragma unroll
     for (int i = 0; i < kPer; ++i) cnt += __popcll(__ballot(k[i] >= cand));
     if (cnt >= n) t = cand;
+    if (cnt >= n && cnt <= most) break;
   }
   return t;
+}
+
+// Largest x of a wave's lanes, on every lane: four steps inside each row of 16 lanes, then
+// the rows' own into the rows above.
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+  auto take = [&](uint32_t y) { x = y > x ? y : x; };
+  take(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x111, 0xF, 0xF, true));   // row_shr:1
+  take(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x112, 0xF, 0xF, true));   // row_shr:2
+  take(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x114, 0xF, 0xF, true));   // row_shr:4
+  take(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x118, 0xF, 0xF, true));   // row_shr:8
+  take(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x142, 0xA, 0xF, false));  // row_bcast:15
+  take(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x143, 0xC, 0xF, false));  // row_bcast:31
+  return __builtin_amdgcn_readlane(x, 63);
 }
 
 // Appends a part's token to the candidates (counted, not kept, behind the list's end).
@@ -293,25 +310,27 @@ __device__ __forceinline__ void append(Shared& sh, uint32_t key, int idx) {
   if (at < kCap) sh.cand[at] = ranked(key, static_cast<uint32_t>(idx));
 }
 
-// The tokens of the threads in sh.few whose key is at least `least`.
+// The tokens of the threads in sh.few whose key is at least `least`: their pieces dealt to
+// all threads, so that the loads are one round trip (or few).
 template <typename Tr>
 __device__ __forceinline__ void gather_few(const LogprobArgs& a, const char* xr, int p0, int p1,
                                            uint32_t least, Shared& sh) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int n = min(sh.n_few, kFewThreads);
-  for (int i = wave; i < n; i += kWaves)
-    for (int64_t p = static_cast<int64_t>(p0) + sh.few[i] + static_cast<int64_t>(lane) * kThreads;
-         p < p1; p += 64 * kThreads) {
-      float x[Tr::kE];
-      Tr::unpack(load_piece<Tr>(a, xr, static_cast<int>(p)), x);
+  const int each = (p1 - p0 + kThreads - 1) / kThreads;  // a thread's pieces
+  const int all = min(sh.n_few, kFewThreads) * each;
+  for (int i = threadIdx.x; i < all; i += kThreads) {
+    const int of = i / each;
+    const int p = p0 + sh.few[of] + (i - of * each) * kThreads;
+    if (p >= p1) continue;
+    float x[Tr::kE];
+    Tr::unpack(load_piece<Tr>(a, xr, p), x);
 #pragma unroll
-      for (int e = 0; e < Tr::kE; ++e) {
-        int idx;
-        const bool ok = token_at<Tr>(a, static_cast<int>(p), e, idx);
-        const uint32_t k = key_of(x[e]);
-        if (ok && k >= least) append(sh, k, idx);
-      }
+    for (int e = 0; e < Tr::kE; ++e) {
+      int idx;
+      const bool ok = token_at<Tr>(a, p, e, idx);
+      const uint32_t k = key_of(x[e]);
+      if (ok && k >= least) append(sh, k, idx);
     }
+  }
 }
 
 // Lists the threads where q holds.
@@ -358,7 +377,9 @@ __device__ __forceinline__ void top_tokens(const LogprobArgs& a, const char* xr,
       uint32_t k[kWaves];
 #pragma unroll
       for (int i = 0; i < kWaves; ++i) k[i] = sh.key[64 * i + lane];
-      const uint32_t t = nth_bound(k, n);
+      const int each = (p1 - p0 + kThreads - 1) / kThreads;
+      const int most = each > 0 ? min(kFewThreads, kFewPieces / each) : n;
+      const uint32_t t = nth_bound(k, n, most > n ? most : n);
       if (lane == 0) sh.bound = t;
     }
     __syncthreads();
@@ -375,6 +396,7 @@ __device__ __forceinline__ void top_tokens(const LogprobArgs& a, const char* xr,
     __syncthreads();
     gather_few<Tr>(a, xr, p0, p1, few ? t : t + 1u, sh);
     __syncthreads();
+    // (many reach t by equal values: t is the n-th largest itself, not below it)
     if (!few && sh.n_cand < n) {  // the lowest indices at t itself
       int left = n - sh.n_cand;
       for (int p = p0 + tid; left > 0 && p - tid < p1; p += kThreads) {
@@ -481,10 +503,9 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, const char* xr, 
 }
 
 template <typename Tr, bool kEnt, bool kTop>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4, 4)))
-void logprobs_kernel(LogprobArgs a) {
+__global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
   __shared__ Shared sh;
-  constexpr int E = Tr::kE;
+  constexpr int E = Tr::kE, kBatch = kBatchTokens / E;
   const int tid = threadIdx.x;
   const uint32_t row = blockIdx.x / static_cast<uint32_t>(a.parts);
   const int part = static_cast<int>(blockIdx.x - row * static_cast<uint32_t>(a.parts));
@@ -596,29 +617,20 @@ __global__ __launch_bounds__(kJoinThreads) void logprobs_join_kernel(LogprobArgs
     for (int i = tid; i < all; i += kJoinThreads) s_all[i] = a.part_top[row * all + i];
     __syncthreads();
     if (tid < 64) {
-      // the n-th largest, key and index, bit by bit: n tokens are left, then ranked
-      u64 t = 0;
-      for (int bit = 63; bit >= 0; --bit) {
-        const u64 cand = t | 1ull << bit;
-        int cnt = 0;
-        for (int i = 0; i < all; i += 64)
-          cnt += __popcll(__ballot(i + lane < all && s_all[i + lane] >= cand));
-        if (cnt >= a.top) t = cand;
-      }
-      int at = 0;
-      for (int i = 0; i < all; i += 64) {
-        const u64 r = i + lane < all ? s_all[i + lane] : 0;
-        const uint64_t in = __ballot(r != 0 && r >= t);
-        if (r != 0 && r >= t) {
-          const int slot = at + __popcll(in & ((uint64_t{1} << lane) - 1));
-          if (slot < kMaxTop) s_top[slot] = r;
+      // the parts' lists fall: the largest of their heads, n times, a list a lane
+      int at = lane * a.top;
+      const int end = lane < a.parts ? at + a.top : at;
+      u64 head = at < end ? s_all[at] : 0;
+      for (int r = 0; r < a.top; ++r) {
+        const uint32_t key = key_in(head), low = static_cast<uint32_t>(head);
+        const uint32_t best = wave_max(key);
+        const uint32_t first = wave_max(key == best ? low : 0u);
+        if (key == best && low == first && head != 0) {
+          s_top[r] = head;
+          ++at;
+          head = at < end ? s_all[at] : 0;
         }
-        at += __popcll(in);
       }
-      const u64 r = lane < min(at, kMaxTop) ? s_top[lane] : 0;
-      int rank = 0;
-      for (int j = 0; j < min(at, kMaxTop); ++j) rank += __shfl(r, j, 64) > r ? 1 : 0;
-      if (r != 0) s_top[rank] = r;
     }
     __syncthreads();
   }
@@ -733,11 +745,11 @@ __global__ __launch_bounds__(kGradThreads) void logprobs_grad_kernel(GradArgs g)
 int elements_of(int dtype) { return dtype == 2 ? 4 : 8; }
 int bytes_of(int dtype) { return dtype == 2 ? 4 : 2; }
 
-// Parts of a row: about a thousand workgroups where the rows are fewer, of a round each
-// (512 pieces) at least.
+// Parts of a row: as many workgroups as the device holds at once where the rows are fewer,
+// of a round each (512 pieces) at least.
 int parts_for(int64_t rows, int64_t pieces) {
   const int64_t most = q3::cdiv(pieces, kThreads);
-  int64_t p = q3::cdiv(1024, rows);
+  int64_t p = kResident / rows;
   p = p < most ? p : most;
   p = p < kMaxParts ? p : kMaxParts;
   return static_cast<int>(p < 1 ? 1 : p);

@@ -20,6 +20,7 @@ gradient for the logits.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple
 
@@ -136,6 +137,11 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: torch.Tensor | None  # fp32 (T, n)
 
 
+@functools.lru_cache(maxsize=1024)
+def _logprobs_workspace(*shape) -> int:
+    return int(_lib.load().qwen3_token_logprobs_workspace_bytes(*shape))
+
+
 def _forward(logits, tokens, top_n, entropy, temperature, stats):
     """One call of the kernel: (logprobs, entropy, top_ids, top_logprobs, stats)."""
     T, V = logits.shape
@@ -149,7 +155,7 @@ def _forward(logits, tokens, top_n, entropy, temperature, stats):
     ids = torch.empty(T, top_n, dtype=torch.int64, device=dev) if top_n else None
     top = torch.empty(T, top_n, **f32) if top_n else None
     st = torch.empty(T, 2, **f32) if stats else None
-    need = int(lib.qwen3_token_logprobs_workspace_bytes(T, V, dtype, top_n))
+    need = _logprobs_workspace(T, V, dtype, top_n)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     ptr = _lib.ptr
     with _lib.on_device(dev):
