@@ -30,8 +30,9 @@ from . import _lib
 from .kernels.paged_attention import update_kv_batch_hip
 from .kernels.paged_cache import copy_pages_hip, fork_pages_hip, move_pages_hip
 
-__all__ = ["KVCachePool", "PagedKVCache", "fork_caches", "prefill_slot_mapping", "write_prefill_batch",
-           "reserve_pages_bulk", "set_seq_lens_bulk", "PageIn"]
+__all__ = ["KVCachePool", "PagedKVCache", "fork_caches", "shared_prefix_groups",
+           "prefill_slot_mapping", "write_prefill_batch", "reserve_pages_bulk",
+           "set_seq_lens_bulk", "PageIn"]
 
 
 class KVCachePool:
@@ -370,6 +371,64 @@ def fork_caches(parents: list, tokens: list | None = None) -> list:
         c.num_pages = len(c.block_table)
         children.append(c)
     return children
+
+
+def shared_prefix_groups(caches: list) -> tuple[list, list, list]:
+    """How a batch of handles shares its first pages, for
+    paged_attention_decode_shared_hip: (order, cu_groups, shared_lens), host lists.
+    order: a permutation of the handles that brings each group's together, what shares
+    nothing last; group g is entries cu_groups[g] .. cu_groups[g + 1] - 1 of it, which hold
+    their first shared_lens[g] tokens in the same (whole) pages.  Of nested prefixes (a
+    system prompt, questions behind it) those are taken that save the most pages.  Valid
+    as long as the handles only grow."""
+    pool = caches[0]._pool if caches else None
+    for c in caches:
+        c.check_live()
+        if c._pool is not pool:
+            raise ValueError("handles of several pools in one batch")
+    tables = [c.block_table for c in caches]
+    order = sorted(range(len(caches)), key=lambda i: tables[i])
+
+    def common(a, b):
+        lo, hi = 0, min(len(a), len(b))
+        while lo < hi:  # the first lo pages are common, more than hi are not
+            mid = (lo + hi + 1) // 2
+            if a[lo:mid] == b[lo:mid]:
+                lo = mid
+            else:
+                hi = mid - 1
+        return lo
+
+    # The sorted handles' common prefixes form a tree: a node is a range of them and the
+    # pages that all of it begins with.  Bottom up, a node makes a group of the handles that
+    # have none below it and of those groups that save no more by themselves.
+    #   open node: pages, first handle, handles without a group, groups (handles, pages)
+    stack = [(0, 0, [], [])]
+    for i in range(1, len(order) + 1):
+        pages = common(tables[order[i - 1]], tables[order[i]]) if i < len(order) else 0
+        lo, free, groups = i - 1, order[i - 1:i], []
+        while pages < stack[-1][0]:
+            n, lo, more_free, more_groups = stack.pop()
+            free, groups = more_free + free, more_groups + groups
+            keep = [g for g in groups if (len(g[0]) - 1) * g[1] > len(g[0]) * n]
+            lost = sum((len(g[0]) - 1) * g[1] for g in groups) \
+                - sum((len(g[0]) - 1) * g[1] for g in keep)
+            joined = free + [h for g in groups if g not in keep for h in g[0]]
+            if (len(joined) - 1) * n > lost:
+                free, groups = [], keep + [(joined, n)]
+        if pages > stack[-1][0]:
+            stack.append((pages, lo, free, groups))
+        else:
+            top = stack.pop()
+            stack.append((*top[:2], top[2] + free, top[3] + groups))
+    groups = stack[0][3]  # below the root, which shares nothing
+    grouped = [i for members, _ in groups for i in members]
+    alone = sorted(set(order).difference(grouped))
+    cu = [0]
+    for members, _ in groups:
+        cu.append(cu[-1] + len(members))
+    bs = pool.block_size if pool is not None else 0
+    return grouped + alone, cu, [pages * bs for _, pages in groups]
 
 
 class PageIn:

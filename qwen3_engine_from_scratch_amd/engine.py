@@ -24,6 +24,11 @@ the per-step state lives:
     token computed past it (its page writes land beyond its final length).
 Greedy decoding only (temperature 0), as the reference's benchmark runs.
 
+Requests may ask how probable their tokens were (GenRequest.logprobs; a step with such a
+request computes its logits and is not replayed from a graph), prompts can be scored
+without generating (Engine.score), and requests that share a prefix may attend it
+together (share_prefixes: their shared pages are read once a step).
+
 Prompts may also follow a prefix that is cached already (Engine.cache_prefix,
 GenRequest.prefix: its pages are shared, not computed again), and long ones may be
 prefilled in pieces (prefill_chunk: bounds what each prompt adds to a step; with
@@ -39,11 +44,15 @@ from dataclasses import dataclass, field
 import numpy as np
 import torch
 
-from .PagedKVcache import PageIn, PagedKVCache, fork_caches, set_seq_lens_bulk
+from .PagedKVcache import (PageIn, PagedKVCache, fork_caches, set_seq_lens_bulk,
+                           shared_prefix_groups)
 from .graph_runner import GraphRunner, pow2_buckets
 from .kernels.model_ops import argmax
+from .sampling import MAX_TOP, TokenLogprobs, token_logprobs
 
 __all__ = ["GenRequest", "Engine"]
+
+MAX_SHARED_BATCH = 1024  # sequences of a decode step over shared prefixes
 
 
 @dataclass
@@ -54,7 +63,10 @@ class GenRequest:
     max_new_tokens: int
     eos_token_id: int | None = None
     prefix: PagedKVCache | None = None  # tokens before the prompt; forked, stays the caller's
+    logprobs: int | None = None  # also each token's log probability, and of the n likeliest
     output_ids: list = field(default_factory=list)
+    output_logprobs: list = field(default_factory=list)  # of output_ids, if asked for
+    output_top: list = field(default_factory=list)       # [(id, log probability), ...] each
     cache: PagedKVCache | None = None
     finished: bool = False
     finish_time: float = 0.0
@@ -75,7 +87,7 @@ class GenRequest:
 class Engine:
     def __init__(self, model, pool, max_batch: int = 64, use_graph: bool = True,
                  batch_invariant: bool = False, max_prefill_batch: int | None = None,
-                 prefill_chunk: int | None = None):
+                 prefill_chunk: int | None = None, share_prefixes: bool = False):
         """batch_invariant: decode attention on the batch-invariant kernel,
         so a request's decode tokens do not depend on what else is batched
         with it.  max_prefill_batch: prompts per prefill step (None: as many
@@ -83,8 +95,15 @@ class Engine:
         request running by itself would be (the library GEMMs of the
         prefill pick kernels by row count, so a prompt's prefill bits depend
         on the rows batched with it).  prefill_chunk: tokens of a prompt per
-        prefill step (None: whole prompts)."""
+        prefill step (None: whole prompts).  share_prefixes: decode steps attend
+        the pages that requests share once for all of them (requests with a common
+        prefix handle), up to 1,024 requests; not with batch_invariant.  A prefix's
+        sums are then taken in another order, so near ties may fall differently."""
         assert prefill_chunk is None or prefill_chunk > 0
+        if share_prefixes and (batch_invariant or max_batch > MAX_SHARED_BATCH):
+            raise ValueError("share_prefixes needs batch_invariant off and a max_batch of at most "
+                             f"{MAX_SHARED_BATCH}")
+        self.share_prefixes = share_prefixes
         self.prefill_chunk = prefill_chunk
         self.model = model
         self.pool = pool
@@ -98,7 +117,8 @@ class Engine:
             buckets = pow2_buckets(max_batch)
             self._placeholders = [PagedKVCache(pool) for _ in range(max(buckets))]
             self.runner = GraphRunner(model, pool, self._placeholders, buckets, reserve_pages=1,
-                                      greedy=True, advance=True, positions_from_lengths=True)
+                                      greedy=True, advance=True, positions_from_lengths=True,
+                                      shared=share_prefixes)
         else:
             model.reserve_decode_workspace(max_batch, pool)
         # two pinned landing buffers: a step's tokens are read back while the
@@ -110,12 +130,29 @@ class Engine:
         self._pages = PageIn(pool, max(max_batch * max_pages, 64))
         self._pending = None     # (requests, host view, event) of the last decode launch
         self._last_batch = None  # (bucket, request ids) of the last graph replay
+        self._last_reqs = None   # its requests, in the rows' order
 
     # ---- steps -------------------------------------------------------------
 
-    def _run_chunk(self, caches, tokens, want_logits):
+    @staticmethod
+    def _choose(logits, reqs):
+        """Greedy token of each request from a step's logits; (token, log probability,
+        [(id, log probability), ...]) of those that ask for it."""
+        toks = argmax(logits)
+        if all(r.logprobs is None for r in reqs):
+            return toks.cpu().tolist()
+        top = max(r.logprobs for r in reqs if r.logprobs is not None)
+        got = token_logprobs(logits, toks, top_n=top)
+        lps = got.logprobs.cpu().tolist()
+        ids = got.top_ids.cpu().tolist() if top else [[]] * len(reqs)
+        likely = got.top_logprobs.cpu().tolist() if top else [[]] * len(reqs)
+        return [tok if r.logprobs is None else (tok, lp, list(zip(i, p))[:r.logprobs])
+                for r, tok, lp, i, p in zip(reqs, toks.cpu().tolist(), lps, ids, likely)]
+
+    def _run_chunk(self, caches, tokens, reqs):
         """One chunk step: tokens[i] (a list, not empty) behind what caches[i] holds.
-        Returns the greedy next token of each handle, or None."""
+        Returns what each handle's request takes next (_choose), or None where there
+        are no requests."""
         dev = self.device
         starts, lens = [c.seq_len for c in caches], [len(t) for t in tokens]
         self._pages.reserve(caches, [a + n for a, n in zip(starts, lens)])
@@ -136,14 +173,14 @@ class Engine:
         buf[3 * T + 2 * n + 1:] = [c.row_id for c in caches]
         d = torch.from_numpy(buf).to(dev)
         small = d[3 * T + n:].to(torch.int32)
-        rows = d[3 * T:3 * T + n] if want_logits else d[3 * T:3 * T + 1]
+        rows = d[3 * T:3 * T + n] if reqs else d[3 * T:3 * T + 1]
         logits = self.model.chunk_logits(d[:T], small[:n + 1], max(lens), small[n + 1:],
                                          d[T:2 * T], d[2 * T:3 * T], self.pool, rows)
-        toks = argmax(logits).cpu().tolist() if want_logits else None
+        chosen = self._choose(logits, reqs) if reqs else None
         for c, m in zip(caches, lens):
             c.seq_len += m
         set_seq_lens_bulk(caches)
-        return toks
+        return chosen
 
     def _check_positions(self, tokens: int) -> None:
         """The rotary tables end; a token behind them would be computed wrongly."""
@@ -161,7 +198,7 @@ class Engine:
         step = self.prefill_chunk or max(len(tokens), 1)
         try:
             for i in range(0, len(tokens), step):
-                self._run_chunk([c], [tokens[i:i + step]], False)
+                self._run_chunk([c], [tokens[i:i + step]], None)
         except BaseException:
             c.free()  # nobody else knows it
             raise
@@ -185,12 +222,12 @@ class Engine:
         done = {id(r): 0 for r in reqs}
         left = list(reqs)
         while left:
-            toks = self._run_chunk([r.cache for r in left],
-                                   [r.prompt[done[id(r)]:done[id(r)] + step] for r in left], True)
-            for r, tok in zip(left, toks):
+            chosen = self._run_chunk([r.cache for r in left],
+                                     [r.prompt[done[id(r)]:done[id(r)] + step] for r in left], left)
+            for r, got in zip(left, chosen):
                 done[id(r)] += step
                 if done[id(r)] >= len(r.prompt):
-                    self._take(r, int(tok))
+                    self._take(r, got)
             left = [r for r in left if done[id(r)] < len(r.prompt)]
 
     def _prefill(self, reqs) -> None:
@@ -209,6 +246,8 @@ class Engine:
                     r.cache.free()
                     r.cache = cache
                 del r.output_ids[told:]
+                del r.output_logprobs[told:]
+                del r.output_top[told:]
                 r.eos_hit = eos_hit
             raise
 
@@ -238,17 +277,21 @@ class Engine:
         logits = self.model.prefill_logits(d[:T], d[3 * T + n:].to(torch.int32), max(lens),
                                            d[T:2 * T], d[2 * T:3 * T], self.pool,
                                            d[3 * T:3 * T + n])
-        toks = argmax(logits).cpu().tolist()
-        for r, L, tok in zip(reqs, lens, toks):
+        for r, L, got in zip(reqs, lens, self._choose(logits, reqs)):
             r.cache.seq_len = L
-            self._take(r, int(tok))
+            self._take(r, got)
         set_seq_lens_bulk([r.cache for r in reqs])
 
     @staticmethod
-    def _take(r, tok: int) -> None:
+    def _take(r, got) -> None:
+        """got: the request's next token, or that with its log probabilities (_choose)."""
         if r.eos_hit or len(r.output_ids) >= r.max_new_tokens:
             return  # a step launched before the stop was known: its token is dropped
+        tok, *told = got if isinstance(got, tuple) else (int(got),)
         r.output_ids.append(tok)
+        if told:
+            r.output_logprobs.append(told[0])
+            r.output_top.append(told[1])
         if r.eos_token_id is not None and tok == r.eos_token_id:
             r.eos_hit = True
 
@@ -268,30 +311,47 @@ class Engine:
         of the step before it, so the host's bookkeeping overlaps the GPU."""
         k = len(reqs)
         dev = self.device
-        if self.runner is not None:
-            b = self.runner.bucket_for(k)
-            key = (b, tuple(r.request_id for r in reqs))
-            if key != self._last_batch:
-                # a changed batch takes its input tokens from the host
-                self._drain()
-        else:
+        told = any(r.logprobs is not None for r in reqs)  # needs logits: no replay
+        replay = self.runner is not None and not told
+        key = (self.runner.bucket_for(k), tuple(r.request_id for r in reqs)) if replay else None
+        if not replay or key != self._last_batch:
+            # a changed batch takes its input tokens from the host
             self._drain()
-        caches = [r.cache for r in reqs]
+        if not replay:
+            self._last_batch = None
         # the token of this step lands at position seq_len: reserve its page
+        caches = [r.cache for r in reqs]
         self._pages.reserve(caches, [c.seq_len + 1 for c in caches])
-        if self.runner is not None:
-            if key == self._last_batch:
-                out = self.runner.replay_greedy(k)
+        groups = None
+        if self.share_prefixes and (not replay or key != self._last_batch):
+            order, *groups = shared_prefix_groups(caches)
+            if replay or groups[1]:
+                reqs = [reqs[i] for i in order]
+                caches = [caches[i] for i in order]
             else:
-                ids = torch.tensor([r.output_ids[-1] for r in reqs], dtype=torch.int64)
-                rows = torch.tensor([c.row_id for c in caches], dtype=torch.int32)
-                out = self.runner.replay_greedy(k, ids.to(dev), rows.to(dev))
-                self._last_batch = key
-            toks = out.view(-1)[:k]
+                groups = None
+        if replay and key == self._last_batch:
+            reqs = self._last_reqs
+            caches = [r.cache for r in reqs]
+            out = self.runner.replay_greedy(k)
         else:
             ids = torch.tensor([r.output_ids[-1] for r in reqs], dtype=torch.int64).to(dev)
             rows = torch.tensor([c.row_id for c in caches], dtype=torch.int32).to(dev)
-            toks = self.model.decode_greedy(ids, rows, self.pool)
+            shared = None
+            if replay:
+                if groups is not None:
+                    self.runner.set_groups(k, *groups)
+                out = self.runner.replay_greedy(k, ids, rows)
+                self._last_batch, self._last_reqs = key, list(reqs)
+            elif groups is not None:
+                shared = tuple(torch.tensor(g, dtype=torch.int32).to(dev) for g in groups)
+            if told:
+                self._take_step(reqs, caches, self.model.decode_logits(ids, rows, self.pool,
+                                                                       shared=shared))
+                return
+            if not replay:
+                out = self.model.decode_greedy(ids, rows, self.pool, shared=shared)
+        toks = out.view(-1)[:k]
         host = self._tok_host[self._flip][:k]
         self._flip ^= 1
         host.copy_(toks, non_blocking=True)
@@ -306,6 +366,48 @@ class Engine:
         self._drain()
         self._pending = (list(reqs), host, ev)
 
+    def _take_step(self, reqs, caches, logits) -> None:
+        """Ends a decode step whose logits are at hand: its tokens are read back at once."""
+        for r, got in zip(reqs, self._choose(logits, reqs)):
+            self._take(r, got)
+        for c in caches:
+            c.seq_len += 1
+        set_seq_lens_bulk(caches)
+
+    @torch.no_grad()
+    def score(self, prompts: list, top_n: int = 0, entropy: bool = False,
+              max_tokens: int = 8192) -> list:
+        """How probable each prompt's tokens are, given those before them: for every
+        prompt a TokenLogprobs (CPU) of its tokens but the first, which nothing comes
+        before.  max_tokens: prompts are run together up to so many tokens (one whole
+        prompt at least; each token has a row of logits)."""
+        prompts = [list(p) for p in prompts]
+        for p in prompts:
+            if not p:
+                raise ValueError("an empty prompt has nothing to score")
+            self._check_positions(len(p))
+        scored, at = [], 0
+        while at < len(prompts):
+            take, T = [], 0
+            while at < len(prompts) and (not take or T + len(prompts[at]) <= max_tokens):
+                take.append(prompts[at])
+                T += len(prompts[at])
+                at += 1
+            cu = np.zeros(len(take) + 1, dtype=np.int64)
+            cu[1:] = np.cumsum([len(p) for p in take])
+            ids = torch.tensor([t for p in take for t in p], dtype=torch.int64)
+            pos = torch.from_numpy(np.concatenate([np.arange(len(p)) for p in take]))
+            logits = self.model.prefill_logits(
+                ids.to(self.device), torch.from_numpy(cu).to(torch.int32).to(self.device),
+                max(len(p) for p in take), pos.to(self.device), None, None, None)
+            following = torch.cat((ids[1:], ids[:1]))
+            following[torch.from_numpy(cu[1:] - 1)] = -1  # nothing follows a prompt's last token
+            got = token_logprobs(logits, following.to(self.device), top_n=top_n, entropy=entropy)
+            got = [None if x is None else x.cpu() for x in got]
+            scored += [TokenLogprobs(*(None if x is None else x[a:b - 1] for x in got))
+                       for a, b in zip(cu[:-1].tolist(), cu[1:].tolist())]
+        return scored
+
     # ---- loop --------------------------------------------------------------
 
     @torch.no_grad()
@@ -313,6 +415,10 @@ class Engine:
         """Runs every request to completion; returns timing and counts.
         Timing: prefill_s / decode_s are host wall time per kind of step
         (a decode step's read-back overlaps the next launch)."""
+        most = min(MAX_TOP, self.model.config.vocab_size)
+        for r in requests:
+            if r.logprobs is not None and not 0 <= r.logprobs <= most:
+                raise ValueError(f"request {r.request_id}: logprobs {r.logprobs} outside 0..{most}")
         waiting = deque(requests)
         running: list = []
         self._pending = None

@@ -21,7 +21,9 @@ Two optional stages, used by the batching engine, ride in the same graph:
                  host's per-request writes of advance_seq_len.
 With positions_from_lengths=True RoPE uses seq_lens[row] (the reference's
 drivers always pass those positions), so nothing but the ids and rows of a
-changed batch needs a host->device copy.
+changed batch needs a host->device copy.  With shared=True (greedy runners)
+the step's attention follows the batch's shared prefixes
+(PagedKVcache.shared_prefix_groups), which come with a changed batch too.
 """
 from __future__ import annotations
 
@@ -44,7 +46,8 @@ def pow2_buckets(max_batch: int) -> tuple:
 class GraphRunner:
     def __init__(self, model, pool, caches, buckets=(1, 2, 4, 8), reserve_pages=64, *,
                  greedy: bool = False, advance: bool = False,
-                 positions_from_lengths: bool = False):
+                 positions_from_lengths: bool = False, shared: bool = False):
+        assert greedy or not shared, "shared prefixes ride in greedy runners"
         self.model = model
         self.pool = pool
         self.buckets = tuple(sorted(set(buckets)))
@@ -52,6 +55,7 @@ class GraphRunner:
         self.greedy = greedy
         self.advance = advance
         self.positions_from_lengths = positions_from_lengths
+        self.shared = shared
         assert len(caches) >= self.max_batch, \
             f"{len(caches)} placeholder handles, need >= max bucket {self.max_batch}"
 
@@ -70,6 +74,8 @@ class GraphRunner:
         pool.block_table_2d[self.dummy_row, 0] = self._dummy_phys
 
         model.reserve_decode_workspace(self.max_batch, pool)
+        if shared:
+            model.reserve_shared_workspace(self.max_batch, pool)
         self._pool_handle = torch.cuda.graph_pool_handle()
         self.graphs = {}
         self._capture_all(caches)
@@ -79,7 +85,8 @@ class GraphRunner:
         if self.greedy:
             ids = t["input"].view(-1)
             self.model.decode_greedy(ids, t["rows"], self.pool,
-                                     None if pos is None else pos.view(-1), out=ids)
+                                     None if pos is None else pos.view(-1), out=ids,
+                                     shared=(t["groups"], t["lens"]) if self.shared else None)
             return None
         return self.model.forward_decode(t["input"], pos, t["rows"], caches)
 
@@ -92,6 +99,9 @@ class GraphRunner:
                 "pos": torch.zeros((b, 1), dtype=torch.long, device=device),
                 "rows": torch.tensor([c.row_id for c in caches[:b]], dtype=torch.int32,
                                      device=device),
+                # as many groups as rows, empty ones last
+                "groups": torch.zeros(b + 1, dtype=torch.int32, device=device),
+                "lens": torch.zeros(b, dtype=torch.int32, device=device),
             }
             for _ in range(3):  # warm-up outside the graph: library heuristics, allocator
                 self._step(t, caches[:b])
@@ -123,6 +133,15 @@ class GraphRunner:
             t["rows"][k:].fill_(self.dummy_row)
         g.replay()
         return t["logits"]
+
+    def set_groups(self, k: int, cu_groups: list, shared_lens: list) -> None:
+        """The shared prefixes of the bucket of k rows, for the replays that follow."""
+        assert self.shared and len(cu_groups) == len(shared_lens) + 1 and cu_groups[-1] <= k
+        b = self.bucket_for(k)
+        t = self.graphs[b][1]
+        rest = b - len(shared_lens)
+        t["groups"].copy_(torch.tensor(cu_groups + cu_groups[-1:] * rest, dtype=torch.int32))
+        t["lens"].copy_(torch.tensor(shared_lens + [0] * rest, dtype=torch.int32))
 
     def replay_greedy(self, k: int, input_ids=None, rows=None):
         """Engine entry (greedy=True): replays the bucket of k rows.  With

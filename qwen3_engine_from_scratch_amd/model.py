@@ -42,6 +42,8 @@ from .kernels.model_ops import (DECODE_LINEAR_MAX_ROWS, add_rms_norm, argmax, de
 from . import _lib
 from .kernels.paged_attention import (paged_attention_chunk_hip, paged_attention_decode_hip,
                                       paged_attention_decode_partials_hip,
+                                      paged_attention_decode_shared_hip,
+                                      paged_decode_shared_workspace_bytes,
                                       paged_decode_workspace_bytes)
 from .kernels.pre_attention import qk_norm_rope_decode, qk_norm_rope_prefill, rope_tables
 
@@ -143,6 +145,7 @@ class Qwen3ForCausalLM(nn.Module):
             self.lm_head.weight = self.model.embed_tokens.weight
         self._workspace = None       # decode attention workspace of the current mode
         self._ws_mode = None
+        self._shared_ws = None       # of decode attention over shared prefixes
         self._superseded = []
         self._head_ws = None
         self._chain_sync = None
@@ -202,6 +205,31 @@ class Qwen3ForCausalLM(nn.Module):
             self._head_ws = torch.empty(int(_lib.load().qwen3_lm_head_argmax_workspace_bytes()),
                                         dtype=torch.uint8, device=pool.k_buffer.device)
 
+    def reserve_shared_workspace(self, batch: int, pool) -> None:
+        """The same for decode steps with shared prefixes, any groups."""
+        if self.decode_batch_invariant:
+            raise ValueError("shared prefixes in the batch-invariant mode: how a sequence's "
+                             "attention is summed depends on its group")
+        c = self.config
+        need = paged_decode_shared_workspace_bytes(batch, c.num_attention_heads,
+                                                   c.num_key_value_heads, c.head_dim)
+        if self._shared_ws is None or self._shared_ws.numel() < need:
+            if self._shared_ws is not None:
+                self._superseded.append(self._shared_ws)
+            self._shared_ws = torch.empty(max(need, 1), dtype=torch.uint8,
+                                          device=pool.k_buffer.device)
+
+    def _attend_decode(self, q, i: int, row_ids, pool, shared) -> torch.Tensor:
+        """Decode attention of layer i in the mode that the workspaces were reserved for;
+        shared: (cu_groups, shared_lens) on the device, or None."""
+        kv = (q, pool.k_buffer[:, i], pool.v_buffer[:, i], pool.block_table_2d, pool.seq_lens,
+              row_ids)
+        if shared is not None:
+            return paged_attention_decode_shared_hip(*kv, *shared, pool.block_size,
+                                                     workspace=self._shared_ws)
+        return paged_attention_decode_hip(*kv, pool.block_size, workspace=self._workspace,
+                                          batch_invariant=self._ws_mode)
+
     def fused_decode_ok(self, batch: int) -> bool:
         """Whether a decode step of `batch` rows runs on the fused decode
         linears (at most 64 rows; widths the kernels tile)."""
@@ -210,15 +238,15 @@ class Qwen3ForCausalLM(nn.Module):
         return (batch <= DECODE_LINEAR_MAX_ROWS and all(w % 128 == 0 for w in widths)
                 and c.head_dim == 128 and c.hidden_size <= 4096)
 
-    def _decode_fused(self, ids, row_ids, pool, positions) -> torch.Tensor:
+    def _decode_fused(self, ids, row_ids, pool, positions, shared) -> torch.Tensor:
         """Decode step on the fused kernels; returns the logits."""
-        h, _ = self._decode_layers(ids, row_ids, pool, positions)
+        h, _ = self._decode_layers(ids, row_ids, pool, positions, shared)
         # lm_head streams 311 MB of weights for few rows: the library GEMM
         # after a separate final norm
         final = add_rms_norm(None, h, self.model.norm.weight, self.config.rms_norm_eps)
         return F.linear(final, self.lm_head.weight)
 
-    def _decode_layers(self, ids, row_ids, pool, positions):
+    def _decode_layers(self, ids, row_ids, pool, positions, shared=None):
         """The decoder layers of a decode step on the fused kernels: the
         residual stream ping-pongs between two buffers, each with its
         per-16-column sums of squares, so every RMSNorm is the prologue of
@@ -226,8 +254,9 @@ class Qwen3ForCausalLM(nn.Module):
         linear before it; the qkv projection also applies QK-norm and RoPE
         and writes K/V into the pool, leaving one attention launch (plus its
         merge) per layer.  At most 16 rows: everything between two attention
-        launches is one (decode_chain), with the same results.  Returns the last
-        residual stream and its sums."""
+        launches is one (decode_chain), with the same results; not with shared
+        prefixes, whose attention joins its parts itself.  Returns the last residual
+        stream and its sums."""
         cfg = self.config
         eps = cfg.rms_norm_eps
         layers = self.model.layers
@@ -238,7 +267,8 @@ class Qwen3ForCausalLM(nn.Module):
         h_a, ss_a = embed_ss(ids, self.model.embed_tokens.weight)
         h_b = torch.empty_like(h_a)
         ss_b = torch.empty_like(ss_a)
-        chain = decode_chain_ok(B, cfg.hidden_size, cfg.intermediate_size, Hq, Hkv)
+        chain = shared is None and decode_chain_ok(B, cfg.hidden_size, cfg.intermediate_size, Hq,
+                                                   Hkv)
         if chain:
             # at most 16 rows: the dense work between two attention launches is
             # one launch (with separate ones, launch and load latency is most
@@ -265,10 +295,7 @@ class Qwen3ForCausalLM(nn.Module):
             q = decode_qkv_rope(h_a, ss_a, layer.input_layernorm.weight, eps, at.qkv_proj.weight,
                                 Hq, Hkv, at.q_norm.weight, at.k_norm.weight, eps, cos, sin, pool,
                                 i, row_ids, positions, sync=self._chain_sync)
-            o = paged_attention_decode_hip(q, pool.k_buffer[:, i], pool.v_buffer[:, i],
-                                           pool.block_table_2d, pool.seq_lens, row_ids,
-                                           pool.block_size, workspace=ws,
-                                           batch_invariant=self._ws_mode)
+            o = self._attend_decode(q, i, row_ids, pool, shared)
             decode_linear(o.view(B, Hq * D), at.o_proj.weight, epilogue="residual",
                           residual=h_a, residual_out=h_b, ss_out=ss_b)
             act = decode_linear(h_b, layer.mlp.gate_up_proj.weight, epilogue="silu", ss_in=ss_b,
@@ -280,9 +307,9 @@ class Qwen3ForCausalLM(nn.Module):
     @torch.no_grad()
     def decode_greedy(self, ids: torch.Tensor, row_ids: torch.Tensor, pool,
                       positions: torch.Tensor | None = None,
-                      out: torch.Tensor | None = None) -> torch.Tensor:
+                      out: torch.Tensor | None = None, shared=None) -> torch.Tensor:
         """Greedy tokens (B,) int64 of one decode step, argmax of
-        decode_logits(...).  On the fused path the final norm, lm_head and
+        decode_logits(...) (shared: as there).  On the fused path the final norm, lm_head and
         argmax run as one pass over the tied embedding that never stores the
         logits (qwen3_lm_head_argmax_bf16); out may alias ids (the ids are
         read before the tokens are written)."""
@@ -292,20 +319,22 @@ class Qwen3ForCausalLM(nn.Module):
             out = torch.empty(B, dtype=torch.int64, device=ids.device)
         if self.fused_decode_ok(B) and lm_head_argmax_ok(cfg.hidden_size):
             self.reserve_decode_workspace(B, pool)
+            if shared is not None:
+                self.reserve_shared_workspace(B, pool)
             rows = row_ids if row_ids is not None else torch.arange(
                 B, dtype=torch.int32, device=ids.device)
             h, ss = self._decode_layers(ids.reshape(-1).contiguous(), rows.contiguous(), pool,
-                                        positions)
+                                        positions, shared)
             lm_head_argmax(h, ss, self.model.norm.weight, cfg.rms_norm_eps, self.lm_head.weight,
                            out=out.view(-1), workspace=self._head_ws)
             return out
-        logits = self.decode_logits(ids, row_ids, pool, positions)
+        logits = self.decode_logits(ids, row_ids, pool, positions, shared=shared)
         return argmax(logits, out=out.view(-1))
 
     @torch.no_grad()
     def decode_logits(self, ids: torch.Tensor, row_ids: torch.Tensor, pool,
                       positions: torch.Tensor | None = None,
-                      fused: bool | None = None) -> torch.Tensor:
+                      fused: bool | None = None, shared=None) -> torch.Tensor:
         """One decode step for B requests: ids (B,) int64 (this step's input
         tokens), row_ids (B,) int32 resident-table rows.  Writes each token's
         K/V at position seq_lens[row] (pages must be reserved), attends over
@@ -313,12 +342,16 @@ class Qwen3ForCausalLM(nn.Module):
         (B,) int64: RoPE positions (None: seq_lens[row]).  Does not advance
         seq_lens (the caller's job, as in the reference).  fused (None: when
         possible) selects the fused decode linears over the library GEMMs
-        with separate norm / activation kernels."""
+        with separate norm / activation kernels.  shared: (cu_groups, shared_lens),
+        device int32, where groups of the batch share a prefix
+        (PagedKVcache.shared_prefix_groups; the batch in its order): attention reads
+        each prefix once."""
         B = ids.numel()
         cfg = self.config
         cos, sin = self.model.rotary_emb.tables(ids.device)
         self.reserve_decode_workspace(B, pool)
-        ws = self._workspace
+        if shared is not None:
+            self.reserve_shared_workspace(B, pool)
         Hq, D = cfg.num_attention_heads, cfg.head_dim
 
         def attend(i, at, qkv):
@@ -326,11 +359,7 @@ class Qwen3ForCausalLM(nn.Module):
             qr = qk_norm_rope_decode(q, k, v, at.q_norm.weight, at.k_norm.weight,
                                      cfg.rms_norm_eps, cos, sin, pool, i, row_ids,
                                      positions=positions)
-            o = paged_attention_decode_hip(qr, pool.k_buffer[:, i], pool.v_buffer[:, i],
-                                           pool.block_table_2d, pool.seq_lens, row_ids,
-                                           pool.block_size, workspace=ws,
-                                           batch_invariant=self._ws_mode)
-            return o.view(B, Hq * D)
+            return self._attend_decode(qr, i, row_ids, pool, shared).view(B, Hq * D)
 
         if fused is None:
             fused = self.fused_decode_ok(B)
@@ -338,7 +367,7 @@ class Qwen3ForCausalLM(nn.Module):
             rows = row_ids if row_ids is not None else torch.arange(
                 B, dtype=torch.int32, device=ids.device)
             return self._decode_fused(ids.reshape(-1).contiguous(), rows.contiguous(), pool,
-                                      positions)
+                                      positions, shared)
         return self._run(ids.reshape(-1), attend, None)
 
     @torch.no_grad()
