@@ -133,8 +133,8 @@ __device__ __forceinline__ uint32_t tile_dma(const Args& a, const LaneOffsets& o
 // One 64-key tile (staged in kt / vt) folded into this wave's online softmax
 // state; c: the softmax scale times log2(e).  mask(s) sets the scores of masked
 // keys to -inf: s[kb][r] of a lane is key 32 kb + 8 (r / 4) + r % 4 + 4 (lane / 32)
-// of the tile.  kTwo: P meets V as two bf16 terms, hi = bf16(p) and lo = bf16(p - hi).
-template <bool kTwo = false, typename Off, typename Mask>
+// of the tile.
+template <typename Off, typename Mask>
 __device__ __forceinline__ void tile_fold(const Off& off, float c, const Mask& mask,
                                           const uint16_t* kt, const uint16_t* vt, const q3::bf16x8 (&qv)[8],
                                           float& m_run, float& l_run, q3::f32x16 (&acc)[4]) {
@@ -188,7 +188,7 @@ __device__ __forceinline__ void tile_fold(const Off& off, float c, const Mask& m
   // key chunk u / 4, dims 32 (u % 4) .. +31.  Chunk 0 is computed first;
   // the exponentials of chunk g + 1 are issued between the four MFMAs of
   // chunk g, two per step, so the VALU works while the matrix core runs.
-  q3::u32x4 pk[4], pl[4];
+  q3::u32x4 pk[4];
   float psum[4];  // four independent sum chains, started by chunk 0
   auto exp_pair = [&](int g, int h) {  // scores 2h, 2h + 1 of chunk g
     const int kb = g >> 1, kc = g & 1;
@@ -202,8 +202,6 @@ __device__ __forceinline__ void tile_fold(const Off& off, float c, const Mask& m
       psum[(2 * h + 1) & 3] += e1;
     }
     pk[g][h] = q3::pack_bf16x2(e0, e1);
-    if constexpr (kTwo)
-      pl[g][h] = q3::pack_bf16x2(e0 - q3::bf16_lo(pk[g][h]), e1 - q3::bf16_hi(pk[g][h]));
   };
 #pragma unroll
   for (int h = 0; h < 4; ++h) exp_pair(0, h);
@@ -211,8 +209,6 @@ __device__ __forceinline__ void tile_fold(const Off& off, float c, const Mask& m
 #pragma unroll
   for (int u = 0; u < 16; ++u) {
     acc[u & 3] = q3::mfma32x32x16(vf[u % kAhead], q3::as_bf16x8(pk[u >> 2]), acc[u & 3]);
-    if constexpr (kTwo)
-      acc[u & 3] = q3::mfma32x32x16(vf[u % kAhead], q3::as_bf16x8(pl[u >> 2]), acc[u & 3]);
     if (u + kAhead < 16) vf[u % kAhead] = lds_vt(vt, pv_operand(off, u + kAhead));
     if (u < 12) exp_pair((u >> 2) + 1, u & 3);
     __builtin_amdgcn_sched_barrier(0);

@@ -20,7 +20,7 @@
 // that have another half, are left in the workspace (normalised, with the log2 of their
 // sum), and the second launch joins each row's.  P is floored to whole tiles of 16 keys
 // and bounded by what the group's first sequence holds; the rest counts as each
-// sequence's own.  P meets V as two bf16 terms, as in the decode.
+// sequence's own, and so does all of a sequence that ends inside P.  P meets V as two bf16 terms, as in the decode.
 #include <algorithm>
 
 #include "paged_decode_merge.hpp"
@@ -100,7 +100,7 @@ struct Tables {
   int32_t gs[kMaxSeqs + 1];    // of groups, streamed
   int32_t gt[kMaxSeqs + 1];    // of groups, staged
   int32_t gp[kMaxSeqs];        // tiles of 16 keys of the prefix
-  uint16_t grp[kMaxSeqs];      // a sequence's group
+  uint16_t grp[kMaxSeqs];      // the group whose prefix a sequence shares
   int16_t g0[kMaxSeqs + 2];    // first sequence (-1, B + 1: outside the batch)
   int32_t wsum[3][kRounds][kShWaves];
 };
@@ -178,8 +178,11 @@ __device__ __forceinline__ void tabulate_shared(const SharedArgs& a, Tables& t, 
     if (b < B) {
       const int g = NG > 0 ? last_at_most(t.g0, NG, b) : -1;
       const bool in = g >= 0 && b < t.g0[g] + members(t, g, B);
-      if (in) skip = t.gp[g];
-      t.grp[b] = static_cast<uint16_t>(in ? g : kNoGroup);
+      // (one that ends inside the prefix attends alone: masked, infinities and NaN among the
+      // values behind its end would reach it by their products with zero)
+      const bool shares = in && t.len[b] >= t.gp[g] * kTile;
+      if (shares) skip = t.gp[g];
+      t.grp[b] = static_cast<uint16_t>(shares ? g : kNoGroup);
       const int tiles = (t.len[b] + kTile - 1) / kTile;
       own[i] = tiles > skip ? tiles - skip + kSegTiles : 0;
     }
@@ -395,7 +398,7 @@ __device__ __forceinline__ void stream_range(const SharedArgs& a, const Tables& 
       first = 0;
     }
     chead = kvh * d.G + (mine ? head : 0);
-    col.last = min(c.L, t.len[cb]) - 1;
+    col.last = c.L - 1;
     reset(col.st);
     const uint16_t* qp = d.q + cb * d.q_sb + static_cast<int64_t>(chead) * d.q_sh + hi * 8;
 #pragma unroll
@@ -690,11 +693,6 @@ __device__ __forceinline__ void staged_range(const SharedArgs& a, const Tables& 
       for (int c = 0; c < 8; ++c)
         qv[c] = q3::as_bf16x8(mine ? q3::ld16(qp + 16 * c) : q3::u32x4{0u, 0u, 0u, 0u});
     }
-    const int last = (mine ? min(t.len[b], keys) : keys) - 1;
-    int lo_last = last;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) lo_last = min(lo_last, __shfl_xor(lo_last, o, 64));
-    lo_last = uniform(lo_last);
     const int64_t row = uniform(t.row[s0]);
     const uint16_t* kv = loader.base + kvh * (wave < 4 ? a.k_sh : a.v_sh);
     float m_run = q3::kNegInf, l_run = 0.f;
@@ -723,17 +721,15 @@ __device__ __forceinline__ void staged_range(const SharedArgs& a, const Tables& 
         if (ja + u < je) ok[u] = stage(ja + u, next_tile(pages, u, loader));
       Next ahead = next_tile(pages, min(kStages - 1, je - ja - 1), loader);
 
-      // a tile's scores, masked: x[i] is key n0 + 4 (lane / 32) + kr of group 2 half + i / 8
+      // a tile's scores, masked: x[i] is a key of group 2 half + i / 8, and the prefix ends
+      // with a group
       auto mask = [&](q3::f32x16& x, int j, uint32_t okj) {
-        const int n0 = j * kBN + 32 * half;
-        if (n0 + 31 > lo_last || okj != 15u) {
-          const int lim = last - n0 - 4 * (lane >> 5);
+        const int left = keys - j * kBN;
+        if (left < kBN) okj &= (1u << (left / kGroup)) - 1u;
+        if (okj != 15u) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int kr = 8 * (i / 4) + (i % 4);
-            const int l = (okj >> (2 * half + i / 8)) & 1u ? lim : -1;
-            x[i] = kr <= l ? x[i] : q3::kNegInf;
-          }
+          for (int i = 0; i < 16; ++i)
+            x[i] = (okj >> (2 * half + i / 8)) & 1u ? x[i] : q3::kNegInf;
         }
       };
       const int rest = half < 2 ? half * 32 * kD : 0;  // where a wave's keys begin in a tile

@@ -339,9 +339,7 @@ class Engine:
             rows = torch.tensor([c.row_id for c in caches], dtype=torch.int32).to(dev)
             shared = None
             if replay:
-                if groups is not None:
-                    self.runner.set_groups(k, *groups)
-                out = self.runner.replay_greedy(k, ids, rows)
+                out = self.runner.replay_greedy(k, ids, rows, groups)
                 self._last_batch, self._last_reqs = key, list(reqs)
             elif groups is not None:
                 shared = tuple(torch.tensor(g, dtype=torch.int32).to(dev) for g in groups)

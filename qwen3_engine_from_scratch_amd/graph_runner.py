@@ -134,21 +134,13 @@ class GraphRunner:
         g.replay()
         return t["logits"]
 
-    def set_groups(self, k: int, cu_groups: list, shared_lens: list) -> None:
-        """The shared prefixes of the bucket of k rows, for the replays that follow."""
-        assert self.shared and len(cu_groups) == len(shared_lens) + 1 and cu_groups[-1] <= k
-        b = self.bucket_for(k)
-        t = self.graphs[b][1]
-        rest = b - len(shared_lens)
-        t["groups"].copy_(torch.tensor(cu_groups + cu_groups[-1:] * rest, dtype=torch.int32))
-        t["lens"].copy_(torch.tensor(shared_lens + [0] * rest, dtype=torch.int32))
-
-    def replay_greedy(self, k: int, input_ids=None, rows=None):
+    def replay_greedy(self, k: int, input_ids=None, rows=None, groups=None):
         """Engine entry (greedy=True): replays the bucket of k rows.  With
         input_ids / rows None the captured tensors already hold them (the
         previous replay of this bucket wrote its tokens there and the batch
-        is unchanged).  Returns the bucket's (b, 1) int64 token tensor, the
-        first k rows valid."""
+        is unchanged).  groups (a runner with shared=True): (cu_groups,
+        shared_lens) host lists of the rows given, None: they share nothing.
+        Returns the bucket's (b, 1) int64 token tensor, the first k rows valid."""
         assert self.greedy
         b = self.bucket_for(k)
         g, t = self.graphs[b]
@@ -158,6 +150,12 @@ class GraphRunner:
             t["rows"][:k].copy_(rows)
             if k < b:
                 t["rows"][k:].fill_(self.dummy_row)
+            if self.shared:
+                cu, lens = groups if groups is not None else ([0], [])
+                assert len(cu) == len(lens) + 1 and cu[-1] <= k
+                cu, lens = cu + cu[-1:] * (b - len(lens)), lens + [0] * (b - len(lens))
+                t["groups"].copy_(torch.tensor(cu, dtype=torch.int32))
+                t["lens"].copy_(torch.tensor(lens, dtype=torch.int32))
         g.replay()
         return t["input"]
 

@@ -336,8 +336,8 @@ def paged_attention_decode_shared_hip(q, k_buffer, v_buffer, block_table_2d, seq
                     cu_groups[g] .. cu_groups[g + 1] - 1
     shared_lens:    int32 (num_groups,): the tokens that all of the group's sequences hold
                     in the same pages (counted in whole multiples of 16, and as far as the
-                    group's first sequence goes).  PagedKVcache.shared_prefix_groups
-                    makes both from handles
+                    group's first sequence goes; one that ends before that attends alone).
+                    PagedKVcache.shared_prefix_groups makes both from handles
     Returns out (B, num_heads, head_dim) bf16.  Entries of no group attend alone.  Groups
     and lengths are read on the device: a captured call follows them.  workspace:
     paged_decode_shared_workspace_bytes(...) bytes, a fresh one per call by default.
@@ -370,7 +370,8 @@ def paged_attention_decode_shared_hip(q, k_buffer, v_buffer, block_table_2d, seq
     strides = _lib.outer_strides
     with _lib.on_device(dev):
         need = _shared_workspace(dev.index, B, num_heads, num_kv_heads, head_dim)
-        if workspace is None or workspace.numel() * workspace.element_size() < need:
+        if (workspace is None or workspace.numel() * workspace.element_size() < need
+                or not workspace.is_contiguous()):
             workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
         rc = _lib.load().qwen3_paged_decode_shared_bf16(
             q.data_ptr(), strides(q), k_buffer.data_ptr(), strides(k_buffer),

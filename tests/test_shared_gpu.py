@@ -164,6 +164,26 @@ def test_lengths_inside_the_prefix(gpu, n):
     assert not run(t, gpu).any()
 
 
+@pytest.mark.parametrize("n", [4, 30])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_values_behind_a_sequences_end(gpu, n, bad):
+    """What the shared pages hold behind the end of a sequence that is shorter than its
+    group's prefix does not reach it: the same bits whatever stands there."""
+    announce(f"shared: {n} sequences, {bad} behind the end of some")
+    t = make_shared([(320, [20] * n)], 16, 4, 16, gpu, seed=n)
+    rows = t["row_ids"].long()
+    short = [1, 2, n - 1]
+    for i, length in zip(short, (288, 7, 290)):
+        t["seq_lens"][rows[i]] = length - 1
+    clean = run(t, gpu)
+    check(clean, t, "clean")
+    page = int(t["table"][rows[0], 18])  # tokens 288 .. 303
+    for x in (t["k"], t["v"]):
+        x[page, :, 2:] = bad
+    out = run(t, gpu)
+    assert torch.equal(out[short], clean[short])
+
+
 def test_claims_of_odd_lengths(gpu):
     """shared_lens inside a page or a tile, beyond the first sequence, none, negative."""
     announce("shared: claims of odd lengths")
