@@ -577,6 +577,13 @@ __device__ __forceinline__ float max3_half(const q3::f32x16& a) {
   return m;
 }
 
+// (The builtin alone is no memory operation to the compiler.)
+__device__ __forceinline__ void wait_all_waves() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // A wave's probabilities of 32 keys, in two bf16 terms, not yet met with their values.
 struct Probs {
   q3::u32x4 hi[2], lo[2];
@@ -737,7 +744,7 @@ __device__ __forceinline__ void staged_range(const SharedArgs& a, const Tables& 
       if (ja + 2 < je) __builtin_amdgcn_s_waitcnt(0x0f70 | 2 * kShare);
       else if (ja + 1 < je) __builtin_amdgcn_s_waitcnt(0x0f70 | kShare);
       else wait_loads();
-      __builtin_amdgcn_s_barrier();
+      wait_all_waves();
       Probs probs;
       if (active) {
         q3::f32x16 x = score(off, tiles_at + rest, qv);
@@ -758,7 +765,7 @@ __device__ __forceinline__ void staged_range(const SharedArgs& a, const Tables& 
         // then everybody's has, and nobody reads tile j - 1 any more
         if (j + 2 < je) __builtin_amdgcn_s_waitcnt(0x0f70 | kShare);
         else wait_loads();
-        __builtin_amdgcn_s_barrier();
+        wait_all_waves();
         const uint32_t ok1 = ok[1];
         ok[1] = ok[2];
         if (j + kStages - 1 < je) {

@@ -132,6 +132,23 @@ def test_masked_rows_and_ties(gpu, dtype, kind):
         check(x, t, one, top_n=20, what=f"{kind} {dtype} {vocab}")
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("kind", ["few left (-inf)", "few left (lowest)", "one left", "equal",
+                                  "two values", "rising", "one thread's"])
+@pytest.mark.parametrize("copies,top", [(1, 9), (1, 64), (1, 3), (10, 64), (13, 20)])
+def test_parts_lists_joined(gpu, dtype, kind, copies, top):
+    """Rows of 2 to 16 parts, whose lists are joined by rank or head by head."""
+    x = special_rows(30011, dtype, kind)
+    t = torch.tensor([5, 2, 30010, 0, 15005, 4292])
+    announce(f"logprobs {kind} {dtype}, {6 * copies} rows, top {top}")
+    got = call(x.repeat(copies, 1).to(gpu), t.repeat(copies).to(gpu), top_n=top, entropy=True)
+    torch.cuda.synchronize()
+    for i in range(1, copies):
+        assert torch.equal(got.top_ids[:6], got.top_ids[6 * i:6 * i + 6])
+    check(x, t, type(got)(*(None if v is None else v[:6] for v in got)), top_n=top,
+          what=f"{kind} {dtype} {copies} x {top}")
+
+
 def test_rows_without_a_distribution(gpu):
     for vocab in (50, 40013):
         announce(f"logprobs without a distribution {vocab}")
@@ -288,7 +305,7 @@ def test_gradient_uses(gpu):
     r = call(base[:, 3:1010], t, entropy=True)
     r.logprobs.mean().backward()
     want, off = Rows(base.detach()[:, 3:1010].cpu()).gradient(t.cpu(), torch.full((6,), 1 / 6))
-    assert ((base.grad[:, 3:1010].cpu().double() - want).abs() <= off + want.abs() * 2.0 ** -24 + 1e-9 * 0 + 2.0 ** -126).all()
+    assert ((base.grad[:, 3:1010].cpu().double() - want).abs() <= off + want.abs() * 2.0 ** -24 + 2.0 ** -126).all()
     assert not base.grad[:, :3].any() and not base.grad[:, 1010:].any()
     with torch.no_grad():
         assert not call(base, t).logprobs.requires_grad
