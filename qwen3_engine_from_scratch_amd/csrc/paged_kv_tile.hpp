@@ -1,6 +1,6 @@
-// What the kernels that stage K/V tiles of a paged cache in LDS share (paged_chunk.hip,
-// paged_shared.hip): pages to 64-key tiles by buffer loads that write LDS, and a tile's
-// fold into 32 query rows of a wave.  Args: a kernel's arguments, with k, k_blk, k_sh,
+// K/V tiles of a paged cache in LDS (paged_chunk.hip; paged_shared.hip takes the groups, the
+// read offsets and the slack): pages to 64-key tiles by buffer loads that write LDS, and a
+// tile's fold into 32 query rows of a wave.  Args: a kernel's arguments, with k, k_blk, k_sh,
 // k_slot (elements), the same for v, num_blocks, bt, bt_stride, max_pages, and gpb and
 // per_group (groups of kGroup keys of a block, and its reciprocal).
 #pragma once

@@ -9,18 +9,34 @@
 // sequences packed together, and its K and V are read once instead of once a sequence.
 //
 // One launch attends, a second joins.  In the first, a workgroup does one of two things:
-//  * prefixes of more than 16 rows: K/V tiles of 64 keys staged in LDS (paged_kv_tile.hpp),
-//    four stages, so that the loads of three tiles are on their way while one is computed;
-//    eight waves, 128 rows an item.  The items' tiles lie end to end and are cut
-//    into equal ranges, a workgroup each;
+//  * prefixes of more than 16 rows: K/V tiles of 64 keys staged in LDS, four stages, so
+//    that the loads of three tiles are on their way while one is computed; eight waves, 128
+//    rows an item.  The items' tiles lie end to end and are cut into equal ranges, a
+//    workgroup each;
 //  * what each sequence has of its own, and prefixes of up to 16 rows: the streaming
 //    decode's loop (paged_decode.hip), K and V straight into MFMA operands, the 16-key
-//    tiles of all items end to end, cut into equal ranges, a wave each.
+//    tiles of all items end to end, cut into equal ranges, a wave each.  (Staged instead,
+//    prefixes of 4 sequences and 4 query heads a KV head: one group behind 30,000 tokens
+//    39.9 us for 41.3, behind 100,000 99 for 85, sixteen behind 2,048 60.0 for 54.4.)
 // The workgroups are divided by the tiles' weights.  Parts of cut items, and whole ones
 // that have another half, are left in the workspace (normalised, with the log2 of their
 // sum), and the second launch joins each row's.  P is floored to whole tiles of 16 keys
 // and bounded by what the group's first sequence holds; the rest counts as each
 // sequence's own, and so does all of a sequence that ends inside P.  P meets V as two bf16 terms, as in the decode.
+//
+// What bounds it: HBM, where sequences have much of their own (256 of 50-2,500 tokens behind
+// 2,000, 16/8 heads: 225 us, 5.7 TB/s); behind long prefixes the staged tiles, 1.87 us each
+// on each CU, where their loads alone take 1.4 (5.9 TB/s) and their products and softmax
+// alone 1.45, MFMA busy a third of the time, VALU as long, LDS without conflicts (32
+// sequences behind 100,000, 32/8 heads: 115 us, 3.8 TB/s; 64 behind 8,192 of 1-1,000 of
+// their own 47 us, 3.2 TB/s); in small calls the latency of the steps, 2.5 us until the batch is
+// tabulated, 10 of the first tiles, 5 of the join (4 behind 896, 16/8 heads: 14 us).
+// Attended one by one (paged_decode.hip) the same batches take 489, 1,817, 296 and 15 us.
+//
+// Measured against it (32 behind 100,000; 64 behind 8,192): the values' products of both
+// halves of a tile's keys after the scores 117.7 us for 115.2; scores of one half taken a tile
+// ahead in stages of their own 113 for 113, 48 for 48; items of 256 rows 2.65 us a tile; parts
+// stored past the caches 54.8 us for 52.6; waves' priorities no difference.
 #include <algorithm>
 
 #include "paged_decode_merge.hpp"
@@ -37,8 +53,11 @@ constexpr int kRowsT = 128;           // rows of an item whose tiles are staged
 constexpr int kRowsS = 16;            // rows of one that is streamed
 constexpr int kMaxWgs = 512;
 constexpr int kStages = 4;
-// Weight, in streamed tiles of 16 keys, of a staged tile of 64; what an item's start and
-// end weigh, in tiles of its kind; tiles that a range takes at least.
+// Weight, in streamed tiles of 16 keys, of a staged tile of 64 (64 behind 8,192: 47.4 us; of
+// 4 51.3, of 6 49.8); what an item's start and end weigh, in tiles of its kind (staged, none
+// 51.6, of 8 48.3; streamed, none 52.7, of 3 48.7); tiles that a range takes at least
+// (staged, 1 to 4 the same; streamed, a chunk: 4 behind 4,096 23.8 us for 21.8, 16 behind
+// 4,096 23.2 for 23.8; four chunks 23.5 and 26.2).
 constexpr int kStagedUnits = 5;
 constexpr int kItemTiles = 4;
 constexpr int kSegTiles = 1;
@@ -774,6 +793,7 @@ __device__ __forceinline__ void staged_range(const SharedArgs& a, const Tables& 
         }
         if (active) {
           const uint16_t* vt = here + kTileElems + rest;
+          // (the halves in different order, or a SIMD's two waves are at the same step)
           if (half == 1) add_values(off, vt, probs, [](int) {}, acc);
           q3::f32x16 x = score(off, next + rest, qv);
           mask(x, j + 1, ok1);
@@ -894,6 +914,11 @@ void paged_shared_kernel(SharedArgs a) {
 
 // ---- the join ---------------------------------------------------------------------------
 
+// Rows (query heads of sequences) up to which a row's parts are dealt to eight waves, a CU
+// reading what a few do too slowly: 4 sequences behind 30,000 tokens 41.7 us for 62.3, 40
+// behind 30,000, 640 rows, 51 for 51; of 2,048 rows 57 for 48.
+constexpr int kSplitRows = 1024;
+
 // Parts of a row: `n` slots from `first` on, `step` apart; the first one may lie elsewhere.
 struct Parts {
   const float* po;
@@ -902,16 +927,17 @@ struct Parts {
   int step, n;
 };
 
-// One workgroup per (KV head, sequence), one wave per query head of the group: lane i
-// fetches the sums of part i of up to 64 parts at once, then every lane owns two
-// dimensions and sums the weighted parts, kBatch loads in flight.
-__global__ __launch_bounds__(kMaxG * 64) void paged_shared_join_kernel(SharedArgs a) {
+// One workgroup of kSplit waves per (query head, sequence): lane i of a wave fetches the
+// sum of the i-th of its parts, of up to 64 at once, then every lane owns two dimensions and
+// sums the weighted parts, kBatch loads in flight; the waves are joined in LDS.
+template <int kSplit>
+__global__ __launch_bounds__(kSplit * 64) void paged_shared_join_kernel(SharedArgs a) {
   constexpr int kBatch = 8;
   const DecodeArgs& d = a.d;
   const int lane = threadIdx.x & 63;
-  const int g = uniform(threadIdx.x >> 6);
-  const int hkv = blockIdx.x, b = blockIdx.y;
-  const int hq = hkv * d.G + g;
+  const int split = uniform(threadIdx.x >> 6);
+  const int hq = blockIdx.x, b = blockIdx.y;
+  const int hkv = hq / d.G, g = hq - hkv * d.G;
   const SeqMeta m = a.seqs[b];
   const CallMeta call = *a.call;
   const int64_t direct = static_cast<int64_t>(b) * d.Hq + hq;
@@ -961,43 +987,67 @@ __global__ __launch_bounds__(kMaxG * 64) void paged_shared_join_kernel(SharedArg
       x.next = 2 * vf * a.rows_t + row;
     }
   }
+  const int all = part[0].n + part[1].n;
+  auto row_at = [&](int i) {  // part i, in its own list
+    const Parts& x = part[i < part[0].n ? 0 : 1];
+    const int k = i < part[0].n ? i : i - part[0].n;
+    return k == 0 ? x.first : x.next + static_cast<int64_t>(k) * x.step;
+  };
   float M = q3::kNegInf, sw = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int i0 = split; i0 < all; i0 += 64 * kSplit) {
+    const int i = i0 + kSplit * lane;
+    const float lse = i < all ? (i < part[0].n ? part[0].lse : part[1].lse)[row_at(i)] : q3::kNegInf;
+    float top = lse;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const Parts& x = part[h];
-    for (int i0 = 0; i0 < x.n; i0 += 64) {
-      const int i = i0 + lane;
-      const float lse = i < x.n ? x.lse[i == 0 ? x.first : x.next + static_cast<int64_t>(i) * x.step]
-                                : q3::kNegInf;
-      float top = lse;
+    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, q3::shfl_xor(top, o));
+    const float m_new = fmaxf(M, top), use = m_new == q3::kNegInf ? 0.f : m_new;
+    const float f = q3::fast_exp2(M - use);
+    M = m_new;
+    const float wt = q3::fast_exp2(lse - use);
+    float wsum = wt;
 #pragma unroll
-      for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, q3::shfl_xor(top, o));
-      const float m_new = fmaxf(M, top), use = m_new == q3::kNegInf ? 0.f : m_new;
-      const float f = q3::fast_exp2(M - use);
-      M = m_new;
-      const float wt = q3::fast_exp2(lse - use);
-      float wsum = wt;
+    for (int o = 1; o < 64; o <<= 1) wsum += q3::shfl_xor(wsum, o);
+    sw = sw * f + wsum;
+    o0 *= f;
+    o1 *= f;
+    const int cnt = min(64, (all - i0 + kSplit - 1) / kSplit);
+    for (int j0 = 0; j0 < cnt; j0 += kBatch) {
+      float2 ov[kBatch];
 #pragma unroll
-      for (int o = 1; o < 64; o <<= 1) wsum += q3::shfl_xor(wsum, o);
-      sw = sw * f + wsum;
-      o0 *= f;
-      o1 *= f;
-      const int cnt = min(64, x.n - i0);
-      for (int j0 = 0; j0 < cnt; j0 += kBatch) {
-        float2 ov[kBatch];
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const int i = min(i0 + j0 + j, x.n - 1);
-          const int64_t row = i == 0 ? x.first : x.next + static_cast<int64_t>(i) * x.step;
-          ov[j] = *reinterpret_cast<const float2*>(x.po + row * kD + 2 * lane);
-        }
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const float u = j0 + j < cnt ? __shfl(wt, j0 + j, 64) : 0.f;
-          o0 += u * ov[j].x;
-          o1 += u * ov[j].y;
-        }
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = i0 + kSplit * min(j0 + j, cnt - 1);
+        const float* po = i < part[0].n ? part[0].po : part[1].po;
+        ov[j] = *reinterpret_cast<const float2*>(po + row_at(i) * kD + 2 * lane);
       }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const float u = j0 + j < cnt ? __shfl(wt, j0 + j, 64) : 0.f;
+        o0 += u * ov[j].x;
+        o1 += u * ov[j].y;
+      }
+    }
+  }
+  if constexpr (kSplit > 1) {
+    __shared__ float s_m[kSplit], s_w[kSplit];
+    __shared__ float2 s_o[kSplit][64];
+    s_o[split][lane] = float2{o0, o1};
+    if (lane == 0) {
+      s_m[split] = M;
+      s_w[split] = sw;
+    }
+    __syncthreads();
+    if (split != 0) return;
+#pragma unroll
+    for (int x = 1; x < kSplit; ++x) M = fmaxf(M, s_m[x]);
+    const float use = M == q3::kNegInf ? 0.f : M;
+    sw = o0 = o1 = 0.f;
+#pragma unroll
+    for (int x = 0; x < kSplit; ++x) {
+      const float f = q3::fast_exp2(s_m[x] - use);
+      const float2 o = s_o[x][lane];
+      sw += f * s_w[x];
+      o0 += f * o.x;
+      o1 += f * o.y;
     }
   }
   const float inv = sw > 0.f ? 1.f / sw : 0.f;
@@ -1127,6 +1177,10 @@ extern "C" int qwen3_paged_decode_shared_bf16(
   q3::clear_error();
   hipLaunchKernelGGL(paged_shared_kernel, dim3(shared_workgroups()), dim3(kThreads), 0, s, a);
   if (const int rc = q3::launch_status(who)) return rc;
-  hipLaunchKernelGGL(paged_shared_join_kernel, dim3(num_kv_heads, B), dim3(64 * a.d.G), 0, s, a);
+  const dim3 grid(num_heads, B);
+  if (B * num_heads <= kSplitRows)
+    hipLaunchKernelGGL(paged_shared_join_kernel<8>, grid, dim3(8 * 64), 0, s, a);
+  else
+    hipLaunchKernelGGL(paged_shared_join_kernel<1>, grid, dim3(64), 0, s, a);
   return q3::launch_status(who);
 }
