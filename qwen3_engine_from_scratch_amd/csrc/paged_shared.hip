@@ -27,15 +27,18 @@
 // What bounds it: HBM, where sequences have much of their own (256 of 50-2,500 tokens behind
 // 2,000, 16/8 heads: 225 us, 5.7 TB/s); behind long prefixes the staged tiles, 1.87 us each
 // on each CU, where their loads alone take 1.4 (5.9 TB/s) and their products and softmax
-// alone 1.45, MFMA busy a third of the time, VALU as long, LDS without conflicts (32
-// sequences behind 100,000, 32/8 heads: 115 us, 3.8 TB/s; 64 behind 8,192 of 1-1,000 of
-// their own 47 us, 3.2 TB/s); in small calls the latency of the steps, 2.5 us until the batch is
-// tabulated, 10 of the first tiles, 5 of the join (4 behind 896, 16/8 heads: 14 us).
+// alone 1.45: a SIMD's two waves issue 48 MFMAs of 32 cycles and 340 other vector
+// instructions a tile, and the time is near the sum of the two, 3,300 cycles, however they
+// are interleaved (32 sequences behind 100,000, 32/8 heads: 115 us, 3.8 TB/s; 64 behind
+// 8,192 and 1-1,000 tokens of their own 47 us, 3.2 TB/s); in small calls the latency of the
+// steps, 2.5 us until the batch is tabulated, 10 of the first tiles, 5 of the join (4 behind
+// 896, 16/8 heads: 14 us).
 // Attended one by one (paged_decode.hip) the same batches take 489, 1,817, 296 and 15 us.
 //
 // Measured against it (32 behind 100,000; 64 behind 8,192): the values' products of both
 // halves of a tile's keys after the scores 117.7 us for 115.2; scores of one half taken a tile
-// ahead in stages of their own 113 for 113, 48 for 48; items of 256 rows 2.65 us a tile; parts
+// ahead in stages of their own 113 for 113, 48 for 48, and all operands read from LDS a step
+// before they are used 121 for 119, 48 for 48; items of 256 rows 2.65 us a tile; parts
 // stored past the caches 54.8 us for 52.6; waves' priorities no difference.
 #include <algorithm>
 
@@ -917,7 +920,7 @@ void paged_shared_kernel(SharedArgs a) {
 // Rows (query heads of sequences) up to which a row's parts are dealt to eight waves, a CU
 // reading what a few do too slowly: 4 sequences behind 30,000 tokens 41.7 us for 62.3, 40
 // behind 30,000, 640 rows, 51 for 51; of 2,048 rows 57 for 48.
-constexpr int kSplitRows = 1024;
+constexpr int kSplitRows = 512;
 
 // Parts of a row: `n` slots from `first` on, `step` apart; the first one may lie elsewhere.
 struct Parts {
