@@ -241,6 +241,9 @@ class Qwen3ForCausalLM(nn.Module):
     def _decode_fused(self, ids, row_ids, pool, positions, shared) -> torch.Tensor:
         """Decode step on the fused kernels; returns the logits."""
         h, _ = self._decode_layers(ids, row_ids, pool, positions, shared)
+        return self._final_logits(h)
+
+    def _final_logits(self, h) -> torch.Tensor:
         # lm_head streams 311 MB of weights for few rows: the library GEMM
         # after a separate final norm
         final = add_rms_norm(None, h, self.model.norm.weight, self.config.rms_norm_eps)
@@ -307,12 +310,14 @@ class Qwen3ForCausalLM(nn.Module):
     @torch.no_grad()
     def decode_greedy(self, ids: torch.Tensor, row_ids: torch.Tensor, pool,
                       positions: torch.Tensor | None = None,
-                      out: torch.Tensor | None = None, shared=None) -> torch.Tensor:
+                      out: torch.Tensor | None = None, shared=None, with_logits: bool = False):
         """Greedy tokens (B,) int64 of one decode step, argmax of
         decode_logits(...) (shared: as there).  On the fused path the final norm, lm_head and
         argmax run as one pass over the tied embedding that never stores the
         logits (qwen3_lm_head_argmax_bf16); out may alias ids (the ids are
-        read before the tokens are written)."""
+        read before the tokens are written).  with_logits: (tokens, logits), the same
+        tokens; on the fused path the logits come from the library product, whose sums
+        differ in order, so a near tie's token may not be its row's argmax."""
         B = ids.numel()
         cfg = self.config
         if out is None:
@@ -327,9 +332,10 @@ class Qwen3ForCausalLM(nn.Module):
                                         positions, shared)
             lm_head_argmax(h, ss, self.model.norm.weight, cfg.rms_norm_eps, self.lm_head.weight,
                            out=out.view(-1), workspace=self._head_ws)
-            return out
+            return (out, self._final_logits(h)) if with_logits else out
         logits = self.decode_logits(ids, row_ids, pool, positions, shared=shared)
-        return argmax(logits, out=out.view(-1))
+        out = argmax(logits, out=out.view(-1))
+        return (out, logits) if with_logits else out
 
     @torch.no_grad()
     def decode_logits(self, ids: torch.Tensor, row_ids: torch.Tensor, pool,

@@ -215,7 +215,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     entropy:  the distributions' entropy too (in nats)
     Returns TokenLogprobs; differentiable with respect to the logits (once), by the log
     probabilities, the entropy and the top log probabilities.  Logits of -inf have no
-    mass; a row of nothing else, or with NaN or +inf, gives NaN.
+    mass; a row of nothing else, or with NaN or +inf, gives NaN.  (A backward pass is
+    captured into a graph for logits made inside the capture, or a leaf of which no eager
+    graph lives: torch ends the process otherwise, whatever the operator.)
     """
     if logits.ndim != 2:
         raise ValueError(f"logits must be (T, V), got shape {tuple(logits.shape)}")

@@ -338,3 +338,54 @@ def test_another_stream_and_a_graph(gpu):
         torch.cuda.synchronize()
         want = call(y, t, top_n=7, entropy=True)
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_gradient_in_a_graph(gpu):
+    """Forward and backward captured, replayed with other logits and upstream gradients."""
+    announce("logprobs: gradient captured")
+    x = make(5, 4099, "bf16", seed=3).to(gpu)
+    t = torch.tensor([[1, 2], [3, 3], [-1, 4098], [7, 0], [9, 4]], device=gpu)
+    up = [torch.randn(5, 2, device=gpu), torch.randn(5, device=gpu), torch.randn(5, 3, device=gpu)]
+
+    def step():
+        leaf = x.detach().requires_grad_()
+        r = call(leaf, t, top_n=3, entropy=True, temperature=0.7)
+        return torch.autograd.grad([r.logprobs, r.entropy, r.top_logprobs], leaf, up)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        d = step()
+    for i in range(4):
+        x.copy_(make(5, 4099, "bf16", seed=20 + i))
+        for u in up:
+            u.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(d, step())
+
+
+def test_logits_past_32_bits(gpu):
+    """Rows whose bytes and elements lie past 2^32 and 2^31, of logits and gradient; strided."""
+    announce("logprobs: 4.5 GB of logits")
+    vocab, rows, stride = 151936, 15000, 152000
+    x = torch.zeros(rows, stride, dtype=torch.bfloat16, device=gpu)[:, 8:8 + vocab]
+    assert x.stride(0) * (rows - 1) > 2 ** 31
+    last = make(5, vocab, "bf16", seed=5)
+    x[-5:] = last.to(gpu)
+    t = torch.zeros(rows, dtype=torch.long, device=gpu)
+    t[-5:] = torch.tensor([0, 7, vocab - 1, 151000, 64], device=gpu)
+    x.requires_grad_()
+    r = call(x, t, top_n=3, entropy=True)
+    end = type(r)(*(v.detach()[-5:] for v in r))
+    check(last, t[-5:].cpu(), end, top_n=3, what="the last rows")
+    up = torch.ones(rows, device=gpu)
+    dx, = torch.autograd.grad(r.logprobs, x, up)
+    alone = last.to(gpu).requires_grad_()
+    few, = torch.autograd.grad(call(alone, t[-5:], top_n=3, entropy=True).logprobs, alone, up[-5:])
+    assert (dx[-5:].float() - few.float()).abs().max() <= few.abs().max().float() * 2.0 ** -7
+    assert not dx[:8, 1:].ne(dx[0, 1]).any()
