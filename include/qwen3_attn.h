@@ -403,8 +403,7 @@ int qwen3_paged_chunk_bf16(const void* q, const int64_t q_strides[2],
  * sequences must lie in the same pages (those that the table names for the group's
  * first sequence are read).  A prefix counts as far as the first sequence's length and
  * in whole multiples of 16; entries of no group, and groups of one, attend alone.
- * Sequences of a group may be shorter than its prefix; the values of shared positions
- * behind such a sequence must be finite.
+ * A sequence of a group that ends inside its prefix attends alone too.
  *   q .. out    as qwen3_paged_decode_bf16; scale positive and finite
  *   workspace   qwen3_paged_decode_shared_workspace_bytes(...) bytes, 16-byte aligned,
  *               no initialisation; calls that share one must not overlap.  Depends on
