@@ -331,7 +331,7 @@ class Engine:
         groups = None
         if self.share_prefixes and (not replay or key != self._last_batch):
             order, *groups = shared_prefix_groups(caches)
-            if replay or groups[1]:
+            if self.runner is not None or groups[1]:
                 reqs = [reqs[i] for i in order]
                 caches = [caches[i] for i in order]
             else:
@@ -341,8 +341,13 @@ class Engine:
             caches = [r.cache for r in reqs]
             out = self.runner.replay_greedy(k)
         else:
-            ids = torch.tensor([r.output_ids[-1] for r in reqs], dtype=torch.int64).to(dev)
-            rows = torch.tensor([c.row_id for c in caches], dtype=torch.int32).to(dev)
+            ids = [r.output_ids[-1] for r in reqs]
+            rows = [c.row_id for c in caches]
+            if self.runner is not None and told:  # as the replay would run it: the same bits
+                pad = self.runner.bucket_for(k) - k
+                ids, rows = ids + [0] * pad, rows + [self.runner.dummy_row] * pad
+            ids = torch.tensor(ids, dtype=torch.int64).to(dev)
+            rows = torch.tensor(rows, dtype=torch.int32).to(dev)
             shared = None
             if replay:
                 out = self.runner.replay_greedy(k, ids, rows, groups)
@@ -352,7 +357,7 @@ class Engine:
             if told:
                 toks, logits = self.model.decode_greedy(ids, rows, self.pool, shared=shared,
                                                         with_logits=True)
-                for r, got in zip(reqs, self._choose(logits, reqs, toks)):
+                for r, got in zip(reqs, self._choose(logits[:k], reqs, toks[:k])):
                     self._take(r, got)
                 for c in caches:
                     c.seq_len += 1

@@ -145,15 +145,16 @@ def test_asking_changes_no_token(gpu, share):
     model = model.to(gpu)
     g = torch.Generator().manual_seed(6)
     system = torch.randint(0, cfg.vocab_size, (70,), generator=g).tolist()
-    asks = [torch.randint(0, cfg.vocab_size, (3 + i,), generator=g).tolist() for i in range(7)]
+    asks = [torch.randint(0, cfg.vocab_size, (3 + i,), generator=g).tolist() for i in range(19)]
     announce(f"log probabilities asked for or not, shared prefixes {share}")
     told = []
     for ask in (None, 0, 5):
-        pool = _pool(cfg, gpu, blocks=120, max_requests=32)
-        engine = Engine(model, pool, max_batch=8, share_prefixes=share)
+        pool = _pool(cfg, gpu, blocks=200, max_requests=64)
+        engine = Engine(model, pool, max_batch=20, share_prefixes=share)
         prefix = engine.cache_prefix(system)
-        reqs = [GenRequest(i, a, 4 + i, prefix=prefix) for i, a in enumerate(asks)]
-        reqs[2].logprobs = reqs[5].logprobs = ask
+        reqs = [GenRequest(i, a, 4 + i, prefix=prefix if i % 4 else None)
+                for i, a in enumerate(asks)]
+        reqs[2].logprobs = reqs[14].logprobs = ask
         engine.generate(reqs)
         told.append([r.output_ids for r in reqs])
         prefix.free()
