@@ -30,15 +30,21 @@
 
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWaves = kThreads / 64;
+// Threads of a workgroup (512: 20 listed of 2,000 x 16,000 bf16 40 us for 30, of 1 and of 64
+// rows of a step 17.4 and 24.3 for 16.0 and 22.1; 64 listed of 12 x 151,936 37 for 42), and
+// where whole rows have up to kShort 16-byte pieces (256 there: 5,571 x 796, 50 listed, 40
+// us for 27, 2,000 x 8,000, 20 listed, 26 for 21; 128 for 3,000 x 8,000 fp32, 50 listed, 42
+// for 38).
+constexpr int kThreads = 256;
+constexpr int kShortThreads = 128;
+constexpr int kShort = 1024;
 constexpr int kMaxTop = 64;      // most likely tokens a row
 constexpr int kMaxGiven = 64;    // given tokens a row
 constexpr int kMaxParts = 64;
-constexpr int kResident = 512;   // workgroups that run at once (2 a CU)
+constexpr int kResident = 512;   // parts of all rows: 2 a CU (1,024: 64 rows 24.6 us for 22.1)
 constexpr int kCap = 1024;       // candidates of a part
-constexpr int kFewThreads = 128; // threads that reach T and are read again one by one
-constexpr int kBatchTokens = 16; // a thread's tokens of a load (600 rows 42 us, of 32 46)
+constexpr int kFewThreads = 64;  // threads that reach T and are read again one by one
+constexpr int kBatchTokens = 16; // a thread's tokens of a load (64 rows of a step 22.6 us, of 32 24.2)
 constexpr int kFewPieces = 256;  // pieces that are read again for a bound looser than n needs
 constexpr uint32_t kMinusInf = 0x007fffffu;  // key of -inf
 constexpr float kFloor = -1e38f; // R of a state without finite terms
@@ -214,10 +220,13 @@ __device__ __forceinline__ void fold(Sums& st, const float (&x)[N], float c) {
   if constexpr (kEnt) st.s1 += (s1[0] + s1[1]) + (s1[2] + s1[3]);
 }
 
+template <int kT>
 struct Shared {
+  static constexpr int kWaves = kT / 64;
+  static_assert(kMaxTop <= kFewThreads && kT / 4 <= kFewThreads);
   Sums sums[kWaves];
   u64 best[kWaves];
-  uint32_t key[kThreads];
+  uint32_t key[kT];
   int count[kWaves];
   u64 cand[kCap];
   u64 top[kMaxTop];
@@ -241,7 +250,9 @@ __device__ __forceinline__ void join_wave(Sums& st) {
 }
 
 // The block's threads' states in one, on every thread.
-__device__ __forceinline__ void join_block(Sums& st, Shared& sh) {
+template <int kT>
+__device__ __forceinline__ void join_block(Sums& st, Shared<kT>& sh) {
+  constexpr int kWaves = kT / 64;
   join_wave(st);
   if ((threadIdx.x & 63) == 0) sh.sums[threadIdx.x >> 6] = st;
   __syncthreads();
@@ -267,7 +278,8 @@ __device__ __forceinline__ bool extreme(float max, float c) {
   return !(__builtin_fabsf(max * c) < kExtreme) && __builtin_fabsf(max) < __builtin_inff();
 }
 
-__device__ __forceinline__ u64 block_max(u64 v, Shared& sh) {
+template <int kT>
+__device__ __forceinline__ u64 block_max(u64 v, Shared<kT>& sh) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const u64 y = __shfl_xor(v, o, 64);
@@ -277,7 +289,7 @@ __device__ __forceinline__ u64 block_max(u64 v, Shared& sh) {
   if ((threadIdx.x & 63) == 0) sh.best[threadIdx.x >> 6] = v;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) v = sh.best[w] > v ? sh.best[w] : v;
+  for (int w = 0; w < kT / 64; ++w) v = sh.best[w] > v ? sh.best[w] : v;
   return v;
 }
 
@@ -307,7 +319,8 @@ __device__ __forceinline__ uint32_t nth_bound(const uint32_t (&k)[kPer], int n, 
 
 // The same of the block's threads' keys.  Fewer finite ones than n are told beforehand: the
 // search for -inf or 0 would pass all 32 bits (rows masked but for 12 tokens: 4 us of 24).
-__device__ __forceinline__ uint32_t bound_of(const uint32_t (&k)[kWaves], int n, int most) {
+template <int kPer>
+__device__ __forceinline__ uint32_t bound_of(const uint32_t (&k)[kPer], int n, int most) {
   if (reaching(k, kMinusInf + 1u) < n) return reaching(k, kMinusInf) < n ? 0u : kMinusInf;
   return nth_bound(k, n, most);
 }
@@ -326,21 +339,22 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
 }
 
 // Appends a part's token to the candidates (counted, not kept, behind the list's end).
-__device__ __forceinline__ void append(Shared& sh, uint32_t key, int idx) {
+template <int kT>
+__device__ __forceinline__ void append(Shared<kT>& sh, uint32_t key, int idx) {
   const int at = atomicAdd(&sh.n_cand, 1);
   if (at < kCap) sh.cand[at] = ranked(key, static_cast<uint32_t>(idx));
 }
 
 // The tokens of the threads in sh.few whose key is at least `least`: their pieces dealt to
 // all threads, so that the loads are one round trip (or few).
-template <typename Tr>
+template <typename Tr, int kT>
 __device__ __forceinline__ void gather_few(const LogprobArgs& a, const char* xr, int p0, int p1,
-                                           uint32_t least, Shared& sh) {
-  const int each = (p1 - p0 + kThreads - 1) / kThreads;  // a thread's pieces
+                                           uint32_t least, Shared<kT>& sh) {
+  const int each = (p1 - p0 + kT - 1) / kT;  // a thread's pieces
   const int all = min(sh.n_few, kFewThreads) * each;
-  for (int i = threadIdx.x; i < all; i += kThreads) {
+  for (int i = threadIdx.x; i < all; i += kT) {
     const int of = i / each;
-    const int p = p0 + sh.few[of] + (i - of * each) * kThreads;
+    const int p = p0 + sh.few[of] + (i - of * each) * kT;
     if (p >= p1) continue;
     float x[Tr::kE];
     Tr::unpack(load_piece<Tr>(a, xr, p), x);
@@ -355,7 +369,8 @@ __device__ __forceinline__ void gather_few(const LogprobArgs& a, const char* xr,
 }
 
 // Lists the threads where q holds.
-__device__ __forceinline__ void list_few(bool q, Shared& sh) {
+template <int kT>
+__device__ __forceinline__ void list_few(bool q, Shared<kT>& sh) {
   if (q) {
     const int at = atomicAdd(&sh.n_few, 1);
     if (at < kFewThreads) sh.few[at] = threadIdx.x;
@@ -381,9 +396,10 @@ __device__ __forceinline__ u64 best_in_piece(const LogprobArgs& a, const char* x
 
 // sh.top: the part's most likely tokens.  max: this thread's; nan: the part holds NaN or
 // +inf.  Every thread of the block calls it.
-template <typename Tr>
+template <typename Tr, int kT>
 __device__ __forceinline__ void top_tokens(const LogprobArgs& a, const char* xr, int p0, int p1,
-                                           float max, bool nan, Shared& sh) {
+                                           float max, bool nan, Shared<kT>& sh) {
+  constexpr int kWaves = kT / 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int n = a.top;
   const bool some = p0 + tid < p1;
@@ -398,8 +414,9 @@ __device__ __forceinline__ void top_tokens(const LogprobArgs& a, const char* xr,
       uint32_t k[kWaves];
 #pragma unroll
       for (int i = 0; i < kWaves; ++i) k[i] = sh.key[64 * i + lane];
-      const int each = (p1 - p0 + kThreads - 1) / kThreads;
-      const int most = each > 0 ? min(kFewThreads, kFewPieces / each) : n;
+      const int each = (p1 - p0 + kT - 1) / kT;
+      // (looser than a quarter of the threads, each that reaches it holds several tokens)
+      const int most = each > 0 ? min(min(p1 - p0, kT) / 4, kFewPieces / each) : n;
       const uint32_t t = bound_of(k, n, most > n ? most : n);
       if (lane == 0) sh.bound = t;
     }
@@ -412,15 +429,15 @@ __device__ __forceinline__ void top_tokens(const LogprobArgs& a, const char* xr,
     cnt = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) cnt += sh.count[w];
-    const bool few = cnt <= kFewThreads;
+    const bool few = cnt <= (n > kT / 4 ? n : kT / 4);
     list_few(few ? reaches : mine > t, sh);
     __syncthreads();
-    gather_few<Tr>(a, xr, p0, p1, few ? t : t + 1u, sh);
+    gather_few<Tr, kT>(a, xr, p0, p1, few ? t : t + 1u, sh);
     __syncthreads();
     // (many reach t by equal values: t is the n-th largest itself, not below it)
     if (!few && sh.n_cand < n) {  // the lowest indices at t itself
       int left = n - sh.n_cand;
-      for (int p = p0 + tid; left > 0 && p - tid < p1; p += kThreads) {
+      for (int p = p0 + tid; left > 0 && p - tid < p1; p += kT) {
         uint32_t hit = 0;
         if (p < p1) {
           float x[Tr::kE];
@@ -456,9 +473,10 @@ __device__ __forceinline__ void top_tokens(const LogprobArgs& a, const char* xr,
     const int nc = sh.n_cand;
     done = nc <= kCap;
     if (done) {
-      for (int i = tid; i < nc; i += kThreads) {
+      for (int i = tid; i < nc; i += kT) {
         const u64 r = sh.cand[i];
         int rank = 0;
+#pragma unroll 4
         for (int j = 0; j < nc; ++j) rank += sh.cand[j] > r ? 1 : 0;
         if (rank < n) sh.top[rank] = r;
       }
@@ -466,7 +484,7 @@ __device__ __forceinline__ void top_tokens(const LogprobArgs& a, const char* xr,
   }
   if (!done) {  // one token a round
     u64 best = 0;
-    for (int p = p0 + tid; p < p1; p += kThreads) {
+    for (int p = p0 + tid; p < p1; p += kT) {
       const u64 b = best_in_piece<Tr>(a, xr, p, ~0ull);
       best = b > best ? b : best;
     }
@@ -474,10 +492,10 @@ __device__ __forceinline__ void top_tokens(const LogprobArgs& a, const char* xr,
       const u64 w = block_max(best, sh);
       if (w == 0) break;  // (the same for every thread)
       if (tid == 0) sh.top[r] = w;
-      const int owner = (static_cast<int>(index_in(w)) / Tr::kE - p0) % kThreads;
+      const int owner = (static_cast<int>(index_in(w)) / Tr::kE - p0) % kT;
       u64 next = 0;
-      for (int64_t p = static_cast<int64_t>(p0) + owner + static_cast<int64_t>(tid) * kThreads;
-           p < p1; p += static_cast<int64_t>(kThreads) * kThreads) {
+      for (int64_t p = static_cast<int64_t>(p0) + owner + static_cast<int64_t>(tid) * kT;
+           p < p1; p += static_cast<int64_t>(kT) * kT) {
         const u64 b = best_in_piece<Tr>(a, xr, static_cast<int>(p), w);
         next = b > next ? b : next;
       }
@@ -523,9 +541,9 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, const char* xr, 
   }
 }
 
-template <typename Tr, bool kEnt, bool kTop>
-__global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
-  __shared__ Shared sh;
+template <typename Tr, int kT, bool kEnt, bool kTop>
+__global__ __launch_bounds__(kT) void logprobs_kernel(LogprobArgs a) {
+  __shared__ Shared<kT> sh;
   constexpr int E = Tr::kE, kBatch = kBatchTokens / E;
   const int tid = threadIdx.x;
   const uint32_t row = blockIdx.x / static_cast<uint32_t>(a.parts);
@@ -539,18 +557,18 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       // (a piece that this thread does not have: another one of the part, not used)
-      const int q = p + u * kThreads;
+      const int q = p + u * kT;
       w[u] = load_piece<Tr>(a, xr, q < p1 ? q : p0);
     }
   };
   if (p0 < p1) {
     q3::u32x4 next[kBatch];
     load(p0 + tid, next);
-    for (int base = p0; base < p1; base += kBatch * kThreads) {
+    for (int base = p0; base < p1; base += kBatch * kT) {
       q3::u32x4 w[kBatch];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) w[u] = next[u];
-      if (base + kBatch * kThreads < p1) load(base + kBatch * kThreads + tid, next);
+      if (base + kBatch * kT < p1) load(base + kBatch * kT + tid, next);
       float x[kBatch * E];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
@@ -559,10 +577,10 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
 #pragma unroll
         for (int e = 0; e < E; ++e) x[u * E + e] = y[e];
       }
-      if (base + kBatch * kThreads > whole) {
+      if (base + kBatch * kT > whole) {
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-          const int p = base + tid + u * kThreads;
+          const int p = base + tid + u * kT;
 #pragma unroll
           for (int e = 0; e < E; ++e) {
             int idx;
@@ -577,7 +595,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
   join_block(st, sh);
   if (extreme(st.max, a.c)) {  // the sums again, of (x - max) c
     Sums ex{st.max, 0.f, 0.f, 0.f};
-    for (int p = p0 + tid; p < p1; p += kThreads) {
+    for (int p = p0 + tid; p < p1; p += kT) {
       float x[E];
       Tr::unpack(load_piece<Tr>(a, xr, p), x);
 #pragma unroll
@@ -593,7 +611,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
     st.s = ex.s;
     st.s1 = ex.s1;
   }
-  if constexpr (kTop) top_tokens<Tr>(a, xr, p0, p1, mine, st.s != st.s, sh);
+  if constexpr (kTop) top_tokens<Tr, kT>(a, xr, p0, p1, mine, st.s != st.s, sh);
   if (a.parts == 1) {
     write_row<Tr>(a, xr, row, st, sh.top);
     return;
@@ -601,16 +619,16 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a) {
   const int64_t at = static_cast<int64_t>(row) * a.parts + part;
   if (tid == 0) a.part_sums[at] = st;
   if constexpr (kTop)
-    for (int k = tid; k < a.top; k += kThreads) a.part_top[at * a.top + k] = sh.top[k];
+    for (int k = tid; k < a.top; k += kT) a.part_top[at * a.top + k] = sh.top[k];
 }
 
 // Joins a row's parts.
 constexpr int kJoinThreads = 256;
 
 // Whether the parts' most likely tokens are joined by rank, some 0.9 us for eight lists and
-// a token a thread, or head by head, some 0.1 us each: 64 rows of 8 parts, 64 tokens 32.5 us
-// by rank and 37.7 by heads, 20 tokens 24.1 and 24.7, 5 tokens 22.1 and 21.5; 16 rows of 32
-// parts, 20 tokens 33 and 22.
+// a token a thread, or head by head, some 0.1 us each: 64 rows of 8 parts, 64 tokens 34.8 us
+// by rank and 40.4 by heads, 20 tokens 22.0 and 22.6, 5 tokens 20.2 and 19.4; 16 rows of 32
+// parts, 20 tokens 37.6 and 21.6.
 __device__ __forceinline__ bool ranked_join(int parts, int top) {
   return 9 * ((parts + 7) / 8) * ((parts * top + kJoinThreads - 1) / kJoinThreads) <= top;
 }
@@ -799,7 +817,7 @@ int elements_of(int dtype) { return dtype == 2 ? 4 : 8; }
 int bytes_of(int dtype) { return dtype == 2 ? 4 : 2; }
 
 // Parts of a row: as many workgroups as the device holds at once where the rows are fewer,
-// of a round each (512 pieces) at least.
+// of a round each (kThreads pieces) at least.
 int parts_for(int64_t rows, int64_t pieces) {
   const int64_t most = q3::cdiv(pieces, kThreads);
   int64_t p = kResident / rows;
@@ -853,17 +871,23 @@ LogprobArgs args_of(const void* logits, int64_t row_stride, int dtype, int64_t v
   return a;
 }
 
+template <typename Tr, int kT>
+void launch_rows(const LogprobArgs& a, int64_t rows, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(rows * a.parts)), block(kT);
+  if (a.entropy) {
+    if (a.top) hipLaunchKernelGGL((logprobs_kernel<Tr, kT, true, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((logprobs_kernel<Tr, kT, true, false>), grid, block, 0, s, a);
+  } else {
+    if (a.top) hipLaunchKernelGGL((logprobs_kernel<Tr, kT, false, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((logprobs_kernel<Tr, kT, false, false>), grid, block, 0, s, a);
+  }
+}
+
 template <typename Tr>
 int launch(const LogprobArgs& a, int64_t rows, hipStream_t s, const char* who) {
-  const dim3 grid(static_cast<unsigned>(rows * a.parts)), block(kThreads);
   q3::clear_error();
-  if (a.entropy) {
-    if (a.top) hipLaunchKernelGGL((logprobs_kernel<Tr, true, true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((logprobs_kernel<Tr, true, false>), grid, block, 0, s, a);
-  } else {
-    if (a.top) hipLaunchKernelGGL((logprobs_kernel<Tr, false, true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((logprobs_kernel<Tr, false, false>), grid, block, 0, s, a);
-  }
+  if (a.parts > 1 || a.pieces > kShort) launch_rows<Tr, kThreads>(a, rows, s);
+  else launch_rows<Tr, kShortThreads>(a, rows, s);
   if (const int rc = q3::launch_status(who)) return rc;
   if (a.parts == 1) return QWEN3_OK;
   hipLaunchKernelGGL(logprobs_join_kernel<Tr>, dim3(static_cast<unsigned>(rows)),
