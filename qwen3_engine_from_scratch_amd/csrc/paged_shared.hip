@@ -22,7 +22,8 @@
 // that have another half, are left in the workspace (normalised, with the log2 of their
 // sum), and the second launch joins each row's.  P is floored to whole tiles of 16 keys
 // and bounded by what the group's first sequence holds; the rest counts as each
-// sequence's own, and so does all of a sequence that ends inside P.  P meets V as two bf16 terms, as in the decode.
+// sequence's own, and so does all of a sequence that ends inside P.  The probabilities meet
+// the values as two bf16 terms, as in the decode.
 //
 // What bounds it: HBM, where sequences have much of their own (256 of 50-2,500 tokens behind
 // 2,000, 16/8 heads: 225 us, 5.7 TB/s); behind long prefixes the staged tiles, 1.87 us each
@@ -210,8 +211,9 @@ __device__ __forceinline__ void tabulate_shared(const SharedArgs& a, Tables& t, 
     }
     if (b < NG) {
       const int rows = members(t, b, B) * a.d.G, gp = t.gp[b];
-      if (rows > kRowsS) gt[i] = gp > 0 ? (staged_tiles(gp) + kItemTiles) * ((rows + kRowsT - 1) / kRowsT) : 0;
-      else gs[i] = gp > 0 ? gp + kSegTiles : 0;
+      const int items = (rows + kRowsT - 1) / kRowsT;
+      if (gp > 0 && rows > kRowsS) gt[i] = (staged_tiles(gp) + kItemTiles) * items;
+      else if (gp > 0) gs[i] = gp + kSegTiles;
     }
     own_i[i] = wave_prefix_sum(own[i]);
     gs_i[i] = wave_prefix_sum(gs[i]);
