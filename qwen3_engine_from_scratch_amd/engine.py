@@ -114,7 +114,7 @@ class Engine:
         self.pool = pool
         self.max_batch = max_batch
         self.max_prefill_batch = max_prefill_batch
-        model.decode_batch_invariant = batch_invariant
+        self.batch_invariant = model.decode_batch_invariant = batch_invariant
         self.device = pool.k_buffer.device
         self.runner = None
         self._placeholders = []
@@ -325,6 +325,8 @@ class Engine:
             self._drain()
         if not replay:
             self._last_batch = None
+            # (another engine of this model may have set its own)
+            self.model.decode_batch_invariant = self.batch_invariant
         # the token of this step lands at position seq_len: reserve its page
         caches = [r.cache for r in reqs]
         self._pages.reserve(caches, [c.seq_len + 1 for c in caches])

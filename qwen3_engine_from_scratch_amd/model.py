@@ -145,6 +145,7 @@ class Qwen3ForCausalLM(nn.Module):
             self.lm_head.weight = self.model.embed_tokens.weight
         self._workspace = None       # decode attention workspace of the current mode
         self._ws_mode = None
+        self._mode_ws = {}           # of each mode
         self._shared_ws = None       # of decode attention over shared prefixes
         self._superseded = []
         self._head_ws = None
@@ -190,15 +191,16 @@ class Qwen3ForCausalLM(nn.Module):
                                             self.config.num_key_value_heads,
                                             self.config.head_dim, pool.block_table_2d.shape[1],
                                             pool.block_size, batch_invariant=inv)
-        if self._workspace is None or self._ws_mode != inv or self._workspace.numel() < need:
-            if self._workspace is not None:
+        ws = self._mode_ws.get(inv)
+        if ws is None or ws.numel() < need:
+            if ws is not None:
                 # a graph captured earlier may still replay on the old buffer
-                self._superseded.append(self._workspace)
+                self._superseded.append(ws)
             # zeroed once: the batch-invariant kernel's hand-off tickets start
             # at zero and every call leaves them there
-            self._workspace = torch.zeros(max(need, 1), dtype=torch.uint8,
-                                          device=pool.k_buffer.device)
-            self._ws_mode = inv
+            ws = self._mode_ws[inv] = torch.zeros(max(need, 1), dtype=torch.uint8,
+                                                  device=pool.k_buffer.device)
+        self._workspace, self._ws_mode = ws, inv
         if self._chain_sync is None:
             self._chain_sync = decode_chain_sync(pool.k_buffer.device)
         if self._head_ws is None:

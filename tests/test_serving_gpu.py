@@ -162,6 +162,42 @@ def test_asking_changes_no_token(gpu, share):
     assert told[0] == told[1] == told[2]
 
 
+def test_engines_of_both_modes_on_one_model(gpu):
+    """Steps that are not replayed keep their engine's mode whatever engine was made last,
+    and going to and fro takes no new workspaces."""
+    from qwen3_engine_from_scratch_amd.engine import Engine, GenRequest
+
+    model, state, cfg = _tiny(seed=15)
+    model = model.to(gpu)
+    g = torch.Generator().manual_seed(7)
+    asks = [torch.randint(0, cfg.vocab_size, (40 + i,), generator=g).tolist() for i in range(5)]
+    pool = _pool(cfg, gpu, blocks=120, max_requests=64)
+    announce("a batch-invariant engine, a sharing and an eager one, in turn")
+    exact = Engine(model, pool, max_batch=8, batch_invariant=True, max_prefill_batch=1)
+    share = Engine(model, pool, max_batch=8, share_prefixes=True)
+    eager = Engine(model, pool, max_batch=8, use_graph=False, share_prefixes=True)
+
+    def run(engine, ask):
+        reqs = [GenRequest(i, a, 6, logprobs=ask if i == 2 else None) for i, a in enumerate(asks)]
+        engine.generate(reqs)
+        return [r.output_ids for r in reqs]
+
+    want, seen = None, None
+    for _ in range(3):
+        for ask in (None, 2):
+            got = run(exact, ask)
+            assert model._ws_mode is True or ask is None
+            want = want or got
+            assert got == want
+            run(share, ask)
+            run(eager, ask)
+            assert model._ws_mode is False
+        seen = seen or len(model._superseded)
+        assert len(model._superseded) == seen
+    for e in (exact, share, eager):
+        e.close()
+
+
 def test_sharing_changes_no_token_of_clear_choices(gpu):
     """The same requests with and without sharing: a token differs only where the oracle's
     two greatest logits are near each other (0.15, as above), and then the rest is not
