@@ -5,9 +5,12 @@
 // R (the largest x c so far), s = sum 2^(x c - R) and s1 = sum 2^(x c - R) (x c - R).
 // Two such states join with f = 2^(R - R'): s' = f s, s1' = f (s1 + s (R - R')).  Then
 //   log p_t = (x_t - max) / T - ln 2 log2 s  (R being max c),   H = ln 2 (log2 s - s1 / s).
-// x c - R is one multiply-add with the same rounded R everywhere, so its rounding is no
-// common shift of the row.  Rows whose |max c| is 1e38 or more (all logits at the type's
-// lowest value, say) overflow there and are passed over once more in the form (x - max) c.
+// x c - R is one multiply-add with the same rounded R everywhere: what R is off, max c - R,
+// is a common factor of the sums, known and taken out again (logprob_of).  R's half step is
+// 1/2 up to 2^24, doubles with every power of two behind it and would leave the exponents'
+// range from 2^31 on, so rows whose |max c| is 2^24 or more (finite masks everywhere, small
+// temperatures) are passed over once more in the form (x - max) c.  R is no lower than
+// -2^24 itself: what lies below vanishes beside anything above, or the row is such a one.
 //
 // The n most likely tokens come out of the same pass: a thread keeps the maximum of its
 // own tokens, and the n-th largest of these maxima, T, is a bound that n tokens reach.  Only
@@ -48,8 +51,8 @@ constexpr int kFewThreads = 64;  // threads that reach T and are read again one 
 constexpr int kBatchTokens = 16; // a thread's tokens of a load (64 rows of a step 22.6 us, of 32 24.2)
 constexpr int kFewPieces = 256;  // pieces that are read again for a bound looser than n needs
 constexpr uint32_t kMinusInf = 0x007fffffu;  // key of -inf
-constexpr float kFloor = -1e38f; // R of a state without finite terms
-constexpr float kExtreme = 1e38f;
+constexpr float kExtreme = 0x1p24f;   // |max c| from which the sums are relative to max itself
+constexpr float kFloor = -kExtreme;   // least R, and that of a state without terms
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kTiny = -200.f;  // 2^x is zero below it: keeps 0 * -inf out of the sums
 
@@ -119,7 +122,7 @@ struct Fp32 {
 struct Sums {
   float max;  // largest logit (-inf: none above it)
   float ref;  // R
-  float s, s1;
+  float s, s1; // relative to R, of an extreme max to max c itself
 };
 
 struct LogprobArgs {
@@ -522,7 +525,7 @@ template <typename Tr>
 __device__ __forceinline__ void write_row(const LogprobArgs& a, const char* xr, int64_t row,
                                           const Sums& st, const u64* top) {
   const int tid = threadIdx.x, step = blockDim.x;
-  // (s is relative to R: max * c, or max itself where that is no number to speak of)
+  // (s is relative to R, the rounded max * c, or to max * c itself of an extreme max)
   const float log2s = __builtin_log2f(st.s);
   if (tid == 0) {
     if (a.entropy) a.entropy[row] = kLn2 * (log2s - st.s1 / st.s);
@@ -646,9 +649,16 @@ __global__ __launch_bounds__(kJoinThreads) void logprobs_join_kernel(LogprobArgs
   float max = st.max;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) max = fmaxf(max, q3::shfl_xor(max, o));
-  if (extreme(max, a.c)) {
-    // each part's sums are relative to its own maximum
-    const float d = fmaxf((st.max - max) * a.c, -3e38f), f = q3::fast_exp2(d);
+  {
+    // a part's own reference, R or max c, over the row's: parts of one row may have either
+    const bool far = extreme(max, a.c), part_far = extreme(st.max, a.c);
+    const float ref = fmaxf(kFloor, max * a.c);
+    float d = st.ref - ref;
+    if (far) d = part_far ? (st.max - max) * a.c : -__builtin_fmaf(max, a.c, -st.ref);
+    else if (part_far) d = __builtin_fmaf(st.max, a.c, -ref);
+    // (no number below the row's largest one: s is 0 or NaN)
+    d = st.max == q3::kNegInf ? -3e38f : fmaxf(d, -3e38f);
+    const float f = q3::fast_exp2(d);
     st.s1 = f * (st.s1 + st.s * fmaxf(d, 2.f * kTiny));
     st.s *= f;
 #pragma unroll
@@ -657,8 +667,6 @@ __global__ __launch_bounds__(kJoinThreads) void logprobs_join_kernel(LogprobArgs
       st.s1 += q3::shfl_xor(st.s1, o);
     }
     st.max = max;
-  } else {
-    join_wave(st);
   }
   const int all = a.parts * a.top;
   if (a.top) {
