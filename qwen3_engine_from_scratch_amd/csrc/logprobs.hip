@@ -144,9 +144,11 @@ struct LogprobArgs {
   u64* part_top;         // (rows, parts, top), descending, 0: none
 };
 
-// Order of logits as whole numbers: larger value, larger key; equal zeros, NaN on top.
+// Order of logits as whole numbers: larger value, larger key; equal zeros, NaN on top (one
+// above the key of +inf, so that no token ranks as high as the ~0 that bounds a search).
+constexpr uint32_t kNanKey = 0xff800001u;
 __device__ __forceinline__ uint32_t key_of(float x) {
-  if (x != x) return 0xffffffffu;
+  if (x != x) return kNanKey;
   const uint32_t b = __float_as_uint(x + 0.f);
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }

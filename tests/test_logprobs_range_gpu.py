@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from conftest import announce
-from oracle.logprobs import Rows
+from oracle.logprobs import Rows, ranking
 from test_logprobs_gpu import call, check, make
 
 pytestmark = pytest.mark.gpu
@@ -107,3 +107,20 @@ def test_gradient_of_far_logits(gpu, kind):
         over = (dx.cpu().double() - want).abs() - (off + gone + want.abs() * 2.0 ** -24 + 2.0 ** -126)
         print(f"[err] {what}: worst excess {over.max().item():.2e}", flush=True)
         assert (over <= 0).all(), what
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_nan_at_the_first_tokens(gpu, dtype):
+    """NaN at token 0, in every token, with as many listed as there are tokens."""
+    for vocab, top in ((1, 1), (5, 5), (64, 64), (997, 12), (40013, 12), (150001, 64)):
+        announce(f"logprobs NaN at token 0: {vocab} {dtype}, top {top}")
+        x = make(4, vocab, dtype, seed=vocab)
+        x[0, 0] = float("nan")
+        x[1] = float("nan")
+        x[2, ::3] = -float("nan")
+        x[2, 1::3] = float("inf")
+        x[3, -1] = float("nan")
+        got = call(x.to(gpu), None, top_n=top)
+        torch.cuda.synchronize()
+        assert torch.equal(got.top_ids.cpu(), ranking(x, top))
+        assert torch.isnan(got.top_logprobs).all()
