@@ -530,7 +530,10 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, const char* xr, 
   // (s is relative to R, the rounded max * c, or to max * c itself of an extreme max)
   const float log2s = __builtin_log2f(st.s);
   if (tid == 0) {
-    if (a.entropy) a.entropy[row] = kLn2 * (log2s - st.s1 / st.s);
+    if (a.entropy) {
+      const float h = kLn2 * (log2s - st.s1 / st.s);
+      a.entropy[row] = h < 0.f ? 0.f : h;  // (one token left: the difference's rounding)
+    }
     if (a.stats) a.stats[row] = float2{st.max, log2s};
   }
   for (int k = tid; k < a.given; k += step) {

@@ -124,3 +124,19 @@ def test_nan_at_the_first_tokens(gpu, dtype):
         torch.cuda.synchronize()
         assert torch.equal(got.top_ids.cpu(), ranking(x, top))
         assert torch.isnan(got.top_logprobs).all()
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.37, 1e-9])
+def test_entropy_is_not_below_zero(gpu, temperature):
+    """One token with all of the mass, in rows of one part and of several."""
+    for rows, vocab in ((4096, 300), (40, 30011)):
+        announce(f"logprobs: entropy of one token, {rows} x {vocab}, T {temperature}")
+        x = torch.full((rows, vocab), float("-inf"))
+        x[:, 5] = torch.linspace(-900, 900, rows)
+        peaked = make(rows, vocab, "fp32", seed=3, std=60.0)
+        for y in (x, peaked):
+            got = call(y.to(gpu), None, entropy=True, temperature=temperature)
+            torch.cuda.synchronize()
+            assert (got.entropy >= 0).all()
+            check(y[:50], None, type(got)(*(v if v is None else v[:50] for v in got)),
+                  temperature=temperature, what=f"entropy {rows} x {vocab}")
