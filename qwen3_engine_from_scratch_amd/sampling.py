@@ -25,6 +25,7 @@ import math
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -215,7 +216,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     entropy:  the distributions' entropy too (in nats)
     Returns TokenLogprobs; differentiable with respect to the logits (once), by the log
     probabilities, the entropy and the top log probabilities.  Logits of -inf have no
-    mass; a row of nothing else, or with NaN or +inf, gives NaN.  (A backward pass is
+    mass; a row of nothing else, or with NaN or +inf, gives NaN.  Logits with a forward-mode
+    tangent are refused (NotImplementedError).  (A backward pass is
     captured into a graph for logits made inside the capture, or a leaf of which no eager
     graph lives: torch ends the process otherwise, whatever the operator.)
     """
@@ -244,6 +246,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
         raise ValueError(f"temperature {temperature} must be positive and finite")
     if tokens is None and not top_n and not entropy:
         raise ValueError("nothing asked for: no tokens, no top_n, no entropy")
+    if forward_ad.unpack_dual(logits).tangent is not None:
+        raise NotImplementedError("token_logprobs has no forward-mode derivative")
     dev = _lib.require_hip(logits, tokens)
     if T == 0:
         f32 = dict(dtype=torch.float32, device=dev)

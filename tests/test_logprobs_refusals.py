@@ -99,3 +99,17 @@ def test_wrapper_refuses():
                      ((x, None), {}), ((x[:, :0], t), {}), ((x[:1].expand(4, 100), t), {})):
         with pytest.raises(ValueError):
             token_logprobs(*args, **kw)
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor needs no gradient and has a data pointer: its tangent would be lost."""
+    x, t = torch.zeros(4, 100), torch.zeros(4, dtype=torch.int64)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for logits in (dual, dual[1:3]):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                token_logprobs(logits, t[:len(logits)])
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            token_logprobs(x, t)  # (one without a tangent is not meant)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda z: token_logprobs(z, t).logprobs, (x,), (x,))
