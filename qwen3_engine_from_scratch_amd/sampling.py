@@ -143,19 +143,26 @@ def _logprobs_workspace(*shape) -> int:
     return int(_lib.load().qwen3_token_logprobs_workspace_bytes(*shape))
 
 
+def _given(tokens) -> int:
+    """Given tokens a row."""
+    return 0 if tokens is None else 1 if tokens.ndim == 1 else tokens.shape[1]
+
+
 def _forward(logits, tokens, top_n, entropy, temperature, stats):
     """One call of the kernel: (logprobs, entropy, top_ids, top_logprobs, stats)."""
     T, V = logits.shape
     dev = logits.device
     lib = _lib.load()
     dtype = _DTYPES[logits.dtype]
-    given = 0 if tokens is None else tokens.numel() // T
+    given = _given(tokens)
     f32 = dict(dtype=torch.float32, device=dev)
     lp = None if tokens is None else torch.empty(tokens.shape, **f32)
     ent = torch.empty(T, **f32) if entropy else None
     ids = torch.empty(T, top_n, dtype=torch.int64, device=dev) if top_n else None
     top = torch.empty(T, top_n, **f32) if top_n else None
     st = torch.empty(T, 2, **f32) if stats else None
+    if T == 0:
+        return lp, ent, ids, top, st
     need = _logprobs_workspace(T, V, dtype, top_n)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     ptr = _lib.ptr
@@ -192,11 +199,13 @@ class _TokenLogprobs(torch.autograd.Function):
         g_lp, g_ent, g_top = (None if g is None else g.to(torch.float32).contiguous()
                               for g in (g_lp, g_ent, g_top))
         grad = torch.empty(T, V, dtype=logits.dtype, device=dev)
+        if T == 0:
+            return grad, None, None, None, None
         ptr = _lib.ptr
         with _lib.on_device(dev):
             rc = _lib.load().qwen3_token_logprobs_grad(
                 logits.data_ptr(), logits.stride(0), _DTYPES[logits.dtype], T, V, ptr(tokens),
-                0 if tokens is None else tokens.numel() // T, ctx.temperature, ptr(ent),
+                _given(tokens), ctx.temperature, ptr(ent),
                 0 if ids is None else ids.shape[1], ptr(ids), stats.data_ptr(), ptr(g_lp),
                 ptr(g_ent), ptr(g_top), grad.data_ptr(), V, _lib.stream_of(dev))
         _lib.check(rc, "qwen3_token_logprobs_grad")
@@ -248,14 +257,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
         raise ValueError("nothing asked for: no tokens, no top_n, no entropy")
     if forward_ad.unpack_dual(logits).tangent is not None:
         raise NotImplementedError("token_logprobs has no forward-mode derivative")
-    dev = _lib.require_hip(logits, tokens)
-    if T == 0:
-        f32 = dict(dtype=torch.float32, device=dev)
-        out = (None if tokens is None else torch.empty(tokens.shape, **f32),
-               torch.empty(0, **f32) if entropy else None,
-               torch.empty(0, top_n, dtype=torch.int64, device=dev) if top_n else None,
-               torch.empty(0, top_n, **f32) if top_n else None)
-        return TokenLogprobs(*out)
+    _lib.require_hip(logits, tokens)
     if tokens is not None:
         tokens = tokens.contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:

@@ -140,3 +140,24 @@ def test_entropy_is_not_below_zero(gpu, temperature):
             assert (got.entropy >= 0).all()
             check(y[:50], None, type(got)(*(v if v is None else v[:50] for v in got)),
                   temperature=temperature, what=f"entropy {rows} x {vocab}")
+
+
+@pytest.mark.parametrize("given", [None, 1, 3])
+def test_a_batch_without_rows_has_a_gradient(gpu, given):
+    """An empty one: a training step without rows runs as any other."""
+    announce(f"logprobs: no rows, {given} given")
+    w = torch.randn(8, 50, device=gpu, requires_grad=True)
+    hidden = torch.empty(0, 8, device=gpu)
+    t = None if given is None else torch.empty((0,) if given == 1 else (0, given), dtype=torch.int64,
+                                               device=gpu)
+    r = call(hidden @ w, t, top_n=2, entropy=True)
+    assert r.top_logprobs.requires_grad and not r.top_ids.requires_grad
+    loss = r.entropy.sum() + r.top_logprobs.sum()
+    if given is not None:
+        assert r.logprobs.shape == t.shape
+        loss = loss + r.logprobs.sum()
+    loss.backward()
+    assert w.grad.shape == w.shape and not w.grad.any()
+    with torch.no_grad():
+        r = call(hidden @ w, t, top_n=2, entropy=True)
+    assert not r.entropy.requires_grad and r.top_ids.shape == (0, 2)
