@@ -91,7 +91,8 @@ class Engine:
                  prefill_chunk: int | None = None, share_prefixes: bool = False):
         """batch_invariant: decode attention on the batch-invariant kernel,
         so a request's decode tokens do not depend on what else is batched
-        with it.  max_prefill_batch: prompts per prefill step (None: as many
+        with it (an eager engine follows model.decode_batch_invariant where that is
+        set afterwards).  max_prefill_batch: prompts per prefill step (None: as many
         as there are free rows); 1 prefills every prompt alone, as a
         request running by itself would be (the library GEMMs of the
         prefill pick kernels by row count, so a prompt's prefill bits depend
@@ -114,7 +115,9 @@ class Engine:
         self.pool = pool
         self.max_batch = max_batch
         self.max_prefill_batch = max_prefill_batch
-        self.batch_invariant = model.decode_batch_invariant = batch_invariant
+        # (as the model's mode too, for direct calls, but not as one that a program set)
+        self.batch_invariant = model._invariant = bool(batch_invariant)
+        self._invariant_set = model._invariant_set
         self.device = pool.k_buffer.device
         self.runner = None
         self._placeholders = []
@@ -312,6 +315,15 @@ class Engine:
             r.inflight -= 1
             self._take(r, int(tok))
 
+    def _mode(self) -> bool:
+        """Whether a step that is not replayed runs batch-invariant: in the mode that the
+        engine was made with, whatever other engines of this model were made with (and
+        captured in, if it captures); an eager one follows a program that has set the
+        model's decode_batch_invariant since."""
+        if self.runner is None and self.model._invariant_set != self._invariant_set:
+            return self.model._invariant_asked
+        return self.batch_invariant
+
     def _decode(self, reqs) -> None:
         """Launches one decode step for `reqs` and then reads back the tokens
         of the step before it, so the host's bookkeeping overlaps the GPU."""
@@ -325,8 +337,6 @@ class Engine:
             self._drain()
         if not replay:
             self._last_batch = None
-            # (another engine of this model may have set its own)
-            self.model.decode_batch_invariant = self.batch_invariant
         # the token of this step lands at position seq_len: reserve its page
         caches = [r.cache for r in reqs]
         self._pages.reserve(caches, [c.seq_len + 1 for c in caches])
@@ -357,8 +367,9 @@ class Engine:
             elif groups is not None:
                 shared = tuple(torch.tensor(g, dtype=torch.int32).to(dev) for g in groups)
             if told:
-                toks, logits = self.model.decode_greedy(ids, rows, self.pool, shared=shared,
-                                                        with_logits=True)
+                with self.model.decode_mode(self._mode()):
+                    toks, logits = self.model.decode_greedy(ids, rows, self.pool, shared=shared,
+                                                            with_logits=True)
                 for r, got in zip(reqs, self._choose(logits[:k], reqs, toks[:k])):
                     self._take(r, got)
                 for c in caches:
@@ -366,7 +377,8 @@ class Engine:
                 set_seq_lens_bulk(caches)
                 return
             if not replay:
-                out = self.model.decode_greedy(ids, rows, self.pool, shared=shared)
+                with self.model.decode_mode(self._mode()):
+                    out = self.model.decode_greedy(ids, rows, self.pool, shared=shared)
         toks = out.view(-1)[:k]
         host = self._tok_host[self._flip][:k]
         self._flip ^= 1

@@ -26,6 +26,7 @@ Entry points:
 """
 from __future__ import annotations
 
+import contextlib
 import zlib
 
 import numpy as np
@@ -150,10 +151,30 @@ class Qwen3ForCausalLM(nn.Module):
         self._superseded = []
         self._head_ws = None
         self._chain_sync = None
-        # Decode attention with the batch-invariant kernel: each sequence's
-        # tokens independent of the rest of the batch (batched == serial),
-        # at some HBM time where sequences are split across waves.
-        self.decode_batch_invariant = False
+        self._invariant = self._invariant_asked = False
+        self._invariant_set = 0      # how often a program has set the mode
+
+    @property
+    def decode_batch_invariant(self) -> bool:
+        """Decode attention with the batch-invariant kernel: each sequence's
+        tokens independent of the rest of the batch (batched == serial),
+        at some HBM time where sequences are split across waves."""
+        return self._invariant
+
+    @decode_batch_invariant.setter
+    def decode_batch_invariant(self, on: bool) -> None:
+        self._invariant = self._invariant_asked = bool(on)
+        self._invariant_set += 1
+
+    @contextlib.contextmanager
+    def decode_mode(self, batch_invariant: bool):
+        """Decode steps inside run in that mode; decode_batch_invariant is afterwards as
+        it was."""
+        kept, self._invariant = self._invariant, bool(batch_invariant)
+        try:
+            yield
+        finally:
+            self._invariant = kept
 
     # ---- shared layer loop -------------------------------------------------
 
