@@ -405,6 +405,9 @@ class Engine:
         for p in prompts:
             if not p:
                 raise ValueError("an empty prompt has nothing to score")
+            if not (0 <= min(p) and max(p) < self.model.config.vocab_size):
+                # (a negative id would count as no token, with a log probability of 0)
+                raise ValueError("a prompt to score has a token outside the vocabulary")
             self._check_positions(len(p))
         scored, at = [], 0
         while at < len(prompts):
