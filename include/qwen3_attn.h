@@ -402,7 +402,8 @@ int qwen3_paged_chunk_bf16(const void* q, const int64_t q_strides[2],
  * num_groups + 1, ascending); the first shared_lens[g] positions of each of its
  * sequences must lie in the same pages (those that the table names for the group's
  * first sequence are read).  A prefix counts as far as the first sequence's length and
- * in whole multiples of 16; entries of no group, and groups of one, attend alone.
+ * in whole multiples of 16; entries of no group, and groups of one, attend alone.  If
+ * the bounds do not ascend, there are no groups.
  * A sequence of a group that ends inside its prefix attends alone too.
  *   q .. out    as qwen3_paged_decode_bf16; scale positive and finite
  *   workspace   qwen3_paged_decode_shared_workspace_bytes(...) bytes, 16-byte aligned,

@@ -126,6 +126,7 @@ struct Tables {
   uint16_t grp[kMaxSeqs];      // the group whose prefix a sequence shares
   int16_t g0[kMaxSeqs + 2];    // first sequence (-1, B + 1: outside the batch)
   int32_t wsum[3][kRounds][kShWaves];
+  int32_t falling;             // whether the groups' bounds do not ascend
 };
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -160,6 +161,7 @@ __device__ __forceinline__ void tabulate_shared(const SharedArgs& a, Tables& t, 
                                                 int& all_gs, int& all_gt) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int B = a.d.B, NG = a.groups;
+  if (tid == 0) t.falling = 0;
   int64_t row[R];
   int32_t cap[R];
 #pragma unroll
@@ -186,12 +188,16 @@ __device__ __forceinline__ void tabulate_shared(const SharedArgs& a, Tables& t, 
   for (int i = 0; i < R; ++i) {
     const int g = i * kThreads + tid;
     if (g < NG) {
+      if (t.g0[g] > t.g0[g + 1]) t.falling = 1;
       const int n = members(t, g, B);
       const int most = n > 1 ? min(cap[i], t.len[t.g0[g]]) : 0;
       t.gp[g] = most > 0 ? most / kTile : 0;
     }
   }
   __syncthreads();
+  // (bounds that fall back make groups overlap: two prefixes of one row, whose parts share
+  // their places, and more tiles than the host has counted on.  There are no groups then)
+  const bool falling = t.falling != 0;
   int own[R], gs[R], gt[R], own_i[R], gs_i[R], gt_i[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -199,7 +205,7 @@ __device__ __forceinline__ void tabulate_shared(const SharedArgs& a, Tables& t, 
     int skip = 0;
     own[i] = gs[i] = gt[i] = 0;
     if (b < B) {
-      const int g = NG > 0 ? last_at_most(t.g0, NG, b) : -1;
+      const int g = falling ? -1 : last_at_most(t.g0, NG, b);
       const bool in = g >= 0 && b < t.g0[g] + members(t, g, B);
       // (one that ends inside the prefix attends alone: masked, infinities and NaN among the
       // values behind its end would reach it by their products with zero)
@@ -210,7 +216,7 @@ __device__ __forceinline__ void tabulate_shared(const SharedArgs& a, Tables& t, 
       own[i] = tiles > skip ? tiles - skip + kSegTiles : 0;
     }
     if (b < NG) {
-      const int rows = members(t, b, B) * a.d.G, gp = t.gp[b];
+      const int rows = members(t, b, B) * a.d.G, gp = falling ? 0 : t.gp[b];
       const int items = (rows + kRowsT - 1) / kRowsT;
       if (gp > 0 && rows > kRowsS) gt[i] = (staged_tiles(gp) + kItemTiles) * items;
       else if (gp > 0) gs[i] = gp + kSegTiles;

@@ -332,8 +332,8 @@ def paged_attention_decode_shared_hip(q, k_buffer, v_buffer, block_table_2d, seq
 
     q, k_buffer/v_buffer, block_table_2d, seq_lens_full, row_ids: as there; up to 1,024
                     sequences, a group's sequences next to each other
-    cu_groups:      int32 (num_groups + 1,), ascending: group g is the batch entries
-                    cu_groups[g] .. cu_groups[g + 1] - 1
+    cu_groups:      int32 (num_groups + 1,), ascending (else there are no groups): group
+                    g is the batch entries cu_groups[g] .. cu_groups[g + 1] - 1
     shared_lens:    int32 (num_groups,): the tokens that all of the group's sequences hold
                     in the same pages (counted in whole multiples of 16, and as far as the
                     group's first sequence goes; one that ends before that attends alone).
