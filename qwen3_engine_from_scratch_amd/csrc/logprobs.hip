@@ -1,16 +1,16 @@
 // Log probabilities of given tokens, the entropy of their distribution and its most
 // likely tokens, from rows of logits, and the logits' gradient.
 //
-// With z = x / T and c = log2(e) / T, in one pass over a row: a thread keeps a reference
-// R (the largest x c so far), s = sum 2^(x c - R) and s1 = sum 2^(x c - R) (x c - R).
-// Two such states join with f = 2^(R - R'): s' = f s, s1' = f (s1 + s (R - R')).  Then
-//   log p_t = (x_t - max) / T - ln 2 log2 s  (R being max c),   H = ln 2 (log2 s - s1 / s).
-// x c - R is one multiply-add with the same rounded R everywhere: what R is off, max c - R,
-// is a common factor of the sums, known and taken out again (logprob_of).  R's half step is
-// 1/2 up to 2^24, doubles with every power of two behind it and would leave the exponents'
-// range from 2^31 on, so rows whose |max c| is 2^24 or more (finite masks everywhere, small
-// temperatures) are passed over once more in the form (x - max) c.  R is no lower than
-// -2^24 itself: what lies below vanishes beside anything above, or the row is such a one.
+// With z = x / T and c = log2(e) / T, in one pass over a row: a thread keeps the largest x
+// so far, m, a point P beside m c, s = sum 2^(x c - P) and s1 = sum 2^(x c - P) (x c - P).
+// Two such states join with f = 2^(P - P'): s' = f s, s1' = f (s1 + s (P - P')).  Then
+//   log p_t = (x_t - m) / T - ln 2 (log2 s - (m c - P)),   H = ln 2 (log2 s - s1 / s).
+// P is m c rounded, so that x c - P is one multiply-add; what it is off, m c - P, is a factor
+// of the sums, known and taken out again.  P's half step is 1/2 up to 2^24, doubles with
+// every power of two behind it and would leave the exponents' range from 2^31 on: where
+// |m c| is 2^24 or more (finite masks, small temperatures) P is m c itself and the exponents
+// are (x - m) c.  (That form everywhere: 4,096 x 151,936 bf16 206 us for 200; sums of far
+// rows in a second pass: 64 rows of a step masked by -1e9 26.4 us for 20.)
 //
 // The n most likely tokens come out of the same pass: a thread keeps the maximum of its
 // own tokens, and the n-th largest of these maxima, T, is a bound that n tokens reach.  Only
@@ -51,8 +51,7 @@ constexpr int kFewThreads = 64;  // threads that reach T and are read again one 
 constexpr int kBatchTokens = 16; // a thread's tokens of a load (64 rows of a step 22.6 us, of 32 24.2)
 constexpr int kFewPieces = 256;  // pieces that are read again for a bound looser than n needs
 constexpr uint32_t kMinusInf = 0x007fffffu;  // key of -inf
-constexpr float kExtreme = 0x1p24f;   // |max c| from which the sums are relative to max itself
-constexpr float kFloor = -kExtreme;   // least R, and that of a state without terms
+constexpr float kFar = 0x1p24f;  // |m c| from which P is m c itself
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kTiny = -200.f;  // 2^x is zero below it: keeps 0 * -inf out of the sums
 
@@ -119,10 +118,9 @@ struct Fp32 {
 };
 
 // A row's (or part's) sums.
-struct Sums {
+struct alignas(16) Sums {
   float max;  // largest logit (-inf: none above it)
-  float ref;  // R
-  float s, s1; // relative to R, of an extreme max to max c itself
+  float s, s1;
 };
 
 struct LogprobArgs {
@@ -198,32 +196,62 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return m;
 }
 
-// The states' join: a with another reference.
-__device__ __forceinline__ void move_ref(Sums& a, float ref) {
-  const float d = fmaxf(a.ref - ref, -3e38f), f = q3::fast_exp2(d);
+// Whether P of the largest logit `max` is max c itself.
+__device__ __forceinline__ bool far(float max, float c) {
+  return !(__builtin_fabsf(max * c) < kFar) && __builtin_fabsf(max) < __builtin_inff();
+}
+// P where it is not (of no logit but -inf the least that one can be).
+__device__ __forceinline__ float point(float max, float c) { return fmaxf(max * c, -kFar); }
+
+// The states' join: a with a larger maximum, by d = P - P'.
+__device__ __forceinline__ void raise_by(Sums& a, float max, float d) {
+  d = fmaxf(d, -3e38f);
+  const float f = q3::fast_exp2(d);
   a.s1 = f * (a.s1 + a.s * fmaxf(d, 2.f * kTiny));
   a.s *= f;
-  a.ref = ref;
+  a.max = max;
+}
+// The same where either may be far.
+__device__ __forceinline__ void raise(Sums& a, float max, float c) {
+  float d = point(a.max, c) - point(max, c);
+  if (far(max, c))
+    d = far(a.max, c) ? (a.max - max) * c : -__builtin_fmaf(max, c, -point(a.max, c));
+  else if (far(a.max, c))
+    d = __builtin_fmaf(a.max, c, -point(max, c));
+  // (a state of -inf alone: s is 0, whatever its point)
+  raise_by(a, max, a.max == q3::kNegInf ? -3e38f : d);
 }
 
-// Folds N tokens (-inf: none) into a state.
-template <int N, bool kEnt>
-__device__ __forceinline__ void fold(Sums& st, const float (&x)[N], float c) {
-  float m = st.max;
-#pragma unroll
-  for (int i = 0; i < N; i += 2) m = max3(m, x[i], x[i + 1]);
-  st.max = m;
-  move_ref(st, fmaxf(st.ref, m * c));
+// Adds N tokens (-inf: none) at y(x) = x c - P.
+template <int N, bool kEnt, typename Y>
+__device__ __forceinline__ void add(Sums& st, const float (&x)[N], const Y& exponent) {
   float s[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const float y = __builtin_fmaf(x[i], c, -st.ref);
+    const float y = exponent(x[i]);
     const float e = q3::fast_exp2(y);
     s[i & 3] += e;
     if constexpr (kEnt) s1[i & 3] = __builtin_fmaf(e, fmaxf(y, kTiny), s1[i & 3]);
   }
   st.s += (s[0] + s[1]) + (s[2] + s[3]);
   if constexpr (kEnt) st.s1 += (s1[0] + s1[1]) + (s1[2] + s1[3]);
+}
+
+// Folds N tokens into a state.
+template <int N, bool kEnt>
+__device__ __forceinline__ void fold(Sums& st, const float (&x)[N], float c) {
+  float m = st.max;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) m = max3(m, x[i], x[i + 1]);
+  const float p = point(m, c);
+  if (!__any(far(st.max, c) || far(m, c))) {
+    raise_by(st, m, point(st.max, c) - p);
+    add<N, kEnt>(st, x, [&](float v) { return __builtin_fmaf(v, c, -p); });
+  } else {
+    const bool off = far(m, c);
+    raise(st, m, c);
+    add<N, kEnt>(st, x, [&](float v) { return off ? (v - m) * c : __builtin_fmaf(v, c, -p); });
+  }
 }
 
 template <int kT>
@@ -241,13 +269,11 @@ struct Shared {
   uint32_t bound;
 };
 
-__device__ __forceinline__ void join_wave(Sums& st) {
+__device__ __forceinline__ void join_wave(Sums& st, float c) {
+  float max = st.max;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) st.max = fmaxf(st.max, q3::shfl_xor(st.max, o));
-  float ref = st.ref;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) ref = fmaxf(ref, q3::shfl_xor(ref, o));
-  move_ref(st, ref);
+  for (int o = 1; o < 64; o <<= 1) max = fmaxf(max, q3::shfl_xor(max, o));
+  raise(st, max, c);
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     st.s += q3::shfl_xor(st.s, o);
@@ -257,31 +283,24 @@ __device__ __forceinline__ void join_wave(Sums& st) {
 
 // The block's threads' states in one, on every thread.
 template <int kT>
-__device__ __forceinline__ void join_block(Sums& st, Shared<kT>& sh) {
+__device__ __forceinline__ void join_block(Sums& st, float c, Shared<kT>& sh) {
   constexpr int kWaves = kT / 64;
-  join_wave(st);
+  join_wave(st, c);
   if ((threadIdx.x & 63) == 0) sh.sums[threadIdx.x >> 6] = st;
   __syncthreads();
   Sums r = sh.sums[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) {
-    r.max = fmaxf(r.max, sh.sums[w].max);
-    r.ref = fmaxf(r.ref, sh.sums[w].ref);
-  }
+  for (int w = 1; w < kWaves; ++w) r.max = fmaxf(r.max, sh.sums[w].max);
   r.s = r.s1 = 0.f;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
     Sums o = sh.sums[w];
-    move_ref(o, r.ref);
+    raise(o, r.max, c);
     r.s += o.s;
     r.s1 += o.s1;
   }
   st = r;
   __syncthreads();
-}
-
-__device__ __forceinline__ bool extreme(float max, float c) {
-  return !(__builtin_fabsf(max * c) < kExtreme) && __builtin_fabsf(max) < __builtin_inff();
 }
 
 template <int kT>
@@ -512,12 +531,10 @@ __device__ __forceinline__ void top_tokens(const LogprobArgs& a, const char* xr,
   __syncthreads();
 }
 
-// log p of a logit: (x - max) / T - log(sum exp((x' - max) / T)), the sum from s, which is
-// relative to R, the rounded max c.
+// log p of a logit: (x - max) / T - log(sum exp((x' - max) / T)), the sum from s.
 __device__ __forceinline__ float logprob_of(const LogprobArgs& a, float x, float max,
                                             float log2s) {
-  const float mc = max * a.c;
-  const float shift = extreme(max, a.c) ? 0.f : __builtin_fmaf(max, a.c, -mc);
+  const float shift = far(max, a.c) ? 0.f : __builtin_fmaf(max, a.c, -point(max, a.c));
   const float r = __builtin_fmaf(x - max, a.inv_t, -kLn2 * (log2s - shift));
   return r > 0.f ? 0.f : r;  // by a rounding of the sum
 }
@@ -527,7 +544,6 @@ template <typename Tr>
 __device__ __forceinline__ void write_row(const LogprobArgs& a, const char* xr, int64_t row,
                                           const Sums& st, const u64* top) {
   const int tid = threadIdx.x, step = blockDim.x;
-  // (s is relative to R, the rounded max * c, or to max * c itself of an extreme max)
   const float log2s = __builtin_log2f(st.s);
   if (tid == 0) {
     if (a.entropy) {
@@ -561,7 +577,7 @@ __global__ __launch_bounds__(kT) void logprobs_kernel(LogprobArgs a) {
   const int p0 = min(part * a.per_part, a.pieces), p1 = min(p0 + a.per_part, a.pieces);
   const int whole = min(p1, a.vocab / E);  // pieces before it are whole ones
 
-  Sums st{q3::kNegInf, kFloor, 0.f, 0.f};
+  Sums st{q3::kNegInf, 0.f, 0.f};
   auto load = [&](int p, q3::u32x4 (&w)[kBatch]) {
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
@@ -601,25 +617,7 @@ __global__ __launch_bounds__(kT) void logprobs_kernel(LogprobArgs a) {
     }
   }
   const float mine = st.max;
-  join_block(st, sh);
-  if (extreme(st.max, a.c)) {  // the sums again, of (x - max) c
-    Sums ex{st.max, 0.f, 0.f, 0.f};
-    for (int p = p0 + tid; p < p1; p += kT) {
-      float x[E];
-      Tr::unpack(load_piece<Tr>(a, xr, p), x);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        int idx;
-        if (!token_at<Tr>(a, p, e, idx)) continue;
-        const float y = (x[e] - st.max) * a.c, v = q3::fast_exp2(y);
-        ex.s += v;
-        ex.s1 = __builtin_fmaf(v, fmaxf(y, kTiny), ex.s1);
-      }
-    }
-    join_block(ex, sh);
-    st.s = ex.s;
-    st.s1 = ex.s1;
-  }
+  join_block(st, a.c, sh);
   if constexpr (kTop) top_tokens<Tr, kT>(a, xr, p0, p1, mine, st.s != st.s, sh);
   if (a.parts == 1) {
     write_row<Tr>(a, xr, row, st, sh.top);
@@ -649,30 +647,9 @@ __global__ __launch_bounds__(kJoinThreads) void logprobs_join_kernel(LogprobArgs
   const int tid = threadIdx.x, lane = tid & 63;
   const int64_t row = blockIdx.x;
   const char* xr = a.x + row * a.row_bytes;
-  Sums st{q3::kNegInf, kFloor, 0.f, 0.f};
+  Sums st{q3::kNegInf, 0.f, 0.f};
   if (lane < a.parts) st = a.part_sums[row * a.parts + lane];  // (every wave)
-  float max = st.max;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) max = fmaxf(max, q3::shfl_xor(max, o));
-  {
-    // a part's own reference, R or max c, over the row's: parts of one row may have either
-    const bool far = extreme(max, a.c), part_far = extreme(st.max, a.c);
-    const float ref = fmaxf(kFloor, max * a.c);
-    float d = st.ref - ref;
-    if (far) d = part_far ? (st.max - max) * a.c : -__builtin_fmaf(max, a.c, -st.ref);
-    else if (part_far) d = __builtin_fmaf(st.max, a.c, -ref);
-    // (no number below the row's largest one: s is 0 or NaN)
-    d = st.max == q3::kNegInf ? -3e38f : fmaxf(d, -3e38f);
-    const float f = q3::fast_exp2(d);
-    st.s1 = f * (st.s1 + st.s * fmaxf(d, 2.f * kTiny));
-    st.s *= f;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      st.s += q3::shfl_xor(st.s, o);
-      st.s1 += q3::shfl_xor(st.s1, o);
-    }
-    st.max = max;
-  }
+  join_wave(st, a.c);
   const int all = a.parts * a.top;
   if (a.top) {
     for (int i = tid; i < all; i += kJoinThreads) s_all[i] = a.part_top[row * all + i];
@@ -783,8 +760,8 @@ __global__ __launch_bounds__(kGradThreads) void logprobs_grad_kernel(GradArgs g)
   for (int k = 0; k < special; ++k) sum += s_g[k];
   const float gh = g.g_entropy ? g.g_entropy[row] : 0.f;
   const float2 stats = g.stats[row];
-  const bool far = extreme(stats.x, a.c);
-  const float mc = stats.x * a.c, log2s = stats.y;
+  const bool off = far(stats.x, a.c);
+  const float p_max = point(stats.x, a.c), log2s = stats.y;
   // p_i (b + gh ln 2 log2 p_i)
   const float b = sum + (g.g_entropy ? gh * g.entropy[row] : 0.f), gl = gh * kLn2;
 #pragma unroll
@@ -795,7 +772,7 @@ __global__ __launch_bounds__(kGradThreads) void logprobs_grad_kernel(GradArgs g)
     Tr::unpack(w[u], x);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const float y = (far ? (x[e] - stats.x) * a.c : __builtin_fmaf(x[e], a.c, -mc)) - log2s;
+      const float y = (off ? (x[e] - stats.x) * a.c : __builtin_fmaf(x[e], a.c, -p_max)) - log2s;
       const float pr = q3::fast_exp2(y);
       x[e] = -pr * __builtin_fmaf(gl, fmaxf(y, kTiny), b);
     }
