@@ -310,7 +310,7 @@ int qwen3_sample_ws_bf16(const void* logits, int64_t row_stride, int64_t rows, i
  * temperature and log p = z - log(sum exp z):
  *   logprobs[r, k]      log p of tokens[r, k] (int64, rows x given, at most 64 a row).
  *                       A negative id is no token: 0.  One of vocab or more: NaN
- *   entropy[r]          -sum p log p (nullable)
+ *   entropy[r]          -sum p log p (nullable), at least 0
  *   top_ids[r, j], top_logprobs[r, j]   the top_n (at most 64 and vocab) largest logits,
  *                       descending, the lower index first among equal ones (-0 is 0;
  *                       NaN ranks above every number)

@@ -24,8 +24,9 @@
 // A row is cut into parts of whole rounds where there are too few rows for the device; a
 // second launch joins the parts.
 //
-// What bounds it: HBM where there are rows enough (4,096 x 151,936 bf16 198 us, 6.3 TB/s;
-// 1,003 x 50,021 fp32, 4 given, 8 listed, 40.7 us, 4.9 TB/s, of which the list some 5),
+// What bounds it: HBM where there are rows enough (4,096 x 151,936 bf16 200 us, 6.2 TB/s, with
+// 5 listed 226, with 20 listed 292; 1,003 x 50,021 fp32, 4 given, 8 listed, 41 us, 4.9 TB/s, of
+// which the list some 5),
 // latency in a decode step (64 rows, 20 listed: 12.7 us, of which the list 4, and 6.2 of the
 // join; one row, 5 listed, 7.3 and 4.4) and, with a list, in short rows.  The gradient reads
 // and writes 1.25 GB of 2,048 x 151,936 in 222 us, 5.6 TB/s, after 100 of the log

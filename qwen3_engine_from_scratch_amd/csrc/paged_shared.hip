@@ -23,15 +23,19 @@
 // sum), and the second launch joins each row's.  P is floored to whole tiles of 16 keys
 // and bounded by what the group's first sequence holds; the rest counts as each
 // sequence's own, and so does all of a sequence that ends inside P.  The probabilities meet
-// the values as two bf16 terms, as in the decode.
+// the values as two bf16 terms, as in the decode: what both leave of a probability is below
+// 2^-16 of it (each term's half step, 2^-8), against 2^-8 of the output's own rounding; one
+// term alone would be as far off as that.  A third would cost the staged tiles 8 more MFMAs
+// of 24.
 //
 // What bounds it: HBM, where sequences have much of their own (256 of 50-2,500 tokens behind
 // 2,000, 16/8 heads: 225 us, 5.7 TB/s); behind long prefixes the staged tiles, 1.87 us each
 // on each CU, where their loads alone take 1.4 (5.9 TB/s) and their products and softmax
 // alone 1.45: a SIMD's two waves issue 48 MFMAs of 32 cycles and 340 other vector
-// instructions a tile, and the time is near the sum of the two, 3,300 cycles, however they
-// are interleaved (32 sequences behind 100,000, 32/8 heads: 115 us, 3.8 TB/s; 64 behind
-// 8,192 and 1-1,000 tokens of their own 47 us, 3.2 TB/s); in small calls the latency of the
+// instructions a tile, near the sum of the two, 3,300 cycles, however they are interleaved.
+// The other 0.4 us are loads and products that wait for one another at the barrier of every
+// tile (32 sequences behind 100,000, 32/8 heads: 115-120 us, 3.7 TB/s; 64 behind 8,192 and
+// 1-1,000 tokens of their own 47-50 us, 3.1 TB/s); in small calls the latency of the
 // steps, 2.5 us until the batch is tabulated, 10 of the first tiles, 5 of the join (4 behind
 // 896, 16/8 heads: 14 us).
 // Attended one by one (paged_decode.hip) the same batches take 489, 1,817, 296 and 15 us.
@@ -39,7 +43,8 @@
 // Measured against it (32 behind 100,000; 64 behind 8,192): the values' products of both
 // halves of a tile's keys after the scores 117.7 us for 115.2; scores of one half taken a tile
 // ahead in stages of their own 113 for 113, 48 for 48, and all operands read from LDS a step
-// before they are used 121 for 119, 48 for 48; items of 256 rows 2.65 us a tile; parts
+// before they are used 121 for 119, 48 for 48; items of 256 rows 2.65 us a tile, for 3.74 of two
+// of 128 rows (not timed in a whole call of a batch that large); parts
 // stored past the caches 54.8 us for 52.6; waves' priorities no difference.
 #include <algorithm>
 
@@ -59,7 +64,8 @@ constexpr int kMaxWgs = 512;
 constexpr int kStages = 4;
 // Weight, in streamed tiles of 16 keys, of a staged tile of 64 (64 behind 8,192: 47.4 us; of
 // 4 51.3, of 6 49.8); what an item's start and end weigh, in tiles of its kind (staged, none
-// 51.6, of 8 48.3; streamed, none 52.7, of 3 48.7); tiles that a range takes at least
+// 51.6, of 8 48.3; streamed, none 52.7, of 3 48.7), all swept on that batch, whose items have
+// 128 rows, and taken for smaller ones too; tiles that a range takes at least
 // (staged, 1 to 4 the same; streamed, a chunk: 4 behind 4,096 23.8 us for 21.8, 16 behind
 // 4,096 23.2 for 23.8; four chunks 23.5 and 26.2).
 constexpr int kStagedUnits = 5;

@@ -101,10 +101,10 @@ class Engine:
         the pages that requests share once for all of them (requests with a common
         prefix handle), up to 1,024 requests; not with batch_invariant.  A prefix's
         sums are then taken in another order, so near ties may fall differently.  A
-        step of Qwen3-0.6B, 64 requests behind 8,192 tokens: 9.46 -> 2.00 ms, 32
-        behind 900 1.96 -> 1.67; up to 16 requests it goes without the chained
-        launches, so short prefixes lose (4 behind 900 1.11 -> 1.43, 16 behind 900
-        1.34 -> 1.55, behind 4,096 2.33 -> 1.65)."""
+        step of Qwen3-0.6B, 64 requests behind 8,192 tokens: 9.49 -> 2.00 ms, 32
+        behind 900 1.97 -> 1.71; up to 16 requests it goes without the chained
+        launches, whatever they share, so short prefixes lose (4 behind 900 1.11 -> 1.42,
+        16 behind 900 1.34 -> 1.56, behind 4,096 2.35 -> 1.63)."""
         assert prefill_chunk is None or prefill_chunk > 0
         if share_prefixes and (batch_invariant or max_batch > MAX_SHARED_BATCH):
             raise ValueError("share_prefixes needs batch_invariant off and a max_batch of at most "
